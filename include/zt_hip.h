@@ -656,6 +656,145 @@ int zt_gemm_int4_f32_rmul(const void* W, const float* B, float* C, const float* 
                           int in_features, int out_features, int group_size, zt_stream_t stream);
 int zt_gemm_int8_f32(const void* A, const float* B, float* C, int M, int K, int N, zt_stream_t stream);
 
+/* ---- a decode step between its linear layers --------------------------- */
+
+/* Rotary positions, an int8 paged key/value cache (written, read back and
+ * attended to), the pages' bookkeeping, and the choice of a token.  Host
+ * structures are read during the call only.  Where a value on the device
+ * cannot be checked by the host (a position, slot, page, length), the kernels
+ * check it themselves: nothing outside the buffers is read or written. */
+
+#define ZT_F32 0
+#define ZT_F16 1
+
+/* [tokens, heads, head_dim] rows, neighbouring values of a head next to each
+ * other; strides in elements.  The tokens' number and the head size are
+ * arguments of the call. */
+typedef struct zt_rows {
+    void* p;
+    long token_stride;
+    long head_stride;
+    int heads;
+    int reserved; /* 0 */
+} zt_rows;
+
+#define ZT_ROPE_INTERLEAVED 1 /* pairs (2i, 2i + 1); else (i, i + rot_dim / 2) */
+#define ZT_ROPE_INVERSE 2     /* by the negative angle: the gradient's way */
+
+/* out[i] = in[i] with the first rot_dim values of each head turned by its
+ * token's position, the others as they are: (a, b) -> (a c - b s, b c + a s),
+ * c and s from `table`, fp32 [max_pos][2][rot_dim / 2], cosines then sines, of
+ * the position (any scaling for long contexts is the table's).  Up to two
+ * tensors (q and k) in one launch; products and sums in fp32, each rounded by
+ * itself, the result rounded once to `type`.  out[i] may be in[i] itself.  A
+ * position outside 0 .. max_pos - 1 gives NaN in the turned values. rot_dim
+ * even, 0 < rot_dim <= head_dim, n 1 or 2, else InvalidValue. */
+int zt_rope(const zt_rows* in, const zt_rows* out, int n, const int* positions, const float* table, int tokens,
+            int head_dim, int rot_dim, int max_pos, int type, int flags, zt_stream_t stream);
+
+/* The cache: pages of page_tokens (16, 32, 64 or 128) tokens, a value is its
+ * code times the scale of its page and head.  Dp = head_dim to the next
+ * multiple of 64; codes past head_dim are 0.  head_dim % 8 == 0, at most 256;
+ * k and v 16-byte aligned. */
+typedef struct zt_kv8_cache {
+    void* k;        /* int8 [pages][kv_heads][page_tokens][Dp] */
+    void* v;        /* int8 [pages][kv_heads][Dp][page_tokens] */
+    float* k_scale; /* [pages][kv_heads] */
+    float* v_scale;
+    int pages;
+    int kv_heads;
+    int head_dim;
+    int page_tokens;
+} zt_kv8_cache;
+
+/* Puts the keys and values of `tokens` tokens at their slots (page *
+ * page_tokens + place; outside the cache: that token is left out).  Tokens of
+ * one page stand next to each other in ascending order, and no page comes
+ * twice, as zt_kv8_plan gives them.  A page's scale becomes the largest of
+ * what it was (0 if the page's first place is among the slots: it starts
+ * anew, its other places become 0) and the new values' largest magnitude
+ * times 1/127; where it grows, the codes that the page holds are taken over as
+ * rint(code * old / new).  A new code is rint(x / scale), x in fp32.  A value
+ * that is not finite makes its page's scale NaN, so that no reader takes the
+ * page for sound.  With `table` the keys are turned first (zt_rope's rule
+ * in fp32, not rounded in between), and q into q_out in the same launch; q,
+ * q_out NULL: none.  table NULL: keys as they are, positions are not read. */
+int zt_kv8_append(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v, const long* slots, const zt_rows* q,
+                  const zt_rows* q_out, const int* positions, const float* table, int tokens, int rot_dim, int max_pos,
+                  int type, int flags, zt_stream_t stream);
+
+/* The values of n pages: keys and values fp32 [n][kv_heads][page_tokens]
+ * [head_dim], code * scale.  A page outside the cache gives NaN. */
+int zt_kv8_dequant(const zt_kv8_cache* cache, const int* pages, int n, float* keys, float* values,
+                   zt_stream_t stream);
+
+/* Pages and slots of a step.  Request r holds kv_lens[r] tokens in the pages
+ * of its row of table [requests][width] and adds add[r] more.  Pages come off
+ * the end of the free list (free_pages[free_count - 1] first), to the requests
+ * in their order; table_out is table with them (it may be table itself).
+ * Token t of the step, the requests' tokens in their order, gets its slot and
+ * its position, request r's are q_start[r] .. q_start[r + 1] - 1 (requests + 1
+ * values), kv_lens_out[r] = kv_lens[r] + add[r], and free_count_out is what is
+ * left of the list.  A request whose pages are not there, or do not fit its
+ * row, gets none: its tokens' slots are -1 and its length stays.  Tokens past
+ * the last request's, up to `tokens`, get slot -1 and position 0.  Negative
+ * lengths count as 0.  free_capacity: the entries of free_pages. */
+int zt_kv8_plan(const int* kv_lens, const int* add, const int* table, int requests, int width, const int* free_pages,
+                const int* free_count, int free_capacity, int page_tokens, int tokens, int* table_out, long* slots,
+                int* positions, int* q_start, int* kv_lens_out, int* free_count_out, zt_stream_t stream);
+
+/* Causal attention over the cache: of request r's q rows q_start[r] ..
+ * q_start[r + 1] - 1, n of them, row i is at position kv_lens[r] - n + i (the
+ * step's own tokens are in the cache already) and sees the tokens up to its
+ * own, with window > 0 the last `window` of them.  q head h reads key/value
+ * head h / (q.heads / kv_heads).  out = softmax(scale q k^T) v; scale: one
+ * fp32 on the device, NULL: 1 / sqrt(head_dim).  q and out have one type; sums
+ * and softmax in fp32.  A row that sees nothing (no length, pages outside the
+ * cache) gives zeros, and so do rows that belong to no request.  Tokens on a
+ * page outside the cache are not seen.  max_q and max_kv are bounds that the
+ * host knows for the largest n and length (they choose the launch; a larger
+ * one is still computed).  Workspace: zt_kv8_attention_workspace_bytes (-1
+ * for a call that is refused), 16-byte aligned; short or missing ->
+ * InvalidValue.  Results do not depend on what else runs. */
+typedef struct zt_kv8_attn {
+    zt_kv8_cache cache;
+    zt_rows q;
+    zt_rows out;
+    const int* table;   /* [requests][width] */
+    const int* kv_lens; /* [requests] */
+    const int* q_start; /* [requests + 1] */
+    const float* scale;
+    int requests;
+    int width;
+    int tokens; /* rows of q and out */
+    int max_q;
+    int max_kv;
+    int window;
+    int type;
+    int reserved; /* 0 */
+} zt_kv8_attn;
+long zt_kv8_attention_workspace_bytes(const zt_kv8_attn* a);
+int zt_kv8_attention(const zt_kv8_attn* a, void* workspace, long workspace_bytes, zt_stream_t stream);
+
+/* A token of each row of logits [rows][vocab] (row_stride elements apart) from
+ * u[row] in [0, 1).  With z the row's values (NaN counts as -inf) and m their
+ * largest, token i weighs w_i = exp((z_i - m) / T), taken down to a whole
+ * multiple of 2^-40 (1 where z_i = m).  Of the tokens in order of falling z,
+ * equal ones by index, stay the first n: n is at most top_k (<= 0 or > vocab:
+ * all) and the number of tokens with w_i >= min_p (at most 1); with top_p < 1
+ * it is the least whose weights reach top_p of those n's.  The token is the
+ * first, in order of the index, at which the running sum of the kept weights
+ * exceeds floor(u times their sum).  T <= 0 or NaN: the largest, lowest index
+ * first.  The sums are of whole numbers, so their order does not matter.
+ * logprob: log of the token's share of the kept weights.  A row without a
+ * value above -inf: token -1, logprob NaN.  NULL temperature, top_k, top_p,
+ * min_p: 1, off, off, off for every row.  vocab from 1 to 2^20; workspace as
+ * above. */
+long zt_sample_workspace_bytes(int rows, int vocab);
+int zt_sample(const void* logits, long row_stride, int rows, int vocab, int type, const float* u,
+              const float* temperature, const int* top_k, const float* top_p, const float* min_p, long* token,
+              float* logprob, void* workspace, long workspace_bytes, zt_stream_t stream);
+
 /* ---- measurement ------------------------------------------------------- */
 
 /* No counterpart in the reference: a plain streaming read of nbytes at p

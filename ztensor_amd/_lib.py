@@ -132,6 +132,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "zt_dequant_iq3s_f32": (I, [P, L, P, L, P]),
     "zt_gemm_wide_workspace_bytes": (L, [I, I, I, I, I]),
     "zt_gemm_wide_f32": (I, [I, P, L, L, P, I, P, I, P, I, I, I, P, L, P]),
+    "zt_rope": (I, [P, P, I, P, P, I, I, I, I, I, I, P]),
+    "zt_kv8_append": (I, [P, P, P, P, P, P, P, P, I, I, I, I, I, P]),
+    "zt_kv8_dequant": (I, [P, P, I, P, P, P]),
+    "zt_kv8_plan": (I, [P, P, P, I, I, P, P, I, I, I, P, P, P, P, P, P, P]),
+    "zt_kv8_attention_workspace_bytes": (L, [P]),
+    "zt_kv8_attention": (I, [P, P, L, P]),
+    "zt_sample_workspace_bytes": (L, [I, I]),
+    "zt_sample": (I, [P, L, I, I, I, P, P, P, P, P, P, P, P, L, P]),
     "zt_gemm_int8_f32": (I, [P, P, P, I, I, I, P]),
     "zt_gemm_int4_f32": (I, [P, P, P, P, P, I, I, I, I, P]),
     "zt_gemm_int4_f32_rmul": (I, [P, P, P, P, P, I, I, I, I, P]),
@@ -185,6 +193,33 @@ def w4a16_gemv_descs(entries) -> C.Array:
     for i, (w, szr, y, rows) in enumerate(entries):
         arr[i].W, arr[i].szr, arr[i].y, arr[i].rows, arr[i].reserved = w, szr, y, rows, 0
     return arr
+
+
+F32, F16 = 0, 1  # ZT_F32, ZT_F16
+ROPE_INTERLEAVED, ROPE_INVERSE = 1, 2  # ZT_ROPE_*
+
+
+class Rows(C.Structure):
+    """zt_rows: a [tokens, heads, head_dim] operand, strides in elements."""
+
+    _fields_ = [("p", C.c_void_p), ("token_stride", C.c_long), ("head_stride", C.c_long), ("heads", C.c_int),
+                ("reserved", C.c_int)]
+
+
+class KV8(C.Structure):
+    """zt_kv8_cache: the buffers and sizes of an int8 paged cache."""
+
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("pages", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("page_tokens", C.c_int)]
+
+
+class KV8Attn(C.Structure):
+    """zt_kv8_attn: one attention call."""
+
+    _fields_ = [("cache", KV8), ("q", Rows), ("out", Rows), ("table", C.c_void_p), ("kv_lens", C.c_void_p),
+                ("q_start", C.c_void_p), ("scale", C.c_void_p), ("requests", C.c_int), ("width", C.c_int),
+                ("tokens", C.c_int), ("max_q", C.c_int), ("max_kv", C.c_int), ("window", C.c_int),
+                ("type", C.c_int), ("reserved", C.c_int)]
 
 
 class ZTError(RuntimeError):

@@ -1,0 +1,501 @@
+// Rotary positions, and the int8 paged cache of keys and values: its writer,
+// its dequantizer, and the pages' bookkeeping.  The attention that reads it is
+// in zt_attn.hip.
+//
+// All of it moves bytes: a page holds, for each head, page x Dp codes of keys
+// [token][dim] and as many of values [dim][token] (the order in which the
+// attention's two products read them), and one fp32 scale of each.
+#include "zt_kv8.h"
+
+namespace zt {
+
+constexpr int kThreads = 256;
+
+// ------------------------------------------------------------------- rotary
+
+struct RopeArgs {
+    Rows in[2], out[2];
+    Turn turn;
+    int tokens, dim;
+    int units;       // of one head
+    int all;         // of one token
+    int per_block;   // tokens that a workgroup takes (1 where a token fills more than one)
+    int chunks;      // workgroups that such a token takes
+};
+
+// One unit of 2 V values a thread.
+template <class T, int V>
+__device__ __forceinline__ void rope_block(const RopeArgs& g, int block) {
+    const int group = g.chunks == 1 ? block : block / g.chunks;
+    const int i = (block - group * g.chunks) * kThreads + threadIdx.x;
+    if (i >= g.per_block * g.all) return;
+    const int tl = g.per_block == 1 ? 0 : i / g.all, r = i - tl * g.all;
+    const long t = (long)group * g.per_block + tl;
+    if (t >= g.tokens) return;
+    int h = r / g.units;
+    const int u = r - h * g.units;
+    const int w = h >= g.in[0].heads;
+    h -= w ? g.in[0].heads : 0;
+    const Rows &x = g.in[w], &y = g.out[w];
+    float a[V], b[V];
+    int first, second;
+    turned<T, V>((const T*)x.p + t * x.token + h * x.head, u, g.turn.positions[t], g.turn, a, b, first, second);
+    T* o = (T*)y.p + t * y.token + h * y.head;
+    store_values<T, V>(o + first, a);
+    store_values<T, V>(o + second, b);
+}
+
+template <class T, int V>
+__global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs g) {
+    rope_block<T, V>(g, blockIdx.x);
+}
+
+// The launch of n operands, and the units' size: V.
+__host__ inline long rope_blocks(RopeArgs& g, int n, int V) {
+    const int heads = g.in[0].heads + (n > 1 ? g.in[1].heads : 0);
+    g.units = g.turn.half / V + (g.dim - 2 * g.turn.half) / (2 * V);
+    g.all = heads * g.units;
+    g.per_block = g.all >= kThreads ? 1 : kThreads / g.all;
+    g.chunks = ceil_div(g.per_block * g.all, kThreads);
+    return (long)ceil_div(g.tokens, g.per_block) * g.chunks;
+}
+
+// The widest V that all operands allow: 16 bytes of fp16 or fp32, 4 values, else one by one.
+__host__ inline int rope_width(const zt_rows* const* r, int n, int dim, int half, int type) {
+    const int widths[2] = {8, 4};
+    for (int v : widths) {
+        bool ok = units_fit(v, dim, half) && (v == 4 || type == ZT_F16);
+        for (int i = 0; i < n && ok; i++) ok = rows_vector(*r[i], v, type);
+        if (ok) return v;
+    }
+    return 1;
+}
+
+}  // namespace zt
+
+using namespace zt;
+
+ZT_EXPORT int zt_rope(const zt_rows* in, const zt_rows* out, int n, const int* positions, const float* table, int tokens,
+                      int head_dim, int rot_dim, int max_pos, int type, int flags, zt_stream_t stream) {
+    if (!in || !out || n < 1 || n > 2 || tokens < 0 || head_dim < 2 || head_dim % 2 || rot_dim < 2 || rot_dim % 2 ||
+        rot_dim > head_dim || max_pos < 1 || !type_ok(type) || (flags & ~(ZT_ROPE_INTERLEAVED | ZT_ROPE_INVERSE)))
+        return kInvalid;
+    const zt_rows* all[4];
+    for (int i = 0; i < n; i++) {
+        if (in[i].heads != out[i].heads || in[i].heads > (1 << 20) / head_dim) return kInvalid;
+        all[2 * i] = in + i;
+        all[2 * i + 1] = out + i;
+    }
+    if (tokens == 0) return 0;
+    for (int i = 0; i < 2 * n; i++)
+        if (!rows_ok(*all[i], type)) return kInvalid;
+    if (!positions || !table || ((uintptr_t)positions & 3) || ((uintptr_t)table & 3)) return kInvalid;
+    RopeArgs g{};
+    for (int i = 0; i < n; i++) {
+        g.in[i] = rows_of(in[i]);
+        g.out[i] = rows_of(out[i]);
+    }
+    g.turn = {positions, table, rot_dim / 2, max_pos, flags};
+    g.tokens = tokens;
+    g.dim = head_dim;
+    const int v = rope_width(all, 2 * n, head_dim, rot_dim / 2, type);
+    const long blocks = rope_blocks(g, n, v);
+    if (blocks >= 1l << 31) return kInvalid;
+    if (type == ZT_F32) {
+        if (v == 4)
+            rope_kernel<float, 4><<<blocks, kThreads, 0, stream>>>(g);
+        else
+            rope_kernel<float, 1><<<blocks, kThreads, 0, stream>>>(g);
+    } else if (v == 8) {
+        rope_kernel<_Float16, 8><<<blocks, kThreads, 0, stream>>>(g);
+    } else if (v == 4) {
+        rope_kernel<_Float16, 4><<<blocks, kThreads, 0, stream>>>(g);
+    } else {
+        rope_kernel<_Float16, 1><<<blocks, kThreads, 0, stream>>>(g);
+    }
+    return (int)hipGetLastError();
+}
+
+// ------------------------------------------------------------------- append
+
+namespace zt {
+
+struct AppendArgs {
+    Kv8 c;
+    Rows x[2];  // keys, values
+    const long* slots;
+    Turn turn;  // half == 0: keys as they are
+    int tokens;
+    int window;  // tokens whose pages a workgroup looks after, for one head of keys or of values
+    long blocks;
+};
+
+// The largest m of the workgroup, and whether any of its threads said bad.
+__device__ __forceinline__ void block_peak(float& m, bool& bad, float* red) {
+    bad = __any(bad);
+    m = max_step<1>(max_step<2>(max_step<4>(max_step<8>(max_step<16>(max_step<32>(m))))));
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) red[wave] = bad ? __builtin_inff() : m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    bad = m > kMaxFloat;
+}
+
+__device__ __forceinline__ int code_of(float x, float scale) {
+    const float q = rintf(x / scale);
+    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
+}
+
+// The n tokens from t on, which go to one page from place `off` on: the page's
+// new scale, and its codes by way of an image of it in LDS.
+template <class T, int V, bool VALUES>
+__device__ __forceinline__ void append_page(const AppendArgs& g, int t, int n, int page, int off, int head,
+                                            uint32_t* image, float* red) {
+    const Kv8& c = g.c;
+    const Rows& x = g.x[VALUES];
+    Turn turn = g.turn;
+    if (VALUES) turn.half = 0;
+    const int units = units_of<V>(c.dim, turn.half);
+    const T* rows = (const T*)x.p + (long)t * x.token + (long)head * x.head;
+    float a[V], b[V];
+    int first, second;
+
+    float m = 0.0f;
+    bool bad = false;
+    for (int i = threadIdx.x; i < n * units; i += kThreads) {
+        const int tl = i / units, u = i - tl * units;
+        const int pos = turn.half ? turn.positions[t + tl] : 0;
+        turned<T, V>(rows + tl * x.token, u, pos, turn, a, b, first, second);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            m = fmaxf(m, fmaxf(fabsf(a[j]), fabsf(b[j])));
+            bad |= !(fabsf(a[j]) <= kMaxFloat) || !(fabsf(b[j]) <= kMaxFloat);
+        }
+    }
+    block_peak(m, bad, red);
+
+    float* scales = VALUES ? c.v_scale : c.k_scale;
+    const long place = (long)page * c.heads + head;
+    const bool fresh = off == 0;
+    const float had = fresh ? 0.0f : scales[place];
+    const float now = bad || had != had ? __builtin_nanf("") : fmaxf(had, m * (1.0f / 127.0f));
+    const bool grown = now > had, whole = fresh || grown;
+    u32x4* codes = reinterpret_cast<u32x4*>((VALUES ? c.v : c.k) + c.at(page, head));
+    u32x4* image4 = reinterpret_cast<u32x4*>(image);
+    const int pieces = c.bytes() / 16;
+    const float ratio = grown ? had / now : 0.0f;
+    if (grown && !fresh) {
+        for (int i = threadIdx.x; i < pieces; i += kThreads) {
+            u32x4 w = codes[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t o = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    o |= ((uint32_t)(int)rintf((float)(int8_t)(w[j] >> 8 * e) * ratio) & 0xFFu) << 8 * e;
+                w[j] = o;
+            }
+            image4[i] = w;
+        }
+    } else if (whole || !VALUES) {  // zeros where nothing new comes; of a page that goes on, its new keys' rows
+        const int lo = whole ? 0 : off * c.dp / 16, hi = whole ? pieces : (off + n) * c.dp / 16;
+        for (int i = lo + threadIdx.x; i < hi; i += kThreads) image4[i] = (u32x4){0, 0, 0, 0};
+    }
+    __syncthreads();  // (the scale has been read by everybody, too)
+
+    int8_t* bytes = reinterpret_cast<int8_t*>(image);
+    const float step = now > 0.0f ? now : 1.0f;  // 1 for a NaN, whose codes nobody takes for values
+    for (int i = threadIdx.x; i < n * units; i += kThreads) {
+        const int tl = i / units, u = i - tl * units;
+        const int pos = turn.half ? turn.positions[t + tl] : 0;
+        turned<T, V>(rows + tl * x.token, u, pos, turn, a, b, first, second);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const int p = code_of(a[j], step), q = code_of(b[j], step);
+            if (VALUES) {
+                bytes[(first + j) * c.page + off + tl] = (int8_t)p;
+                bytes[(second + j) * c.page + off + tl] = (int8_t)q;
+            } else {
+                bytes[(off + tl) * c.dp + first + j] = (int8_t)p;
+                bytes[(off + tl) * c.dp + second + j] = (int8_t)q;
+            }
+        }
+    }
+    __syncthreads();
+
+    if (whole || !VALUES) {
+        const int lo = whole ? 0 : off * c.dp / 16, hi = whole ? pieces : (off + n) * c.dp / 16;
+        for (int i = lo + threadIdx.x; i < hi; i += kThreads) codes[i] = image4[i];
+    } else {
+        int8_t* out = reinterpret_cast<int8_t*>(codes);
+        for (int i = threadIdx.x; i < c.dim * n; i += kThreads) {
+            const int d = i / n, at = d * c.page + off + i - d * n;
+            out[at] = bytes[at];
+        }
+    }
+    if (threadIdx.x == 0) scales[place] = now;
+    __syncthreads();  // the image is free again
+}
+
+template <class T, int V>
+__global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, RopeArgs q) {
+    __shared__ __align__(16) uint32_t image[128 * 256 / 4];
+    __shared__ float red[4];
+    __shared__ int count;
+    if (blockIdx.x >= g.blocks) {
+        rope_block<T, V>(q, blockIdx.x - g.blocks);
+        return;
+    }
+    const Kv8& c = g.c;
+    const int values = blockIdx.x & 1, head = (blockIdx.x >> 1) % c.heads;
+    const int from = (blockIdx.x >> 1) / c.heads * g.window, to = min(g.tokens, from + g.window);
+    const long slots = (long)c.pages << c.shift;
+    for (int t = from; t < to; t++) {
+        const long s = g.slots[t];
+        const int off = (int)(s & (c.page - 1));
+        // tokens that go on from the one before, in its page, belong to that one's workgroup
+        if (s < 0 || s >= slots || (t > 0 && off != 0 && g.slots[t - 1] == s - 1)) continue;
+        if (threadIdx.x == 0) count = min(c.page - off, g.tokens - t);
+        __syncthreads();
+        if ((int)threadIdx.x < count && g.slots[t + threadIdx.x] != s + threadIdx.x) atomicMin(&count, (int)threadIdx.x);
+        __syncthreads();
+        const int n = count, page = (int)(s >> c.shift);
+        if (values)
+            append_page<T, V, true>(g, t, n, page, off, head, image, red);
+        else
+            append_page<T, V, false>(g, t, n, page, off, head, image, red);
+    }
+}
+
+}  // namespace zt
+
+ZT_EXPORT int zt_kv8_append(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v, const long* slots,
+                            const zt_rows* q, const zt_rows* q_out, const int* positions, const float* table, int tokens,
+                            int rot_dim, int max_pos, int type, int flags, zt_stream_t stream) {
+    if (!cache || !kv8_ok(*cache) || !k || !v || tokens < 0 || !type_ok(type) || (flags & ~ZT_ROPE_INTERLEAVED) ||
+        (q == nullptr) != (q_out == nullptr) || (q && !table))
+        return kInvalid;
+    const int dim = cache->head_dim, half = table ? rot_dim / 2 : 0;
+    if (table && (rot_dim < 2 || rot_dim % 2 || rot_dim > dim || max_pos < 1)) return kInvalid;
+    if (k->heads != cache->kv_heads || v->heads != cache->kv_heads) return kInvalid;
+    if (q && (q->heads != q_out->heads || q->heads > (1 << 20) / dim)) return kInvalid;
+    if (tokens == 0) return 0;
+    const zt_rows* all[4] = {k, v, q, q_out};
+    const int n = q ? 4 : 2;
+    for (int i = 0; i < n; i++)
+        if (!rows_ok(*all[i], type)) return kInvalid;
+    if (!slots || ((uintptr_t)slots & 7) || (table && (!positions || ((uintptr_t)positions & 3) || ((uintptr_t)table & 3))))
+        return kInvalid;
+    // values are not turned: their units are those of a head without pairs, which 8 values divide
+    const int width = rope_width(all, n, dim, half, ZT_F32) == 4 && rope_width(all, n, dim, half, type) >= 4 ? 4 : 1;
+    AppendArgs g{};
+    g.c = kv8_of(*cache);
+    g.x[0] = rows_of(*k);
+    g.x[1] = rows_of(*v);
+    g.slots = slots;
+    g.turn = {positions, table, half, max_pos, flags};
+    g.tokens = tokens;
+    // a workgroup for each token's page while they are few, else for 16 tokens' pages: most tokens of a prompt are not
+    // the first of their page, and a workgroup that finds none to do costs its launch
+    g.window = tokens <= 2048 ? 1 : 16;
+    g.blocks = 2l * cache->kv_heads * ceil_div(tokens, g.window);
+    RopeArgs r{};
+    long blocks = g.blocks;
+    if (q) {
+        r.in[0] = rows_of(*q);
+        r.out[0] = rows_of(*q_out);
+        r.turn = g.turn;
+        r.tokens = tokens;
+        r.dim = dim;
+        blocks += rope_blocks(r, 1, width);
+    }
+    if (blocks >= 1l << 31) return kInvalid;
+    if (type == ZT_F32) {
+        if (width == 4)
+            append_kernel<float, 4><<<blocks, kThreads, 0, stream>>>(g, r);
+        else
+            append_kernel<float, 1><<<blocks, kThreads, 0, stream>>>(g, r);
+    } else if (width == 4) {
+        append_kernel<_Float16, 4><<<blocks, kThreads, 0, stream>>>(g, r);
+    } else {
+        append_kernel<_Float16, 1><<<blocks, kThreads, 0, stream>>>(g, r);
+    }
+    return (int)hipGetLastError();
+}
+
+// ------------------------------------------------------------------ dequant
+
+namespace zt {
+
+// One page and head of keys or of values a workgroup, 4 values a store.  Values
+// go through LDS, in rows 4 bytes longer than a page so that neighbouring dims
+// of one token lie in different banks.
+__global__ __launch_bounds__(kThreads) void dequant_kernel(Kv8 c, const int* pages, float* keys, float* values) {
+    __shared__ uint32_t image[256 * (128 + 4) / 4];
+    const int is_v = blockIdx.x & 1, head = (blockIdx.x >> 1) % c.heads, i = (blockIdx.x >> 1) / c.heads;
+    const int p = pages[i];
+    const bool held = c.holds(p);
+    float* out = (is_v ? values : keys) + ((long)i * c.heads + head) * c.page * c.dim;
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>((is_v ? c.v : c.k) + (held ? c.at(p, head) : 0));
+    const float scale = held ? (is_v ? c.v_scale : c.k_scale)[(long)p * c.heads + head] : __builtin_nanf("");
+    const int row = is_v ? c.page / 4 : 0;
+    if (is_v && held) {
+        for (int j = threadIdx.x; j < c.dim * row; j += kThreads) image[j / row * (row + 1) + j % row] = codes[j];
+    }
+    __syncthreads();
+    const int8_t* bytes = reinterpret_cast<const int8_t*>(image);
+    const int quads = c.dim / 4;
+    for (int j = threadIdx.x; j < c.page * quads; j += kThreads) {
+        const int t = j / quads, d = (j - t * quads) * 4;
+        float o[4];
+        if (is_v) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = (float)bytes[(d + e) * (c.page + 4) + t] * scale;
+        } else {
+            const uint32_t w = held ? codes[(t * c.dp + d) / 4] : 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = (float)(int8_t)(w >> 8 * e) * scale;
+        }
+        store16(out + (long)t * c.dim + d, o);
+    }
+}
+
+}  // namespace zt
+
+ZT_EXPORT int zt_kv8_dequant(const zt_kv8_cache* cache, const int* pages, int n, float* keys, float* values,
+                             zt_stream_t stream) {
+    if (!cache || !kv8_ok(*cache) || n < 0) return kInvalid;
+    if (n == 0) return 0;
+    if (!pages || !keys || !values || (((uintptr_t)pages | (uintptr_t)keys | (uintptr_t)values) & 3)) return kInvalid;
+    const long blocks = 2l * n * cache->kv_heads;
+    if (blocks >= 1l << 31) return kInvalid;
+    dequant_kernel<<<blocks, kThreads, 0, stream>>>(kv8_of(*cache), pages, keys, values);
+    return (int)hipGetLastError();
+}
+
+// --------------------------------------------------------------------- plan
+
+namespace zt {
+
+struct PlanArgs {
+    const int *kv_lens, *add, *table, *free_pages, *free_count;
+    int requests, width, free_capacity, shift, tokens;
+    int *table_out, *positions, *q_start, *kv_lens_out, *free_count_out;
+    long* slots;
+};
+
+struct Request {
+    int held, add, have, need;  // tokens held and added, pages held and wanted
+    bool fits;
+};
+
+__device__ __forceinline__ Request request(const PlanArgs& g, int r) {
+    Request q;
+    q.held = max(0, g.kv_lens[r]);
+    q.add = max(0, g.add[r]);
+    const long end = (long)q.held + q.add, room = (1l << g.shift) - 1;
+    q.fits = end <= (long)g.width << g.shift;
+    q.have = (int)((q.held + room) >> g.shift);
+    q.need = q.fits ? (int)((end + room) >> g.shift) - q.have : 0;
+    return q;
+}
+
+// The workgroup's sum of v, in every thread.
+__device__ __forceinline__ long block_sum(long v, long* red) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return red[0] + red[1] + red[2] + red[3];
+}
+
+// Workgroup r: request r's row, tokens and length.  Each sums up what the
+// requests before it add and want by itself (a few loads a thread: no second
+// launch, no order among the workgroups).  The last one has the tokens past
+// the last request's, and what is left of the free list: a request that wants
+// pages gets them if the wants up to its own are there, so once one does not,
+// no later one does, and the largest sum that is there has been given away.
+__global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs g) {
+    __shared__ long red[4];
+    const int r = blockIdx.x;
+    const int free = min(max(0, *g.free_count), g.free_capacity);
+    long before = 0, wanted = 0;
+    for (int i = threadIdx.x; i < r; i += kThreads) {
+        const Request q = request(g, i);
+        before += q.add;
+        wanted += q.need;
+    }
+    before = block_sum(before, red);
+    wanted = block_sum(wanted, red);
+    if (r < g.requests) {
+        const Request q = request(g, r);
+        const bool done = q.fits && (q.need == 0 || wanted + q.need <= free);
+        const int* row = g.table + (long)r * g.width;
+        int* out = g.table_out + (long)r * g.width;
+        const int* fresh = g.free_pages + (free - 1 - wanted + q.have);  // read at -j: page j of the row, if it is new
+        for (int j = threadIdx.x; j < g.width; j += kThreads)
+            out[j] = done && j >= q.have && j < q.have + q.need ? fresh[-j] : row[j];
+        for (long i = threadIdx.x; i < q.add && before + i < g.tokens; i += kThreads) {
+            const long pos = q.held + i;
+            const int j = (int)(pos >> g.shift);
+            const int page = !done ? -1 : j >= q.have ? fresh[-j] : row[j];
+            g.slots[before + i] = page < 0 ? -1 : ((long)page << g.shift) + (pos & ((1l << g.shift) - 1));
+            g.positions[before + i] = (int)pos;
+        }
+        if (threadIdx.x == 0) {
+            g.q_start[r] = (int)min(before, 0x7FFFFFFFl);
+            g.kv_lens_out[r] = done ? q.held + q.add : q.held;
+        }
+        return;
+    }
+    for (long i = before + threadIdx.x; i < g.tokens; i += kThreads) {
+        g.slots[i] = -1;
+        g.positions[i] = 0;
+    }
+    __shared__ int sums[2][kThreads];
+    __shared__ int given;
+    if (threadIdx.x == 0) {
+        g.q_start[r] = (int)min(before, 0x7FFFFFFFl);
+        given = 0;
+    }
+    int base = 0;
+    for (int i0 = 0; i0 < g.requests; i0 += kThreads) {  // running sums, 256 requests at a time
+        const int i = i0 + (int)threadIdx.x, need = i < g.requests ? request(g, i).need : 0;
+        int upto = need, at = 0;
+        sums[0][threadIdx.x] = upto;
+        __syncthreads();
+        for (int o = 1; o < kThreads; o <<= 1, at ^= 1) {
+            upto += (int)threadIdx.x >= o ? sums[at][threadIdx.x - o] : 0;
+            sums[at ^ 1][threadIdx.x] = upto;
+            __syncthreads();
+        }
+        if (need > 0 && base + upto <= free) atomicMax(&given, base + upto);
+        base += sums[at][kThreads - 1];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *g.free_count_out = free - given;
+}
+
+}  // namespace zt
+
+ZT_EXPORT int zt_kv8_plan(const int* kv_lens, const int* add, const int* table, int requests, int width,
+                          const int* free_pages, const int* free_count, int free_capacity, int page_tokens, int tokens,
+                          int* table_out, long* slots, int* positions, int* q_start, int* kv_lens_out,
+                          int* free_count_out, zt_stream_t stream) {
+    if (requests < 0 || width < 1 || tokens < 0 || free_capacity < 0 || !page_tokens_ok(page_tokens) ||
+        (long)requests * width >= 1l << 31 || requests >= 1 << 24)
+        return kInvalid;
+    if (requests && (!kv_lens || !add || !table || !table_out || !kv_lens_out)) return kInvalid;
+    if ((free_capacity && !free_pages) || !free_count || !free_count_out || !q_start || (tokens && (!slots || !positions)))
+        return kInvalid;
+    const void* ints[] = {kv_lens,   add,       table,   free_pages,  free_count,
+                          table_out, positions, q_start, kv_lens_out, free_count_out};
+    for (const void* p : ints)
+        if ((uintptr_t)p & 3) return kInvalid;
+    if ((uintptr_t)slots & 7) return kInvalid;
+    PlanArgs g{kv_lens,  add,     table,     free_pages, free_count, requests,    width,         free_capacity, __builtin_ctz(page_tokens),
+               tokens,   table_out, positions, q_start,  kv_lens_out, free_count_out, slots};
+    plan_kernel<<<requests + 1, kThreads, 0, stream>>>(g);
+    return (int)hipGetLastError();
+}

@@ -26,6 +26,8 @@ import numpy as np
 import torch
 
 from . import _lib
+from ._stream import _on_engine_stream
+from .decode import DecodeOps
 from .storage import (
     AWQStorage,
     Float16Storage,
@@ -53,28 +55,6 @@ def _p(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _on_engine_stream(fn):
-    """Runs an engine method with the engine's stream as torch's current
-    stream, so every temporary it makes (clones, transposes, pads, outputs,
-    tiled copies, the workspace) is allocated and written in the same stream
-    order as the kernels that read it, and the caching allocator never hands
-    one of them to other work while a kernel on the engine stream still uses
-    it.  Inputs made on another stream must be ready before the call, and
-    outputs used on another stream must wait for the engine stream, as with
-    any stream-ordered library.  Where the caller's current stream is the
-    engine's own already, there is nothing to switch (a call on 1024 x 4096
-    Q4_0 weights spent 6 of its 24 us on the two switches)."""
-
-    def wrapped(self, *args, **kwargs):
-        if self._is_current():
-            return fn(self, *args, **kwargs)
-        with torch.cuda.stream(self.stream):
-            return fn(self, *args, **kwargs)
-
-    wrapped.__name__, wrapped.__doc__, wrapped.__wrapped__ = fn.__name__, fn.__doc__, fn  # type: ignore[attr-defined]
-    return wrapped
-
-
 def _tiled_cached(s: Any, key: tuple):
     """The tiled device copy cached on a storage for `key`
     (format tag, rows, K, source buffer address), or None."""
@@ -84,7 +64,7 @@ def _tiled_cached(s: Any, key: tuple):
     return None
 
 
-class ROCmEngine:
+class ROCmEngine(DecodeOps):
     def __init__(self, device: int = 0, stream: torch.cuda.Stream | None = None, q6k_split: bool = True,
                  split_reserve_bytes: int = 1 << 30, token_copies: bool = True):
         """q6k_split: Q6_K batch 1 on a split copy of the super-blocks (35-55%
