@@ -33,13 +33,29 @@ __device__ __forceinline__ int find_request(const AttnArgs& g, int t, int& lo, i
 
 // ------------------------------------------------- few rows: a long axis split
 
-struct FewArgs {
+// Workgroups of one request and head along its tokens, and the tiles of 64
+// tokens that each takes (the last one: all that are left).
+struct Split {
+    int splits, tiles;
+};
+
+struct Work {
     AttnArgs a;
-    int splits, tiles;  // workgroups of one request and head along its tokens, tiles of 64 tokens of each (the last: all)
-    int few;            // requests of more rows than that (a row: a token and one of the heads of a group) are others' work
-    int vec;            // q and out in pieces of 4 values
-    float* part;        // [splits][tokens][q heads][dp] sums of the splits, not yet divided,
-    float2* stat;       // [splits][tokens][q heads] and their (maximum, sum of weights)
+    Split few, many;
+    int most;    // requests of up to so many rows (a row: a token and one of the heads of a group) are the few kernel's
+    int qtiles;  // workgroups along the rows of the other kernel
+    int vec;     // q and out in pieces of 4 values
+    int room;    // rows of a request and head whose splits' sums there is room for
+    long others; // where the other kernel's begin
+    float* part;   // [][dp]: sums of a row's split, not yet divided,
+    float2* stat;  // and their (maximum, sum of weights)
+    // the place of a row's sums: of the few kernel's, and of the other's
+    __device__ __forceinline__ long few_at(int split, int r, int kv, int row) const {
+        return (((long)split * a.requests + r) * a.c.heads + kv) * room + row;
+    }
+    __device__ __forceinline__ long many_at(int split, int t, int h) const {
+        return others + ((long)split * a.tokens + t) * a.q.heads + h;
+    }
 };
 
 // 8 codes as fp16, exact: each byte, its sign bit turned over, goes under the
@@ -115,9 +131,73 @@ __device__ __forceinline__ Span span_of(const AttnArgs& g, int r) {
     return s;
 }
 
-// Splits that a request's tiles fill.
-__device__ __forceinline__ int splits_of(const FewArgs& f, const Span& s) {
-    return min(f.splits, max(1, (s.tile1 - s.tile0 + f.tiles - 1) / f.tiles));
+// Splits that so many tiles fill.
+__device__ __forceinline__ int splits_of(const Split& f, int tiles) {
+    return min(f.splits, max(1, (tiles + f.tiles - 1) / f.tiles));
+}
+
+// Row `row` of a request and key/value head as this lane's operands: dims 64 d
+// + 16 (lane / 16) .. +16 of each d, fp32 rows in two parts after a power of
+// two; factor: what a product of it is to be multiplied by for a score in
+// units of log 2; the tokens lo .. hi - 1 that it sees (hi 0: no such row).
+template <class T, int DN>
+__device__ __forceinline__ void load_query(const Work& f, const Span& sp, int kv, int row, int rows, float scale,
+                                           half8v (&q)[DN][2], half8v (&ql)[DN][2], float& factor, int& lo, int& hi) {
+    constexpr bool SPLIT = sizeof(T) == 4;
+    const AttnArgs& g = f.a;
+    const int i = row / g.group, h = kv * g.group + row - i * g.group, quad = (threadIdx.x & 63) >> 4;
+    const bool there = row < rows;
+    hi = there ? sp.len - sp.n + i + 1 : 0;
+    lo = g.window > 0 ? max(0, hi - g.window) : 0;
+    const T* x = there ? (const T*)g.q.p + (long)(sp.start + i) * g.q.token + (long)h * g.q.head : nullptr;
+    float v[DN][16];
+    float m = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DN; d++) {
+        load16<T>(x, 64 * d + 16 * quad, g.c.dim, f.vec, v[d]);
+#pragma unroll
+        for (int e = 0; e < 16; e++) m = fmaxf(m, finite(fabsf(v[d][e])));
+    }
+    int e2 = 0;
+    if (SPLIT) e2 = scale_exponent(max_step<16>(max_step<32>(m)));
+    factor = ldexpf(scale, -e2);
+#pragma unroll
+    for (int d = 0; d < DN; d++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            if constexpr (SPLIT) {
+                float x8[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) x8[k] = ldexpf(v[d][8 * e + k], e2);
+                split_hi_lo(x8, q[d][e], ql[d][e]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; k++) q[d][e][k] = (_Float16)v[d][8 * e + k];
+            }
+        }
+}
+
+// What a lane holds of a row, dims 16 i + 4 (lane / 16) .. +4: the result, or
+// the sum that the other splits' are to be added to.
+template <class T, int DN>
+__device__ __forceinline__ void store_row(const Work& f, const Span& sp, int kv, int row, int rows, int ns, long at,
+                                          float top, float sum, int ev, const float4v (&o)[4 * DN]) {
+    if (row >= rows) return;
+    const AttnArgs& g = f.a;
+    const int i = row / g.group, h = kv * g.group + row - i * g.group, quad = (threadIdx.x & 63) >> 4;
+    const long t = sp.start + i;
+    const float by = ldexpf(ns > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum, ev - 14);
+    if (ns > 1 && quad == 0) f.stat[at] = make_float2(top, sum);
+    T* out = (T*)g.out.p + t * g.out.token + (long)h * g.out.head;
+#pragma unroll
+    for (int k = 0; k < 4 * DN; k++) {
+        const float4v x = o[k] * by;
+        const int d = 16 * k + 4 * quad;
+        if (ns > 1)
+            *reinterpret_cast<float4v*>(f.part + at * g.c.dp + d) = x;
+        else
+            store4<T>(out, d, g.c.dim, f.vec, {x[0], x[1], x[2], x[3]});
+    }
 }
 
 // One workgroup: a request, a key/value head and a range of its tokens; up to
@@ -135,7 +215,7 @@ __device__ __forceinline__ int splits_of(const FewArgs& f, const Span& s) {
 // (the largest so far, 2^(e - 14)): fp16 then holds 39 bits below the largest.
 // fp32 rows: queries and weights in two fp16 parts (22 bits).
 template <class T, int DN, int CT>
-__global__ __launch_bounds__(256, 2) void attn_few_kernel(FewArgs f) {
+__global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int ROW = 64 * DN + 4;  // floats of a row in LDS: 16 rows' pieces of 4 in different banks
     __shared__ float sums[2][16 * CT][ROW];
@@ -146,7 +226,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(FewArgs f) {
     int b = blockIdx.x;
     const int kv = b % c.heads;
     b /= c.heads;
-    const int split = b % f.splits, r = b / f.splits;
+    const int split = b % f.few.splits, r = b / f.few.splits;
     if (r == g.requests) {  // rows of no request
         if (split || blockIdx.y) return;
         const int from = g.requests ? max(0, g.q_start[g.requests]) : 0;
@@ -159,10 +239,10 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(FewArgs f) {
     }
     const Span sp = span_of(g, r);
     const int rows = sp.n * g.group;
-    if (sp.n <= 0 || rows > f.few) return;
-    const int ns = splits_of(f, sp);
+    if (sp.n <= 0 || rows > f.most) return;
+    const int ns = rows <= f.room ? splits_of(f.few, sp.tile1 - sp.tile0) : 1;
     if (split >= ns) return;
-    const int first = sp.tile0 + split * f.tiles, last = split == ns - 1 ? sp.tile1 : first + f.tiles;
+    const int first = sp.tile0 + split * f.few.tiles, last = split == ns - 1 ? sp.tile1 : first + f.few.tiles;
     const float scale = (g.scale ? *g.scale : 1.0f / sqrtf((float)c.dim)) * kLog2e;
     const int* table = g.table + (long)r * g.width;
     const int krow = (col >> 2) * 16 + (col & 3);  // this lane's token of a key tile, less 4 j
@@ -173,42 +253,12 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(FewArgs f) {
     };
 
     for (int cg = blockIdx.y; cg * 16 * CT < rows; cg += gridDim.y) {
-        half8v q[CT][DN][2], ql[SPLIT ? CT : 1][DN][2];
+        half8v q[CT][DN][2], ql[CT][DN][2];
         float factor[CT];
         int lo[CT], hi[CT];
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++) {
-            const int row = (cg * CT + ct) * 16 + col, i = row / g.group, h = kv * g.group + row - i * g.group;
-            const bool there = row < rows;
-            hi[ct] = there ? sp.len - sp.n + i + 1 : 0;
-            lo[ct] = g.window > 0 ? max(0, hi[ct] - g.window) : 0;
-            const T* x = there ? (const T*)g.q.p + (long)(sp.start + i) * g.q.token + (long)h * g.q.head : nullptr;
-            float v[DN][16];
-            float m = 0.0f;
-#pragma unroll
-            for (int d = 0; d < DN; d++) {
-                load16<T>(x, 64 * d + 16 * quad, c.dim, f.vec, v[d]);
-#pragma unroll
-                for (int e = 0; e < 16; e++) m = fmaxf(m, finite(fabsf(v[d][e])));
-            }
-            int e2 = 0;
-            if (SPLIT) e2 = scale_exponent(max_step<16>(max_step<32>(m)));
-            factor[ct] = ldexpf(scale, -e2);
-#pragma unroll
-            for (int d = 0; d < DN; d++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    float x8[8];
-#pragma unroll
-                    for (int k = 0; k < 8; k++) x8[k] = SPLIT ? ldexpf(v[d][8 * e + k], e2) : v[d][8 * e + k];
-                    if constexpr (SPLIT) {
-                        split_hi_lo(x8, q[ct][d][e], ql[ct][d][e]);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 8; k++) q[ct][d][e][k] = (_Float16)x8[k];
-                    }
-                }
-        }
+        for (int ct = 0; ct < CT; ct++)
+            load_query<T, DN>(f, sp, kv, (cg * CT + ct) * 16 + col, rows, scale, q[ct], ql[ct], factor[ct], lo[ct], hi[ct]);
         // every row of these columns sees tokens all_lo .. all_hi - 1
         const int row0 = cg * 16 * CT, row1 = min(rows, row0 + 16 * CT) - 1;
         const int all_hi = sp.len - sp.n + row0 / g.group + 1;
@@ -370,24 +420,239 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(FewArgs f) {
         }
         if (wave == 0) {
 #pragma unroll
-            for (int ct = 0; ct < CT; ct++) {
-                const int row = (cg * CT + ct) * 16 + col, i = row / g.group, h = kv * g.group + row - i * g.group;
-                if (row >= rows) continue;
-                const long t = sp.start + i;
-                const float out = ldexpf(ns > 1 ? 1.0f : sum[ct] == 0.0f ? 0.0f : 1.0f / sum[ct], e - 14);
-                const long at = ((long)split * g.tokens + t) * g.q.heads + h;
-                if (ns > 1 && quad == 0) f.stat[at] = make_float2(top[ct], sum[ct]);
+            for (int ct = 0; ct < CT; ct++)
+            {
+                const int row = (cg * CT + ct) * 16 + col;
+                store_row<T, DN>(f, sp, kv, row, rows, ns, f.few_at(split, r, kv, row), top[ct], sum[ct], e, o[ct]);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------ prompts: tiled
+
+// Columns of 16 rows that a wave of the tiled kernel holds.
+template <int DN>
+constexpr int kCols = DN <= 2 ? 2 : 1;
+template <int DN>
+constexpr int kRows = 64 * kCols<DN>;  // rows of a workgroup
+
+// The workgroup's rows that `row` is among: the tiles that they see.
+struct RowTiles {
+    int row0, tile0, tile1;
+};
+template <int DN>
+__device__ __forceinline__ RowTiles tiles_of(const AttnArgs& g, const Span& sp, int row) {
+    RowTiles w;
+    w.row0 = row / kRows<DN> * kRows<DN>;
+    const int last = min(w.row0 + kRows<DN>, sp.n * g.group) - 1;
+    const int lo = g.window > 0 ? max(0, sp.len - sp.n + w.row0 / g.group + 1 - g.window) : 0;
+    w.tile0 = lo >> 6;
+    w.tile1 = max((max(0, sp.len - sp.n + last / g.group + 1) + 63) >> 6, w.tile0);
+    return w;
+}
+
+// As the few kernel, with the roles of its operands and its numbers, but the
+// rows of a prompt read a tile many times: four waves of 16 CT rows each share
+// tiles of 64 tokens that they bring to LDS as fp16, decoded once for the
+// workgroup's 64 CT rows, each fragment in the order of the lanes that read it
+// (16 bytes a lane side by side, no bank conflicts).  The next tile's codes are
+// on their way to registers while a tile is worked on, and go to the other
+// buffer after it: one barrier a tile.
+template <class T, int DN>
+__global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
+    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr int CT = kCols<DN>, FRAGS = 16 * DN;  // fragments of 64 lanes x 16 bytes in a buffer: keys', then values'
+    extern __shared__ __align__(16) half8v tiles[];  // [2][FRAGS][64]
+    const AttnArgs& g = f.a;
+    const Kv8& c = g.c;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
+    int b = blockIdx.x;
+    const int kv = b % c.heads;
+    b /= c.heads;
+    const int split = b % f.many.splits, at = b / f.many.splits, r = blockIdx.y;
+    const Span sp = span_of(g, r);
+    const int rows = sp.n * g.group;
+    if (sp.n <= 0 || rows <= f.most) return;
+    const float scale = (g.scale ? *g.scale : 1.0f / sqrtf((float)c.dim)) * kLog2e;
+    const int* table = g.table + (long)r * g.width;
+    const int krow = (col >> 2) * 16 + (col & 3);
+    auto page_at = [&](int token) {
+        const int p = token < sp.len ? table[token >> c.shift] : -1;
+        return c.holds(p) ? p : -1;
+    };
+
+    // the later a row, the more tokens it sees: those first
+    const int all = (rows + kRows<DN> - 1) / kRows<DN>;
+    for (int qt = all - 1 - at; qt >= 0; qt -= f.qtiles) {
+        const RowTiles w = tiles_of<DN>(g, sp, qt * kRows<DN>);
+        const int ns = splits_of(f.many, w.tile1 - w.tile0);
+        if (split >= ns) continue;
+        const int first = w.tile0 + split * f.many.tiles, last = split == ns - 1 ? w.tile1 : first + f.many.tiles;
+
+        half8v q[CT][DN][2], ql[CT][DN][2];
+        float factor[CT];
+        int lo[CT], hi[CT];
+        const int row0 = w.row0 + wave * 16 * CT, row1 = min(rows, row0 + 16 * CT) - 1;
 #pragma unroll
-                for (int k = 0; k < 4 * DN; k++) {
-                    const float4v x = o[ct][k] * out;
-                    const int d = 16 * k + 4 * quad;
-                    if (ns > 1)
-                        *reinterpret_cast<float4v*>(f.part + at * c.dp + d) = x;
-                    else
-                        store4<T>((T*)g.out.p + t * g.out.token + (long)h * g.out.head, d, c.dim, f.vec,
-                                  {x[0], x[1], x[2], x[3]});
+        for (int ct = 0; ct < CT; ct++)
+            load_query<T, DN>(f, sp, kv, row0 + 16 * ct + col, rows, scale, q[ct], ql[ct], factor[ct], lo[ct], hi[ct]);
+        const int all_hi = sp.len - sp.n + row0 / g.group + 1;
+        const int all_lo = g.window > 0 ? max(0, sp.len - sp.n + row1 / g.group + 1 - g.window) : 0;
+
+        float4v o[CT][4 * DN];
+        float m[CT], l[CT];
+        int ev = -127;
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            m[ct] = kNone;
+            l[ct] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4 * DN; i++) o[ct][i] = (float4v){0, 0, 0, 0};
+        }
+
+        // this wave's share of a tile: key tile j = wave (DN loads), values' dims 16 (DN wave + i) (DN loads)
+        u32x4 kw[DN], vw[DN];
+        float ks, vs;
+        bool seen;
+        auto fetch = [&](int tile, int pk, int pv) {
+            const int t0 = tile * 64;
+            const int p = max(pv, 0);
+            const int8_t* kp = c.k + c.at(max(pk, 0), kv) + (long)((t0 + krow + 4 * wave) & (c.page - 1)) * c.dp + 16 * quad;
+            const int8_t* vp = c.v + c.at(p, kv) + (long)(16 * DN * wave + col) * c.page + ((t0 + 16 * quad) & (c.page - 1));
+#pragma unroll
+            for (int d = 0; d < DN; d++) {
+                kw[d] = *reinterpret_cast<const u32x4*>(kp + 64 * d);
+                vw[d] = *reinterpret_cast<const u32x4*>(vp + (long)16 * d * c.page);
+            }
+            ks = c.k_scale[(long)p * c.heads + kv];
+            vs = c.v_scale[(long)p * c.heads + kv];
+            seen = pv >= 0;
+        };
+        auto put = [&](int buffer) {
+            half8v* to = tiles + buffer * FRAGS * 64 + lane;
+#pragma unroll
+            for (int d = 0; d < DN; d++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    to[((wave * DN + d) * 2 + h) * 64] = codes8(kw[d][2 * h], kw[d][2 * h + 1]);
+                    to[(8 * DN + (wave * DN + d) * 2 + h) * 64] = codes8(vw[d][2 * h], vw[d][2 * h + 1]);
+                }
+        };
+        int pk = page_at(first * 64 + (col >> 2) * 16), pv = page_at(first * 64 + quad * 16);
+        __syncthreads();  // nobody reads the buffers of the rows before any more
+        if (first < last) {
+            fetch(first, pk, pv);
+            pk = page_at(first * 64 + 64 + (col >> 2) * 16);
+            pv = page_at(first * 64 + 64 + quad * 16);
+            put(0);
+        }
+        __syncthreads();
+        for (int tile = first, buffer = 0; tile < last; tile++, buffer ^= 1) {
+            const int t0 = tile * 64;
+            const float fs = ks, fvs = vs;
+            const bool there = seen;
+            const bool whole = t0 + 64 <= all_hi && t0 >= all_lo && __all(there);
+            if (tile + 1 < last) {
+                fetch(tile + 1, pk, pv);
+                pk = page_at(t0 + 128 + (col >> 2) * 16);
+                pv = page_at(t0 + 128 + quad * 16);
+            }
+            const half8v* from = tiles + buffer * FRAGS * 64 + lane;
+
+            int e = max(ev, exponent_of(fvs));
+            e = max(e, __shfl_xor(e, 16));
+            e = max(e, __shfl_xor(e, 32));
+            const float fv = ldexpf(fvs, 14 - e);
+
+            float4v s[CT][4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) s[ct][j] = (float4v){0, 0, 0, 0};
+#pragma unroll
+                for (int d = 0; d < DN; d++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const half8v k8 = from[((j * DN + d) * 2 + h) * 64];
+#pragma unroll
+                        for (int ct = 0; ct < CT; ct++) {
+                            s[ct][j] = mfma(k8, q[ct][d][h], s[ct][j]);
+                            if constexpr (SPLIT) s[ct][j] = mfma(k8, ql[ct][d][h], s[ct][j]);
+                        }
+                    }
+            }
+            half8v p[CT][2], pl[CT][2];
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                const float fk = factor[ct] * fs;
+                float x[16], top = kNone;
+#pragma unroll
+                for (int k = 0; k < 16; k++) x[k] = s[ct][k >> 2][k & 3] * fk;
+                if (!whole) {
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        const int t = t0 + 16 * quad + k;
+                        if (!(there && t >= lo[ct] && t < hi[ct])) x[k] = kNone;
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 16; k++) top = fmaxf(top, x[k]);
+                top = fmaxf(m[ct], max_step<16>(max_step<32>(top)));
+                const float base = top == kNone ? 0.0f : top;
+                const float old = __builtin_amdgcn_exp2f(m[ct] - base), keep = ldexpf(old, ev - e);
+                float sum = 0.0f;
+                float y[2][8];
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    const float z = __builtin_amdgcn_exp2f(x[k] - base);
+                    sum += z;
+                    y[k >> 3][k & 7] = z * fv;
+                }
+                if (!whole) {  // (a page that a row does not see may have any scale)
+#pragma unroll
+                    for (int k = 0; k < 16; k++)
+                        if (x[k] == kNone) y[k >> 3][k & 7] = 0.0f;
+                }
+                l[ct] = l[ct] * old + sum;
+                m[ct] = top;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if constexpr (SPLIT) {
+                        split_hi_lo(y[h], p[ct][h], pl[ct][h]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; k++) p[ct][h][k] = (_Float16)y[h][k];
+                    }
+                }
+                if (__any(keep != 1.0f)) {
+#pragma unroll
+                    for (int i = 0; i < 4 * DN; i++) o[ct][i] *= keep;
                 }
             }
+            ev = e;
+#pragma unroll
+            for (int i = 0; i < 4 * DN; i++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const half8v v8 = from[(8 * DN + 2 * i + h) * 64];
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) {
+                        o[ct][i] = mfma(v8, p[ct][h], o[ct][i]);
+                        if constexpr (SPLIT) o[ct][i] = mfma(v8, pl[ct][h], o[ct][i]);
+                    }
+                }
+            if (tile + 1 < last) put(buffer ^ 1);
+            __syncthreads();
+        }
+
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            l[ct] += __shfl_xor(l[ct], 16);
+            l[ct] += __shfl_xor(l[ct], 32);
+            const int row = row0 + 16 * ct + col, i = row / g.group;
+            store_row<T, DN>(f, sp, kv, row, rows, ns, f.many_at(split, sp.start + i, kv * g.group + row - i * g.group), m[ct],
+                             l[ct], ev, o[ct]);
         }
     }
 }
@@ -395,7 +660,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(FewArgs f) {
 // Joins the splits' sums in their order: a workgroup a row and q head, 16 lanes
 // x 4 dims x DN of its threads a split, 16 / DN splits at a time.
 template <class T, int DN>
-__global__ __launch_bounds__(256) void attn_join_kernel(FewArgs f) {
+__global__ __launch_bounds__(256) void attn_join_kernel(Work f) {
     constexpr int G = 16 / DN;  // groups of 16 DN lanes
     __shared__ float4 part[G][16 * DN];
     const AttnArgs& g = f.a;
@@ -404,10 +669,20 @@ __global__ __launch_bounds__(256) void attn_join_kernel(FewArgs f) {
     const int r = find_request(g, t, lo, hi);
     if (g.requests == 0 || t < g.q_start[0] || t >= g.q_start[g.requests]) return;
     const Span sp = span_of(g, r);
-    if (sp.n * g.group > f.few) return;
-    const int ns = splits_of(f, sp);
+    const int rows = sp.n * g.group, kv = h / g.group, row = (t - sp.start) * g.group + h % g.group;
+    int ns;
+    long at, step;
+    if (rows <= f.most) {
+        ns = rows <= f.room ? splits_of(f.few, sp.tile1 - sp.tile0) : 1;
+        at = f.few_at(0, r, kv, row);
+        step = f.few_at(1, r, kv, row) - at;
+    } else {
+        const RowTiles w = tiles_of<DN>(g, sp, row);
+        ns = splits_of(f.many, w.tile1 - w.tile0);
+        at = f.many_at(0, t, h);
+        step = f.many_at(1, t, h) - at;
+    }
     if (ns == 1) return;
-    const long step = (long)g.tokens * g.q.heads, at = (long)t * g.q.heads + h;
     float top = kNone;
     for (int s = threadIdx.x & 63; s < ns; s += 64) top = fmaxf(top, f.stat[s * step + at].x);
     top = max_step<1>(max_step<2>(max_step<4>(max_step<8>(max_step<16>(max_step<32>(top))))));
@@ -448,71 +723,6 @@ __global__ __launch_bounds__(256) void attn_join_kernel(FewArgs f) {
               {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv});
 }
 
-// One wave for a row and a q head; a lane for each of 64 tokens in the first
-// product, for every 64th dim in the second.
-template <class T>
-__global__ __launch_bounds__(256) void attn_simple_kernel(AttnArgs g, int few) {
-    __shared__ float qs[4][256];
-    __shared__ float ps[4][64];
-    __shared__ int pages[4][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int hb = (g.q.heads + 3) / 4;
-    const int t = blockIdx.x / hb, h = (blockIdx.x - t * hb) * 4 + wave;
-    if (h >= g.q.heads) return;
-    const Kv8& c = g.c;
-    const int kv = h / g.group;
-    int lo, hi;
-    const int r = find_request(g, t, lo, hi);
-    if (g.requests == 0 || t < g.q_start[0] || t >= g.q_start[g.requests] || span_of(g, r).n * g.group <= few) return;
-    const float scale = (g.scale ? *g.scale : 1.0f / sqrtf((float)c.dim)) * kLog2e;
-    const T* q = (const T*)g.q.p + (long)t * g.q.token + (long)h * g.q.head;
-    for (int d = lane; d < c.dp; d += 64) qs[wave][d] = d < c.dim ? (float)q[d] : 0.0f;
-    float m = -__builtin_inff(), l = 0.0f, o[4] = {0, 0, 0, 0};
-    const int nd = c.dp / 64;
-    for (int k0 = lo & ~63; k0 < hi; k0 += 64) {
-        const int k = k0 + lane;
-        const int j = k >> c.shift;
-        int page = -1;
-        if (k >= lo && k < hi) page = g.table[(long)r * g.width + j];
-        if (!c.holds(page)) page = -1;
-        float s = -__builtin_inff();
-        if (page >= 0) {
-            const u32x4* row = reinterpret_cast<const u32x4*>(c.k + c.at(page, kv) + (long)(k & (c.page - 1)) * c.dp);
-            float acc = 0.0f;
-            for (int i = 0; i < c.dp / 16; i++) {
-                const u32x4 w = row[i];
-#pragma unroll
-                for (int e = 0; e < 16; e++) acc += qs[wave][16 * i + e] * (float)(int8_t)(w[e / 4] >> 8 * (e % 4));
-            }
-            s = acc * (c.k_scale[(long)page * c.heads + kv] * scale);
-        }
-        const float top = fmaxf(m, max_step<1>(max_step<2>(max_step<4>(max_step<8>(max_step<16>(max_step<32>(s)))))));
-        const float base = top == -__builtin_inff() ? 0.0f : top;
-        const float p = page >= 0 ? exp2f(s - base) : 0.0f, old = exp2f(m - base);
-        float sum = p;
-        for (int x = 32; x >= 1; x >>= 1) sum += __shfl_xor(sum, x);
-        l = l * old + sum;
-        m = top;
-        ps[wave][lane] = page >= 0 ? p * c.v_scale[(long)page * c.heads + kv] : 0.0f;
-        pages[wave][lane] = page;
-        for (int n = 0; n < nd; n++) o[n] *= old;
-        for (int i = 0; i < 64; i += 16) {
-            int any = -1;  // 16 tokens lie on one page
-            for (int e = 0; e < 16; e++) any = max(any, pages[wave][i + e]);
-            if (any < 0) continue;
-            for (int n = 0; n < nd; n++) {
-                const u32x4 w = *reinterpret_cast<const u32x4*>(c.v + c.at(any, kv) + (long)(n * 64 + lane) * c.page +
-                                                                ((k0 + i) & (c.page - 1)));
-#pragma unroll
-                for (int e = 0; e < 16; e++) o[n] += ps[wave][i + e] * (float)(int8_t)(w[e / 4] >> 8 * (e % 4));
-            }
-        }
-    }
-    T* out = (T*)g.out.p + (long)t * g.out.token + (long)h * g.out.head;
-    for (int n = 0; n < nd; n++)
-        if (n * 64 + lane < c.dim) out[n * 64 + lane] = (T)(l == 0.0f ? 0.0f : o[n] / l);
-}
-
 }  // namespace zt
 
 using namespace zt;
@@ -524,48 +734,73 @@ static bool attn_ok(const zt_kv8_attn* a) {
            (long)a->tokens * a->q.heads < (1l << 31) && (long)a->requests * a->width < (1l << 31);
 }
 
-// How a call is split: for the rows that a launch covers, splits along the
-// tokens until about 4 workgroups a CU are there, none of less than 4 tiles (one
-// a wave).
+// How a call is launched.
 struct AttnPlan {
-    int ct, groups;     // column tiles a wave, workgroups along the rows
-    int splits, tiles;
-    int few;            // most rows of a request that the split kernel takes; others: the tiled one
-    long part, stat;    // bytes of the splits' sums
+    int ct, groups;  // the few kernel: column tiles a wave, workgroups along the rows
+    Split few, many;
+    int most, qtiles, room;
+    long others;
+    long part, stat;  // bytes of the splits' sums
 };
+
+// Along the tokens until about `want` workgroups are there, none of less than
+// 4 tiles.
+static Split split_of(long tiles, long have, long want) {
+    const long splits = std::max(1l, std::min((want + have - 1) / have, tiles / 4));
+    Split s;
+    s.tiles = (int)((tiles + splits - 1) / splits);
+    s.splits = (int)((tiles + s.tiles - 1) / s.tiles);
+    return s;
+}
 
 static AttnPlan attn_plan(const zt_kv8_attn* a) {
     AttnPlan p{};
     const int group = a->q.heads / a->cache.kv_heads, dp = (a->cache.head_dim + 63) & ~63;
+    const long requests = std::max(1, a->requests), heads = a->cache.kv_heads;
     const long most = (long)std::min(a->max_q, a->tokens) * group;
-    p.few = most <= 64 ? 0x7FFFFFFF : 64;
+    p.most = most <= 64 ? 0x7FFFFFFF : 64;
     const int rows = (int)std::max(1l, std::min(most, 64l));
     p.ct = rows > 16 && dp <= 128 ? 2 : 1;
     p.groups = ceil_div(rows, 16 * p.ct);
     long kv = std::min((long)a->max_kv, (long)a->width * a->cache.page_tokens);
     if (a->window > 0) kv = std::min(kv, (long)a->window + a->max_q + 63);
     const long tiles = std::max(1l, (kv + 63) / 64);
-    const long have = (long)std::max(1, a->requests) * a->cache.kv_heads * p.groups;
-    const long splits = std::max(1l, std::min((1024 + have - 1) / have, tiles / 4));
-    p.tiles = (int)((tiles + splits - 1) / splits);
-    p.splits = (int)((tiles + p.tiles - 1) / p.tiles);
-    if (p.splits > 1) {
-        const long rows_all = (long)p.splits * a->tokens * a->q.heads;
-        p.stat = (rows_all * 8 + 15) & ~15l;
-        p.part = rows_all * dp * 4;
+    p.few = split_of(tiles, requests * heads * p.groups, 1024);
+    p.many = {1, 1};
+    if (most > 64) {
+        p.qtiles = ceil_div(most, dp <= 128 ? 128 : 64);
+        p.many = split_of(tiles, requests * heads * p.qtiles, 512);
     }
+    p.room = p.groups * 16 * p.ct;
+    if (p.few.splits > 1) p.others = (long)p.few.splits * a->requests * heads * p.room;
+    const long all = p.others + (p.many.splits > 1 ? (long)p.many.splits * a->tokens * a->q.heads : 0);
+    p.stat = (all * 8 + 15) & ~15l;
+    p.part = all * dp * 4;
     return p;
 }
 
 template <class T, int DN>
-static void launch_few(const FewArgs& f, const AttnPlan& p, long blocks, hipStream_t stream) {
-    const dim3 grid((unsigned)blocks, p.groups);
+static int launch(const Work& f, const AttnPlan& p, hipStream_t stream) {
+    const long few = ((long)f.a.requests + 1) * p.few.splits * f.a.c.heads;
+    const long many = (long)p.qtiles * p.many.splits * f.a.c.heads;
+    if (few >= 1l << 31 || many >= 1l << 31 || (p.qtiles && f.a.requests > 65535)) return kInvalid;
+    if (p.qtiles && f.a.requests) {
+        static std::atomic<uint64_t> raised{0};
+        constexpr int lds = 2 * 16 * DN * 1024;
+        if constexpr (lds > 65536) {
+            const hipError_t rc = raise_lds((const void*)attn_many_kernel<T, DN>, lds, raised);
+            if (rc != hipSuccess) return (int)rc;
+        }
+        attn_many_kernel<T, DN><<<dim3((unsigned)many, f.a.requests), 256, lds, stream>>>(f);
+    }
+    const dim3 grid((unsigned)few, p.groups);
     if (p.ct == 2) {
         if constexpr (DN <= 2) attn_few_kernel<T, DN, 2><<<grid, 256, 0, stream>>>(f);
     } else {
         attn_few_kernel<T, DN, 1><<<grid, 256, 0, stream>>>(f);
     }
-    if (p.splits > 1) attn_join_kernel<T, DN><<<(unsigned)(f.a.tokens * f.a.q.heads), 256, 0, stream>>>(f);
+    if (p.part) attn_join_kernel<T, DN><<<(unsigned)(f.a.tokens * f.a.q.heads), 256, 0, stream>>>(f);
+    return (int)hipGetLastError();
 }
 
 ZT_EXPORT long zt_kv8_attention_workspace_bytes(const zt_kv8_attn* a) {
@@ -585,23 +820,13 @@ ZT_EXPORT int zt_kv8_attention(const zt_kv8_attn* a, void* workspace, long works
     if (p.part + p.stat > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.part + p.stat)) return kInvalid;
     const AttnArgs g{kv8_of(a->cache), rows_of(a->q), rows_of(a->out), a->table, a->kv_lens, a->q_start, a->scale,
                      a->requests,      a->width,      a->tokens,       a->window, a->q.heads / a->cache.kv_heads};
-    const FewArgs f{g, p.splits, p.tiles, p.few, rows_vector(a->q, 4, a->type) && rows_vector(a->out, 4, a->type),
-                    (float*)workspace, (float2*)((char*)workspace + p.part)};
-    const long blocks = ((long)a->requests + 1) * p.splits * a->cache.kv_heads;
-    if (blocks >= 1l << 31) return kInvalid;
+    const Work f{g,        p.few, p.many, p.most, p.qtiles, rows_vector(a->q, 4, a->type) && rows_vector(a->out, 4, a->type),
+                 p.room,   p.others, (float*)workspace, (float2*)((char*)workspace + p.part)};
     const bool f32 = a->type == ZT_F32;
     switch (g.c.dp) {
-        case 64: f32 ? launch_few<float, 1>(f, p, blocks, stream) : launch_few<_Float16, 1>(f, p, blocks, stream); break;
-        case 128: f32 ? launch_few<float, 2>(f, p, blocks, stream) : launch_few<_Float16, 2>(f, p, blocks, stream); break;
-        case 192: f32 ? launch_few<float, 3>(f, p, blocks, stream) : launch_few<_Float16, 3>(f, p, blocks, stream); break;
-        default: f32 ? launch_few<float, 4>(f, p, blocks, stream) : launch_few<_Float16, 4>(f, p, blocks, stream); break;
+        case 64: return f32 ? launch<float, 1>(f, p, stream) : launch<_Float16, 1>(f, p, stream);
+        case 128: return f32 ? launch<float, 2>(f, p, stream) : launch<_Float16, 2>(f, p, stream);
+        case 192: return f32 ? launch<float, 3>(f, p, stream) : launch<_Float16, 3>(f, p, stream);
+        default: return f32 ? launch<float, 4>(f, p, stream) : launch<_Float16, 4>(f, p, stream);
     }
-    if (p.few == 64) {
-        const long many = (long)a->tokens * ((a->q.heads + 3) / 4);
-        if (f32)
-            attn_simple_kernel<float><<<many, 256, 0, stream>>>(g, p.few);
-        else
-            attn_simple_kernel<_Float16><<<many, 256, 0, stream>>>(g, p.few);
-    }
-    return (int)hipGetLastError();
 }
