@@ -410,6 +410,7 @@ def test_sample_gives_every_token_its_share(eng, vocab, dtype):
     every_token(eng, z, dtype)
     every_token(eng, z, dtype, temperature=0.6, top_k=7)
     every_token(eng, z, dtype, temperature=1.7, min_p=0.03)
+    every_token(eng, z, dtype, top_k=vocab * 2 // 3)
     # a threshold in the middle between two sums: no rounding moves it over one
     zd = cuda(z.astype(np.float32)).to(DT[dtype]).double().cpu().numpy()
     for k, n in ((0, 1), (0, vocab // 2), (40, 12), (40, 30)):
@@ -417,6 +418,10 @@ def test_sample_gives_every_token_its_share(eng, vocab, dtype):
         if 0 < n < len(order):
             mass = np.cumsum(w[order])
             every_token(eng, z, dtype, 0.9, k, float((mass[n - 1] - w[order[n - 1]] / 2) / mass[-1]), 1e-6)
+    order, w = ref.kept(zd, 1.1, vocab * 3 // 4, 1.0, 1e-3)
+    mass = np.cumsum(w[order])
+    for n in {1, len(order) // 3 + 1, len(order)}:
+        every_token(eng, z, dtype, 1.1, vocab * 3 // 4, float((mass[n - 1] - w[order[n - 1]] / 2) / mass[-1]), 1e-3)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
