@@ -61,23 +61,36 @@ struct Scan {
     uint64_t part[kSampleThreads / 64];
 };
 
+// x + (x of the lane that a DPP move takes it from; 0 where none)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t add_moved(uint64_t x) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xF, true);
+    return x + ((uint64_t)hi << 32 | lo);
+}
+
 // Running sums in the order of the threads: v becomes the sum before the
-// thread's own, the result is the sum of all.
+// thread's own, the result is the sum of all.  In a wave by moves of 1, 2, 4 and
+// 8 lanes in rows of 16, then each row's last to the rows after it; across the
+// 16 waves every thread adds up the waves' sums.
 __device__ __forceinline__ uint64_t block_scan(uint64_t& v, Scan& s) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint64_t x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
+    x = add_moved<0x111, 0xF>(x);
+    x = add_moved<0x112, 0xF>(x);
+    x = add_moved<0x114, 0xF>(x);
+    x = add_moved<0x118, 0xF>(x);
+    x = add_moved<0x142, 0xA>(x);  // lanes 15 and 47 to the next row
+    x = add_moved<0x143, 0xC>(x);  // lane 31 to the upper two
     __syncthreads();
     if (lane == 63) s.part[wave] = x;
     __syncthreads();
     uint64_t before = 0, all = 0;
-    for (int i = 0; i < (int)blockDim.x / 64; i++) {
-        if (i < wave) before += s.part[i];
-        all += s.part[i];
+#pragma unroll
+    for (int i = 0; i < kSampleThreads / 64; i++) {
+        const uint64_t p = s.part[i];
+        before += i < wave ? p : 0;
+        all += p;
     }
     v = before + x - v;
     return all;
@@ -480,8 +493,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs 
         if (at + i < kListed) w.list[at + i] = list[i];
 }
 
-// Falling order of n <= kListed values, n2 the power of two above (the rest of
-// them 0), by compare and exchange over strides that halve.
+// Falling order of n2 values, a power of two, by compare and exchange over
+// strides that halve.
 __device__ __forceinline__ void sort_falling(unsigned long long* v, int n2) {
     for (int size = 2; size <= n2; size <<= 1)
         for (int stride = size >> 1; stride >= 1; stride >>= 1) {
@@ -539,7 +552,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(SampleArgs 
     const uint64_t above = block_scan(before, scan);
     uint64_t total = above;
     if (listed) {
-        int n2 = 2;
+        int n2 = 16;
         while (n2 < listed) n2 *= 2;
 #pragma unroll
         for (int e = 0; e < kTurns; e++) {
@@ -547,7 +560,19 @@ __global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(SampleArgs 
             if (i < n2) u.order[i] = i < listed ? mine[e] : 0;
         }
         __syncthreads();
-        sort_falling(u.order, n2);
+        if (n2 <= 256) {
+            // few: each counts those before it, four threads or more for one (128: 1 us less than by exchanges)
+            const int each = min(64, kSampleThreads / n2), i = tid / each;
+            const unsigned long long o = i < listed ? u.order[i] : 0;
+            int rank = 0;
+            for (int j = tid & (each - 1); j < n2; j += each) rank += u.order[j] > o;
+            for (int x = 1; x < each; x <<= 1) rank += __shfl_xor(rank, x);
+            __syncthreads();
+            if (i < listed && (tid & (each - 1)) == 0) u.order[rank] = o;
+            __syncthreads();
+        } else {
+            sort_falling(u.order, n2);
+        }
         // this thread's tokens, neighbours in that order: their weights, and which cut they are listed for
         uint64_t f[kTurns];
         bool ranked[kTurns], weighed[kTurns], likely[kTurns];
