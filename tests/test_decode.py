@@ -28,6 +28,18 @@ BAD_CACHES = [dict(k=0), dict(v=P + 8), dict(k_scale=0), dict(v_scale=0), dict(p
               dict(pages=1 << 28)]
 
 
+def test_packed_structures_are_the_c_ones():
+    from ztensor_amd import decode
+
+    for packed, c in ((decode._ROWS, _lib.Rows), (decode._ROWS2, _lib.Rows * 2), (decode._CACHE, _lib.KV8),
+                      (decode._ATTN, _lib.KV8Attn)):
+        assert packed.size == ctypes.sizeof(c)
+    fields = decode._ATTN.pack(*range(1, 31))
+    a = _lib.KV8Attn.from_buffer_copy(fields)
+    assert (a.cache.k, a.cache.page_tokens, a.q.p, a.q.heads, a.out.p, a.out.head_stride, a.table, a.scale, a.requests,
+            a.type, a.reserved) == (1, 8, 9, 12, 14, 16, 19, 22, 23, 29, 30)
+
+
 def test_rope_refuses():
     lib, two = _lib.load(), (_lib.Rows * 2)(rows(), rows())
 

@@ -17,8 +17,8 @@ passed as numbers.
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from typing import NamedTuple
 
 import torch
@@ -118,41 +118,60 @@ def rope_table(rot_dim: int, max_pos: int, base: float = 10000.0, scaling: dict 
     return (torch.stack((angle.cos(), angle.sin()), 1) * mult).float().to(device)
 
 
+# The C structures (zt_rows, zt_kv8_cache, zt_kv8_attn) as bytes that a call takes for a pointer to them: packing one
+# costs a third of building a ctypes.Structure (0.5 us of a call's 10 instead of 2).
+_ROWS = struct.Struct("@Pqqii")
+_ROWS2 = struct.Struct("@PqqiiPqqii")
+_CACHE = struct.Struct("@PPPPiiii")
+_ATTN = struct.Struct("@PPPPiiiiPqqiiPqqiiPPPPiiiiiiii")
+
+
+def _like(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 class DecodeOps:
     """ROCmEngine's methods for the operators between the linear layers."""
 
-    def _rows(self, x: torch.Tensor, name: str) -> _lib.Rows:
-        if x.dim() != 3 or x.device != self.device or (x.stride(2) != 1 and x.shape[2] > 1):
-            raise ValueError(f"{name} is [tokens, heads, head_dim] on the engine's device, values of a head neighbours")
+    def _rows(self, x: torch.Tensor, name: str) -> tuple:
+        """zt_rows' fields of a [tokens, heads, head_dim] tensor."""
         st = x.stride()
-        return _lib.Rows(x.data_ptr(), st[0], st[1], x.shape[1], 0)
+        if len(st) != 3 or x.device != self.device or (st[2] != 1 and x.shape[2] > 1):
+            raise ValueError(f"{name} is [tokens, heads, head_dim] on the engine's device, values of a head neighbours")
+        return x.data_ptr(), st[0], st[1], x.shape[1], 0
 
     def _dense(self, x: torch.Tensor | None, name: str, dtype: torch.dtype, shape: tuple) -> int:
         """The address of a contiguous tensor of that type and shape (None: any size) on the engine's device."""
         if x is None:
             return 0
-        if (x.dtype != dtype or x.device != self.device or x.dim() != len(shape) or not x.is_contiguous()
-                or any(n is not None and n != m for n, m in zip(shape, x.shape))):
-            raise ValueError(f"{name} is a contiguous {dtype} tensor {list(shape)} on the engine's device")
-        return x.data_ptr()
+        if x.dtype is dtype and x.is_contiguous() and x.device == self.device:
+            have = x.shape
+            if have == shape or (len(have) == len(shape) and all(n is None or n == m for n, m in zip(shape, have))):
+                return x.data_ptr()
+        raise ValueError(f"{name} is a contiguous {dtype} tensor {list(shape)} on the engine's device")
 
-    def _type(self, name: str, *xs: torch.Tensor) -> int:
-        t = _TYPES.get(xs[0].dtype)
-        if t is None or any(x.dtype != xs[0].dtype for x in xs):
+    def _type(self, name: str, x: torch.Tensor, *more: torch.Tensor) -> int:
+        dtype = x.dtype
+        t = _TYPES.get(dtype)
+        for y in more:
+            if y.dtype is not dtype:
+                t = None
+        if t is None:
             raise TypeError(f"{name} takes float32 or float16 tensors of one type")
         return t
 
-    def _kv8(self, cache, head_dim: int) -> _lib.KV8:
+    def _kv8(self, cache, head_dim: int) -> tuple:
+        """zt_kv8_cache's fields."""
         k, v, ks, vs = cache
-        if (k.dim() != 4 or v.dim() != 4 or k.dtype != torch.int8 or v.dtype != torch.int8
-                or k.device != self.device or v.device != self.device):
+        shape, i8, dev = k.shape, torch.int8, self.device
+        if len(shape) != 4 or k.dtype is not i8 or v.dtype is not i8 or k.device != dev or v.device != dev:
             raise ValueError("a cache is int8 [pages, kv_heads, page_tokens, Dp] keys and [.., Dp, page_tokens] values")
-        pages, heads, page, dp = k.shape
+        pages, heads, page, dp = shape
         if (v.shape != (pages, heads, dp, page) or not k.is_contiguous() or not v.is_contiguous()
-                or dp != -(-head_dim // 64) * 64):
+                or dp != (head_dim + 63) // 64 * 64):
             raise ValueError(f"cache of {tuple(k.shape)} keys and {tuple(v.shape)} values for heads of {head_dim}")
-        return _lib.KV8(k.data_ptr(), v.data_ptr(), self._dense(ks, "k_scale", torch.float32, (pages, heads)),
-                        self._dense(vs, "v_scale", torch.float32, (pages, heads)), pages, heads, head_dim, page)
+        return (k.data_ptr(), v.data_ptr(), self._dense(ks, "k_scale", torch.float32, (pages, heads)),
+                self._dense(vs, "v_scale", torch.float32, (pages, heads)), pages, heads, head_dim, page)
 
     @_on_engine_stream
     def rope(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table: torch.Tensor, *,
@@ -164,21 +183,28 @@ class DecodeOps:
         Returns (q, k); with k None, (q, None).  table: rope_table's, of all
         of the head or its first part.  inverse: by the negative angle, which
         is how a gradient goes back."""
-        xs = [q] if k is None else [q, k]
-        given = [q_out] if k is None else [q_out, k_out]
-        outs = [torch.empty(x.shape, dtype=x.dtype, device=x.device) if o is None else o for x, o in zip(xs, given)]
-        t = self._type("rope", *xs, *outs)
-        if any(x.shape != o.shape for x, o in zip(xs, outs)) or any(
-                x.shape[0] != q.shape[0] or x.shape[2] != q.shape[2] for x in xs[1:]):
+        if q_out is None:
+            q_out = _like(q)
+        rows = self._rows
+        if k is None:
+            t, n = self._type("rope", q, q_out), 1
+            ins, outs = _ROWS.pack(*rows(q, "q")), _ROWS.pack(*rows(q_out, "q_out"))
+        else:
+            if k_out is None:
+                k_out = _like(k)
+            t, n = self._type("rope", q, k, q_out, k_out), 2
+            ins = _ROWS2.pack(*rows(q, "q"), *rows(k, "k"))
+            outs = _ROWS2.pack(*rows(q_out, "q_out"), *rows(k_out, "k_out"))
+            if k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k_out.shape != k.shape:
+                raise ValueError("rope: q, k and their outputs have the same tokens and head size")
+        if q_out.shape != q.shape:
             raise ValueError("rope: q, k and their outputs have the same tokens and head size")
-        n = len(xs)
-        ins, to = (_lib.Rows * n)(*[self._rows(x, "q and k") for x in xs]), (_lib.Rows * n)(*[self._rows(o, "outputs") for o in outs])
-        tokens, dim = q.shape[0], q.shape[2]
-        self.lib.call("zt_rope", ins, to, n, self._dense(positions, "positions", torch.int32, (tokens,)),
-                      self._dense(table, "table", torch.float32, (None, 2, None)), tokens, dim, 2 * table.shape[2],
-                      table.shape[0], t, (_lib.ROPE_INTERLEAVED if interleaved else 0)
+        tokens, _, dim = q.shape
+        tab = self._dense(table, "table", torch.float32, (None, 2, None))
+        self.lib.call("zt_rope", ins, outs, n, self._dense(positions, "positions", torch.int32, (tokens,)), tab, tokens,
+                      dim, 2 * table.shape[2], table.shape[0], t, (_lib.ROPE_INTERLEAVED if interleaved else 0)
                       | (_lib.ROPE_INVERSE if inverse else 0), self._s)
-        return outs[0], (outs[1] if n == 2 else None)
+        return q_out, k_out if n == 2 else None
 
     @_on_engine_stream
     def kv8_append(self, k: torch.Tensor, v: torch.Tensor, cache, slots: torch.Tensor, *,
@@ -193,28 +219,37 @@ class DecodeOps:
         A page's scale grows where the new values need it, and the codes that
         it holds are rounded to the new scale; a page that starts anew forgets
         what it held.  Tokens whose slot is outside the cache are left out."""
-        t = self._type("kv8_append", k, v, *([] if q is None else [q]))
-        tokens, dim = k.shape[0], k.shape[2]
-        if k.shape != v.shape:
+        rows, pack = self._rows, _ROWS.pack
+        krows, vrows = rows(k, "k"), rows(v, "v")
+        tokens, heads, dim = k.shape
+        if v.shape != k.shape:
             raise ValueError("kv8_append: k and v have one shape")
-        if q is not None and (table is None or q.shape[0] != tokens or q.shape[2] != dim):
-            raise ValueError("kv8_append: q goes with a rope table, and has k's tokens and head size")
-        if table is not None and positions is None:
-            raise ValueError("kv8_append: a rope table needs positions")
-        if q is not None and q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        elif q_out is not None and (q is None or q_out.shape != q.shape or q_out.dtype != q.dtype):
-            raise ValueError("kv8_append: q_out is q's shape and type")
+        qr = qo = None
+        if q is not None:
+            if table is None or q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != dim:
+                raise ValueError("kv8_append: q goes with a rope table, and has k's tokens and head size")
+            if q_out is None:
+                q_out = _like(q)
+            elif q_out.shape != q.shape:
+                raise ValueError("kv8_append: q_out has q's shape")
+            t = self._type("kv8_append", k, v, q, q_out)
+            qr, qo = pack(*rows(q, "q")), pack(*rows(q_out, "q_out"))
+        elif q_out is not None:
+            raise ValueError("kv8_append: q_out goes with q")
+        else:
+            t = self._type("kv8_append", k, v)
         c = self._kv8(cache, dim)
-        if k.shape[1] != c.kv_heads:
-            raise ValueError(f"kv8_append: {k.shape[1]} heads for a cache of {c.kv_heads}")
-        rows, ref = self._rows, ctypes.byref
-        self.lib.call("zt_kv8_append", ref(c), ref(rows(k, "k")), ref(rows(v, "v")),
-                      self._dense(slots, "slots", torch.int64, (tokens,)),
-                      None if q is None else ref(rows(q, "q")), None if q is None else ref(rows(q_out, "q_out")),
-                      0 if table is None else self._dense(positions, "positions", torch.int32, (tokens,)),
-                      self._dense(table, "table", torch.float32, (None, 2, None)), tokens,
-                      0 if table is None else 2 * table.shape[2], 0 if table is None else table.shape[0], t,
+        if heads != c[5]:
+            raise ValueError(f"kv8_append: {heads} heads for a cache of {c[5]}")
+        pos = tab = half = most = 0
+        if table is not None:
+            if positions is None:
+                raise ValueError("kv8_append: a rope table needs positions")
+            pos = self._dense(positions, "positions", torch.int32, (tokens,))
+            tab = self._dense(table, "table", torch.float32, (None, 2, None))
+            most, _, half = table.shape
+        self.lib.call("zt_kv8_append", _CACHE.pack(*c), pack(*krows), pack(*vrows),
+                      self._dense(slots, "slots", torch.int64, (tokens,)), qr, qo, pos, tab, tokens, 2 * half, most, t,
                       _lib.ROPE_INTERLEAVED if interleaved else 0, self._s)
         return q_out
 
@@ -224,9 +259,8 @@ class DecodeOps:
         [n, kv_heads, page_tokens, head_dim], code * scale."""
         c, n = self._kv8(cache, head_dim), pages.numel()
         p = self._dense(pages, "pages", torch.int32, (n,))
-        keys, values = torch.empty((2, n, c.kv_heads, c.page_tokens, head_dim), dtype=torch.float32,
-                                   device=self.device).unbind()
-        self.lib.call("zt_kv8_dequant", ctypes.byref(c), p, n, keys.data_ptr(), values.data_ptr(), self._s)
+        keys, values = torch.empty((2, n, c[5], c[7], head_dim), dtype=torch.float32, device=self.device).unbind()
+        self.lib.call("zt_kv8_dequant", _CACHE.pack(*c), p, n, keys.data_ptr(), values.data_ptr(), self._s)
         return keys, values
 
     @_on_engine_stream
@@ -239,19 +273,19 @@ class DecodeOps:
         few, or whose row of block_table (int32 [requests, width]) is full,
         gets none: its slots are -1 and its length stays.  in_place: the new
         pages are written into block_table itself, not a copy."""
-        r = kv_lens.numel()
-        width = block_table.shape[-1]
-        dense, i32 = self._dense, torch.int32
-        args = (dense(kv_lens, "kv_lens", i32, (r,)), dense(new, "new", i32, (r,)),
-                dense(block_table, "block_table", i32, (r, None)), r, width,
+        r, width = block_table.shape
+        dense, i32, one = self._dense, torch.int32, (r,)
+        args = (dense(kv_lens, "kv_lens", i32, one), dense(new, "new", i32, one),
+                dense(block_table, "block_table", i32, (r, width)), r, width,
                 dense(free_pages, "free_pages", i32, (None,)), dense(free_count, "free_count", i32, (1,)),
-                free_pages.numel(), page_tokens, tokens)
-        table = block_table if in_place else torch.empty((r, width), dtype=i32, device=self.device)
+                free_pages.shape[0], page_tokens, tokens)
+        table = block_table if in_place else torch.empty_like(block_table)
         slots = torch.empty(tokens, dtype=torch.int64, device=self.device)
         small = torch.empty(tokens + 2 * r + 2, dtype=i32, device=self.device)
         positions, q_start, lens, left = small.split_with_sizes((tokens, r + 1, r, 1))
-        self.lib.call("zt_kv8_plan", *args, table.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-                      q_start.data_ptr(), lens.data_ptr(), left.data_ptr(), self._s)
+        at = small.data_ptr()
+        self.lib.call("zt_kv8_plan", *args, table.data_ptr(), slots.data_ptr(), at, at + 4 * tokens,
+                      at + 4 * (tokens + r + 1), at + 4 * (tokens + 2 * r + 1), self._s)
         return KV8Plan(table, slots, positions, q_start, lens, left)
 
     @_on_engine_stream
@@ -268,24 +302,23 @@ class DecodeOps:
         block_table allow): they choose the launch, not the result's meaning.
         Rows that see nothing are zeros."""
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = _like(q)
         elif out.shape != q.shape:
             raise ValueError("kv8_attention: out has q's shape")
         t = self._type("kv8_attention", q, out)
-        c = self._kv8(cache, q.shape[2])
+        rows, dense, i32 = self._rows, self._dense, torch.int32
+        qrows, orows = rows(q, "q"), rows(out, "out")
+        tokens, heads, dim = q.shape
+        c = self._kv8(cache, dim)
         r, width = block_table.shape
-        if q.shape[1] % c.kv_heads:
-            raise ValueError(f"kv8_attention: {q.shape[1]} heads over {c.kv_heads} of the cache")
-        a = _lib.KV8Attn(c, self._rows(q, "q"), self._rows(out, "out"),
-                         self._dense(block_table, "block_table", torch.int32, (r, width)),
-                         self._dense(kv_lens, "kv_lens", torch.int32, (r,)),
-                         self._dense(q_start, "q_start", torch.int32, (r + 1,)),
-                         self._dense(scale, "scale", torch.float32, (1,)), r, width, q.shape[0],
-                         q.shape[0] if max_q is None else max_q, width * c.page_tokens if max_kv is None else max_kv,
-                         window, t, 0)
-        ref = ctypes.byref(a)
-        ws, wsb = self._workspace(self.lib.zt_kv8_attention_workspace_bytes(ref))
-        self.lib.call("zt_kv8_attention", ref, ws, wsb, self._s)
+        if heads % c[5]:
+            raise ValueError(f"kv8_attention: {heads} heads over {c[5]} of the cache")
+        a = _ATTN.pack(*c, *qrows, *orows, dense(block_table, "block_table", i32, (r, width)),
+                       dense(kv_lens, "kv_lens", i32, (r,)), dense(q_start, "q_start", i32, (r + 1,)),
+                       dense(scale, "scale", torch.float32, (1,)), r, width, tokens, tokens if max_q is None else max_q,
+                       width * c[7] if max_kv is None else max_kv, window, t, 0)
+        ws, wsb = self._workspace(self.lib.zt_kv8_attention_workspace_bytes(a))
+        self.lib.call("zt_kv8_attention", a, ws, wsb, self._s)
         return out
 
     @_on_engine_stream
@@ -297,16 +330,17 @@ class DecodeOps:
         kept probability (float32 [rows]).  temperature, top_p, min_p: float32
         [rows], top_k: int32 [rows], None: off.  temperature <= 0: the largest
         logit.  A row with no logit above -inf gives token -1."""
-        if logits.dim() != 2 or logits.device != self.device or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        st = logits.stride()
+        if len(st) != 2 or logits.device != self.device or (st[1] != 1 and logits.shape[1] > 1):
             raise ValueError("sample: logits are [rows, vocab] on the engine's device, a row's values neighbours")
         rows, vocab = logits.shape
-        t, f32, dense = self._type("sample", logits), torch.float32, self._dense
-        args = (dense(u, "u", f32, (rows,)), dense(temperature, "temperature", f32, (rows,)),
-                dense(top_k, "top_k", torch.int32, (rows,)), dense(top_p, "top_p", f32, (rows,)),
-                dense(min_p, "min_p", f32, (rows,)))
+        t, f32, dense, one = self._type("sample", logits), torch.float32, self._dense, (rows,)
+        args = (dense(u, "u", f32, one), dense(temperature, "temperature", f32, one),
+                dense(top_k, "top_k", torch.int32, one), dense(top_p, "top_p", f32, one),
+                dense(min_p, "min_p", f32, one))
         token = torch.empty(rows, dtype=torch.int64, device=self.device)
-        logprob = torch.empty(rows, dtype=f32, device=self.device)
+        logprob = torch.empty_like(u)
         ws, wsb = self._workspace(self.lib.zt_sample_workspace_bytes(rows, vocab))
-        self.lib.call("zt_sample", logits.data_ptr(), logits.stride(0), rows, vocab, t, *args, token.data_ptr(),
+        self.lib.call("zt_sample", logits.data_ptr(), st[0], rows, vocab, t, *args, token.data_ptr(),
                       logprob.data_ptr(), ws, wsb, self._s)
         return token, logprob
