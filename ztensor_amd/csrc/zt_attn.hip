@@ -41,18 +41,15 @@ struct Split {
 
 struct Work {
     AttnArgs a;
-    Split few, many;
     int most;    // requests of up to so many rows (a row: a token and one of the heads of a group) are the few kernel's
+    int shares;  // waves of the few kernel
+    Split many;
     int qtiles;  // workgroups along the rows of the other kernel
     int vec;     // q and out in pieces of 4 values
-    int room;    // rows of a request and head whose splits' sums there is room for
-    long others; // where the other kernel's begin
-    float* part;   // [][dp]: sums of a row's split, not yet divided,
+    long others; // rows of sums that the few kernel has room for; the other kernel's follow
+    float* part;   // [][dp]: sums of a row over some of its tokens, not yet divided,
     float2* stat;  // and their (maximum, sum of weights)
-    // the place of a row's sums: of the few kernel's, and of the other's
-    __device__ __forceinline__ long few_at(int split, int r, int kv, int row) const {
-        return (((long)split * a.requests + r) * a.c.heads + kv) * room + row;
-    }
+    // the place of a row's sums in the other kernel's
     __device__ __forceinline__ long many_at(int split, int t, int h) const {
         return others + ((long)split * a.tokens + t) * a.q.heads + h;
     }
@@ -127,7 +124,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs& g, int r) {
     s.len = g.c.pages ? (int)min((long)max(0, g.kv_lens[r]), most) : 0;
     const int lo = g.window > 0 ? max(0, s.len - s.n + 1 - g.window) : 0;
     s.tile0 = lo >> 6;
-    s.tile1 = max((s.len + 63) >> 6, s.tile0);
+    s.tile1 = max((s.len + 63) >> 6, s.tile0 + 1);  // (one where there is nothing to see: it gives zeros)
     return s;
 }
 
@@ -180,56 +177,94 @@ __device__ __forceinline__ void load_query(const Work& f, const Span& sp, int kv
 // What a lane holds of a row, dims 16 i + 4 (lane / 16) .. +4: the result, or
 // the sum that the other splits' are to be added to.
 template <class T, int DN>
-__device__ __forceinline__ void store_row(const Work& f, const Span& sp, int kv, int row, int rows, int ns, long at,
+__device__ __forceinline__ void store_row(const Work& f, const Span& sp, int kv, int row, int rows, bool part, long at,
                                           float top, float sum, int ev, const float4v (&o)[4 * DN]) {
     if (row >= rows) return;
     const AttnArgs& g = f.a;
     const int i = row / g.group, h = kv * g.group + row - i * g.group, quad = (threadIdx.x & 63) >> 4;
     const long t = sp.start + i;
-    const float by = ldexpf(ns > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum, ev - 14);
-    if (ns > 1 && quad == 0) f.stat[at] = make_float2(top, sum);
+    const float by = ldexpf(part ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum, ev - 14);
+    if (part && quad == 0) f.stat[at] = make_float2(top, sum);
     T* out = (T*)g.out.p + t * g.out.token + (long)h * g.out.head;
 #pragma unroll
     for (int k = 0; k < 4 * DN; k++) {
         const float4v x = o[k] * by;
         const int d = 16 * k + 4 * quad;
-        if (ns > 1)
+        if (part)
             *reinterpret_cast<float4v*>(f.part + at * g.c.dp + d) = x;
         else
             store4<T>(out, d, g.c.dim, f.vec, {x[0], x[1], x[2], x[3]});
     }
 }
 
-// One workgroup: a request, a key/value head and a range of its tokens; up to
-// 16 CT rows (tokens x the group's q heads) are the columns of the products
+// The few kernel's work is a row of tiles: request after request, and of each
+// request its column groups (of 16 CT rows) and key/value heads, each with the
+// tiles of 64 tokens that the request sees, after a place for what it takes to
+// begin.  Every wave takes an equal share of the row, wherever that begins and
+// ends: sequences of any lengths keep all CUs busy to the end.  What a share
+// holds of a head's tiles goes to `out` if it is all of them, else to the
+// share's place for its first part or its last.
+constexpr int kBegin = 1;  // a head's queries and first pages take as long as a tile of a busy card
+struct Shares {
+    long all, each;  // places, and of one share
+};
+__device__ __forceinline__ long places_of(const Work& f, const Span& sp, int rows_of_group) {
+    const int rows = sp.n * f.a.group;
+    if (sp.n <= 0 || rows > f.most) return 0;
+    return (long)((rows + rows_of_group - 1) / rows_of_group) * f.a.c.heads * (sp.tile1 - sp.tile0 + kBegin);
+}
+
+// Running sums over the lanes, the lane's own included.
+__device__ __forceinline__ long wave_scan(long v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long x = __shfl_up(v, o);
+        if (lane >= o) v += x;
+    }
+    return v;
+}
+
+// The shares, and the places of the requests before r (each wave by itself).
+__device__ __forceinline__ Shares shares_of(const Work& f, int rows_of_group, int r, long& before) {
+    const int lane = threadIdx.x & 63;
+    long all = 0;
+    before = 0;
+    for (int r0 = 0; r0 < f.a.requests; r0 += 64) {
+        const long n = r0 + lane < f.a.requests ? places_of(f, span_of(f.a, r0 + lane), rows_of_group) : 0;
+        const long upto = wave_scan(n);
+        if (r >= r0 && r < r0 + 64) before = all + __shfl(upto - n, r - r0);
+        all += __shfl(upto, 63);
+    }
+    return {all, (all + f.shares - 1) / f.shares};
+}
+
+// A wave takes its share; up to 16 CT rows (tokens x the group's q heads) of one
+// request and head are the columns of the products
 //     S^T = K Q^T  (64 tokens x 16)   and   O^T += V^T P^T  (dims x 16),
 // whose operands K and V^T come from the cache straight into registers, 16
 // bytes a lane: the codes of a lane's tokens and dims are neighbours in both
 // layouts, and a lane's scores of the first product are its weights in the
 // second.  Row i of the first product's tile j is token 16 (i / 4) + 4 j + i % 4:
 // lane (n, g) then holds tokens 16 g .. 16 g + 15 of column n, all on one page,
-// and needs the values of just these.  Each wave takes every fourth tile of 64
-// tokens with its own running maximum; the four are joined through LDS.
+// and needs the values of just these.  The waves of a workgroup share nothing; a
+// lane's queries lie in LDS for itself.
 //
 // Weights enter the second product times their page's scale over a power of two
 // (the largest so far, 2^(e - 14)): fp16 then holds 39 bits below the largest.
 // fp32 rows: queries and weights in two fp16 parts (22 bits).
 template <class T, int DN, int CT>
-__global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
+__global__ __launch_bounds__(256, DN * CT <= 2 && sizeof(T) == 2 ? 3 : 2) void attn_few_kernel(Work f) {
     constexpr bool SPLIT = sizeof(T) == 4;
-    constexpr int ROW = 64 * DN + 4;  // floats of a row in LDS: 16 rows' pieces of 4 in different banks
-    __shared__ float sums[2][16 * CT][ROW];
-    __shared__ float4 stats[4][16 * CT];
+    constexpr int PARTS = SPLIT ? 2 : 1;
+    extern __shared__ __align__(16) half8v queries[];  // [4 waves][CT][DN][2][PARTS][64]
     const AttnArgs& g = f.a;
     const Kv8& c = g.c;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
-    int b = blockIdx.x;
-    const int kv = b % c.heads;
-    b /= c.heads;
-    const int split = b % f.few.splits, r = b / f.few.splits;
-    if (r == g.requests) {  // rows of no request
-        if (split || blockIdx.y) return;
-        const int from = g.requests ? max(0, g.q_start[g.requests]) : 0;
+    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int blocks = (f.shares + 3) / 4, share = blockIdx.x * 4 + wave;
+    if ((int)blockIdx.x >= blocks) {  // rows of no request
+        const int kv = blockIdx.x - blocks, from = g.requests ? max(0, g.q_start[g.requests]) : 0;
         for (int t = from; t < g.tokens; t++)
             for (int i = threadIdx.x; i < g.group * c.dim; i += 256) {
                 const int h = i / c.dim;
@@ -237,28 +272,75 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
             }
         return;
     }
-    const Span sp = span_of(g, r);
-    const int rows = sp.n * g.group;
-    if (sp.n <= 0 || rows > f.most) return;
-    const int ns = rows <= f.room ? splits_of(f.few, sp.tile1 - sp.tile0) : 1;
-    if (split >= ns) return;
-    const int first = sp.tile0 + split * f.few.tiles, last = split == ns - 1 ? sp.tile1 : first + f.few.tiles;
+    if (share >= f.shares) return;
+    // the share, and the request of its first place
+    long all = 0, before = 0, upto = 0, places = 0;
+    for (int r0 = 0; r0 < g.requests; r0 += 64) {
+        places = r0 + lane < g.requests ? places_of(f, span_of(g, r0 + lane), 16 * CT) : 0;
+        upto = wave_scan(places);
+        all += __shfl(upto, 63);
+    }
+    const long each = (all + f.shares - 1) / f.shares;
+    long pos = share * each;
+    const long end = min(all, pos + each);
+    if (pos >= end) return;
+    int r = 0;
+    for (int r0 = 0;; r0 += 64) {
+        if (g.requests > 64) {
+            places = r0 + lane < g.requests ? places_of(f, span_of(g, r0 + lane), 16 * CT) : 0;
+            upto = wave_scan(places);
+        }
+        const uint64_t past = __ballot(before + upto > pos);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            r = r0 + l;
+            before += __shfl(upto - places, l);
+            break;
+        }
+        before += __shfl(upto, 63);
+    }
+    r = __builtin_amdgcn_readfirstlane(r);
     const float scale = (g.scale ? *g.scale : 1.0f / sqrtf((float)c.dim)) * kLog2e;
-    const int* table = g.table + (long)r * g.width;
     const int krow = (col >> 2) * 16 + (col & 3);  // this lane's token of a key tile, less 4 j
 
-    auto page_at = [&](int token) {  // -1: nothing to see there
-        const int p = token < sp.len ? table[token >> c.shift] : -1;
-        return c.holds(p) ? p : -1;
-    };
-
-    for (int cg = blockIdx.y; cg * 16 * CT < rows; cg += gridDim.y) {
-        half8v q[CT][DN][2], ql[CT][DN][2];
+    while (pos < end) {
+        const Span sp = span_of(g, r);
+        const int rows = sp.n * g.group, tiles = sp.tile1 - sp.tile0;
+        const long mine = places_of(f, sp, 16 * CT);
+        if (pos - before >= mine) {
+            before += mine;
+            r++;
+            continue;
+        }
+        const int seg = __builtin_amdgcn_readfirstlane((int)((pos - before) / (tiles + kBegin)));
+        const int at0 = __builtin_amdgcn_readfirstlane((int)(pos - before - (long)seg * (tiles + kBegin)));
+        const int at1 = (int)min(at0 + end - pos, (long)(tiles + kBegin));
+        const int cg = seg / c.heads, kv = seg - cg * c.heads;
+        const int into = max(0, at0 - kBegin), n = at1 - kBegin - into;
+        const int first = sp.tile0 + into, last = first + n;
+        pos += at1 - at0;
+        if (n <= 0) continue;
+        const int* table = g.table + (long)r * g.width;
+        auto page_at = [&](int token) {  // -1: nothing to see there
+            const int p = token < sp.len ? table[token >> c.shift] : -1;
+            return c.holds(p) ? p : -1;
+        };
+        int pk = page_at(first * 64 + (col >> 2) * 16), pv = page_at(first * 64 + quad * 16);
+        half8v* mine_q = queries + wave * (CT * DN * 2 * PARTS * 64);
         float factor[CT];
         int lo[CT], hi[CT];
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++)
-            load_query<T, DN>(f, sp, kv, (cg * CT + ct) * 16 + col, rows, scale, q[ct], ql[ct], factor[ct], lo[ct], hi[ct]);
+        for (int ct = 0; ct < CT; ct++) {
+            half8v q[DN][2], ql[DN][2];
+            load_query<T, DN>(f, sp, kv, (cg * CT + ct) * 16 + col, rows, scale, q, ql, factor[ct], lo[ct], hi[ct]);
+#pragma unroll
+            for (int d = 0; d < DN; d++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    mine_q[(((ct * DN + d) * 2 + h) * PARTS) * 64 + lane] = q[d][h];
+                    if constexpr (SPLIT) mine_q[(((ct * DN + d) * 2 + h) * PARTS + 1) * 64 + lane] = ql[d][h];
+                }
+        }
         // every row of these columns sees tokens all_lo .. all_hi - 1
         const int row0 = cg * 16 * CT, row1 = min(rows, row0 + 16 * CT) - 1;
         const int all_hi = sp.len - sp.n + row0 / g.group + 1;
@@ -275,10 +357,10 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
             for (int i = 0; i < 4 * DN; i++) o[ct][i] = (float4v){0, 0, 0, 0};
         }
 
-        int tile = first + wave;
-        int pk = page_at(tile * 64 + (col >> 2) * 16), pv = page_at(tile * 64 + quad * 16);
-        for (; tile < last; tile += 4) {
+        for (int tile = first; tile < last && c.pages; tile++) {
             const int t0 = tile * 64;
+            int qlane = lane;
+            asm volatile("" : "+v"(qlane));  // the queries are read from LDS for each tile: held, they cost 16 to 64 registers
             const int at = max(pv, 0);
             const int8_t* kp = c.k + c.at(max(pk, 0), kv) + (long)((t0 + krow) & (c.page - 1)) * c.dp + 16 * quad;
             const int8_t* vp = c.v + c.at(at, kv) + (long)col * c.page + ((t0 + 16 * quad) & (c.page - 1));
@@ -293,8 +375,8 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
             const bool seen = pv >= 0;
             const bool whole = t0 + 64 <= all_hi && t0 >= all_lo && __all(seen);
             // the next tile's pages, while this one's codes are on their way
-            pk = page_at(t0 + 256 + (col >> 2) * 16);
-            pv = page_at(t0 + 256 + quad * 16);
+            pk = page_at(t0 + 64 + (col >> 2) * 16);
+            pv = page_at(t0 + 64 + quad * 16);
 
             int e = max(ev, exponent_of(vs));
             e = max(e, __shfl_xor(e, 16));
@@ -315,8 +397,8 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
                         const half8v k8 = codes8(kw[j][d][2 * h], kw[j][d][2 * h + 1]);
 #pragma unroll
                         for (int ct = 0; ct < CT; ct++) {
-                            s[ct][j] = mfma(k8, q[ct][d][h], s[ct][j]);
-                            if constexpr (SPLIT) s[ct][j] = mfma(k8, ql[ct][d][h], s[ct][j]);
+#pragma unroll
+                            for (int part = 0; part < PARTS; part++) s[ct][j] = mfma(k8, mine_q[(((ct * DN + d) * 2 + h) * PARTS + part) * 64 + qlane], s[ct][j]);
                         }
                     }
 
@@ -373,58 +455,12 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
                 }
         }
 
-        // the four waves' sums as one: common maximum and exponent, then 3 to 1, 2 to 0, 1 to 0
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             l[ct] += __shfl_xor(l[ct], 16);
             l[ct] += __shfl_xor(l[ct], 32);
-            if (quad == 0) stats[wave][16 * ct + col] = make_float4(m[ct], l[ct], (float)ev, 0.0f);
-        }
-        __syncthreads();
-        float sum[CT], top[CT];
-        int e = -127;
-#pragma unroll
-        for (int ct = 0; ct < CT; ct++) {
-            top[ct] = kNone;
-            sum[ct] = 0.0f;
-            for (int w = 0; w < 4; w++) {
-                top[ct] = fmaxf(top[ct], stats[w][16 * ct + col].x);
-                e = max(e, (int)stats[w][16 * ct + col].z);
-            }
-            const float base = top[ct] == kNone ? 0.0f : top[ct];
-            for (int w = 0; w < 4; w++) {
-                const float4 t = stats[w][16 * ct + col];
-                sum[ct] += t.y * __builtin_amdgcn_exp2f(t.x - base);
-            }
-            const float keep = ldexpf(__builtin_amdgcn_exp2f(m[ct] - base), ev - e);
-#pragma unroll
-            for (int i = 0; i < 4 * DN; i++) o[ct][i] *= keep;
-        }
-        for (int to = 2; to >= 1; to >>= 1) {
-            if (wave >= to && wave < 2 * to) {
-#pragma unroll
-                for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                    for (int i = 0; i < 4 * DN; i++)
-                        *reinterpret_cast<float4v*>(&sums[wave - to][16 * ct + col][16 * i + 4 * quad]) = o[ct][i];
-            }
-            __syncthreads();
-            if (wave < to) {
-#pragma unroll
-                for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                    for (int i = 0; i < 4 * DN; i++)
-                        o[ct][i] += *reinterpret_cast<const float4v*>(&sums[wave][16 * ct + col][16 * i + 4 * quad]);
-            }
-            __syncthreads();
-        }
-        if (wave == 0) {
-#pragma unroll
-            for (int ct = 0; ct < CT; ct++)
-            {
-                const int row = (cg * CT + ct) * 16 + col;
-                store_row<T, DN>(f, sp, kv, row, rows, ns, f.few_at(split, r, kv, row), top[ct], sum[ct], e, o[ct]);
-            }
+            const long at = ((long)share * 2 + (into == 0)) * (16 * CT) + 16 * ct + col;
+            store_row<T, DN>(f, sp, kv, (cg * CT + ct) * 16 + col, rows, n < tiles, at, m[ct], l[ct], ev, o[ct]);
         }
     }
 }
@@ -651,76 +687,103 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
             l[ct] += __shfl_xor(l[ct], 16);
             l[ct] += __shfl_xor(l[ct], 32);
             const int row = row0 + 16 * ct + col, i = row / g.group;
-            store_row<T, DN>(f, sp, kv, row, rows, ns, f.many_at(split, sp.start + i, kv * g.group + row - i * g.group), m[ct],
+            store_row<T, DN>(f, sp, kv, row, rows, ns > 1, f.many_at(split, sp.start + i, kv * g.group + row - i * g.group), m[ct],
                              l[ct], ev, o[ct]);
         }
     }
 }
 
-// Joins the splits' sums in their order: a workgroup a row and q head, 16 lanes
-// x 4 dims x DN of its threads a split, 16 / DN splits at a time.
-template <class T, int DN>
-__global__ __launch_bounds__(256) void attn_join_kernel(Work f) {
-    constexpr int G = 16 / DN;  // groups of 16 DN lanes
-    __shared__ float4 part[G][16 * DN];
+// Joins what several waves or workgroups hold of a row, in their order: W waves
+// a row and q head, 16 DN lanes x 4 dims a part, 4 W / DN parts at a time.  One
+// wave does for a batch, whose heads are split in few parts; of one long
+// sequence there are hundreds.
+template <class T, int DN, int W>
+__global__ __launch_bounds__(512) void attn_join_kernel(Work f, int rows_of_group, int each_n, bool many) {
+    constexpr int G = W == 1 ? 4 / DN : 32 / DN;  // groups of 16 DN lanes
+    constexpr int LANES = W == 1 ? 64 : 512, SETS = 512 / LANES;
+    __shared__ float4 part[SETS][G][16 * DN];
+    __shared__ float ls[SETS][G];
     const AttnArgs& g = f.a;
-    const int t = blockIdx.x / g.q.heads, h = blockIdx.x - t * g.q.heads;
-    int lo, hi;
-    const int r = find_request(g, t, lo, hi);
-    if (g.requests == 0 || t < g.q_start[0] || t >= g.q_start[g.requests]) return;
-    const Span sp = span_of(g, r);
-    const int rows = sp.n * g.group, kv = h / g.group, row = (t - sp.start) * g.group + h % g.group;
-    int ns;
-    long at, step;
-    if (rows <= f.most) {
-        ns = rows <= f.room ? splits_of(f.few, sp.tile1 - sp.tile0) : 1;
-        at = f.few_at(0, r, kv, row);
-        step = f.few_at(1, r, kv, row) - at;
-    } else {
-        const RowTiles w = tiles_of<DN>(g, sp, row);
-        ns = splits_of(f.many, w.tile1 - w.tile0);
-        at = f.many_at(0, t, h);
-        step = f.many_at(1, t, h) - at;
-    }
-    if (ns == 1) return;
-    float top = kNone;
-    for (int s = threadIdx.x & 63; s < ns; s += 64) top = fmaxf(top, f.stat[s * step + at].x);
-    top = max_step<1>(max_step<2>(max_step<4>(max_step<8>(max_step<16>(max_step<32>(top))))));
-    if (top == kNone) top = 0.0f;
-    const int group = threadIdx.x / (16 * DN), piece = threadIdx.x % (16 * DN);
-    float4 sum = make_float4(0, 0, 0, 0);
-    float l = 0.0f;
-    if (group < G) {
-#pragma unroll 4
-        for (int s = group; s < ns; s += G) {
-            const float2 st = f.stat[s * step + at];
-            const float w = __builtin_amdgcn_exp2f(st.x - top);
-            const float4 x = reinterpret_cast<const float4*>(f.part + (s * step + at) * g.c.dp)[piece];
-            l += st.y * w;
-            sum.x += x.x * w;
-            sum.y += x.y * w;
-            sum.z += x.z * w;
-            sum.w += x.w * w;
+    const int set = W == 1 ? threadIdx.x >> 6 : 0, tid = threadIdx.x & (LANES - 1);
+    long b = (long)blockIdx.x * SETS + set;
+    const int h = (int)(b % g.q.heads);
+    b /= g.q.heads;
+    const int i0 = (int)(b % each_n), r = (int)(b / each_n);
+    const bool there = r < g.requests;
+    Span sp{};
+    if (there) sp = span_of(g, r);
+    const int rows = sp.n * g.group, kv = h / g.group;
+    const bool mine = there && sp.n > 0 && many == (rows > f.most);
+    long before = 0;
+    Shares sh{0, 1};
+    if (!many) sh = shares_of(f, rows_of_group, r, before);
+    for (int i = i0; __any(mine && i < sp.n); i += each_n) {  // (any: the same for all of a row's threads)
+        const int row = i * g.group + h % g.group, t = sp.start + i;
+        int ns;
+        long at0, at, step;  // the place of the first part, of the second, and on from there
+        if (!many) {
+            const int tiles = sp.tile1 - sp.tile0;
+            const long a = before + ((long)(row / rows_of_group) * g.c.heads + kv) * (tiles + kBegin) + kBegin;
+            const long s0 = a / sh.each, s1 = (a + tiles - 1) / sh.each;
+            ns = (int)(s1 - s0) + 1;
+            at0 = (2 * s0 + 1) * rows_of_group + row % rows_of_group;
+            at = at0 + rows_of_group;
+            step = 2l * rows_of_group;
+        } else {
+            const RowTiles w = tiles_of<DN>(g, sp, row);
+            ns = splits_of(f.many, w.tile1 - w.tile0);
+            at0 = f.many_at(0, t, h);
+            at = f.many_at(1, t, h);
+            step = at - at0;
         }
-        part[group][piece] = sum;
+        if (ns == 1) continue;
+        auto place = [&](int s) { return s ? at + (s - 1) * step : at0; };
+        float top = kNone;
+        for (int s = tid & 63; s < ns; s += 64) top = fmaxf(top, f.stat[place(s)].x);
+        top = max_step<1>(max_step<2>(max_step<4>(max_step<8>(max_step<16>(max_step<32>(top))))));
+        if (top == kNone) top = 0.0f;
+        const int group = tid / (16 * DN), piece = tid % (16 * DN);
+        float4 sum = make_float4(0, 0, 0, 0);
+        float l = 0.0f;
+        if (group < G) {
+#pragma unroll 8
+            for (int s = group; s < ns; s += G) {
+                const float2 st = f.stat[place(s)];
+                const float w = __builtin_amdgcn_exp2f(st.x - top);
+                const float4 x = reinterpret_cast<const float4*>(f.part + place(s) * g.c.dp)[piece];
+                l += st.y * w;
+                sum.x += x.x * w;
+                sum.y += x.y * w;
+                sum.z += x.z * w;
+                sum.w += x.w * w;
+            }
+            part[set][group][piece] = sum;
+            if (piece == 0) ls[set][group] = l;
+        }
+        if (W > 1)
+            __syncthreads();
+        else
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        if (tid < 16 * DN) {
+            l = 0.0f;
+            sum = make_float4(0, 0, 0, 0);
+            for (int k = 0; k < G; k++) {
+                const float4 x = part[set][k][piece];
+                l += ls[set][k];
+                sum.x += x.x;
+                sum.y += x.y;
+                sum.z += x.z;
+                sum.w += x.w;
+            }
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            store4<T>((T*)g.out.p + (long)t * g.out.token + (long)h * g.out.head, 4 * piece, g.c.dim, f.vec,
+                      {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv});
+        }
+        if (W > 1)
+            __syncthreads();
+        else
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
     }
-    __shared__ float ls[G];
-    if (group < G && piece == 0) ls[group] = l;
-    __syncthreads();
-    if (threadIdx.x >= 16 * DN) return;
-    l = 0.0f;
-    sum = make_float4(0, 0, 0, 0);
-    for (int i = 0; i < G; i++) {
-        const float4 x = part[i][piece];
-        l += ls[i];
-        sum.x += x.x;
-        sum.y += x.y;
-        sum.z += x.z;
-        sum.w += x.w;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    store4<T>((T*)g.out.p + (long)t * g.out.token + (long)h * g.out.head, 4 * piece, g.c.dim, f.vec,
-              {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv});
 }
 
 }  // namespace zt
@@ -736,22 +799,13 @@ static bool attn_ok(const zt_kv8_attn* a) {
 
 // How a call is launched.
 struct AttnPlan {
-    int ct, groups;  // the few kernel: column tiles a wave, workgroups along the rows
-    Split few, many;
-    int most, qtiles, room;
+    int ct;  // column tiles of a wave of the few kernel
+    int most, shares, qtiles;
+    int few_n, many_n;  // bounds of the tokens of one request
+    Split many;
     long others;
-    long part, stat;  // bytes of the splits' sums
+    long part, stat;  // bytes of the parts' sums
 };
-
-// Along the tokens until about `want` workgroups are there, none of less than
-// 4 tiles.
-static Split split_of(long tiles, long have, long want) {
-    const long splits = std::max(1l, std::min((want + have - 1) / have, tiles / 4));
-    Split s;
-    s.tiles = (int)((tiles + splits - 1) / splits);
-    s.splits = (int)((tiles + s.tiles - 1) / s.tiles);
-    return s;
-}
 
 static AttnPlan attn_plan(const zt_kv8_attn* a) {
     AttnPlan p{};
@@ -759,20 +813,24 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
     const long requests = std::max(1, a->requests), heads = a->cache.kv_heads;
     const long most = (long)std::min(a->max_q, a->tokens) * group;
     p.most = most <= 64 ? 0x7FFFFFFF : 64;
-    const int rows = (int)std::max(1l, std::min(most, 64l));
-    p.ct = rows > 16 && dp <= 128 ? 2 : 1;
-    p.groups = ceil_div(rows, 16 * p.ct);
+    p.ct = most > 16 && dp <= 128 ? 2 : 1;
     long kv = std::min((long)a->max_kv, (long)a->width * a->cache.page_tokens);
     if (a->window > 0) kv = std::min(kv, (long)a->window + a->max_q + 63);
     const long tiles = std::max(1l, (kv + 63) / 64);
-    p.few = split_of(tiles, requests * heads * p.groups, 1024);
+    // a tile each as far as the bounds go, up to the waves that the card holds
+    const long groups = (std::max(1l, std::min(most, 64l)) + 16 * p.ct - 1) / (16 * p.ct);
+    p.shares = (int)std::min(2048l, requests * heads * groups * (tiles + kBegin));
+    p.others = 2l * p.shares * 16 * p.ct;
+    p.many_n = std::max(1, std::min(a->max_q, a->tokens));
+    p.few_n = std::max(1, std::min(p.many_n, 64 / group));
     p.many = {1, 1};
     if (most > 64) {
         p.qtiles = ceil_div(most, dp <= 128 ? 128 : 64);
-        p.many = split_of(tiles, requests * heads * p.qtiles, 512);
+        // along the tokens until about 512 workgroups are there, none of less than 4 tiles
+        const long have = requests * heads * p.qtiles, splits = std::max(1l, std::min((512 + have - 1) / have, tiles / 4));
+        p.many.tiles = (int)((tiles + splits - 1) / splits);
+        p.many.splits = (int)((tiles + p.many.tiles - 1) / p.many.tiles);
     }
-    p.room = p.groups * 16 * p.ct;
-    if (p.few.splits > 1) p.others = (long)p.few.splits * a->requests * heads * p.room;
     const long all = p.others + (p.many.splits > 1 ? (long)p.many.splits * a->tokens * a->q.heads : 0);
     p.stat = (all * 8 + 15) & ~15l;
     p.part = all * dp * 4;
@@ -781,9 +839,8 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
 
 template <class T, int DN>
 static int launch(const Work& f, const AttnPlan& p, hipStream_t stream) {
-    const long few = ((long)f.a.requests + 1) * p.few.splits * f.a.c.heads;
     const long many = (long)p.qtiles * p.many.splits * f.a.c.heads;
-    if (few >= 1l << 31 || many >= 1l << 31 || (p.qtiles && f.a.requests > 65535)) return kInvalid;
+    if (many >= 1l << 31 || (p.qtiles && f.a.requests > 65535)) return kInvalid;
     if (p.qtiles && f.a.requests) {
         static std::atomic<uint64_t> raised{0};
         constexpr int lds = 2 * 16 * DN * 1024;
@@ -793,13 +850,23 @@ static int launch(const Work& f, const AttnPlan& p, hipStream_t stream) {
         }
         attn_many_kernel<T, DN><<<dim3((unsigned)many, f.a.requests), 256, lds, stream>>>(f);
     }
-    const dim3 grid((unsigned)few, p.groups);
+    const int few = (f.shares + 3) / 4 + f.a.c.heads;
+    constexpr int lds = DN * 2 * (sizeof(T) / 2) * 4096;  // of a column tile, at most 64 KB in all
     if (p.ct == 2) {
-        if constexpr (DN <= 2) attn_few_kernel<T, DN, 2><<<grid, 256, 0, stream>>>(f);
+        if constexpr (DN <= 2) attn_few_kernel<T, DN, 2><<<few, 256, 2 * lds, stream>>>(f);
     } else {
-        attn_few_kernel<T, DN, 1><<<grid, 256, 0, stream>>>(f);
+        attn_few_kernel<T, DN, 1><<<few, 256, lds, stream>>>(f);
     }
-    if (p.part) attn_join_kernel<T, DN><<<(unsigned)(f.a.tokens * f.a.q.heads), 256, 0, stream>>>(f);
+    // rows that may be in parts: of each request up to so many tokens
+    const auto join = [&](int each, bool many, bool wide) {
+        const long rows = (long)f.a.requests * each * f.a.q.heads;
+        if (wide)
+            attn_join_kernel<T, DN, 8><<<(unsigned)rows, 512, 0, stream>>>(f, 16 * p.ct, each, many);
+        else
+            attn_join_kernel<T, DN, 1><<<(unsigned)((rows + 7) / 8), 512, 0, stream>>>(f, 16 * p.ct, each, many);
+    };
+    if (f.a.requests && p.shares > 1) join(p.few_n, false, (long)f.a.requests * f.a.c.heads * 8 < p.shares);
+    if (f.a.requests && p.many.splits > 1) join(p.many_n, true, p.many.splits > 8);
     return (int)hipGetLastError();
 }
 
@@ -820,8 +887,8 @@ ZT_EXPORT int zt_kv8_attention(const zt_kv8_attn* a, void* workspace, long works
     if (p.part + p.stat > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.part + p.stat)) return kInvalid;
     const AttnArgs g{kv8_of(a->cache), rows_of(a->q), rows_of(a->out), a->table, a->kv_lens, a->q_start, a->scale,
                      a->requests,      a->width,      a->tokens,       a->window, a->q.heads / a->cache.kv_heads};
-    const Work f{g,        p.few, p.many, p.most, p.qtiles, rows_vector(a->q, 4, a->type) && rows_vector(a->out, 4, a->type),
-                 p.room,   p.others, (float*)workspace, (float2*)((char*)workspace + p.part)};
+    const Work f{g,        p.most, p.shares, p.many, p.qtiles, rows_vector(a->q, 4, a->type) && rows_vector(a->out, 4, a->type),
+                 p.others, (float*)workspace, (float2*)((char*)workspace + p.part)};
     const bool f32 = a->type == ZT_F32;
     switch (g.c.dp) {
         case 64: return f32 ? launch<float, 1>(f, p, stream) : launch<_Float16, 1>(f, p, stream);
