@@ -43,12 +43,14 @@ struct Work {
     AttnArgs a;
     int most;    // requests of up to so many rows (a row: a token and one of the heads of a group) are the few kernel's
     int shares;  // waves of the few kernel
+    bool single; // each takes whole heads
     Split many;
     int qtiles;  // workgroups along the rows of the other kernel
     int vec;     // q and out in pieces of 4 values
     long others; // rows of sums that the few kernel has room for; the other kernel's follow
     float* part;   // [][dp]: sums of a row over some of its tokens, not yet divided,
     float2* stat;  // and their (maximum, sum of weights)
+    int2* parts;   // [tokens][q heads]: of each row, the place of its first part's sums, and how many parts there are
     // the place of a row's sums in the other kernel's
     __device__ __forceinline__ long many_at(int split, int t, int h) const {
         return others + ((long)split * a.tokens + t) * a.q.heads + h;
@@ -204,14 +206,15 @@ __device__ __forceinline__ void store_row(const Work& f, const Span& sp, int kv,
 // ends: sequences of any lengths keep all CUs busy to the end.  What a share
 // holds of a head's tiles goes to `out` if it is all of them, else to the
 // share's place for its first part or its last.
-constexpr int kBegin = 1;  // a head's queries and first pages take as long as a tile of a busy card
-struct Shares {
-    long all, each;  // places, and of one share
-};
+// That place counts as two tiles: 64 sequences of up to 8000 tokens, 76 us at one, 75 at two or three.  Where the
+// host knows of few tiles, a head's are one place: nothing is split, nothing to be joined.
+constexpr int kBegin = 2;
+__device__ __forceinline__ int begin_of(const Work& f) { return f.single ? 0 : kBegin; }
+__device__ __forceinline__ int length_of(const Work& f, const Span& sp) { return f.single ? 1 : sp.tile1 - sp.tile0 + kBegin; }
 __device__ __forceinline__ long places_of(const Work& f, const Span& sp, int rows_of_group) {
     const int rows = sp.n * f.a.group;
     if (sp.n <= 0 || rows > f.most) return 0;
-    return (long)((rows + rows_of_group - 1) / rows_of_group) * f.a.c.heads * (sp.tile1 - sp.tile0 + kBegin);
+    return (long)((rows + rows_of_group - 1) / rows_of_group) * f.a.c.heads * length_of(f, sp);
 }
 
 // Running sums over the lanes, the lane's own included.
@@ -223,20 +226,6 @@ __device__ __forceinline__ long wave_scan(long v) {
         if (lane >= o) v += x;
     }
     return v;
-}
-
-// The shares, and the places of the requests before r (each wave by itself).
-__device__ __forceinline__ Shares shares_of(const Work& f, int rows_of_group, int r, long& before) {
-    const int lane = threadIdx.x & 63;
-    long all = 0;
-    before = 0;
-    for (int r0 = 0; r0 < f.a.requests; r0 += 64) {
-        const long n = r0 + lane < f.a.requests ? places_of(f, span_of(f.a, r0 + lane), rows_of_group) : 0;
-        const long upto = wave_scan(n);
-        if (r >= r0 && r < r0 + 64) before = all + __shfl(upto - n, r - r0);
-        all += __shfl(upto, 63);
-    }
-    return {all, (all + f.shares - 1) / f.shares};
 }
 
 // A wave takes its share; up to 16 CT rows (tokens x the group's q heads) of one
@@ -254,7 +243,7 @@ __device__ __forceinline__ Shares shares_of(const Work& f, int rows_of_group, in
 // (the largest so far, 2^(e - 14)): fp16 then holds 39 bits below the largest.
 // fp32 rows: queries and weights in two fp16 parts (22 bits).
 template <class T, int DN, int CT>
-__global__ __launch_bounds__(256, DN * CT <= 2 && sizeof(T) == 2 ? 3 : 2) void attn_few_kernel(Work f) {
+__global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int PARTS = SPLIT ? 2 : 1;
     extern __shared__ __align__(16) half8v queries[];  // [4 waves][CT][DN][2][PARTS][64]
@@ -268,28 +257,32 @@ __global__ __launch_bounds__(256, DN * CT <= 2 && sizeof(T) == 2 ? 3 : 2) void a
         for (int t = from; t < g.tokens; t++)
             for (int i = threadIdx.x; i < g.group * c.dim; i += 256) {
                 const int h = i / c.dim;
+                if (i - h * c.dim == 0) f.parts[(long)t * g.q.heads + kv * g.group + h] = make_int2(0, 1);
                 ((T*)g.out.p)[(long)t * g.out.token + (long)(kv * g.group + h) * g.out.head + i - h * c.dim] = (T)0.0f;
             }
         return;
     }
     if (share >= f.shares) return;
-    // the share, and the request of its first place
+    // the share, and the request of its first place; 64 requests' spans lie in the lanes at a time
+    Span span{};
     long all = 0, before = 0, upto = 0, places = 0;
-    for (int r0 = 0; r0 < g.requests; r0 += 64) {
-        places = r0 + lane < g.requests ? places_of(f, span_of(g, r0 + lane), 16 * CT) : 0;
+    auto load_spans = [&](int r0) {
+        span = Span{};
+        if (r0 + lane < g.requests) span = span_of(g, r0 + lane);
+        places = places_of(f, span, 16 * CT);
         upto = wave_scan(places);
+    };
+    for (int r0 = 0; r0 < g.requests; r0 += 64) {
+        load_spans(r0);
         all += __shfl(upto, 63);
     }
     const long each = (all + f.shares - 1) / f.shares;
     long pos = share * each;
     const long end = min(all, pos + each);
     if (pos >= end) return;
-    int r = 0;
-    for (int r0 = 0;; r0 += 64) {
-        if (g.requests > 64) {
-            places = r0 + lane < g.requests ? places_of(f, span_of(g, r0 + lane), 16 * CT) : 0;
-            upto = wave_scan(places);
-        }
+    int r = 0, r0 = 0;
+    for (;; r0 += 64) {
+        if (g.requests > 64) load_spans(r0);
         const uint64_t past = __ballot(before + upto > pos);
         if (past) {
             const int l = __builtin_ctzll(past);
@@ -304,7 +297,16 @@ __global__ __launch_bounds__(256, DN * CT <= 2 && sizeof(T) == 2 ? 3 : 2) void a
     const int krow = (col >> 2) * 16 + (col & 3);  // this lane's token of a key tile, less 4 j
 
     while (pos < end) {
-        const Span sp = span_of(g, r);
+        if (r >= r0 + 64) {
+            r0 += 64;
+            load_spans(r0);
+        }
+        Span sp;
+        sp.start = __builtin_amdgcn_readlane(span.start, r - r0);
+        sp.n = __builtin_amdgcn_readlane(span.n, r - r0);
+        sp.len = __builtin_amdgcn_readlane(span.len, r - r0);
+        sp.tile0 = __builtin_amdgcn_readlane(span.tile0, r - r0);
+        sp.tile1 = __builtin_amdgcn_readlane(span.tile1, r - r0);
         const int rows = sp.n * g.group, tiles = sp.tile1 - sp.tile0;
         const long mine = places_of(f, sp, 16 * CT);
         if (pos - before >= mine) {
@@ -312,14 +314,17 @@ __global__ __launch_bounds__(256, DN * CT <= 2 && sizeof(T) == 2 ? 3 : 2) void a
             r++;
             continue;
         }
-        const int seg = __builtin_amdgcn_readfirstlane((int)((pos - before) / (tiles + kBegin)));
-        const int at0 = __builtin_amdgcn_readfirstlane((int)(pos - before - (long)seg * (tiles + kBegin)));
-        const int at1 = (int)min(at0 + end - pos, (long)(tiles + kBegin));
+        const int length = length_of(f, sp), begin = begin_of(f);
+        const int seg = __builtin_amdgcn_readfirstlane((int)((pos - before) / length));
+        const int at0 = __builtin_amdgcn_readfirstlane((int)(pos - before - (long)seg * length));
+        const int at1 = (int)min(at0 + end - pos, (long)length);
         const int cg = seg / c.heads, kv = seg - cg * c.heads;
-        const int into = max(0, at0 - kBegin), n = at1 - kBegin - into;
+        const int into = max(0, at0 - begin), n = f.single ? tiles : at1 - begin - into;
         const int first = sp.tile0 + into, last = first + n;
+        const long first_place = pos - at0 + begin;
         pos += at1 - at0;
         if (n <= 0) continue;
+        const int parts = f.single ? 1 : (int)((first_place + tiles - 1) / each) - share + 1;  // (of the first part's share)
         const int* table = g.table + (long)r * g.width;
         auto page_at = [&](int token) {  // -1: nothing to see there
             const int p = token < sp.len ? table[token >> c.shift] : -1;
@@ -460,7 +465,10 @@ __global__ __launch_bounds__(256, DN * CT <= 2 && sizeof(T) == 2 ? 3 : 2) void a
             l[ct] += __shfl_xor(l[ct], 16);
             l[ct] += __shfl_xor(l[ct], 32);
             const long at = ((long)share * 2 + (into == 0)) * (16 * CT) + 16 * ct + col;
-            store_row<T, DN>(f, sp, kv, (cg * CT + ct) * 16 + col, rows, n < tiles, at, m[ct], l[ct], ev, o[ct]);
+            const int row = (cg * CT + ct) * 16 + col, i = row / g.group;
+            if (into == 0 && row < rows && quad == 0)
+                f.parts[(long)(sp.start + i) * g.q.heads + kv * g.group + row - i * g.group] = make_int2((int)at, parts);
+            store_row<T, DN>(f, sp, kv, row, rows, n < tiles, at, m[ct], l[ct], ev, o[ct]);
         }
     }
 }
@@ -687,6 +695,8 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
             l[ct] += __shfl_xor(l[ct], 16);
             l[ct] += __shfl_xor(l[ct], 32);
             const int row = row0 + 16 * ct + col, i = row / g.group;
+            if (f.many.splits > 1 && split == 0 && row < rows && quad == 0)
+                f.parts[(long)(sp.start + i) * g.q.heads + kv * g.group + row - i * g.group] = make_int2(0, ns);
             store_row<T, DN>(f, sp, kv, row, rows, ns > 1, f.many_at(split, sp.start + i, kv * g.group + row - i * g.group), m[ct],
                              l[ct], ev, o[ct]);
         }
@@ -694,86 +704,103 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
 }
 
 // Joins what several waves or workgroups hold of a row, in their order: W waves
-// a row and q head, 16 DN lanes x 4 dims a part, 4 W / DN parts at a time.  One
-// wave does for a batch, whose heads are split in few parts; of one long
-// sequence there are hundreds.
+// a row and q head, 16 DN lanes x 4 dims a part, 4 W / DN parts at a time; then
+// those sets' sums, all with maxima of their own.  One wave does for a batch,
+// whose heads are split in few parts; of one long sequence there are hundreds.
+// The rows: ROWS all of them, FEW up to each_n of each request, MANY as FEW, of
+// the other kernel's.
+enum class Join { ROWS, FEW, MANY };
 template <class T, int DN, int W>
-__global__ __launch_bounds__(512) void attn_join_kernel(Work f, int rows_of_group, int each_n, bool many) {
+__global__ __launch_bounds__(512) void attn_join_kernel(Work f, int rows_of_group, int each_n, Join which) {
     constexpr int G = W == 1 ? 4 / DN : 32 / DN;  // groups of 16 DN lanes
     constexpr int LANES = W == 1 ? 64 : 512, SETS = 512 / LANES;
     __shared__ float4 part[SETS][G][16 * DN];
-    __shared__ float ls[SETS][G];
+    __shared__ float2 stats[SETS][G];
     const AttnArgs& g = f.a;
     const int set = W == 1 ? threadIdx.x >> 6 : 0, tid = threadIdx.x & (LANES - 1);
     long b = (long)blockIdx.x * SETS + set;
     const int h = (int)(b % g.q.heads);
     b /= g.q.heads;
-    const int i0 = (int)(b % each_n), r = (int)(b / each_n);
-    const bool there = r < g.requests;
-    Span sp{};
-    if (there) sp = span_of(g, r);
-    const int rows = sp.n * g.group, kv = h / g.group;
-    const bool mine = there && sp.n > 0 && many == (rows > f.most);
-    long before = 0;
-    Shares sh{0, 1};
-    if (!many) sh = shares_of(f, rows_of_group, r, before);
-    for (int i = i0; __any(mine && i < sp.n); i += each_n) {  // (any: the same for all of a row's threads)
-        const int row = i * g.group + h % g.group, t = sp.start + i;
-        int ns;
-        long at0, at, step;  // the place of the first part, of the second, and on from there
-        if (!many) {
-            const int tiles = sp.tile1 - sp.tile0;
-            const long a = before + ((long)(row / rows_of_group) * g.c.heads + kv) * (tiles + kBegin) + kBegin;
-            const long s0 = a / sh.each, s1 = (a + tiles - 1) / sh.each;
-            ns = (int)(s1 - s0) + 1;
-            at0 = (2 * s0 + 1) * rows_of_group + row % rows_of_group;
-            at = at0 + rows_of_group;
-            step = 2l * rows_of_group;
-        } else {
-            const RowTiles w = tiles_of<DN>(g, sp, row);
-            ns = splits_of(f.many, w.tile1 - w.tile0);
-            at0 = f.many_at(0, t, h);
-            at = f.many_at(1, t, h);
-            step = at - at0;
+    int t = (int)b, to = min(t + 1, g.tokens), step_t = 1;
+    if (which != Join::ROWS) {
+        const int r = (int)(b / each_n);
+        t = to = 0;
+        if (r < g.requests) {
+            const int start = g.q_start[r], n = min(g.q_start[r + 1], g.tokens) - start;
+            if (start >= 0 && (which == Join::MANY) == (n * g.group > f.most)) {
+                t = start + (int)(b % each_n);
+                to = start + n;
+            }
         }
+        step_t = each_n;
+    }
+    const int group = tid / (16 * DN), piece = tid % (16 * DN);
+    for (; t < to; t += step_t) {
+        const int2 of = f.parts[(long)t * g.q.heads + h];
+        const int ns = of.y;
         if (ns == 1) continue;
-        auto place = [&](int s) { return s ? at + (s - 1) * step : at0; };
-        float top = kNone;
-        for (int s = tid & 63; s < ns; s += 64) top = fmaxf(top, f.stat[place(s)].x);
-        top = max_step<1>(max_step<2>(max_step<4>(max_step<8>(max_step<16>(max_step<32>(top))))));
-        if (top == kNone) top = 0.0f;
-        const int group = tid / (16 * DN), piece = tid % (16 * DN);
+        // the place of the first part, of the second, and on from there
+        const long at0 = which == Join::MANY ? f.many_at(0, t, h) : of.x;
+        const long at = which == Join::MANY ? f.many_at(1, t, h) : at0 + rows_of_group;
+        const long step = which == Join::MANY ? at - at0 : 2l * rows_of_group;
+        float top = kNone, l = 0.0f;
         float4 sum = make_float4(0, 0, 0, 0);
-        float l = 0.0f;
         if (group < G) {
-#pragma unroll 8
-            for (int s = group; s < ns; s += G) {
-                const float2 st = f.stat[place(s)];
-                const float w = __builtin_amdgcn_exp2f(st.x - top);
-                const float4 x = reinterpret_cast<const float4*>(f.part + place(s) * g.c.dp)[piece];
-                l += st.y * w;
-                sum.x += x.x * w;
-                sum.y += x.y * w;
-                sum.z += x.z * w;
-                sum.w += x.w * w;
+            for (int s = group; s < ns; s += 8 * G) {  // 8 parts' loads at a time
+                float2 st[8];
+                float4 x[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int k = s + e * G;
+                    const long place = k ? at + (long)(k - 1) * step : at0;
+                    st[e] = make_float2(kNone, 0.0f);
+                    x[e] = make_float4(0, 0, 0, 0);
+                    if (k < ns) {
+                        st[e] = f.stat[place];
+                        x[e] = reinterpret_cast<const float4*>(f.part + place * g.c.dp)[piece];
+                    }
+                }
+                float m = top;
+#pragma unroll
+                for (int e = 0; e < 8; e++) m = fmaxf(m, st[e].x);
+                const float base = m == kNone ? 0.0f : m, old = __builtin_amdgcn_exp2f(top - base);
+                top = m;
+                l *= old;
+                sum.x *= old;
+                sum.y *= old;
+                sum.z *= old;
+                sum.w *= old;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float w = __builtin_amdgcn_exp2f(st[e].x - base);
+                    l += st[e].y * w;
+                    sum.x += x[e].x * w;
+                    sum.y += x[e].y * w;
+                    sum.z += x[e].z * w;
+                    sum.w += x[e].w * w;
+                }
             }
             part[set][group][piece] = sum;
-            if (piece == 0) ls[set][group] = l;
+            if (piece == 0) stats[set][group] = make_float2(top, l);
         }
         if (W > 1)
             __syncthreads();
         else
             __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
         if (tid < 16 * DN) {
+            top = kNone;
+            for (int k = 0; k < G; k++) top = fmaxf(top, stats[set][k].x);
+            const float base = top == kNone ? 0.0f : top;
             l = 0.0f;
             sum = make_float4(0, 0, 0, 0);
             for (int k = 0; k < G; k++) {
                 const float4 x = part[set][k][piece];
-                l += ls[set][k];
-                sum.x += x.x;
-                sum.y += x.y;
-                sum.z += x.z;
-                sum.w += x.w;
+                const float w = __builtin_amdgcn_exp2f(stats[set][k].x - base);
+                l += stats[set][k].y * w;
+                sum.x += x.x * w;
+                sum.y += x.y * w;
+                sum.z += x.z * w;
+                sum.w += x.w * w;
             }
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             store4<T>((T*)g.out.p + (long)t * g.out.token + (long)h * g.out.head, 4 * piece, g.c.dim, f.vec,
@@ -802,9 +829,10 @@ struct AttnPlan {
     int ct;  // column tiles of a wave of the few kernel
     int most, shares, qtiles;
     int few_n, many_n;  // bounds of the tokens of one request
+    bool single, wide;
     Split many;
     long others;
-    long part, stat;  // bytes of the parts' sums
+    long part, stat, parts;  // bytes of the parts' sums, and of where they are
 };
 
 static AttnPlan attn_plan(const zt_kv8_attn* a) {
@@ -817,9 +845,12 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
     long kv = std::min((long)a->max_kv, (long)a->width * a->cache.page_tokens);
     if (a->window > 0) kv = std::min(kv, (long)a->window + a->max_q + 63);
     const long tiles = std::max(1l, (kv + 63) / 64);
-    // a tile each as far as the bounds go, up to the waves that the card holds
+    // A tile each as far as the bounds go, up to a wave for each SIMD: each more makes parts to be joined (one sequence
+    // of 40011 tokens 31 us, with 2048 36; 64 of up to 8000 70 and 75).
     const long groups = (std::max(1l, std::min(most, 64l)) + 16 * p.ct - 1) / (16 * p.ct);
-    p.shares = (int)std::min(2048l, requests * heads * groups * (tiles + kBegin));
+    p.single = tiles <= 2;
+    p.shares = (int)std::min(1024l, requests * heads * groups * (p.single ? 1 : tiles + kBegin));
+    p.wide = p.shares > 16 * requests * heads * groups;  // more than 16 parts of a row
     p.others = 2l * p.shares * 16 * p.ct;
     p.many_n = std::max(1, std::min(a->max_q, a->tokens));
     p.few_n = std::max(1, std::min(p.many_n, 64 / group));
@@ -834,6 +865,7 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
     const long all = p.others + (p.many.splits > 1 ? (long)p.many.splits * a->tokens * a->q.heads : 0);
     p.stat = (all * 8 + 15) & ~15l;
     p.part = all * dp * 4;
+    p.parts = ((long)a->tokens * a->q.heads * 8 + 15) & ~15l;
     return p;
 }
 
@@ -857,23 +889,23 @@ static int launch(const Work& f, const AttnPlan& p, hipStream_t stream) {
     } else {
         attn_few_kernel<T, DN, 1><<<few, 256, lds, stream>>>(f);
     }
-    // rows that may be in parts: of each request up to so many tokens
-    const auto join = [&](int each, bool many, bool wide) {
-        const long rows = (long)f.a.requests * each * f.a.q.heads;
+    const auto join = [&](Join which, int each, bool wide) {
+        each = (int)std::min((long)each, std::max(1l, ((1l << 31) - 1) / (std::max(1l, (long)f.a.requests) * f.a.q.heads)));
+        const long rows = which == Join::ROWS ? (long)f.a.tokens * f.a.q.heads : (long)f.a.requests * each * f.a.q.heads;
         if (wide)
-            attn_join_kernel<T, DN, 8><<<(unsigned)rows, 512, 0, stream>>>(f, 16 * p.ct, each, many);
+            attn_join_kernel<T, DN, 8><<<(unsigned)rows, 512, 0, stream>>>(f, 16 * p.ct, each, which);
         else
-            attn_join_kernel<T, DN, 1><<<(unsigned)((rows + 7) / 8), 512, 0, stream>>>(f, 16 * p.ct, each, many);
+            attn_join_kernel<T, DN, 1><<<(unsigned)((rows + 7) / 8), 512, 0, stream>>>(f, 16 * p.ct, each, which);
     };
-    if (f.a.requests && p.shares > 1) join(p.few_n, false, (long)f.a.requests * f.a.c.heads * 8 < p.shares);
-    if (f.a.requests && p.many.splits > 1) join(p.many_n, true, p.many.splits > 8);
+    if (f.a.requests && !p.single) join(p.qtiles ? Join::FEW : Join::ROWS, p.few_n, p.wide);
+    if (f.a.requests && p.many.splits > 1) join(Join::MANY, p.many_n, p.many.splits > 8);
     return (int)hipGetLastError();
 }
 
 ZT_EXPORT long zt_kv8_attention_workspace_bytes(const zt_kv8_attn* a) {
     if (!attn_ok(a)) return -1;
     const AttnPlan p = attn_plan(a);
-    return p.part + p.stat;
+    return p.part + p.stat + p.parts;
 }
 
 ZT_EXPORT int zt_kv8_attention(const zt_kv8_attn* a, void* workspace, long workspace_bytes, zt_stream_t stream) {
@@ -884,11 +916,12 @@ ZT_EXPORT int zt_kv8_attention(const zt_kv8_attn* a, void* workspace, long works
         (((uintptr_t)a->table | (uintptr_t)a->kv_lens | (uintptr_t)a->q_start | (uintptr_t)a->scale) & 3))
         return kInvalid;
     const AttnPlan p = attn_plan(a);
-    if (p.part + p.stat > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.part + p.stat)) return kInvalid;
+    if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.part + p.stat + p.parts) return kInvalid;
     const AttnArgs g{kv8_of(a->cache), rows_of(a->q), rows_of(a->out), a->table, a->kv_lens, a->q_start, a->scale,
                      a->requests,      a->width,      a->tokens,       a->window, a->q.heads / a->cache.kv_heads};
-    const Work f{g,        p.most, p.shares, p.many, p.qtiles, rows_vector(a->q, 4, a->type) && rows_vector(a->out, 4, a->type),
-                 p.others, (float*)workspace, (float2*)((char*)workspace + p.part)};
+    const Work f{g,        p.most, p.shares, p.single, p.many, p.qtiles, rows_vector(a->q, 4, a->type) && rows_vector(a->out, 4, a->type),
+                 p.others, (float*)workspace, (float2*)((char*)workspace + p.part),
+                 (int2*)((char*)workspace + p.part + p.stat)};
     const bool f32 = a->type == ZT_F32;
     switch (g.c.dp) {
         case 64: return f32 ? launch<float, 1>(f, p, stream) : launch<_Float16, 1>(f, p, stream);
