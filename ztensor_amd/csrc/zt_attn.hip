@@ -159,7 +159,13 @@ __device__ __forceinline__ void load_query(const Work& f, const Span& sp, int kv
     }
     int e2 = 0;
     if (SPLIT) e2 = scale_exponent(max_step<16>(max_step<32>(m)));
-    factor = ldexpf(scale, -e2);
+    factor = ldexpf(fabsf(scale), -e2);
+    if (scale < 0.0f) {  // its sign goes to the query: a larger product is a larger score
+#pragma unroll
+        for (int d = 0; d < DN; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) v[d][e] = -v[d][e];
+    }
 #pragma unroll
     for (int d = 0; d < DN; d++)
 #pragma unroll
@@ -176,6 +182,90 @@ __device__ __forceinline__ void load_query(const Work& f, const Span& sp, int kv
         }
 }
 
+// The scale of a lane's values in a tile, over the power of two that their
+// weights are brought to: fp16 holds them up to 2^15.  The logarithm stops where
+// a weight is nothing in fp16 beside those of the largest scale; a scale that is
+// not a number stays that.
+constexpr int kWeightBits = 10;
+struct ValueScale {
+    float by, log, inverse;
+    int e;  // the tile's exponent, at least the one before
+    __device__ __forceinline__ ValueScale(float vs, int ev) {
+        const float most = max_step<16>(max_step<32>(finite(vs)));
+        e = max(ev, exponent_of(most));
+        by = ldexpf(vs, kWeightBits - e);
+        log = by <= 0x1p-60f ? -60.0f : __builtin_amdgcn_logf(by);
+        inverse = __builtin_amdgcn_exp2f(-log);
+    }
+};
+
+// The weights of a tile's 16 tokens in this lane for one row: scores s times fk
+// in units of log 2, against a base that follows their maximum only when it is
+// passed by more than 2^4 (most tiles move some row's maximum a little; so few
+// of them change sums that stand already).  keep: what sums against the base
+// before are to be multiplied by.  MASKED: of tokens t .. t + 15 those that are
+// `there` and in lo .. hi - 1.
+template <bool SPLIT, bool MASKED>
+__device__ __forceinline__ void weights_of(const float4v (&s)[4], float fk, const ValueScale& v, int t, bool there, int lo, int hi,
+                                           float& base, float& l, float& keep, half8v (&p)[2], half8v (&pl)[2]) {
+    float x[16], top = kNone;
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        x[k] = s[k >> 2][k & 3];
+        if (MASKED) x[k] = there && t + k >= lo && t + k < hi ? x[k] * fk : kNone;
+        top = fmaxf(top, x[k]);
+    }
+    if (!MASKED) top *= fk;  // (a scale is not negative)
+    top = max_step<16>(max_step<32>(top));
+    const float before = base;
+    if (top > base + 4.0f) base = top;  // (from nothing: to the first that is seen)
+    const float from = base == kNone ? 0.0f : base;
+    keep = __builtin_amdgcn_exp2f(before == kNone ? kNone : before - from);
+    float sum = 0.0f;
+    if constexpr (SPLIT || MASKED) {
+        float y[2][8];
+#pragma unroll
+        for (int k = 0; k < 16; k++) {
+            const float z = __builtin_amdgcn_exp2f(MASKED ? x[k] - from : __builtin_fmaf(x[k], fk, -from));
+            sum += z;
+            y[k >> 3][k & 7] = MASKED && x[k] == kNone ? 0.0f : z * v.by;  // (a page that nobody sees may have any scale)
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if constexpr (SPLIT) {
+                split_hi_lo(y[h], p[h], pl[h]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; k++) p[h][k] = (_Float16)y[h][k];
+            }
+        }
+    } else {
+        // the scale in the exponent, and the sum of the weights as they are rounded
+        const float at = v.log - from;
+        const half2v one = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+        for (int k = 0; k < 16; k += 2) {
+            const half2v w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[k], fk, at)),
+                              (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[k + 1], fk, at))};
+            sum = __builtin_amdgcn_fdot2(w, one, sum, false);
+            p[k >> 3][k & 7] = w[0];
+            p[k >> 3][(k & 7) + 1] = w[1];
+        }
+        sum *= v.inverse;
+    }
+    l = l * keep + sum;
+}
+
+// The page of a token, as the table has it (a load that nothing waits for until
+// the page is needed; past the length: of the last token), and whether there is
+// something to see there.
+struct Pages {
+    const int* row;
+    int len, shift;
+    __device__ __forceinline__ int operator()(int token) const { return len > 0 ? row[min(token, len - 1) >> shift] : -1; }
+    __device__ __forceinline__ bool seen(const Kv8& c, int page, int token) const { return token < len && c.holds(page); }
+};
+
 // What a lane holds of a row, dims 16 i + 4 (lane / 16) .. +4: the result, or
 // the sum that the other splits' are to be added to.
 template <class T, int DN>
@@ -185,7 +275,7 @@ __device__ __forceinline__ void store_row(const Work& f, const Span& sp, int kv,
     const AttnArgs& g = f.a;
     const int i = row / g.group, h = kv * g.group + row - i * g.group, quad = (threadIdx.x & 63) >> 4;
     const long t = sp.start + i;
-    const float by = ldexpf(part ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum, ev - 14);
+    const float by = ldexpf(part ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum, ev - kWeightBits);
     if (part && quad == 0) f.stat[at] = make_float2(top, sum);
     T* out = (T*)g.out.p + t * g.out.token + (long)h * g.out.head;
 #pragma unroll
@@ -240,7 +330,7 @@ __device__ __forceinline__ long wave_scan(long v) {
 // lane's queries lie in LDS for itself.
 //
 // Weights enter the second product times their page's scale over a power of two
-// (the largest so far, 2^(e - 14)): fp16 then holds 39 bits below the largest.
+// (the largest so far, 2^(e - 10)): fp16 then holds 35 bits below the largest.
 // fp32 rows: queries and weights in two fp16 parts (22 bits).
 template <class T, int DN, int CT>
 __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
@@ -325,12 +415,8 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
         pos += at1 - at0;
         if (n <= 0) continue;
         const int parts = f.single ? 1 : (int)((first_place + tiles - 1) / each) - share + 1;  // (of the first part's share)
-        const int* table = g.table + (long)r * g.width;
-        auto page_at = [&](int token) {  // -1: nothing to see there
-            const int p = token < sp.len ? table[token >> c.shift] : -1;
-            return c.holds(p) ? p : -1;
-        };
-        int pk = page_at(first * 64 + (col >> 2) * 16), pv = page_at(first * 64 + quad * 16);
+        const Pages page_of{g.table + (long)r * g.width, sp.len, c.shift};
+        int pk = page_of(first * 64 + (col >> 2) * 16), pv = page_of(first * 64 + quad * 16);
         half8v* mine_q = queries + wave * (CT * DN * 2 * PARTS * 64);
         float factor[CT];
         int lo[CT], hi[CT];
@@ -366,8 +452,9 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
             const int t0 = tile * 64;
             int qlane = lane;
             asm volatile("" : "+v"(qlane));  // the queries are read from LDS for each tile: held, they cost 16 to 64 registers
-            const int at = max(pv, 0);
-            const int8_t* kp = c.k + c.at(max(pk, 0), kv) + (long)((t0 + krow) & (c.page - 1)) * c.dp + 16 * quad;
+            const bool seen = page_of.seen(c, pv, t0 + 16 * quad);
+            const int at = seen ? pv : 0;
+            const int8_t* kp = c.k + c.at(page_of.seen(c, pk, t0 + (col >> 2) * 16) ? pk : 0, kv) + (long)((t0 + krow) & (c.page - 1)) * c.dp + 16 * quad;
             const int8_t* vp = c.v + c.at(at, kv) + (long)col * c.page + ((t0 + 16 * quad) & (c.page - 1));
             u32x4 kw[4][DN], vw[4 * DN];
 #pragma unroll
@@ -377,16 +464,12 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
             const float ks = c.k_scale[(long)at * c.heads + kv], vs = c.v_scale[(long)at * c.heads + kv];
 #pragma unroll
             for (int i = 0; i < 4 * DN; i++) vw[i] = *reinterpret_cast<const u32x4*>(vp + (long)16 * i * c.page);
-            const bool seen = pv >= 0;
             const bool whole = t0 + 64 <= all_hi && t0 >= all_lo && __all(seen);
             // the next tile's pages, while this one's codes are on their way
-            pk = page_at(t0 + 64 + (col >> 2) * 16);
-            pv = page_at(t0 + 64 + quad * 16);
+            pk = page_of(t0 + 64 + (col >> 2) * 16);
+            pv = page_of(t0 + 64 + quad * 16);
 
-            int e = max(ev, exponent_of(vs));
-            e = max(e, __shfl_xor(e, 16));
-            e = max(e, __shfl_xor(e, 32));
-            const float fv = ldexpf(vs, 14 - e);
+            const ValueScale scales(vs, ev);
 
             float4v s[CT][4];
 #pragma unroll
@@ -408,45 +491,21 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
                     }
 
             half8v p[CT][2], pl[CT][2];
+            float keep[CT];
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
-                const float fk = factor[ct] * ks;
-                float x[16], top = kNone;
+                if (whole)
+                    weights_of<SPLIT, false>(s[ct], factor[ct] * ks, scales, 0, true, 0, 0, m[ct], l[ct], keep[ct], p[ct], pl[ct]);
+                else
+                    weights_of<SPLIT, true>(s[ct], factor[ct] * ks, scales, t0 + 16 * quad, seen, lo[ct], hi[ct], m[ct], l[ct],
+                                            keep[ct], p[ct], pl[ct]);
+                if (scales.e != ev) keep[ct] = ldexpf(keep[ct], ev - scales.e);
+                if (__any(keep[ct] != 1.0f)) {
 #pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    x[k] = s[ct][k >> 2][k & 3] * fk;
-                    const int t = t0 + 16 * quad + k;
-                    if (!whole && !(seen && t >= lo[ct] && t < hi[ct])) x[k] = kNone;
-                    top = fmaxf(top, x[k]);
-                }
-                top = fmaxf(m[ct], max_step<16>(max_step<32>(top)));
-                const float base = top == kNone ? 0.0f : top;
-                const float keep = ldexpf(__builtin_amdgcn_exp2f(m[ct] - base), ev - e);
-                float sum = 0.0f;
-                float w[2][8];
-#pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    const float y = __builtin_amdgcn_exp2f(x[k] - base);
-                    sum += y;
-                    w[k >> 3][k & 7] = x[k] == kNone ? 0.0f : y * fv;  // (a page that nobody sees may have any scale)
-                }
-                l[ct] = l[ct] * __builtin_amdgcn_exp2f(m[ct] - base) + sum;
-                m[ct] = top;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    if constexpr (SPLIT) {
-                        split_hi_lo(w[h], p[ct][h], pl[ct][h]);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 8; k++) p[ct][h][k] = (_Float16)w[h][k];
-                    }
-                }
-                if (__any(keep != 1.0f)) {
-#pragma unroll
-                    for (int i = 0; i < 4 * DN; i++) o[ct][i] *= keep;
+                    for (int i = 0; i < 4 * DN; i++) o[ct][i] *= keep[ct];
                 }
             }
-            ev = e;
+            ev = scales.e;
 #pragma unroll
             for (int i = 0; i < 4 * DN; i++)
 #pragma unroll
@@ -519,12 +578,8 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
     const int rows = sp.n * g.group;
     if (sp.n <= 0 || rows <= f.most) return;
     const float scale = (g.scale ? *g.scale : 1.0f / sqrtf((float)c.dim)) * kLog2e;
-    const int* table = g.table + (long)r * g.width;
     const int krow = (col >> 2) * 16 + (col & 3);
-    auto page_at = [&](int token) {
-        const int p = token < sp.len ? table[token >> c.shift] : -1;
-        return c.holds(p) ? p : -1;
-    };
+    const Pages page_of{g.table + (long)r * g.width, sp.len, c.shift};
 
     // the later a row, the more tokens it sees: those first
     const int all = (rows + kRows<DN> - 1) / kRows<DN>;
@@ -561,8 +616,9 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
         bool seen;
         auto fetch = [&](int tile, int pk, int pv) {
             const int t0 = tile * 64;
-            const int p = max(pv, 0);
-            const int8_t* kp = c.k + c.at(max(pk, 0), kv) + (long)((t0 + krow + 4 * wave) & (c.page - 1)) * c.dp + 16 * quad;
+            seen = page_of.seen(c, pv, t0 + 16 * quad);
+            const int p = seen ? pv : 0;
+            const int8_t* kp = c.k + c.at(page_of.seen(c, pk, t0 + (col >> 2) * 16) ? pk : 0, kv) + (long)((t0 + krow + 4 * wave) & (c.page - 1)) * c.dp + 16 * quad;
             const int8_t* vp = c.v + c.at(p, kv) + (long)(16 * DN * wave + col) * c.page + ((t0 + 16 * quad) & (c.page - 1));
 #pragma unroll
             for (int d = 0; d < DN; d++) {
@@ -571,7 +627,6 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
             }
             ks = c.k_scale[(long)p * c.heads + kv];
             vs = c.v_scale[(long)p * c.heads + kv];
-            seen = pv >= 0;
         };
         auto put = [&](int buffer) {
             half8v* to = tiles + buffer * FRAGS * 64 + lane;
@@ -583,12 +638,12 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
                     to[(8 * DN + (wave * DN + d) * 2 + h) * 64] = codes8(vw[d][2 * h], vw[d][2 * h + 1]);
                 }
         };
-        int pk = page_at(first * 64 + (col >> 2) * 16), pv = page_at(first * 64 + quad * 16);
+        int pk = page_of(first * 64 + (col >> 2) * 16), pv = page_of(first * 64 + quad * 16);
         __syncthreads();  // nobody reads the buffers of the rows before any more
         if (first < last) {
             fetch(first, pk, pv);
-            pk = page_at(first * 64 + 64 + (col >> 2) * 16);
-            pv = page_at(first * 64 + 64 + quad * 16);
+            pk = page_of(first * 64 + 64 + (col >> 2) * 16);
+            pv = page_of(first * 64 + 64 + quad * 16);
             put(0);
         }
         __syncthreads();
@@ -599,15 +654,12 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
             const bool whole = t0 + 64 <= all_hi && t0 >= all_lo && __all(there);
             if (tile + 1 < last) {
                 fetch(tile + 1, pk, pv);
-                pk = page_at(t0 + 128 + (col >> 2) * 16);
-                pv = page_at(t0 + 128 + quad * 16);
+                pk = page_of(t0 + 128 + (col >> 2) * 16);
+                pv = page_of(t0 + 128 + quad * 16);
             }
             const half8v* from = tiles + buffer * FRAGS * 64 + lane;
 
-            int e = max(ev, exponent_of(fvs));
-            e = max(e, __shfl_xor(e, 16));
-            e = max(e, __shfl_xor(e, 32));
-            const float fv = ldexpf(fvs, 14 - e);
+            const ValueScale scales(fvs, ev);
 
             float4v s[CT][4];
 #pragma unroll
@@ -627,54 +679,21 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
                     }
             }
             half8v p[CT][2], pl[CT][2];
+            float keep[CT];
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
-                const float fk = factor[ct] * fs;
-                float x[16], top = kNone;
+                if (whole)
+                    weights_of<SPLIT, false>(s[ct], factor[ct] * fs, scales, 0, true, 0, 0, m[ct], l[ct], keep[ct], p[ct], pl[ct]);
+                else
+                    weights_of<SPLIT, true>(s[ct], factor[ct] * fs, scales, t0 + 16 * quad, there, lo[ct], hi[ct], m[ct], l[ct],
+                                            keep[ct], p[ct], pl[ct]);
+                if (scales.e != ev) keep[ct] = ldexpf(keep[ct], ev - scales.e);
+                if (__any(keep[ct] != 1.0f)) {
 #pragma unroll
-                for (int k = 0; k < 16; k++) x[k] = s[ct][k >> 2][k & 3] * fk;
-                if (!whole) {
-#pragma unroll
-                    for (int k = 0; k < 16; k++) {
-                        const int t = t0 + 16 * quad + k;
-                        if (!(there && t >= lo[ct] && t < hi[ct])) x[k] = kNone;
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < 16; k++) top = fmaxf(top, x[k]);
-                top = fmaxf(m[ct], max_step<16>(max_step<32>(top)));
-                const float base = top == kNone ? 0.0f : top;
-                const float old = __builtin_amdgcn_exp2f(m[ct] - base), keep = ldexpf(old, ev - e);
-                float sum = 0.0f;
-                float y[2][8];
-#pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    const float z = __builtin_amdgcn_exp2f(x[k] - base);
-                    sum += z;
-                    y[k >> 3][k & 7] = z * fv;
-                }
-                if (!whole) {  // (a page that a row does not see may have any scale)
-#pragma unroll
-                    for (int k = 0; k < 16; k++)
-                        if (x[k] == kNone) y[k >> 3][k & 7] = 0.0f;
-                }
-                l[ct] = l[ct] * old + sum;
-                m[ct] = top;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    if constexpr (SPLIT) {
-                        split_hi_lo(y[h], p[ct][h], pl[ct][h]);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 8; k++) p[ct][h][k] = (_Float16)y[h][k];
-                    }
-                }
-                if (__any(keep != 1.0f)) {
-#pragma unroll
-                    for (int i = 0; i < 4 * DN; i++) o[ct][i] *= keep;
+                    for (int i = 0; i < 4 * DN; i++) o[ct][i] *= keep[ct];
                 }
             }
-            ev = e;
+            ev = scales.e;
 #pragma unroll
             for (int i = 0; i < 4 * DN; i++)
 #pragma unroll
