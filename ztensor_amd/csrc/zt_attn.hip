@@ -652,31 +652,39 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
             const float fs = ks, fvs = vs;
             const bool there = seen;
             const bool whole = t0 + 64 <= all_hi && t0 >= all_lo && __all(there);
-            if (tile + 1 < last) {
-                fetch(tile + 1, pk, pv);
-                pk = page_of(t0 + 128 + (col >> 2) * 16);
-                pv = page_of(t0 + 128 + quad * 16);
-            }
+            // (past the last tile: of the last token's page, for nobody)
+            fetch(tile + 1, pk, pv);
+            pk = page_of(t0 + 128 + (col >> 2) * 16);
+            pv = page_of(t0 + 128 + quad * 16);
             const half8v* from = tiles + buffer * FRAGS * 64 + lane;
 
             const ValueScale scales(fvs, ev);
 
+            // four fragments ahead of the products that take them
+            half8v frag[2][2 * DN];
+            auto read = [&](int to, int at) {
+#pragma unroll
+                for (int k = 0; k < 2 * DN; k++) frag[to][k] = from[(at * 2 * DN + k) * 64];
+            };
             float4v s[CT][4];
+            read(0, 0);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
+                read((j + 1) & 1, j + 1);  // (after the last keys: the first values)
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++) s[ct][j] = (float4v){0, 0, 0, 0};
 #pragma unroll
                 for (int d = 0; d < DN; d++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        const half8v k8 = from[((j * DN + d) * 2 + h) * 64];
 #pragma unroll
                         for (int ct = 0; ct < CT; ct++) {
-                            s[ct][j] = mfma(k8, q[ct][d][h], s[ct][j]);
-                            if constexpr (SPLIT) s[ct][j] = mfma(k8, ql[ct][d][h], s[ct][j]);
+                            s[ct][j] = mfma(frag[j & 1][2 * d + h], q[ct][d][h], s[ct][j]);
+                            if constexpr (SPLIT) s[ct][j] = mfma(frag[j & 1][2 * d + h], ql[ct][d][h], s[ct][j]);
                         }
                     }
+                __builtin_amdgcn_sched_group_barrier(0x100, 2 * DN, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 2 * DN * CT * (SPLIT ? 2 : 1), 0);
             }
             half8v p[CT][2], pl[CT][2];
             float keep[CT];
@@ -694,18 +702,20 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
                 }
             }
             ev = scales.e;
+            put(buffer ^ 1);
 #pragma unroll
-            for (int i = 0; i < 4 * DN; i++)
+            for (int j = 0; j < 4; j++) {
+                if (j < 3) read((j + 1) & 1, 5 + j);
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const half8v v8 = from[(8 * DN + 2 * i + h) * 64];
+                for (int k = 0; k < 2 * DN; k++) {
+                    const int i = j * DN + k / 2;
 #pragma unroll
                     for (int ct = 0; ct < CT; ct++) {
-                        o[ct][i] = mfma(v8, p[ct][h], o[ct][i]);
-                        if constexpr (SPLIT) o[ct][i] = mfma(v8, pl[ct][h], o[ct][i]);
+                        o[ct][i] = mfma(frag[j & 1][k], p[ct][k & 1], o[ct][i]);
+                        if constexpr (SPLIT) o[ct][i] = mfma(frag[j & 1][k], pl[ct][k & 1], o[ct][i]);
                     }
                 }
-            if (tile + 1 < last) put(buffer ^ 1);
+            }
             __syncthreads();
         }
 
