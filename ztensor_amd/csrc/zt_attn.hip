@@ -138,16 +138,15 @@ __device__ __forceinline__ int splits_of(const Split& f, int tiles) {
 // Row `row` of a request and key/value head as this lane's operands: dims 64 d
 // + 16 (lane / 16) .. +16 of each d, fp32 rows in two parts after a power of
 // two; factor: what a product of it is to be multiplied by for a score in
-// units of log 2; the tokens lo .. hi - 1 that it sees (hi 0: no such row).
+// units of log 2; hi: it sees tokens before that (0: no such row).
 template <class T, int DN>
 __device__ __forceinline__ void load_query(const Work& f, const Span& sp, int kv, int row, int rows, float scale,
-                                           half8v (&q)[DN][2], half8v (&ql)[DN][2], float& factor, int& lo, int& hi) {
+                                           half8v (&q)[DN][2], half8v (&ql)[DN][2], float& factor, int& hi) {
     constexpr bool SPLIT = sizeof(T) == 4;
     const AttnArgs& g = f.a;
     const int i = row / g.group, h = kv * g.group + row - i * g.group, quad = (threadIdx.x & 63) >> 4;
     const bool there = row < rows;
     hi = there ? sp.len - sp.n + i + 1 : 0;
-    lo = g.window > 0 ? max(0, hi - g.window) : 0;
     const T* x = there ? (const T*)g.q.p + (long)(sp.start + i) * g.q.token + (long)h * g.q.head : nullptr;
     float v[DN][16];
     float m = 0.0f;
@@ -192,52 +191,61 @@ struct ValueScale {
     int e;  // the tile's exponent, at least the one before
     __device__ __forceinline__ ValueScale(float vs, int ev) {
         const float most = max_step<16>(max_step<32>(finite(vs)));
-        e = max(ev, exponent_of(most));
+        e = max(ev, __builtin_amdgcn_readfirstlane(exponent_of(most)));
         by = ldexpf(vs, kWeightBits - e);
         log = by <= 0x1p-60f ? -60.0f : __builtin_amdgcn_logf(by);
         inverse = __builtin_amdgcn_exp2f(-log);
     }
 };
 
+// Of a tile's 16 tokens in this lane, t on, what a row does not see: tokens that
+// are not `there`, before lo or from hi on.  Their scores become -inf; of a lane
+// in which it sees none the scales may be anything, and are set aside.
+__device__ __forceinline__ void mask_scores(float4v (&s)[4], float& fk, ValueScale& v, int t, bool there, int lo, int hi) {
+    if (!there || max(t, lo) >= min(t + 16, hi)) {
+        fk = v.by = v.inverse = 1.0f;
+        v.log = 0.0f;
+        hi = 0;
+    }
+#pragma unroll
+    for (int k = 0; k < 16; k++)
+        if (t + k < lo || t + k >= hi) s[k >> 2][k & 3] = kNone;
+}
+
 // The weights of a tile's 16 tokens in this lane for one row: scores s times fk
 // in units of log 2, against a base that follows their maximum only when it is
 // passed by more than 2^4 (most tiles move some row's maximum a little; so few
-// of them change sums that stand already).  keep: what sums against the base
-// before are to be multiplied by.  MASKED: of tokens t .. t + 15 those that are
-// `there` and in lo .. hi - 1.
-template <bool SPLIT, bool MASKED>
-__device__ __forceinline__ void weights_of(const float4v (&s)[4], float fk, const ValueScale& v, int t, bool there, int lo, int hi,
-                                           float& base, float& l, float& keep, half8v (&p)[2], half8v (&pl)[2]) {
-    float x[16], top = kNone;
+// of them change l and o, which stand already).  Scales of keys and values are
+// not negative; fk of 0 counts as what no score survives, so that -inf stays.
+template <bool SPLIT, int N>
+__device__ __forceinline__ void weights_of(const float4v (&s)[4], float fk, const ValueScale& v, float& base, float& l,
+                                           float4v (&o)[N], half8v (&p)[2], half8v (&pl)[2]) {
+    fk = fk < 1e-37f ? 1e-37f : fk;  // (not a number: stays that)
+    float top = kNone;
 #pragma unroll
-    for (int k = 0; k < 16; k++) {
-        x[k] = s[k >> 2][k & 3];
-        if (MASKED) x[k] = there && t + k >= lo && t + k < hi ? x[k] * fk : kNone;
-        top = fmaxf(top, x[k]);
+    for (int k = 0; k < 16; k++) top = fmaxf(top, s[k >> 2][k & 3]);
+    top = max_step<16>(max_step<32>(top * fk));
+    if (__any(top > base + 4.0f)) {  // (from nothing: to the first that is seen)
+        const bool up = top > base + 4.0f;
+        const float keep = up ? __builtin_amdgcn_exp2f(base - top) : 1.0f;
+        base = up ? top : base;
+        l *= keep;
+#pragma unroll
+        for (int i = 0; i < N; i++) o[i] *= keep;
     }
-    if (!MASKED) top *= fk;  // (a scale is not negative)
-    top = max_step<16>(max_step<32>(top));
-    const float before = base;
-    if (top > base + 4.0f) base = top;  // (from nothing: to the first that is seen)
     const float from = base == kNone ? 0.0f : base;
-    keep = __builtin_amdgcn_exp2f(before == kNone ? kNone : before - from);
     float sum = 0.0f;
-    if constexpr (SPLIT || MASKED) {
-        float y[2][8];
-#pragma unroll
-        for (int k = 0; k < 16; k++) {
-            const float z = __builtin_amdgcn_exp2f(MASKED ? x[k] - from : __builtin_fmaf(x[k], fk, -from));
-            sum += z;
-            y[k >> 3][k & 7] = MASKED && x[k] == kNone ? 0.0f : z * v.by;  // (a page that nobody sees may have any scale)
-        }
+    if constexpr (SPLIT) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            if constexpr (SPLIT) {
-                split_hi_lo(y[h], p[h], pl[h]);
-            } else {
+            float y[8];
 #pragma unroll
-                for (int k = 0; k < 8; k++) p[h][k] = (_Float16)y[h][k];
+            for (int k = 0; k < 8; k++) {
+                const float z = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * h + (k >> 2)][k & 3], fk, -from));
+                sum += z;
+                y[k] = z * v.by;
             }
+            split_hi_lo(y, p[h], pl[h]);
         }
     } else {
         // the scale in the exponent, and the sum of the weights as they are rounded
@@ -245,15 +253,15 @@ __device__ __forceinline__ void weights_of(const float4v (&s)[4], float fk, cons
         const half2v one = {(_Float16)1.0f, (_Float16)1.0f};
 #pragma unroll
         for (int k = 0; k < 16; k += 2) {
-            const half2v w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[k], fk, at)),
-                              (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[k + 1], fk, at))};
+            const half2v w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 2][k & 3], fk, at)),
+                              (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 2][(k & 3) + 1], fk, at))};
             sum = __builtin_amdgcn_fdot2(w, one, sum, false);
             p[k >> 3][k & 7] = w[0];
             p[k >> 3][(k & 7) + 1] = w[1];
         }
         sum *= v.inverse;
     }
-    l = l * keep + sum;
+    l += sum;
 }
 
 // The page of a token, as the table has it (a load that nothing waits for until
@@ -419,11 +427,11 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
         int pk = page_of(first * 64 + (col >> 2) * 16), pv = page_of(first * 64 + quad * 16);
         half8v* mine_q = queries + wave * (CT * DN * 2 * PARTS * 64);
         float factor[CT];
-        int lo[CT], hi[CT];
+        int hi[CT];
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             half8v q[DN][2], ql[DN][2];
-            load_query<T, DN>(f, sp, kv, (cg * CT + ct) * 16 + col, rows, scale, q, ql, factor[ct], lo[ct], hi[ct]);
+            load_query<T, DN>(f, sp, kv, (cg * CT + ct) * 16 + col, rows, scale, q, ql, factor[ct], hi[ct]);
 #pragma unroll
             for (int d = 0; d < DN; d++)
 #pragma unroll
@@ -491,19 +499,18 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
                     }
 
             half8v p[CT][2], pl[CT][2];
-            float keep[CT];
+            if (scales.e != ev) {  // a larger scale of values than any before
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                    for (int i = 0; i < 4 * DN; i++) o[ct][i] *= ldexpf(1.0f, ev - scales.e);
+            }
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
-                if (whole)
-                    weights_of<SPLIT, false>(s[ct], factor[ct] * ks, scales, 0, true, 0, 0, m[ct], l[ct], keep[ct], p[ct], pl[ct]);
-                else
-                    weights_of<SPLIT, true>(s[ct], factor[ct] * ks, scales, t0 + 16 * quad, seen, lo[ct], hi[ct], m[ct], l[ct],
-                                            keep[ct], p[ct], pl[ct]);
-                if (scales.e != ev) keep[ct] = ldexpf(keep[ct], ev - scales.e);
-                if (__any(keep[ct] != 1.0f)) {
-#pragma unroll
-                    for (int i = 0; i < 4 * DN; i++) o[ct][i] *= keep[ct];
-                }
+                float fk = factor[ct] * ks;
+                ValueScale v = scales;
+                if (!whole) mask_scores(s[ct], fk, v, t0 + 16 * quad, seen, g.window > 0 ? hi[ct] - g.window : 0, hi[ct]);
+                weights_of<SPLIT>(s[ct], fk, v, m[ct], l[ct], o[ct], p[ct], pl[ct]);
             }
             ev = scales.e;
 #pragma unroll
@@ -569,7 +576,8 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
     extern __shared__ __align__(16) half8v tiles[];  // [2][FRAGS][64]
     const AttnArgs& g = f.a;
     const Kv8& c = g.c;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
+    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int b = blockIdx.x;
     const int kv = b % c.heads;
     b /= c.heads;
@@ -591,11 +599,11 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
 
         half8v q[CT][DN][2], ql[CT][DN][2];
         float factor[CT];
-        int lo[CT], hi[CT];
+        int hi[CT];
         const int row0 = w.row0 + wave * 16 * CT, row1 = min(rows, row0 + 16 * CT) - 1;
 #pragma unroll
         for (int ct = 0; ct < CT; ct++)
-            load_query<T, DN>(f, sp, kv, row0 + 16 * ct + col, rows, scale, q[ct], ql[ct], factor[ct], lo[ct], hi[ct]);
+            load_query<T, DN>(f, sp, kv, row0 + 16 * ct + col, rows, scale, q[ct], ql[ct], factor[ct], hi[ct]);
         const int all_hi = sp.len - sp.n + row0 / g.group + 1;
         const int all_lo = g.window > 0 ? max(0, sp.len - sp.n + row1 / g.group + 1 - g.window) : 0;
 
@@ -614,19 +622,24 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
         u32x4 kw[DN], vw[DN];
         float ks, vs;
         bool seen;
+        // (a tile begins at a multiple of 64: what a lane adds to that stays in the page, or is taken modulo its tokens)
+        const uint32_t page_bytes = (uint32_t)(c.heads * c.bytes()), head_bytes = (uint32_t)(kv * c.bytes());
+        const uint32_t k_lane = ((krow + 4 * wave) & (c.page - 1)) * c.dp + 16 * quad + head_bytes;
+        const uint32_t v_lane = (16 * DN * wave + col) * c.page + ((16 * quad) & (c.page - 1)) + head_bytes;
         auto fetch = [&](int tile, int pk, int pv) {
-            const int t0 = tile * 64;
+            const int t0 = tile * 64, in = t0 & (c.page - 1);
             seen = page_of.seen(c, pv, t0 + 16 * quad);
-            const int p = seen ? pv : 0;
-            const int8_t* kp = c.k + c.at(page_of.seen(c, pk, t0 + (col >> 2) * 16) ? pk : 0, kv) + (long)((t0 + krow + 4 * wave) & (c.page - 1)) * c.dp + 16 * quad;
-            const int8_t* vp = c.v + c.at(p, kv) + (long)(16 * DN * wave + col) * c.page + ((t0 + 16 * quad) & (c.page - 1));
+            const uint32_t p = seen ? pv : 0, q = page_of.seen(c, pk, t0 + (col >> 2) * 16) ? pk : 0;
+            const int8_t* kp = c.k + ((uint64_t)q * page_bytes + (k_lane + in * c.dp));
+            const int8_t* vp = c.v + ((uint64_t)p * page_bytes + (v_lane + in));
 #pragma unroll
             for (int d = 0; d < DN; d++) {
                 kw[d] = *reinterpret_cast<const u32x4*>(kp + 64 * d);
-                vw[d] = *reinterpret_cast<const u32x4*>(vp + (long)16 * d * c.page);
+                vw[d] = *reinterpret_cast<const u32x4*>(vp + 16 * d * c.page);
             }
-            ks = c.k_scale[(long)p * c.heads + kv];
-            vs = c.v_scale[(long)p * c.heads + kv];
+            const uint32_t at = p * c.heads + kv;
+            ks = c.k_scale[at];
+            vs = c.v_scale[at];
         };
         auto put = [&](int buffer) {
             half8v* to = tiles + buffer * FRAGS * 64 + lane;
@@ -687,19 +700,18 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 2 * DN * CT * (SPLIT ? 2 : 1), 0);
             }
             half8v p[CT][2], pl[CT][2];
-            float keep[CT];
+            if (scales.e != ev) {  // a larger scale of values than any before
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                    for (int i = 0; i < 4 * DN; i++) o[ct][i] *= ldexpf(1.0f, ev - scales.e);
+            }
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
-                if (whole)
-                    weights_of<SPLIT, false>(s[ct], factor[ct] * fs, scales, 0, true, 0, 0, m[ct], l[ct], keep[ct], p[ct], pl[ct]);
-                else
-                    weights_of<SPLIT, true>(s[ct], factor[ct] * fs, scales, t0 + 16 * quad, there, lo[ct], hi[ct], m[ct], l[ct],
-                                            keep[ct], p[ct], pl[ct]);
-                if (scales.e != ev) keep[ct] = ldexpf(keep[ct], ev - scales.e);
-                if (__any(keep[ct] != 1.0f)) {
-#pragma unroll
-                    for (int i = 0; i < 4 * DN; i++) o[ct][i] *= keep[ct];
-                }
+                float fk = factor[ct] * fs;
+                ValueScale v = scales;
+                if (!whole) mask_scores(s[ct], fk, v, t0 + 16 * quad, there, g.window > 0 ? hi[ct] - g.window : 0, hi[ct]);
+                weights_of<SPLIT>(s[ct], fk, v, m[ct], l[ct], o[ct], p[ct], pl[ct]);
             }
             ev = scales.e;
             put(buffer ^ 1);

@@ -29,7 +29,7 @@ __host__ inline bool kv8_ok(const zt_kv8_cache& c) {
     return c.k && c.v && c.k_scale && c.v_scale && ((uintptr_t)c.k & 15) == 0 && ((uintptr_t)c.v & 15) == 0 &&
            c.pages >= 0 && c.kv_heads >= 1 && c.head_dim >= 8 && c.head_dim <= 256 && c.head_dim % 8 == 0 &&
            page_tokens_ok(c.page_tokens) && (long)c.pages * c.page_tokens < (1l << 31) &&
-           (long)c.pages * c.kv_heads < (1l << 31);
+           (long)c.pages * c.kv_heads < (1l << 31) && c.kv_heads <= 1 << 16;  // (a page of all heads: under 2 GiB)
 }
 
 __host__ inline Kv8 kv8_of(const zt_kv8_cache& c) {
