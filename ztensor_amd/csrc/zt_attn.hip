@@ -581,7 +581,9 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
     int b = blockIdx.x;
     const int kv = b % c.heads;
     b /= c.heads;
-    const int split = b % f.many.splits, at = b / f.many.splits, r = blockIdx.y;
+    const int split = b % f.many.splits;
+    b /= f.many.splits;
+    const int r = b % g.requests, at = b / g.requests;  // (the longest rows of all requests first)
     const Span sp = span_of(g, r);
     const int rows = sp.n * g.group;
     if (sp.n <= 0 || rows <= f.most) return;
@@ -755,6 +757,7 @@ template <class T, int DN, int W>
 __global__ __launch_bounds__(512) void attn_join_kernel(Work f, int rows_of_group, int each_n, Join which) {
     constexpr int G = W == 1 ? 4 / DN : 32 / DN;  // groups of 16 DN lanes
     constexpr int LANES = W == 1 ? 64 : 512, SETS = 512 / LANES;
+    constexpr int LOADS = W == 1 ? 2 : 8;  // parts on their way at a time: where rows are many, waves do that
     __shared__ float4 part[SETS][G][16 * DN];
     __shared__ float2 stats[SETS][G];
     const AttnArgs& g = f.a;
@@ -787,11 +790,11 @@ __global__ __launch_bounds__(512) void attn_join_kernel(Work f, int rows_of_grou
         float top = kNone, l = 0.0f;
         float4 sum = make_float4(0, 0, 0, 0);
         if (group < G) {
-            for (int s = group; s < ns; s += 8 * G) {  // 8 parts' loads at a time
-                float2 st[8];
-                float4 x[8];
+            for (int s = group; s < ns; s += LOADS * G) {
+                float2 st[LOADS];
+                float4 x[LOADS];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
+                for (int e = 0; e < LOADS; e++) {
                     const int k = s + e * G;
                     const long place = k ? at + (long)(k - 1) * step : at0;
                     st[e] = make_float2(kNone, 0.0f);
@@ -803,7 +806,7 @@ __global__ __launch_bounds__(512) void attn_join_kernel(Work f, int rows_of_grou
                 }
                 float m = top;
 #pragma unroll
-                for (int e = 0; e < 8; e++) m = fmaxf(m, st[e].x);
+                for (int e = 0; e < LOADS; e++) m = fmaxf(m, st[e].x);
                 const float base = m == kNone ? 0.0f : m, old = __builtin_amdgcn_exp2f(top - base);
                 top = m;
                 l *= old;
@@ -812,7 +815,7 @@ __global__ __launch_bounds__(512) void attn_join_kernel(Work f, int rows_of_grou
                 sum.z *= old;
                 sum.w *= old;
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
+                for (int e = 0; e < LOADS; e++) {
                     const float w = __builtin_amdgcn_exp2f(st[e].x - base);
                     l += st[e].y * w;
                     sum.x += x[e].x * w;
@@ -898,8 +901,10 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
     p.many = {1, 1};
     if (most > 64) {
         p.qtiles = ceil_div(most, dp <= 128 ? 128 : 64);
-        // along the tokens until about 512 workgroups are there, none of less than 4 tiles
-        const long have = requests * heads * p.qtiles, splits = std::max(1l, std::min((512 + have - 1) / have, tiles / 4));
+        // along the tokens while the card's 512 workgroups are not there, none of less than 4 tiles; of a prompt from its
+        // beginning half of the rows see half of the tokens, and half of them are not split
+        const long have = requests * heads * p.qtiles, want = kv >= 2l * a->max_q ? 512 : 768;
+        const long splits = std::max(1l, std::min(want / have, tiles / 4));
         p.many.tiles = (int)((tiles + splits - 1) / splits);
         p.many.splits = (int)((tiles + p.many.tiles - 1) / p.many.tiles);
     }
@@ -912,8 +917,8 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
 
 template <class T, int DN>
 static int launch(const Work& f, const AttnPlan& p, hipStream_t stream) {
-    const long many = (long)p.qtiles * p.many.splits * f.a.c.heads;
-    if (many >= 1l << 31 || (p.qtiles && f.a.requests > 65535)) return kInvalid;
+    const long many = (long)p.qtiles * p.many.splits * f.a.c.heads * f.a.requests;
+    if (many >= 1l << 31) return kInvalid;
     if (p.qtiles && f.a.requests) {
         static std::atomic<uint64_t> raised{0};
         constexpr int lds = 2 * 16 * DN * 1024;
@@ -921,7 +926,7 @@ static int launch(const Work& f, const AttnPlan& p, hipStream_t stream) {
             const hipError_t rc = raise_lds((const void*)attn_many_kernel<T, DN>, lds, raised);
             if (rc != hipSuccess) return (int)rc;
         }
-        attn_many_kernel<T, DN><<<dim3((unsigned)many, f.a.requests), 256, lds, stream>>>(f);
+        attn_many_kernel<T, DN><<<(unsigned)many, 256, lds, stream>>>(f);
     }
     const int few = (f.shares + 3) / 4 + f.a.c.heads;
     constexpr int lds = DN * 2 * (sizeof(T) / 2) * 4096;  // of a column tile, at most 64 KB in all
@@ -939,7 +944,7 @@ static int launch(const Work& f, const AttnPlan& p, hipStream_t stream) {
             attn_join_kernel<T, DN, 1><<<(unsigned)((rows + 7) / 8), 512, 0, stream>>>(f, 16 * p.ct, each, which);
     };
     if (f.a.requests && !p.single) join(p.qtiles ? Join::FEW : Join::ROWS, p.few_n, p.wide);
-    if (f.a.requests && p.many.splits > 1) join(Join::MANY, p.many_n, p.many.splits > 8);
+    if (f.a.requests && p.many.splits > 1) join(Join::MANY, p.many_n, false);
     return (int)hipGetLastError();
 }
 
