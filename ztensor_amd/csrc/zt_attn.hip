@@ -675,32 +675,40 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
 
             const ValueScale scales(fvs, ev);
 
-            // four fragments ahead of the products that take them
-            half8v frag[2][2 * DN];
-            auto read = [&](int to, int at) {
+            // four fragments ahead of the products that take them, sums that depend on each other 8 products apart
+            half8v frag[2][4];
+            auto keys = [&](int to, int k) {
 #pragma unroll
-                for (int k = 0; k < 2 * DN; k++) frag[to][k] = from[(at * 2 * DN + k) * 64];
+                for (int j = 0; j < 4; j++) frag[to][j] = from[(j * 2 * DN + k) * 64];
             };
+            auto values = [&](int to, int at) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) frag[to][k] = from[(8 * DN + 4 * at + k) * 64];
+            };
+            __builtin_amdgcn_s_setprio(1);  // the other workgroup's wave has the vector unit meanwhile
             float4v s[CT][4];
-            read(0, 0);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                read((j + 1) & 1, j + 1);  // (after the last keys: the first values)
+            for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++) s[ct][j] = (float4v){0, 0, 0, 0};
+                for (int j = 0; j < 4; j++) s[ct][j] = (float4v){0, 0, 0, 0};
+            keys(0, 0);
 #pragma unroll
-                for (int d = 0; d < DN; d++)
+            for (int k = 0; k < 2 * DN; k++) {
+                if (k + 1 < 2 * DN) keys((k + 1) & 1, k + 1); else values((k + 1) & 1, 0);
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
+                for (int j = 0; j < 4; j++)
 #pragma unroll
-                        for (int ct = 0; ct < CT; ct++) {
-                            s[ct][j] = mfma(frag[j & 1][2 * d + h], q[ct][d][h], s[ct][j]);
-                            if constexpr (SPLIT) s[ct][j] = mfma(frag[j & 1][2 * d + h], ql[ct][d][h], s[ct][j]);
-                        }
-                    }
-                __builtin_amdgcn_sched_group_barrier(0x100, 2 * DN, 0);
-                __builtin_amdgcn_sched_group_barrier(0x008, 2 * DN * CT * (SPLIT ? 2 : 1), 0);
+                    for (int ct = 0; ct < CT; ct++) s[ct][j] = mfma(frag[k & 1][j], q[ct][k >> 1][k & 1], s[ct][j]);
+                if constexpr (SPLIT) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int ct = 0; ct < CT; ct++) s[ct][j] = mfma(frag[k & 1][j], ql[ct][k >> 1][k & 1], s[ct][j]);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 4 * CT * (SPLIT ? 2 : 1), 0);
             }
+            __builtin_amdgcn_s_setprio(0);
             half8v p[CT][2], pl[CT][2];
             if (scales.e != ev) {  // a larger scale of values than any before
 #pragma unroll
@@ -718,15 +726,21 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
             ev = scales.e;
             put(buffer ^ 1);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (j < 3) read((j + 1) & 1, 5 + j);
+            for (int j = 0; j < 2 * DN; j++) {
+                if (j + 1 < 2 * DN) values((j + 1) & 1, j + 1);
 #pragma unroll
-                for (int k = 0; k < 2 * DN; k++) {
-                    const int i = j * DN + k / 2;
+                for (int h = 0; h < 2; h++) {
 #pragma unroll
-                    for (int ct = 0; ct < CT; ct++) {
-                        o[ct][i] = mfma(frag[j & 1][k], p[ct][k & 1], o[ct][i]);
-                        if constexpr (SPLIT) o[ct][i] = mfma(frag[j & 1][k], pl[ct][k & 1], o[ct][i]);
+                    for (int e = 0; e < 2; e++)
+#pragma unroll
+                        for (int ct = 0; ct < CT; ct++)
+                            o[ct][2 * j + e] = mfma(frag[j & 1][2 * e + h], p[ct][h], o[ct][2 * j + e]);
+                    if constexpr (SPLIT) {
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+#pragma unroll
+                            for (int ct = 0; ct < CT; ct++)
+                                o[ct][2 * j + e] = mfma(frag[j & 1][2 * e + h], pl[ct][h], o[ct][2 * j + e]);
                     }
                 }
             }
