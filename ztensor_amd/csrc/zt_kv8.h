@@ -18,7 +18,7 @@ struct Kv8 {
     int pages, heads, dim, dp;  // dp: dim to the next multiple of 64
     int page, shift;            // page tokens, their logarithm
     // bytes of one page and head, of keys and of values alike
-    __device__ __forceinline__ int bytes() const { return page * dp; }
+    __host__ __device__ __forceinline__ int bytes() const { return page * dp; }
     __device__ __forceinline__ long at(int p, int h) const { return ((long)p * heads + h) * bytes(); }
     __device__ __forceinline__ bool holds(int p) const { return (unsigned)p < (unsigned)pages; }
 };

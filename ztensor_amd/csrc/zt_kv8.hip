@@ -126,7 +126,7 @@ struct AppendArgs {
     const long* slots;
     Turn turn;  // half == 0: keys as they are
     int tokens;
-    int window;  // tokens whose pages a workgroup looks after, for one head of keys or of values
+    int turns;  // workgroups that the pages which 64 tokens begin are dealt out to, for one head of keys or of values
     long blocks;
 };
 
@@ -237,24 +237,34 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, int t, int n, i
     __syncthreads();  // the image is free again
 }
 
-template <class T, int V>
+// A workgroup looks at 64 tokens: those that do not go on from the one before,
+// in its page, begin a page's tokens.  It takes every turns-th of them.
+template <class T, int V, int VQ>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, RopeArgs q) {
-    __shared__ __align__(16) uint32_t image[128 * 256 / 4];
+    extern __shared__ __align__(16) uint32_t image[];  // of one page and head
     __shared__ float red[4];
     __shared__ int count;
     if (blockIdx.x >= g.blocks) {
-        rope_block<T, V>(q, blockIdx.x - g.blocks);
+        rope_block<T, VQ>(q, blockIdx.x - g.blocks);
         return;
     }
     const Kv8& c = g.c;
-    const int values = blockIdx.x & 1, head = (blockIdx.x >> 1) % c.heads;
-    const int from = (blockIdx.x >> 1) / c.heads * g.window, to = min(g.tokens, from + g.window);
+    int b = blockIdx.x;
+    const int values = b & 1, head = (b >> 1) % c.heads;
+    b = (b >> 1) / c.heads;
+    const int turn = b % g.turns, from = b / g.turns * 64, lane = threadIdx.x & 63;
     const long slots = (long)c.pages << c.shift;
-    for (int t = from; t < to; t++) {
-        const long s = g.slots[t];
+    const long here = from + lane < g.tokens ? g.slots[from + lane] : -1;
+    long last = __shfl_up(here, 1);
+    if (lane == 0) last = from > 0 ? g.slots[from - 1] : -1;
+    const bool goes_on = (here & (c.page - 1)) != 0 && last == here - 1;
+    uint64_t begin = __ballot(here >= 0 && here < slots && !goes_on);
+    for (int left = turn; begin; begin &= begin - 1) {
+        if (left-- > 0) continue;
+        left = g.turns - 1;
+        const int i = __builtin_ctzll(begin), t = from + i;
+        const long s = __shfl(here, i);
         const int off = (int)(s & (c.page - 1));
-        // tokens that go on from the one before, in its page, belong to that one's workgroup
-        if (s < 0 || s >= slots || (t > 0 && off != 0 && g.slots[t - 1] == s - 1)) continue;
         if (threadIdx.x == 0) count = min(c.page - off, g.tokens - t);
         __syncthreads();
         if ((int)threadIdx.x < count && g.slots[t + threadIdx.x] != s + threadIdx.x) atomicMin(&count, (int)threadIdx.x);
@@ -286,8 +296,9 @@ ZT_EXPORT int zt_kv8_append(const zt_kv8_cache* cache, const zt_rows* k, const z
         if (!rows_ok(*all[i], type)) return kInvalid;
     if (!slots || ((uintptr_t)slots & 7) || (table && (!positions || ((uintptr_t)positions & 3) || ((uintptr_t)table & 3))))
         return kInvalid;
-    // values are not turned: their units are those of a head without pairs, which 8 values divide
-    const int width = rope_width(all, n, dim, half, ZT_F32) == 4 && rope_width(all, n, dim, half, type) >= 4 ? 4 : 1;
+    // 4 values at a time for keys and values (values are not turned: 8 divide the head, a unit of 4 pairs), q as wide as it allows
+    const int width = units_fit(4, dim, half) && rows_vector(*k, 4, type) && rows_vector(*v, 4, type) ? 4 : 1;
+    const int q_width = q ? rope_width(all + 2, 2, dim, half, type) : 1;
     AppendArgs g{};
     g.c = kv8_of(*cache);
     g.x[0] = rows_of(*k);
@@ -295,10 +306,12 @@ ZT_EXPORT int zt_kv8_append(const zt_kv8_cache* cache, const zt_rows* k, const z
     g.slots = slots;
     g.turn = {positions, table, half, max_pos, flags};
     g.tokens = tokens;
-    // a workgroup for each token's page while they are few, else for 16 tokens' pages: most tokens of a prompt are not
-    // the first of their page, and a workgroup that finds none to do costs its launch
-    g.window = tokens <= 2048 ? 1 : 16;
-    g.blocks = 2l * cache->kv_heads * ceil_div(tokens, g.window);
+    // a workgroup for each token while they are few (a batch's next tokens, each on a page of its own), else for eight: a
+    // prompt's tokens mostly go on in their page, and a workgroup that finds none to do costs its launch (pages of 16,
+    // prompts of 1400 tokens: 8 groups for 64 tokens 40 us, 16 44, 32 53)
+    g.turns = tokens <= 256 ? 64 : 8;
+    g.blocks = 2l * cache->kv_heads * ceil_div(tokens, 64) * g.turns;
+    const int lds = g.c.bytes();
     RopeArgs r{};
     long blocks = g.blocks;
     if (q) {
@@ -307,18 +320,19 @@ ZT_EXPORT int zt_kv8_append(const zt_kv8_cache* cache, const zt_rows* k, const z
         r.turn = g.turn;
         r.tokens = tokens;
         r.dim = dim;
-        blocks += rope_blocks(r, 1, width);
+        blocks += rope_blocks(r, 1, q_width);
     }
     if (blocks >= 1l << 31) return kInvalid;
+    auto run = [&](auto kernel) { kernel<<<blocks, kThreads, lds, stream>>>(g, r); };
     if (type == ZT_F32) {
         if (width == 4)
-            append_kernel<float, 4><<<blocks, kThreads, 0, stream>>>(g, r);
+            q_width == 4 ? run(append_kernel<float, 4, 4>) : run(append_kernel<float, 4, 1>);
         else
-            append_kernel<float, 1><<<blocks, kThreads, 0, stream>>>(g, r);
+            q_width == 4 ? run(append_kernel<float, 1, 4>) : run(append_kernel<float, 1, 1>);
     } else if (width == 4) {
-        append_kernel<_Float16, 4><<<blocks, kThreads, 0, stream>>>(g, r);
+        q_width == 8 ? run(append_kernel<_Float16, 4, 8>) : q_width == 4 ? run(append_kernel<_Float16, 4, 4>) : run(append_kernel<_Float16, 4, 1>);
     } else {
-        append_kernel<_Float16, 1><<<blocks, kThreads, 0, stream>>>(g, r);
+        q_width == 8 ? run(append_kernel<_Float16, 1, 8>) : q_width == 4 ? run(append_kernel<_Float16, 1, 4>) : run(append_kernel<_Float16, 1, 1>);
     }
     return (int)hipGetLastError();
 }
