@@ -566,3 +566,18 @@ def test_engine_arguments(eng):
     assert empty.shape == (0, 2, 64) and eng.sample(t[:0, 0], t[:0, 0, 0])[0].shape == (0,)
     assert eng.rope(t[:0], t[:0], pos[:0], table)[1].shape == (0, 2, 64)
     assert eng.kv8_append(t[:0], t[:0], cache, slots[:0]) is None and eng.kv8_dequant(cache, pos[:0], 64)[0].shape == (0, 2, 16, 64)
+
+
+@pytest.mark.parametrize("new", [1, 24])
+def test_attention_of_fp32_rows_holds_22_bits_of_each_weight(eng, new):
+    """Small scores, so that the weights' own rounding is all there is: two parts that do not belong together (one
+    rounded from the product, the other from its fp32 value) would show as 2^-11 of one weight."""
+    rng = np.random.default_rng(new)
+    lens = list(rng.integers(new, new + 30, 60))
+    host, table = paged(rng, lens, 16, 2, 64)
+    starts = list(range(0, 60 * new + 1, new))
+    q = (0.01 * rng.standard_normal((60 * new, 8, 64))).astype(np.float32)
+    want, most, big = ref.attend(q, host, table, lens, starts)
+    out = eng.kv8_attention(cuda(q), host.device(torch), i32(table), i32(lens), i32(starts)).cpu().numpy()
+    assert most < 1.5
+    assert np.abs(out - want).max() <= ref.attend_bound(0, most, big, False)

@@ -1,5 +1,6 @@
 // Attention over the int8 paged cache.
 #include <algorithm>
+#include <cmath>
 
 #include "zt_kv8.h"
 
@@ -11,6 +12,7 @@ struct AttnArgs {
     const int *table, *kv_lens, *q_start;
     const float* scale;
     int requests, width, tokens, window, group;
+    float unit, unit_lo;  // log2(e) / sqrt(dim) in two parts: a score's factor where no scale is given
 };
 
 // The request of row t, and that row's place: tokens lo .. hi - 1 are seen
@@ -74,7 +76,33 @@ __device__ __forceinline__ float4v mfma(half8v a, half8v b, float4v c) {
 }
 
 constexpr float kNone = -__builtin_inff();
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f, kLog2eLo = (float)(1.44269504088896340736 - (double)kLog2e);
+
+// What makes a product of a query and a key a score in units of log 2, to 48
+// bits: an error in it is one of every score in the same direction, and grows
+// with them.
+struct Factor {
+    float hi, lo;
+};
+__device__ __forceinline__ Factor factor_of(const AttnArgs& g) {
+    if (!g.scale) return {g.unit, g.unit_lo};
+    const float s = *g.scale, hi = s * kLog2e;
+    return {hi, __builtin_fmaf(s, kLog2eLo, __builtin_fmaf(s, kLog2e, -hi))};
+}
+// The same times a page's scale: hi above 0, and for fp32 rows lo, above 0 too
+// (so that both take -inf to -inf).
+template <bool SPLIT>
+__device__ __forceinline__ Factor times(const Factor& f, float ks) {
+    Factor r;
+    r.hi = f.hi * ks;
+    r.hi = r.hi < 1e-30f ? 1e-30f : r.hi;  // (not a number: stays that)
+    r.lo = 0.0f;
+    if (SPLIT) {
+        r.hi = __uint_as_float(__float_as_uint(r.hi) - 1);
+        r.lo = fmaxf(__builtin_fmaf(f.lo, ks, __builtin_fmaf(f.hi, ks, -r.hi)), 1e-37f);
+    }
+    return r;
+}
 
 // 16 values of one row from dim d on, fp32; past the head's size and of no row: 0.
 template <class T>
@@ -140,8 +168,8 @@ __device__ __forceinline__ int splits_of(const Split& f, int tiles) {
 // two; factor: what a product of it is to be multiplied by for a score in
 // units of log 2; hi: it sees tokens before that (0: no such row).
 template <class T, int DN>
-__device__ __forceinline__ void load_query(const Work& f, const Span& sp, int kv, int row, int rows, float scale,
-                                           half8v (&q)[DN][2], half8v (&ql)[DN][2], float& factor, int& hi) {
+__device__ __forceinline__ void load_query(const Work& f, const Span& sp, int kv, int row, int rows, const Factor& scale,
+                                           half8v (&q)[DN][2], half8v (&ql)[DN][2], Factor& factor, int& hi) {
     constexpr bool SPLIT = sizeof(T) == 4;
     const AttnArgs& g = f.a;
     const int i = row / g.group, h = kv * g.group + row - i * g.group, quad = (threadIdx.x & 63) >> 4;
@@ -158,8 +186,9 @@ __device__ __forceinline__ void load_query(const Work& f, const Span& sp, int kv
     }
     int e2 = 0;
     if (SPLIT) e2 = scale_exponent(max_step<16>(max_step<32>(m)));
-    factor = ldexpf(fabsf(scale), -e2);
-    if (scale < 0.0f) {  // its sign goes to the query: a larger product is a larger score
+    const bool negative = scale.hi < 0.0f;
+    factor = {ldexpf(fabsf(scale.hi), -e2), ldexpf(negative ? -scale.lo : scale.lo, -e2)};
+    if (negative) {  // its sign goes to the query: a larger product is a larger score
 #pragma unroll
         for (int d = 0; d < DN; d++)
 #pragma unroll
@@ -201,9 +230,10 @@ struct ValueScale {
 // Of a tile's 16 tokens in this lane, t on, what a row does not see: tokens that
 // are not `there`, before lo or from hi on.  Their scores become -inf; of a lane
 // in which it sees none the scales may be anything, and are set aside.
-__device__ __forceinline__ void mask_scores(float4v (&s)[4], float& fk, ValueScale& v, int t, bool there, int lo, int hi) {
+__device__ __forceinline__ void mask_scores(float4v (&s)[4], Factor& fk, ValueScale& v, int t, bool there, int lo, int hi) {
     if (!there || max(t, lo) >= min(t + 16, hi)) {
-        fk = v.by = v.inverse = 1.0f;
+        fk = {1.0f, 1e-37f};
+        v.by = v.inverse = 1.0f;
         v.log = 0.0f;
         hi = 0;
     }
@@ -216,15 +246,14 @@ __device__ __forceinline__ void mask_scores(float4v (&s)[4], float& fk, ValueSca
 // in units of log 2, against a base that follows their maximum only when it is
 // passed by more than 2^4 (most tiles move some row's maximum a little; so few
 // of them change l and o, which stand already).  Scales of keys and values are
-// not negative; fk of 0 counts as what no score survives, so that -inf stays.
+// not negative.
 template <bool SPLIT, int N>
-__device__ __forceinline__ void weights_of(const float4v (&s)[4], float fk, const ValueScale& v, float& base, float& l,
+__device__ __forceinline__ void weights_of(const float4v (&s)[4], const Factor& fk, const ValueScale& v, float& base, float& l,
                                            float4v (&o)[N], half8v (&p)[2], half8v (&pl)[2]) {
-    fk = fk < 1e-37f ? 1e-37f : fk;  // (not a number: stays that)
     float top = kNone;
 #pragma unroll
     for (int k = 0; k < 16; k++) top = fmaxf(top, s[k >> 2][k & 3]);
-    top = max_step<16>(max_step<32>(top * fk));
+    top = max_step<16>(max_step<32>(top * fk.hi));
     if (__any(top > base + 4.0f)) {  // (from nothing: to the first that is seen)
         const bool up = top > base + 4.0f;
         const float keep = up ? __builtin_amdgcn_exp2f(base - top) : 1.0f;
@@ -241,9 +270,13 @@ __device__ __forceinline__ void weights_of(const float4v (&s)[4], float fk, cons
             float y[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const float z = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * h + (k >> 2)][k & 3], fk, -from));
+                const float x = s[2 * h + (k >> 2)][k & 3];
+                const float z = __builtin_amdgcn_exp2f(__builtin_fmaf(x, fk.hi, __builtin_fmaf(x, fk.lo, -from)));
                 sum += z;
                 y[k] = z * v.by;
+                // one value for both parts: fused into the conversion of one of them, the product would round to another
+                // fp16 near a tie, and the parts would be off by its last bit
+                asm("" : "+v"(y[k]));
             }
             split_hi_lo(y, p[h], pl[h]);
         }
@@ -253,8 +286,8 @@ __device__ __forceinline__ void weights_of(const float4v (&s)[4], float fk, cons
         const half2v one = {(_Float16)1.0f, (_Float16)1.0f};
 #pragma unroll
         for (int k = 0; k < 16; k += 2) {
-            const half2v w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 2][k & 3], fk, at)),
-                              (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 2][(k & 3) + 1], fk, at))};
+            const half2v w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 2][k & 3], fk.hi, at)),
+                              (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 2][(k & 3) + 1], fk.hi, at))};
             sum = __builtin_amdgcn_fdot2(w, one, sum, false);
             p[k >> 3][k & 7] = w[0];
             p[k >> 3][(k & 7) + 1] = w[1];
@@ -391,7 +424,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
         before += __shfl(upto, 63);
     }
     r = __builtin_amdgcn_readfirstlane(r);
-    const float scale = (g.scale ? *g.scale : 1.0f / sqrtf((float)c.dim)) * kLog2e;
+    const Factor scale = factor_of(g);
     const int krow = (col >> 2) * 16 + (col & 3);  // this lane's token of a key tile, less 4 j
 
     while (pos < end) {
@@ -426,7 +459,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
         const Pages page_of{g.table + (long)r * g.width, sp.len, c.shift};
         int pk = page_of(first * 64 + (col >> 2) * 16), pv = page_of(first * 64 + quad * 16);
         half8v* mine_q = queries + wave * (CT * DN * 2 * PARTS * 64);
-        float factor[CT];
+        Factor factor[CT];
         int hi[CT];
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
@@ -507,7 +540,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
             }
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
-                float fk = factor[ct] * ks;
+                Factor fk = times<SPLIT>(factor[ct], ks);
                 ValueScale v = scales;
                 if (!whole) mask_scores(s[ct], fk, v, t0 + 16 * quad, seen, g.window > 0 ? hi[ct] - g.window : 0, hi[ct]);
                 weights_of<SPLIT>(s[ct], fk, v, m[ct], l[ct], o[ct], p[ct], pl[ct]);
@@ -587,7 +620,7 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
     const Span sp = span_of(g, r);
     const int rows = sp.n * g.group;
     if (sp.n <= 0 || rows <= f.most) return;
-    const float scale = (g.scale ? *g.scale : 1.0f / sqrtf((float)c.dim)) * kLog2e;
+    const Factor scale = factor_of(g);
     const int krow = (col >> 2) * 16 + (col & 3);
     const Pages page_of{g.table + (long)r * g.width, sp.len, c.shift};
 
@@ -600,7 +633,7 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
         const int first = w.tile0 + split * f.many.tiles, last = split == ns - 1 ? w.tile1 : first + f.many.tiles;
 
         half8v q[CT][DN][2], ql[CT][DN][2];
-        float factor[CT];
+        Factor factor[CT];
         int hi[CT];
         const int row0 = w.row0 + wave * 16 * CT, row1 = min(rows, row0 + 16 * CT) - 1;
 #pragma unroll
@@ -718,7 +751,7 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
             }
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
-                float fk = factor[ct] * fs;
+                Factor fk = times<SPLIT>(factor[ct], fs);
                 ValueScale v = scales;
                 if (!whole) mask_scores(s[ct], fk, v, t0 + 16 * quad, there, g.window > 0 ? hi[ct] - g.window : 0, hi[ct]);
                 weights_of<SPLIT>(s[ct], fk, v, m[ct], l[ct], o[ct], p[ct], pl[ct]);
@@ -977,8 +1010,10 @@ ZT_EXPORT int zt_kv8_attention(const zt_kv8_attn* a, void* workspace, long works
         return kInvalid;
     const AttnPlan p = attn_plan(a);
     if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.part + p.stat + p.parts) return kInvalid;
+    const double unit = 1.44269504088896340736 / std::sqrt((double)a->cache.head_dim);
     const AttnArgs g{kv8_of(a->cache), rows_of(a->q), rows_of(a->out), a->table, a->kv_lens, a->q_start, a->scale,
-                     a->requests,      a->width,      a->tokens,       a->window, a->q.heads / a->cache.kv_heads};
+                     a->requests,      a->width,      a->tokens,       a->window, a->q.heads / a->cache.kv_heads,
+                     (float)unit,      (float)(unit - (double)(float)unit)};
     const Work f{g,        p.most, p.shares, p.single, p.many, p.qtiles, rows_vector(a->q, 4, a->type) && rows_vector(a->out, 4, a->type),
                  p.others, (float*)workspace, (float2*)((char*)workspace + p.part),
                  (int2*)((char*)workspace + p.part + p.stat)};
