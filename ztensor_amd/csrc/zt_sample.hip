@@ -145,7 +145,7 @@ struct Digits {
 // selections of 8 bits a pass, one by number and one by weight.  Slow, and for
 // every row: those with more tokens in one bin than the list below has room for.
 template <class T>
-__device__ __noinline__ void sample_row(const SampleArgs& g, int b, const Scores& sc, const Settings& st, Scan& scan, Digits& dg) {
+__device__ __forceinline__ void sample_row(const SampleArgs& g, int b, const Scores& sc, const Settings& st, Scan& scan, Digits& dg) {
     const int tid = threadIdx.x, V = g.vocab;
     const T* row = (const T*)g.logits + (long)b * g.row_stride;
     uint64_t want = st.k;  // the weights fall with the logits: those of min_p or more are the first so many, too
@@ -380,15 +380,21 @@ __global__ __launch_bounds__(kSampleThreads) void sample_bins_kernel(SampleArgs 
     __syncthreads();
     const int to = min(g.vocab, (s + 1) * part);
     const Scores sc(bins.top, st.temperature);
-#pragma unroll 4
-    for (int i = s * part + tid; i < to; i += kSampleThreads) {
-        const float z = logit(row, i);
-        const int bin = bins.of(z);
-        if (need.counted) atomicAdd(&count[bin], 1u);
-        if (need.weighed) {
-            float x;
-            const uint64_t f = sc.weight(z, x);
-            if (f && x >= st.min_p) atomicAdd(&mass[bin], (unsigned long long)f);
+    constexpr int kAhead = 4;
+    for (int i0 = s * part + tid; i0 < to; i0 += kSampleThreads * kAhead) {
+        float z[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) z[k] = logit(row, min(i0 + kSampleThreads * k, to - 1));
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            if (i0 + kSampleThreads * k >= to) continue;
+            const int bin = bins.of(z[k]);
+            if (need.counted) atomicAdd(&count[bin], 1u);
+            if (need.weighed) {
+                float x;
+                const uint64_t f = sc.weight(z[k], x);
+                if (f && x >= st.min_p) atomicAdd(&mass[bin], (unsigned long long)f);
+            }
         }
     }
     __syncthreads();
@@ -467,18 +473,23 @@ __global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs 
     const Scores sc(bins.top, st.temperature);
     const int wave = tid >> 6, from = s * part + wave * parts.seg, to = min(g.vocab, from + parts.seg);
     uint64_t sure = 0;
-#pragma unroll 4
-    for (int i = from + (tid & 63); i < to; i += 64) {
-        const float z = logit(row, i);
-        const int bin = bins.of(z);
-        const bool counts = bin < lo, ranks = (bin >= lo && bin <= hi) || (bin >= bin0 && bin <= bin1);
-        if (!counts && !ranks) continue;
-        float x;
-        const uint64_t f = sc.weight(z, x);
-        sure += counts && x >= st.min_p ? f : 0;
-        if (ranks && f) {  // tokens without weight are the last in any order
-            const unsigned n = atomicAdd(&listed, 1u);
-            if (n < kListed) list[n] = order_of(key_of(z), i);
+    constexpr int kAhead = 8;  // values on their way at a time
+    for (int i0 = from + (tid & 63); i0 < to; i0 += 64 * kAhead) {
+        float z[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) z[k] = logit(row, min(i0 + 64 * k, to - 1));
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const int i = i0 + 64 * k, bin = bins.of(z[k]);
+            const bool counts = bin < lo, ranks = (bin >= lo && bin <= hi) || (bin >= bin0 && bin <= bin1);
+            if (i >= to || !(counts || ranks)) continue;
+            float x;
+            const uint64_t f = sc.weight(z[k], x);
+            sure += counts && x >= st.min_p ? f : 0;
+            if (ranks && f) {  // tokens without weight are the last in any order
+                const unsigned n = atomicAdd(&listed, 1u);
+                if (n < kListed) list[n] = order_of(key_of(z[k]), i);
+            }
         }
     }
 #pragma unroll
