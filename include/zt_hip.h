@@ -694,8 +694,8 @@ int zt_rope(const zt_rows* in, const zt_rows* out, int n, const int* positions, 
 
 /* The cache: pages of page_tokens (16, 32, 64 or 128) tokens, a value is its
  * code times the scale of its page and head.  Dp = head_dim to the next
- * multiple of 64; codes past head_dim are 0.  head_dim % 8 == 0, at most 256;
- * k and v 16-byte aligned. */
+ * multiple of 64; codes past head_dim are 0, and a scale is not negative (it
+ * may be NaN).  head_dim % 8 == 0, at most 256; k and v 16-byte aligned. */
 typedef struct zt_kv8_cache {
     void* k;        /* int8 [pages][kv_heads][page_tokens][Dp] */
     void* v;        /* int8 [pages][kv_heads][Dp][page_tokens] */
@@ -736,8 +736,8 @@ int zt_kv8_dequant(const zt_kv8_cache* cache, const int* pages, int n, float* ke
  * its position, request r's are q_start[r] .. q_start[r + 1] - 1 (requests + 1
  * values), kv_lens_out[r] = kv_lens[r] + add[r], and free_count_out is what is
  * left of the list.  A request whose pages are not there, or do not fit its
- * row, gets none: its tokens' slots are -1 and its length stays.  Tokens past
- * the last request's, up to `tokens`, get slot -1 and position 0.  Negative
+ * row (or whose length would pass 2^31 - 1), gets none: its tokens' slots are
+ * -1 and its length stays.  Tokens past the last request's, up to `tokens`, get slot -1 and position 0.  Negative
  * lengths count as 0.  free_capacity: the entries of free_pages. */
 int zt_kv8_plan(const int* kv_lens, const int* add, const int* table, int requests, int width, const int* free_pages,
                 const int* free_count, int free_capacity, int page_tokens, int tokens, int* table_out, long* slots,

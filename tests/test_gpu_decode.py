@@ -237,6 +237,14 @@ def test_plan_of_nothing_and_of_lengths_that_do_not_fit(eng):
     assert p.block_table.tolist() == [[5, 6], [5, 6], [8, 6]]
 
 
+def test_plan_of_a_length_past_31_bits(eng):
+    """A row that would have room for it: the request gets nothing, as one that does not fit its row."""
+    width = 2 ** 24  # of pages of 128: 2^31 tokens
+    p = eng.kv8_plan(i32([2 ** 31 - 1]), i32([1]), torch.zeros((1, width), dtype=torch.int32, device="cuda"), i32([7]),
+                     i32([1]), 128, 1, in_place=True)
+    assert p.kv_lens.tolist() == [2 ** 31 - 1] and p.slots.tolist() == [-1] and p.free_count.tolist() == [1]
+
+
 # ---------------------------------------------------------------- attention
 
 

@@ -15,24 +15,6 @@ struct AttnArgs {
     float unit, unit_lo;  // log2(e) / sqrt(dim) in two parts: a score's factor where no scale is given
 };
 
-// The request of row t, and that row's place: tokens lo .. hi - 1 are seen
-// (hi <= lo: none).
-__device__ __forceinline__ int find_request(const AttnArgs& g, int t, int& lo, int& hi) {
-    int a = 0, b = g.requests;  // q_start[a] <= t < q_start[b], if it is in any
-    lo = hi = 0;
-    if (g.requests == 0 || t < g.q_start[0] || t >= g.q_start[b]) return 0;
-    while (b - a > 1) {
-        const int m = (a + b) >> 1;
-        if (g.q_start[m] <= t) a = m; else b = m;
-    }
-    const long most = (long)g.width << g.c.shift;
-    const int len = (int)min((long)max(0, g.kv_lens[a]), most);
-    const int n = g.q_start[a + 1] - g.q_start[a];
-    hi = len - n + (t - g.q_start[a]) + 1;
-    lo = g.window > 0 ? max(0, hi - g.window) : 0;
-    return a;
-}
-
 // ------------------------------------------------- few rows: a long axis split
 
 // Workgroups of one request and head along its tokens, and the tiles of 64

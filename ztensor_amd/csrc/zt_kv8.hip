@@ -408,7 +408,7 @@ __device__ __forceinline__ Request request(const PlanArgs& g, int r) {
     q.held = max(0, g.kv_lens[r]);
     q.add = max(0, g.add[r]);
     const long end = (long)q.held + q.add, room = (1l << g.shift) - 1;
-    q.fits = end <= (long)g.width << g.shift;
+    q.fits = end <= min((long)g.width << g.shift, 0x7FFFFFFFl);
     q.have = (int)((q.held + room) >> g.shift);
     q.need = q.fits ? (int)((end + room) >> g.shift) - q.have : 0;
     return q;
