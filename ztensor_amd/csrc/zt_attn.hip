@@ -219,9 +219,11 @@ __device__ __forceinline__ void mask_scores(float4v (&s)[4], Factor& fk, ValueSc
         v.log = 0.0f;
         hi = 0;
     }
+    lo -= t;
+    hi -= t;
 #pragma unroll
     for (int k = 0; k < 16; k++)
-        if (t + k < lo || t + k >= hi) s[k >> 2][k & 3] = kNone;
+        if (k < lo || k >= hi) s[k >> 2][k & 3] = kNone;
 }
 
 // The weights of a tile's 16 tokens in this lane for one row: scores s times fk
@@ -235,8 +237,9 @@ __device__ __forceinline__ void weights_of(const float4v (&s)[4], const Factor& 
     float top = kNone;
 #pragma unroll
     for (int k = 0; k < 16; k++) top = fmaxf(top, s[k >> 2][k & 3]);
-    top = max_step<16>(max_step<32>(top * fk.hi));
+    top *= fk.hi;
     if (__any(top > base + 4.0f)) {  // (from nothing: to the first that is seen)
+        top = max_step<16>(max_step<32>(top));
         const bool up = top > base + 4.0f;
         const float keep = up ? __builtin_amdgcn_exp2f(base - top) : 1.0f;
         base = up ? top : base;
