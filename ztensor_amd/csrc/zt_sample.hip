@@ -504,12 +504,14 @@ __global__ __launch_bounds__(kSampleThreads) void sample_list_kernel(SampleArgs 
         if (at + i < kListed) w.list[at + i] = list[i];
 }
 
-// Falling order of n2 values, a power of two, by compare and exchange over
-// strides that halve.
+// Falling order of n2 values, a power of two up to 2 kSampleThreads, by compare
+// and exchange over strides that halve.  At strides up to 64 a wave's pairs are
+// its own 128 values: no barrier between such steps.
 __device__ __forceinline__ void sort_falling(unsigned long long* v, int n2) {
+    const int t = threadIdx.x;
     for (int size = 2; size <= n2; size <<= 1)
         for (int stride = size >> 1; stride >= 1; stride >>= 1) {
-            for (int t = threadIdx.x; t < n2 / 2; t += kSampleThreads) {
+            if (t < n2 / 2) {
                 const int i = 2 * t - (t & (stride - 1)), j = i + stride;
                 const unsigned long long a = v[i], b = v[j];
                 if ((a < b) != ((i & size) != 0)) {
@@ -517,7 +519,10 @@ __device__ __forceinline__ void sort_falling(unsigned long long* v, int n2) {
                     v[j] = a;
                 }
             }
-            __syncthreads();
+            if (stride > 64 || (stride == 1 && (size > 64 || size == n2)))
+                __syncthreads();
+            else
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
 }
 
