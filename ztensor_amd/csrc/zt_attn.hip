@@ -1,4 +1,14 @@
-// Attention over the int8 paged cache.
+// Attention over the int8 paged cache: o = sum_j w_j v_j / sum_j w_j with w_j =
+// 2^(f q.k_j - m), m a running maximum of the scores and f = scale log2(e) times
+// the scale of the keys' page; one pass over the tokens, sums in fp32.
+//
+// Few rows (a batch's next tokens) read their sequences' codes once, and bytes
+// bound them; the rows of a prompt read each tile many times, and the products
+// and exponentials do.  So there are two kernels, and a third that joins what
+// several waves have of one row.  A call whose requests have at most 64 rows of a
+// key/value head (tokens x the group of its q heads) is the first kernel's, which
+// reads a tile for 16 or 32 of them; in a call of longer ones those of up to 64
+// still are, and the others' rows are the second's, up to 128 at a time.
 #include <algorithm>
 #include <cmath>
 
@@ -322,9 +332,10 @@ __device__ __forceinline__ void store_row(const Work& f, const Span& sp, int kv,
 // ends: sequences of any lengths keep all CUs busy to the end.  What a share
 // holds of a head's tiles goes to `out` if it is all of them, else to the
 // share's place for its first part or its last.
-// That place counts as two tiles: 64 sequences of up to 8000 tokens, 76 us at one, 75 at two or three.  Where the
-// host knows of few tiles, a head's are one place: nothing is split, nothing to be joined.
-constexpr int kBegin = 2;
+// That place counts as four tiles: 64 sequences of up to 8000 tokens, fp16, 87 us at one, 74 at two, 68 at four or
+// seven; fp32 74, 68, 67 and 68.  Where the host knows of few tiles, a head's are one place: nothing is split, nothing
+// to be joined.
+constexpr int kBegin = 4;
 __device__ __forceinline__ int begin_of(const Work& f) { return f.single ? 0 : kBegin; }
 __device__ __forceinline__ int length_of(const Work& f, const Span& sp) { return f.single ? 1 : sp.tile1 - sp.tile0 + kBegin; }
 __device__ __forceinline__ long places_of(const Work& f, const Span& sp, int rows_of_group) {
@@ -358,6 +369,12 @@ __device__ __forceinline__ long wave_scan(long v) {
 // Weights enter the second product times their page's scale over a power of two
 // (the largest so far, 2^(e - 10)): fp16 then holds 35 bits below the largest.
 // fp32 rows: queries and weights in two fp16 parts (22 bits).
+//
+// The codes bound it: 64 sequences of up to 8000 tokens (8 heads of 128, fp32,
+// pages of 32) 306 MB in 62 us, 4.9 TB/s, the rate of a large copy; one of 40011
+// (fp16, pages of 64) 82 MB in 21.6 us, 3.8 TB/s, of which about 5 us are the
+// launch and the chain from the lengths to the first codes; 37 tokens 8.6 us, all
+// of it that chain.
 template <class T, int DN, int CT>
 __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
     constexpr bool SPLIT = sizeof(T) == 4;
@@ -587,6 +604,15 @@ __device__ __forceinline__ RowTiles tiles_of(const AttnArgs& g, const Span& sp, 
 // (16 bytes a lane side by side, no bank conflicts).  The next tile's codes are
 // on their way to registers while a tile is worked on, and go to the other
 // buffer after it: one barrier a tile.
+//
+// Two workgroups a CU.  Three prompts (187 GFLOP, 32 heads over 8 of 128, fp16)
+// 255 to 285 us with the card's clock, 0.65 to 0.73 PFLOP/s.  A tile of one wave
+// is 64 matrix instructions (1024 cycles) and some 340 of the vector unit (1800
+// cycles with the exponentials), which bounds it: 80 decode its share of the
+// codes, 5 for each of its scores are the softmax's.  The last fifth of the time
+// is a tail with half of the workgroups; splitting those along their tokens makes
+// parts to be joined and costs more (272 us: 387 with tiles in 24s, 474 in 32s),
+// dealing a late row tile and an early one to one workgroup 273.
 template <class T, int DN>
 __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
     constexpr bool SPLIT = sizeof(T) == 4;
@@ -784,6 +810,10 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
 // whose heads are split in few parts; of one long sequence there are hundreds.
 // The rows: ROWS all of them, FEW up to each_n of each request, MANY as FEW, of
 // the other kernel's.
+//
+// It reads the parts (512 bytes each at 128 dims) after where they are, two loads
+// that wait for each other: the 64 rows of one long sequence, in 128 parts, 4.2
+// us; 64 sequences' 2048 rows 4.8.
 enum class Join { ROWS, FEW, MANY };
 template <class T, int DN, int W>
 __global__ __launch_bounds__(512) void attn_join_kernel(Work f, int rows_of_group, int each_n, Join which) {
@@ -916,27 +946,44 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
     const int group = a->q.heads / a->cache.kv_heads, dp = (a->cache.head_dim + 63) & ~63;
     const long requests = std::max(1, a->requests), heads = a->cache.kv_heads;
     const long most = (long)std::min(a->max_q, a->tokens) * group;
+    // up to 64 rows by the few kernel: 32 requests of 3000 tokens, 64 rows 91 us, by the other 95; 128 rows 136 and 110
     p.most = most <= 64 ? 0x7FFFFFFF : 64;
+    // of more than 16 rows two columns of them share what is read of a tile (those requests, 32 rows: 67 us, one by one
+    // 81); past 128 dims their sums would leave no registers
     p.ct = most > 16 && dp <= 128 ? 2 : 1;
     long kv = std::min((long)a->max_kv, (long)a->width * a->cache.page_tokens);
     if (a->window > 0) kv = std::min(kv, (long)a->window + a->max_q + 63);
     const long tiles = std::max(1l, (kv + 63) / 64);
-    // A tile each as far as the bounds go, up to a wave for each SIMD: each more makes parts to be joined (one sequence
-    // of 40011 tokens 31 us, with 2048 36; 64 of up to 8000 70 and 75).
+    // A tile each as far as the bounds go, up to a wave for each SIMD: fewer leave some without work, each more makes
+    // parts to be joined (one sequence of 40011 tokens 25.6 us, with 512 32.6, with 2048 27.4; 64 of up to 8000 68, 96
+    // and 70).
     const long groups = (std::max(1l, std::min(most, 64l)) + 16 * p.ct - 1) / (16 * p.ct);
     p.single = tiles <= 2;
     p.shares = (int)std::min(1024l, requests * heads * groups * (p.single ? 1 : tiles + kBegin));
-    p.wide = p.shares > 16 * requests * heads * groups;  // more than 16 parts of a row
+    // eight waves to join a row of more than 16 parts (one sequence of 40011 tokens, 128 parts: 26 us, with one 37), else
+    // one (64 sequences 70 us, with eight 80)
+    p.wide = p.shares > 16 * requests * heads * groups;
     p.others = 2l * p.shares * 16 * p.ct;
     p.many_n = std::max(1, std::min(a->max_q, a->tokens));
     p.few_n = std::max(1, std::min(p.many_n, 64 / group));
     p.many = {1, 1};
     if (most > 64) {
         p.qtiles = ceil_div(most, dp <= 128 ? 128 : 64);
-        // along the tokens while the card's 512 workgroups are not there, none of less than 4 tiles; of a prompt from its
-        // beginning half of the rows see half of the tokens, and half of them are not split
-        const long have = requests * heads * p.qtiles, want = kv >= 2l * a->max_q ? 512 : 768;
-        const long splits = std::max(1l, std::min(want / have, tiles / 4));
+        // Along the tokens where that is less time: a tile of 128 rows and dims is 2.2 us while the card's 512 workgroups
+        // are not passed, the parts are written and read at 4.5 TB/s, a launch 4 us.  (32 heads over 8 of 128, fp16, one
+        // sequence: 100 tokens onto 4000 42 us in 16 splits, 124 whole; 1000 onto 4000 129 in two, 151 whole; 1500 from
+        // the beginning 83 in two, 63 whole.)
+        const long have = requests * heads * p.qtiles;
+        const double tile = 2.2 * dp / (dp <= 128 ? 128 : 256), part = 8.0 * a->tokens * a->q.heads * dp / 4.5e6;
+        long splits = 1;
+        double least = 0;
+        for (long s = 1; s <= std::max(1l, std::min(512 / have, tiles / 4)); s++) {
+            const double us = (double)((tiles + s - 1) / s) * tile + (s > 1 ? 4 + s * part : 0);
+            if (s == 1 || us < least) {
+                least = us;
+                splits = s;
+            }
+        }
         p.many.tiles = (int)((tiles + splits - 1) / splits);
         p.many.splits = (int)((tiles + p.many.tiles - 1) / p.many.tiles);
     }
