@@ -376,17 +376,16 @@ __device__ __forceinline__ long wave_scan(long v) {
 // launch and the chain from the lengths to the first codes; 37 tokens 8.6 us, all
 // of it that chain.
 template <class T, int DN, int CT>
-__global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
+__device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queries) {  // [4 waves][CT][DN][2][PARTS][64]
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int PARTS = SPLIT ? 2 : 1;
-    extern __shared__ __align__(16) half8v queries[];  // [4 waves][CT][DN][2][PARTS][64]
     const AttnArgs& g = f.a;
     const Kv8& c = g.c;
     const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int blocks = (f.shares + 3) / 4, share = blockIdx.x * 4 + wave;
-    if ((int)blockIdx.x >= blocks) {  // rows of no request
-        const int kv = blockIdx.x - blocks, from = g.requests ? max(0, g.q_start[g.requests]) : 0;
+    const int blocks = (f.shares + 3) / 4, share = block * 4 + wave;
+    if (block >= blocks) {  // rows of no request
+        const int kv = block - blocks, from = g.requests ? max(0, g.q_start[g.requests]) : 0;
         for (int t = from; t < g.tokens; t++)
             for (int i = threadIdx.x; i < g.group * c.dim; i += 256) {
                 const int h = i / c.dim;
@@ -574,6 +573,12 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
     }
 }
 
+template <class T, int DN, int CT>
+__global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
+    extern __shared__ __align__(16) half8v shared[];
+    few_rows<T, DN, CT>(f, blockIdx.x, shared);
+}
+
 // ------------------------------------------------------------ prompts: tiled
 
 // Columns of 16 rows that a wave of the tiled kernel holds.
@@ -606,7 +611,7 @@ __device__ __forceinline__ RowTiles tiles_of(const AttnArgs& g, const Span& sp, 
 // buffer after it: one barrier a tile.
 //
 // Two workgroups a CU.  Three prompts (187 GFLOP, 32 heads over 8 of 128, fp16)
-// 255 to 285 us with the card's clock, 0.65 to 0.73 PFLOP/s.  A tile of one wave
+// 247 to 275 us with the card's clock, 0.68 to 0.75 PFLOP/s.  A tile of one wave
 // is 64 matrix instructions (1024 cycles) and some 340 of the vector unit (1800
 // cycles with the exponentials), which bounds it: 80 decode its share of the
 // codes, 5 for each of its scores are the softmax's.  The last fifth of the time
@@ -614,15 +619,13 @@ __device__ __forceinline__ RowTiles tiles_of(const AttnArgs& g, const Span& sp, 
 // parts to be joined and costs more (272 us: 387 with tiles in 24s, 474 in 32s),
 // dealing a late row tile and an early one to one workgroup 273.
 template <class T, int DN>
-__global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
+__device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {  // [2][FRAGS][64]
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int CT = kCols<DN>, FRAGS = 16 * DN;  // fragments of 64 lanes x 16 bytes in a buffer: keys', then values'
-    extern __shared__ __align__(16) half8v tiles[];  // [2][FRAGS][64]
     const AttnArgs& g = f.a;
     const Kv8& c = g.c;
     const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int b = blockIdx.x;
     const int kv = b % c.heads;
     b /= c.heads;
     const int split = b % f.many.splits;
@@ -802,6 +805,17 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f) {
                              l[ct], ev, o[ct]);
         }
     }
+}
+
+// The other kernel's workgroups come last in the same launch: they are there while the tiled ones run out (a prompt of
+// 100 tokens 13.5 us, with two launches 15.6; three of up to 4096 252 and 258).
+template <class T, int DN>
+__global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f, int tiled) {
+    extern __shared__ __align__(16) half8v shared[];
+    if ((int)blockIdx.x < tiled)
+        many_rows<T, DN>(f, blockIdx.x, shared);
+    else
+        few_rows<T, DN, (DN <= 2 ? 2 : 1)>(f, blockIdx.x - tiled, shared);
 }
 
 // Joins what several waves or workgroups hold of a row, in their order: W waves
@@ -996,23 +1010,23 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
 
 template <class T, int DN>
 static int launch(const Work& f, const AttnPlan& p, hipStream_t stream) {
-    const long many = (long)p.qtiles * p.many.splits * f.a.c.heads * f.a.requests;
-    if (many >= 1l << 31) return kInvalid;
-    if (p.qtiles && f.a.requests) {
+    const long tiled = (long)p.qtiles * p.many.splits * f.a.c.heads * f.a.requests;
+    const int few = (f.shares + 3) / 4 + f.a.c.heads;
+    if (tiled + few >= 1l << 31) return kInvalid;
+    constexpr int column = DN * 2 * (sizeof(T) / 2) * 4096;  // LDS of the few kernel, at most 64 KB in all
+    if (tiled) {
         static std::atomic<uint64_t> raised{0};
         constexpr int lds = 2 * 16 * DN * 1024;
+        static_assert(lds >= column * (DN <= 2 ? 2 : 1));
         if constexpr (lds > 65536) {
             const hipError_t rc = raise_lds((const void*)attn_many_kernel<T, DN>, lds, raised);
             if (rc != hipSuccess) return (int)rc;
         }
-        attn_many_kernel<T, DN><<<(unsigned)many, 256, lds, stream>>>(f);
-    }
-    const int few = (f.shares + 3) / 4 + f.a.c.heads;
-    constexpr int lds = DN * 2 * (sizeof(T) / 2) * 4096;  // of a column tile, at most 64 KB in all
-    if (p.ct == 2) {
-        if constexpr (DN <= 2) attn_few_kernel<T, DN, 2><<<few, 256, 2 * lds, stream>>>(f);
+        attn_many_kernel<T, DN><<<(unsigned)(tiled + few), 256, lds, stream>>>(f, (int)tiled);
+    } else if (p.ct == 2) {
+        if constexpr (DN <= 2) attn_few_kernel<T, DN, 2><<<few, 256, 2 * column, stream>>>(f);
     } else {
-        attn_few_kernel<T, DN, 1><<<few, 256, lds, stream>>>(f);
+        attn_few_kernel<T, DN, 1><<<few, 256, column, stream>>>(f);
     }
     const auto join = [&](Join which, int each, bool wide) {
         each = (int)std::min((long)each, std::max(1l, ((1l << 31) - 1) / (std::max(1l, (long)f.a.requests) * f.a.q.heads)));
