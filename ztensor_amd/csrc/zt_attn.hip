@@ -371,7 +371,7 @@ __device__ __forceinline__ long wave_scan(long v) {
 // fp32 rows: queries and weights in two fp16 parts (22 bits).
 //
 // The codes bound it: 64 sequences of up to 8000 tokens (8 heads of 128, fp32,
-// pages of 32) 306 MB in 62 us, 4.9 TB/s, the rate of a large copy; one of 40011
+// pages of 32) 306 MB in 63 us, 4.9 TB/s, the rate of a large copy; one of 40011
 // (fp16, pages of 64) 82 MB in 21.6 us, 3.8 TB/s, of which about 5 us are the
 // launch and the chain from the lengths to the first codes; 37 tokens 8.6 us, all
 // of it that chain.
@@ -611,7 +611,7 @@ __device__ __forceinline__ RowTiles tiles_of(const AttnArgs& g, const Span& sp, 
 // buffer after it: one barrier a tile.
 //
 // Two workgroups a CU.  Three prompts (187 GFLOP, 32 heads over 8 of 128, fp16)
-// 247 to 275 us with the card's clock, 0.68 to 0.75 PFLOP/s.  A tile of one wave
+// 247 us, 0.75 PFLOP/s, one call after the other (up to 290 as the first).  A tile of one wave
 // is 64 matrix instructions (1024 cycles) and some 340 of the vector unit (1800
 // cycles with the exponentials), which bounds it: 80 decode its share of the
 // codes, 5 for each of its scores are the softmax's.  The last fifth of the time
