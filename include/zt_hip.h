@@ -1,6 +1,7 @@
 /*
  * zt_hip.h -- C ABI of libzt_hip.so, the MI355X (gfx950) quantized-weight
- * GEMV / small-batch GEMM library for ztensor's decode matmul path.
+ * GEMV / small-batch GEMM library for ztensor's decode matmul path, and the
+ * operators of a decode step between those matmuls.
  *
  * Every entry point takes plain pointers and integers (floats only by device
  * pointer), allocates nothing, launches asynchronously on `stream` and
