@@ -751,7 +751,9 @@ int zt_kv8_plan(const int* kv_lens, const int* add, const int* table, int reques
  * head h / (q.heads / kv_heads).  out = softmax(scale q k^T) v; scale: one
  * fp32 on the device, NULL: 1 / sqrt(head_dim).  q and out have one type; sums
  * and softmax in fp32.  A row that sees nothing (no length, pages outside the
- * cache) gives zeros, and so do rows that belong to no request.  Tokens on a
+ * cache) gives zeros, and so do rows that belong to no request (before
+ * q_start[0], or past the last one's).  A request's rows past `tokens` are not
+ * there; starts that are not in order give values without a meaning.  Tokens on a
  * page outside the cache are not seen.  max_q and max_kv are bounds that the
  * host knows for the largest n and length (they choose the launch; a larger
  * one is still computed).  Workspace: zt_kv8_attention_workspace_bytes (-1

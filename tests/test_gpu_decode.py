@@ -334,6 +334,48 @@ def test_attention_of_uneven_scales_and_large_queries(eng, new, dtype):
     assert (np.abs(out - want) <= bound).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("lens,new", [([40, 700, 3], [1, 2, 1]), ([2500], [2]), ([300, 190], [90, 33])])
+def test_attention_of_rows_before_the_first_request(eng, lens, new, dtype):
+    """q_start need not begin with 0: the rows before it are of no request, and zeros whatever the workspace held."""
+    rng = np.random.default_rng(len(lens))
+    host, table = paged(rng, lens, 16, 2, 128)
+    starts = 5 + np.concatenate([[0], np.cumsum(new)])
+    q = cuda(rng.standard_normal((starts[-1] + 3, 8, 128)).astype(np.float32)).to(DT[dtype])
+    want, most, big = ref.attend(q.float().cpu().numpy(), host, table, lens, starts)
+    bound = ref.attend_bound(want, most, big, dtype == "f16")
+    for bounds in ({"max_q": max(new), "max_kv": max(lens)}, {}):
+        out = eng.kv8_attention(q, host.device(torch), i32(table), i32(lens), i32(starts), **bounds)
+        assert (out[:5] == 0).all() and (out[starts[-1]:] == 0).all()
+        assert (np.abs(out.double().cpu().numpy() - want) <= bound).all()
+
+
+@pytest.mark.parametrize("lens,new,tokens", [([40, 700, 300], [1, 2, 8], 6), ([300, 190, 500], [90, 33, 70], 140)])
+def test_attention_of_requests_that_pass_the_rows(eng, lens, new, tokens):
+    """Rows past q's end are not there; those before them keep their positions."""
+    rng = np.random.default_rng(tokens)
+    host, table = paged(rng, lens, 16, 2, 128)
+    starts = np.concatenate([[0], np.cumsum(new)])
+    q = rng.standard_normal((starts[-1], 8, 128)).astype(np.float32)
+    want, most, big = ref.attend(q, host, table, lens, starts)
+    out = eng.kv8_attention(cuda(q)[:tokens], host.device(torch), i32(table), i32(lens), i32(starts))
+    assert (np.abs(out.double().cpu().numpy() - want[:tokens]) <= ref.attend_bound(want, most, big, False)).all()
+
+
+@pytest.mark.parametrize("most", [1, 40])
+def test_attention_of_starts_out_of_order(eng, most):
+    """No meaning, but nothing outside the buffers is read or written: finite values, and the guard rows untouched."""
+    rng = np.random.default_rng(most)
+    lens = [100, 800, 40, 300]
+    host, table = paged(rng, lens, 16, 2, 128)
+    q = cuda(rng.standard_normal((60, 8, 128)).astype(np.float32))
+    whole = torch.full((64, 8, 128), 7.0, device="cuda")
+    for starts in ([-9, 5, 2, 9, 60], [2 ** 31 - 1, -2 ** 31, 30, -2, 2 ** 31 - 1], [50, 40, 30, 20, 10], [-2 ** 31] * 5):
+        out = eng.kv8_attention(q, host.device(torch), i32(table), i32(lens), i32(starts), max_q=most, max_kv=800,
+                                out=whole[2:62])
+        assert torch.isfinite(out).all() and (whole[:2] == 7).all() and (whole[62:] == 7).all()
+
+
 def test_attention_with_pages_that_are_not_there(eng):
     """Tokens on pages outside the cache are not seen; a row all of whose pages are missing gives zeros; what lies
     behind a length (any codes, NaN scales, wild table entries) does not matter."""

@@ -42,6 +42,8 @@ struct Work {
     int qtiles;  // workgroups along the rows of the other kernel
     int vec;     // q and out in pieces of 4 values
     long others; // rows of sums that the few kernel has room for; the other kernel's follow
+    long places; // of both
+    int most_parts;  // of a row
     float* part;   // [][dp]: sums of a row over some of its tokens, not yet divided,
     float2* stat;  // and their (maximum, sum of weights)
     int2* parts;   // [tokens][q heads]: of each row, the place of its first part's sums, and how many parts there are
@@ -137,13 +139,15 @@ struct Span {
     int start, n, len;  // first row, rows, tokens
     int tile0, tile1;   // tiles of 64 tokens that any row sees
 };
+__device__ __forceinline__ int row_bound(const AttnArgs& g, int r) { return min(max(0, g.q_start[r]), g.tokens); }
 __device__ __forceinline__ Span span_of(const AttnArgs& g, int r) {
     Span s;
-    s.start = g.q_start[r];
-    s.n = min(g.q_start[r + 1], g.tokens) - s.start;
-    if (s.start < 0) s.n = 0;
+    s.start = row_bound(g, r);
+    s.n = row_bound(g, r + 1) - s.start;
     const long most = (long)g.width << g.c.shift;
-    s.len = g.c.pages ? (int)min((long)max(0, g.kv_lens[r]), most) : 0;
+    // (rows that q does not have are the last ones of their request: what only they would see is as good as not there)
+    const long cut = max(0, g.q_start[r + 1]) - (long)(s.start + s.n);
+    s.len = g.c.pages ? (int)max(0l, min((long)max(0, g.kv_lens[r]), most) - max(0l, cut)) : 0;
     const int lo = g.window > 0 ? max(0, s.len - s.n + 1 - g.window) : 0;
     s.tile0 = lo >> 6;
     s.tile1 = max((s.len + 63) >> 6, s.tile0 + 1);  // (one where there is nothing to see: it gives zeros)
@@ -384,9 +388,10 @@ __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queri
     const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int blocks = (f.shares + 3) / 4, share = block * 4 + wave;
-    if (block >= blocks) {  // rows of no request
-        const int kv = block - blocks, from = g.requests ? max(0, g.q_start[g.requests]) : 0;
-        for (int t = from; t < g.tokens; t++)
+    if (block >= blocks) {  // rows of no request: those before the first one's, and past the last one's
+        const int kv = block - blocks, upto = g.requests ? row_bound(g, 0) : 0;
+        const int from = g.requests ? max(upto, row_bound(g, g.requests)) : 0;
+        for (int t = upto ? 0 : from; t < g.tokens; t = t + 1 == upto ? from : t + 1)
             for (int i = threadIdx.x; i < g.group * c.dim; i += 256) {
                 const int h = i / c.dim;
                 if (i - h * c.dim == 0) f.parts[(long)t * g.q.heads + kv * g.group + h] = make_int2(0, 1);
@@ -846,8 +851,8 @@ __global__ __launch_bounds__(512) void attn_join_kernel(Work f, int rows_of_grou
         const int r = (int)(b / each_n);
         t = to = 0;
         if (r < g.requests) {
-            const int start = g.q_start[r], n = min(g.q_start[r + 1], g.tokens) - start;
-            if (start >= 0 && (which == Join::MANY) == (n * g.group > f.most)) {
+            const int start = row_bound(g, r), n = row_bound(g, r + 1) - start;
+            if ((which == Join::MANY) == (n * g.group > f.most)) {
                 t = start + (int)(b % each_n);
                 to = start + n;
             }
@@ -858,7 +863,7 @@ __global__ __launch_bounds__(512) void attn_join_kernel(Work f, int rows_of_grou
     for (; t < to; t += step_t) {
         const int2 of = f.parts[(long)t * g.q.heads + h];
         const int ns = of.y;
-        if (ns == 1) continue;
+        if (ns <= 1 || ns > f.most_parts) continue;
         // the place of the first part, of the second, and on from there
         const long at0 = which == Join::MANY ? f.many_at(0, t, h) : of.x;
         const long at = which == Join::MANY ? f.many_at(1, t, h) : at0 + rows_of_group;
@@ -875,7 +880,7 @@ __global__ __launch_bounds__(512) void attn_join_kernel(Work f, int rows_of_grou
                     const long place = k ? at + (long)(k - 1) * step : at0;
                     st[e] = make_float2(kNone, 0.0f);
                     x[e] = make_float4(0, 0, 0, 0);
-                    if (k < ns) {
+                    if (k < ns && place >= 0 && place < f.places) {  // (a starts' array out of order may lead past them)
                         st[e] = f.stat[place];
                         x[e] = reinterpret_cast<const float4*>(f.part + place * g.c.dp)[piece];
                     }
@@ -953,6 +958,7 @@ struct AttnPlan {
     Split many;
     long others;
     long part, stat, parts;  // bytes of the parts' sums, and of where they are
+    long places;
 };
 
 static AttnPlan attn_plan(const zt_kv8_attn* a) {
@@ -1004,6 +1010,7 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
     const long all = p.others + (p.many.splits > 1 ? (long)p.many.splits * a->tokens * a->q.heads : 0);
     p.stat = (all * 8 + 15) & ~15l;
     p.part = all * dp * 4;
+    p.places = all;
     p.parts = ((long)a->tokens * a->q.heads * 8 + 15) & ~15l;
     return p;
 }
@@ -1061,7 +1068,7 @@ ZT_EXPORT int zt_kv8_attention(const zt_kv8_attn* a, void* workspace, long works
                      a->requests,      a->width,      a->tokens,       a->window, a->q.heads / a->cache.kv_heads,
                      (float)unit,      (float)(unit - (double)(float)unit)};
     const Work f{g,        p.most, p.shares, p.single, p.many, p.qtiles, rows_vector(a->q, 4, a->type) && rows_vector(a->out, 4, a->type),
-                 p.others, (float*)workspace, (float2*)((char*)workspace + p.part),
+                 p.others, p.places, std::max(p.shares, p.many.splits), (float*)workspace, (float2*)((char*)workspace + p.part),
                  (int2*)((char*)workspace + p.part + p.stat)};
     const bool f32 = a->type == ZT_F32;
     switch (g.c.dp) {
