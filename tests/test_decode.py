@@ -82,11 +82,12 @@ def test_plan_refuses():
     lib = _lib.load()
     names = ("lens add table requests width free count capacity page tokens table_out slots positions q_start lens_out "
              "count_out").split()
-    good = dict(zip(names, (P, P, P, 4, 8, P, P, 16, 16, 9, P, P, P, P, P, P)))
+    good = dict(zip(names, (P, P, P, 4, 8, P, P, 16, 16, 9, P, P, P, P, P + 64, P + 128)))
     for bad in [{n: 0} for n in ("lens", "add", "table", "free", "count", "table_out", "slots", "positions", "q_start",
                                  "lens_out", "count_out", "width", "page")] + [
             dict(requests=-1), dict(width=-1), dict(tokens=-1), dict(capacity=-1), dict(page=24), dict(page=256),
-            dict(slots=P + 4), dict(positions=P + 2), dict(requests=1 << 20, width=1 << 12)]:
+            dict(slots=P + 4), dict(positions=P + 2), dict(requests=1 << 20, width=1 << 12), dict(lens_out=P),
+            dict(count_out=P)]:
         assert lib.zt_kv8_plan(*{**good, **bad}.values(), None) == BAD, bad
 
 

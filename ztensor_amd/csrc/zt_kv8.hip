@@ -534,6 +534,8 @@ ZT_EXPORT int zt_kv8_plan(const int* kv_lens, const int* add, const int* table, 
     for (const void* p : ints)
         if ((uintptr_t)p & 3) return kInvalid;
     if ((uintptr_t)slots & 7) return kInvalid;
+    // other workgroups read these while one writes (a table's row has one workgroup)
+    if ((requests && kv_lens_out == kv_lens) || free_count_out == free_count) return kInvalid;
     PlanArgs g{kv_lens,  add,     table,     free_pages, free_count, requests,    width,         free_capacity, __builtin_ctz(page_tokens),
                tokens,   table_out, positions, q_start,  kv_lens_out, free_count_out, slots};
     plan_kernel<<<requests + 1, kThreads, 0, stream>>>(g);
