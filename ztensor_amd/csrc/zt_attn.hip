@@ -211,6 +211,9 @@ __device__ __forceinline__ void load_query(const Work& f, const Span& sp, int kv
 // a weight is nothing in fp16 beside those of the largest scale; a scale that is
 // not a number stays that.
 constexpr int kWeightBits = 10;
+// A weight in fp16 is off by at most 2^-25 where it is small: from this factor on, that is 2^-29 of the sum's unit for a
+// token, 2^-13 for 65536 of them.
+constexpr float kSumBy = 16.0f;
 struct ValueScale {
     float by, log, inverse;
     int e;  // the tile's exponent, at least the one before
@@ -280,9 +283,11 @@ __device__ __forceinline__ void weights_of(const float4v (&s)[4], const Factor& 
             split_hi_lo(y, p[h], pl[h]);
         }
     } else {
-        // the scale in the exponent, and the sum of the weights as they are rounded
+        // the scale in the exponent; the sum is of the weights as fp16 has them, so that their rounding is the same above and
+        // below, but for pages whose scale is so far below the largest that fp16 holds too little of what they add to it
         const float at = v.log - from;
         const half2v one = {(_Float16)1.0f, (_Float16)1.0f};
+        const bool apart = __any(v.by < kSumBy);
 #pragma unroll
         for (int k = 0; k < 16; k += 2) {
             const half2v w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 2][k & 3], fk.hi, at)),
@@ -292,6 +297,11 @@ __device__ __forceinline__ void weights_of(const float4v (&s)[4], const Factor& 
             p[k >> 3][(k & 7) + 1] = w[1];
         }
         sum *= v.inverse;
+        if (apart) {
+            sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 16; k++) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 2][k & 3], fk.hi, -from));
+        }
     }
     l += sum;
 }
