@@ -1,6 +1,7 @@
-"""Attention over pages whose scales of values are far apart, zero among them,
-against the definition in 64 bits.  Each row, head and dim is held to a bound
-of its own, so that small results beside large ones count."""
+"""Attention over pages whose scales are far apart, or are of no matter: zero
+and tiny scales of values among others, large ones that a row does not see or
+gives no weight, against the definition in 64 bits.  Each row, head and dim is
+held to a bound of its own, so that small results beside large ones count."""
 import numpy as np
 import pytest
 
@@ -18,7 +19,7 @@ def attend(q, host, table, lens, starts, half, window=0):
     scores    operands in 22 bits or more and fp32 sums in chains of at most 16 and 64 terms: each weight's share of
               2^-20 (2 + the row's largest sum of |q k| times the scale), in a and once more in the result (the sum)
     weights   the second product takes them as fp16 (two parts for fp32 rows) times their page's scale, in units of which
-              the row's largest, max p scale, is 2^9 or more: what lies below is rounded to steps of 2^-24, and a code is
+              the row's largest, max p scale, is 2^8 or more: what lies below is rounded to steps of 2^-24, and a code is
               at most 127
     fp16      11 bits of each weight, in a and in their sum, and of the result; of the sum besides steps of 2^-24 where
               the unit is 2^4 or more"""
@@ -113,3 +114,79 @@ def test_many_small_weights_in_the_sum(eng, new, dtype):  # noqa: F811
     host.scales[1, table[0, 0]] = 1.0
     q = np.ones((new, 4, 128))
     check(eng, q, host, table, [4000], [0, new], dtype)
+
+
+@TYPES
+@SIZES
+@pytest.mark.parametrize("ratio", [0.0, 1e-6, 1e-12, 1e-30])
+def test_rows_that_see_small_values_only(eng, ratio, new, dtype):  # noqa: F811
+    """Half of the pages' values are nothing, or nearly, beside the others': rows beside those that see the others, and
+    rows that see the others with little weight, keep the precision of their own."""
+    rng = np.random.default_rng(new)
+    host, table = paged(rng, LENS, 16, 2, 128)
+    host.scales[1] *= np.where(rng.random(host.scales[1].shape) < 0.5, ratio, 1.0).astype(np.float32)
+    q, starts = queries(rng, new, 8, 128)
+    check(eng, q, host, table, LENS, starts, dtype)
+    check(eng, q, host, table, LENS, starts, dtype, max_q=1, max_kv=1)
+
+
+@TYPES
+@SIZES
+@pytest.mark.parametrize("heads,kv,dim,page", [(4, 4, 64, 32), (6, 2, 80, 64), (2, 1, 192, 16), (4, 1, 256, 128)])
+def test_pages_of_any_scale(eng, heads, kv, dim, page, new, dtype):  # noqa: F811
+    """From 1e-18 to 1e3 (fp16 results stay finite), some zero."""
+    rng = np.random.default_rng(dim + new)
+    host, table = paged(rng, LENS, page, kv, dim)
+    shape = host.scales[1].shape
+    host.scales[1] = (np.exp(rng.uniform(-41, 5, shape)) * (rng.random(shape) > 0.2)).astype(np.float32)
+    q, starts = queries(rng, new, heads, dim)
+    check(eng, q, host, table, LENS, starts, dtype)
+
+
+@TYPES
+@SIZES
+@pytest.mark.parametrize("large", [1e4, 1e12, 3e38])
+def test_pages_of_nobody_do_not_matter(eng, large, new, dtype):  # noqa: F811
+    """Lanes past a length, and on pages outside the cache, read page 0: any finite scale there leaves every bit."""
+    rng = np.random.default_rng(new)
+    host, table = paged(rng, LENS, 16, 2, 128)
+    table[2, 3:6] = -1, 1 << 20, len(host.codes[0])
+    q, starts = queries(rng, new, 8, 128)
+    host.scales[:, 0] = 0
+    want = check(eng, q, host, table, LENS, starts, dtype)
+    host.scales[:, 0] = large
+    assert torch.equal(check(eng, q, host, table, LENS, starts, dtype), want)
+
+
+@TYPES
+@SIZES
+def test_tokens_that_a_row_does_not_see_do_not_matter(eng, new, dtype):  # noqa: F811
+    """The last tokens' pages hold values 2^40 times the others' (for fp16 rows the others' are as much smaller, so that
+    results stay finite): the rows before them are what they were.  With a window, tokens behind it likewise."""
+    rng = np.random.default_rng(new)
+    small = np.float32(2.0 ** -32) if dtype == "f16" else np.float32(1)
+    for window in (0, 40):
+        host, table = paged(rng, LENS, 16, 2, 128)
+        host.scales[1] *= small
+        for r, size in enumerate(LENS):
+            host.scales[1, table[r, (size - 1) // 16 if not window else max(0, size - new - window) // 16]] *= np.float32(2.0 ** 40)
+        q, starts = queries(rng, new, 8, 128)
+        qd = cuda(q.astype(np.float32)).to(DT[dtype])
+        want, bound = attend(qd.float().cpu().numpy(), host, table, LENS, starts, dtype == "f16", window)
+        out = eng.kv8_attention(qd, host.device(torch), i32(table), i32(LENS), i32(starts), window=window)
+        assert (np.abs(out.double().cpu().numpy() - want) <= bound).all()
+
+
+@TYPES
+@SIZES
+def test_large_values_of_no_weight(eng, new, dtype):  # noqa: F811
+    """A page whose values are 2^40 times the others', and whose tokens weigh about 2^-65 of theirs."""
+    rng = np.random.default_rng(new)
+    host, table = paged(rng, LENS, 16, 2, 128)
+    host.scales[0] *= 0.05
+    for r in range(len(LENS)):
+        host.codes[0, table[r, 1]] = -127
+        host.scales[0, table[r, 1]] = 45 * np.sqrt(128) / (127 * 128)
+        host.scales[1, table[r, 1]] = 2.0 ** 40
+    q, starts = queries(rng, new, 8, 128)
+    check(eng, 1 + 0.01 * q, host, table, LENS, starts, dtype)

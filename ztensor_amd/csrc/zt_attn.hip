@@ -70,6 +70,8 @@ __device__ __forceinline__ float4v mfma(half8v a, half8v b, float4v c) {
 }
 
 constexpr float kNone = -__builtin_inff();
+constexpr float kNothing = -kMaxFloat;  // of a base: below all finite scores, and none of its own differences is not a number
+constexpr float kWeightBits = 10.0f, kSumBits = 4.0f;
 constexpr float kLog2e = 1.44269504088896340736f, kLog2eLo = (float)(1.44269504088896340736 - (double)kLog2e);
 
 // What makes a product of a query and a key a score in units of log 2, to 48
@@ -126,12 +128,6 @@ __device__ __forceinline__ void store4(T* row, int d, int dim, bool vec, const f
 #pragma unroll
         for (int i = 0; i < 4; i++) row[d + i] = (T)v[i];
     }
-}
-
-// The exponent of a scale of values; none of what is not finite.
-__device__ __forceinline__ int exponent_of(float s) {
-    const int e = (int)(__float_as_uint(s) >> 23 & 255) - 127;
-    return e > 127 ? -127 : e;
 }
 
 // The rows of a request and the tokens that they see, by the device's lengths.
@@ -206,23 +202,28 @@ __device__ __forceinline__ void load_query(const Work& f, const Span& sp, int kv
         }
 }
 
-// The scale of a lane's values in a tile, over the power of two that their
-// weights are brought to: fp16 holds them up to 2^15.  The logarithm stops where
-// a weight is nothing in fp16 beside those of the largest scale; a scale that is
-// not a number stays that.
-constexpr int kWeightBits = 10;
-// A weight in fp16 is off by at most 2^-25 where it is small: from this factor on, that is 2^-29 of the sum's unit for a
-// token, 2^-13 for 65536 of them.
-constexpr float kSumBy = 16.0f;
+// The scale of a lane's values in a tile, and its logarithm: fp16 rows add it to
+// a score, fp32 rows, which multiply a weight by the scale, need a whole number
+// that is not below it.  Of nothing: -inf.
 struct ValueScale {
-    float by, log, inverse;
-    int e;  // the tile's exponent, at least the one before
-    __device__ __forceinline__ ValueScale(float vs, int ev) {
-        const float most = max_step<16>(max_step<32>(finite(vs)));
-        e = max(ev, __builtin_amdgcn_readfirstlane(exponent_of(most)));
-        by = ldexpf(vs, kWeightBits - e);
-        log = by <= 0x1p-60f ? -60.0f : __builtin_amdgcn_logf(by);
-        inverse = __builtin_amdgcn_exp2f(-log);
+    float by, log;
+};
+template <bool SPLIT>
+__device__ __forceinline__ ValueScale value_scale(float vs) {
+    if (SPLIT) return {vs, vs > 0.0f ? (float)__builtin_amdgcn_frexp_expf(vs) : kNone};
+    return {vs, __builtin_amdgcn_logf(vs)};
+}
+
+// What the softmax of one row stands on.  Its sums have two units, each a power
+// of two: l is in units of 2^base, base near the largest score so far, and o in
+// units of 2^(unit - 10), unit near the largest product of a weight and its
+// values' scale.  So fp16 has the weights that matter for o, whatever the scales
+// of pages that the row gives no weight, or does not see.
+struct Base {
+    float base, unit;  // kNothing: nothing yet
+    // the factor `by` of sums in o, for the unit of l
+    __device__ __forceinline__ float o_in_l(float by) const {
+        return ldexpf(by, (int)fminf(fmaxf(unit - base - kWeightBits, -1000.0f), 1000.0f));
     }
 };
 
@@ -232,8 +233,7 @@ struct ValueScale {
 __device__ __forceinline__ void mask_scores(float4v (&s)[4], Factor& fk, ValueScale& v, int t, bool there, int lo, int hi) {
     if (!there || max(t, lo) >= min(t + 16, hi)) {
         fk = {1.0f, 1e-37f};
-        v.by = v.inverse = 1.0f;
-        v.log = 0.0f;
+        v = {1.0f, 1000.0f};  // (a logarithm that asks for nothing: see weights_of)
         hi = 0;
     }
     lo -= t;
@@ -246,27 +246,35 @@ __device__ __forceinline__ void mask_scores(float4v (&s)[4], Factor& fk, ValueSc
 // The weights of a tile's 16 tokens in this lane for one row: scores s times fk
 // in units of log 2, against a base that follows their maximum only when it is
 // passed by more than 2^4 (most tiles move some row's maximum a little; so few
-// of them change l and o, which stand already).  Scales of keys and values are
-// not negative.
+// of them change l and o, which stand already), and as the second product takes
+// them, times the values' scale, against a unit that follows in the same way: at
+// most 2^14 in fp16.  Scales of keys and values are not negative.
 template <bool SPLIT, int N>
-__device__ __forceinline__ void weights_of(const float4v (&s)[4], const Factor& fk, const ValueScale& v, float& base, float& l,
+__device__ __forceinline__ void weights_of(const float4v (&s)[4], const Factor& fk, const ValueScale& v, Base& b, float& l,
                                            float4v (&o)[N], half8v (&p)[2], half8v (&pl)[2]) {
     float top = kNone;
 #pragma unroll
     for (int k = 0; k < 16; k++) top = fmaxf(top, s[k >> 2][k & 3]);
     top *= fk.hi;
-    if (__any(top > base + 4.0f)) {  // (from nothing: to the first that is seen)
-        top = max_step<16>(max_step<32>(top));
-        const bool up = top > base + 4.0f;
-        const float keep = up ? __builtin_amdgcn_exp2f(base - top) : 1.0f;
-        base = up ? top : base;
-        l *= keep;
+    const float most = top + v.log;
+    if (__any(top > b.base + 4.0f || most > b.unit + 4.0f)) {  // (from nothing: to the first that is seen)
+        auto follow = [](float& at, float x) {
+            x = ceilf(max_step<16>(max_step<32>(x)));
+            const bool up = x > at + 4.0f;
+            const float keep = up ? __builtin_amdgcn_exp2f(at - x) : 1.0f;
+            at = up ? x : at;
+            return keep;
+        };
+        l *= follow(b.base, top);
+        const float keep = follow(b.unit, most);
 #pragma unroll
         for (int i = 0; i < N; i++) o[i] *= keep;
     }
-    const float from = base == kNone ? 0.0f : base;
+    const float from = b.base, unit = b.unit - kWeightBits;
     float sum = 0.0f;
     if constexpr (SPLIT) {
+        float by = ldexpf(v.by, (int)fminf(from - unit, 1000.0f));
+        by = by > 0x1p100f ? 0x1p100f : by;  // (of weights that are nothing: 0 times it is not to be NaN)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             float y[8];
@@ -275,7 +283,7 @@ __device__ __forceinline__ void weights_of(const float4v (&s)[4], const Factor& 
                 const float x = s[2 * h + (k >> 2)][k & 3];
                 const float z = __builtin_amdgcn_exp2f(__builtin_fmaf(x, fk.hi, __builtin_fmaf(x, fk.lo, -from)));
                 sum += z;
-                y[k] = z * v.by;
+                y[k] = z * by;
                 // one value for both parts: fused into the conversion of one of them, the product would round to another
                 // fp16 near a tie, and the parts would be off by its last bit
                 asm("" : "+v"(y[k]));
@@ -283,11 +291,13 @@ __device__ __forceinline__ void weights_of(const float4v (&s)[4], const Factor& 
             split_hi_lo(y, p[h], pl[h]);
         }
     } else {
-        // the scale in the exponent; the sum is of the weights as fp16 has them, so that their rounding is the same above and
-        // below, but for pages whose scale is so far below the largest that fp16 holds too little of what they add to it
-        const float at = v.log - from;
+        // The scale in the exponent; fp16 holds 11 bits of a weight.  l adds the weights up as fp16 has them, so that their
+        // rounding is the same above and below, but for pages whose scale is so far below that fp16 holds too little of
+        // what they add to it: off by at most 2^-25 each where they are small, from 2^kSumBits on that is 2^-29 of l's unit
+        // for a token, 2^-13 for 65536 of them.
+        const float at = v.log - unit;
         const half2v one = {(_Float16)1.0f, (_Float16)1.0f};
-        const bool apart = __any(v.by < kSumBy);
+        const bool apart = __any(at + from < kSumBits);
 #pragma unroll
         for (int k = 0; k < 16; k += 2) {
             const half2v w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 2][k & 3], fk.hi, at)),
@@ -296,7 +306,7 @@ __device__ __forceinline__ void weights_of(const float4v (&s)[4], const Factor& 
             p[k >> 3][k & 7] = w[0];
             p[k >> 3][(k & 7) + 1] = w[1];
         }
-        sum *= v.inverse;
+        sum *= __builtin_amdgcn_exp2f(-(at + from));
         if (apart) {
             sum = 0.0f;
 #pragma unroll
@@ -320,13 +330,13 @@ struct Pages {
 // the sum that the other splits' are to be added to.
 template <class T, int DN>
 __device__ __forceinline__ void store_row(const Work& f, const Span& sp, int kv, int row, int rows, bool part, long at,
-                                          float top, float sum, int ev, const float4v (&o)[4 * DN]) {
+                                          const Base& b, float sum, const float4v (&o)[4 * DN]) {
     if (row >= rows) return;
     const AttnArgs& g = f.a;
     const int i = row / g.group, h = kv * g.group + row - i * g.group, quad = (threadIdx.x & 63) >> 4;
     const long t = sp.start + i;
-    const float by = ldexpf(part ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum, ev - kWeightBits);
-    if (part && quad == 0) f.stat[at] = make_float2(top, sum);
+    const float by = b.o_in_l(part ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum);
+    if (part && quad == 0) f.stat[at] = make_float2(b.base, sum);
     T* out = (T*)g.out.p + t * g.out.token + (long)h * g.out.head;
 #pragma unroll
     for (int k = 0; k < 4 * DN; k++) {
@@ -381,8 +391,8 @@ __device__ __forceinline__ long wave_scan(long v) {
 // lane's queries lie in LDS for itself.
 //
 // Weights enter the second product times their page's scale over a power of two
-// (the largest so far, 2^(e - 10)): fp16 then holds 35 bits below the largest.
-// fp32 rows: queries and weights in two fp16 parts (22 bits).
+// that keeps the row's largest such product so far in 2^8 to 2^14: fp16 then holds
+// 32 bits below it.  fp32 rows: queries and weights in two fp16 parts (22 bits).
 //
 // The codes bound it: 64 sequences of up to 8000 tokens (8 heads of 128, fp32,
 // pages of 32) 306 MB in 63 us, 4.9 TB/s, the rate of a large copy; one of 40011
@@ -495,11 +505,11 @@ __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queri
         const int all_lo = g.window > 0 ? max(0, sp.len - sp.n + row1 / g.group + 1 - g.window) : 0;
 
         float4v o[CT][4 * DN];
-        float m[CT], l[CT];
-        int ev = -127;
+        Base m[CT];
+        float l[CT];
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
-            m[ct] = kNone;
+            m[ct] = {kNothing, kNothing};
             l[ct] = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4 * DN; i++) o[ct][i] = (float4v){0, 0, 0, 0};
@@ -526,7 +536,7 @@ __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queri
             pk = page_of(t0 + 64 + (col >> 2) * 16);
             pv = page_of(t0 + 64 + quad * 16);
 
-            const ValueScale scales(vs, ev);
+            const ValueScale scales = value_scale<SPLIT>(vs);
 
             float4v s[CT][4];
 #pragma unroll
@@ -548,12 +558,6 @@ __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queri
                     }
 
             half8v p[CT][2], pl[CT][2];
-            if (scales.e != ev) {  // a larger scale of values than any before
-#pragma unroll
-                for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                    for (int i = 0; i < 4 * DN; i++) o[ct][i] *= ldexpf(1.0f, ev - scales.e);
-            }
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
                 Factor fk = times<SPLIT>(factor[ct], ks);
@@ -561,7 +565,6 @@ __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queri
                 if (!whole) mask_scores(s[ct], fk, v, t0 + 16 * quad, seen, g.window > 0 ? hi[ct] - g.window : 0, hi[ct]);
                 weights_of<SPLIT>(s[ct], fk, v, m[ct], l[ct], o[ct], p[ct], pl[ct]);
             }
-            ev = scales.e;
 #pragma unroll
             for (int i = 0; i < 4 * DN; i++)
 #pragma unroll
@@ -583,7 +586,7 @@ __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queri
             const int row = (cg * CT + ct) * 16 + col, i = row / g.group;
             if (into == 0 && row < rows && quad == 0)
                 f.parts[(long)(sp.start + i) * g.q.heads + kv * g.group + row - i * g.group] = make_int2((int)at, parts);
-            store_row<T, DN>(f, sp, kv, row, rows, n < tiles, at, m[ct], l[ct], ev, o[ct]);
+            store_row<T, DN>(f, sp, kv, row, rows, n < tiles, at, m[ct], l[ct], o[ct]);
         }
     }
 }
@@ -672,11 +675,11 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
         const int all_lo = g.window > 0 ? max(0, sp.len - sp.n + row1 / g.group + 1 - g.window) : 0;
 
         float4v o[CT][4 * DN];
-        float m[CT], l[CT];
-        int ev = -127;
+        Base m[CT];
+        float l[CT];
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
-            m[ct] = kNone;
+            m[ct] = {kNothing, kNothing};
             l[ct] = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4 * DN; i++) o[ct][i] = (float4v){0, 0, 0, 0};
@@ -735,7 +738,7 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
             pv = page_of(t0 + 128 + quad * 16);
             const half8v* from = tiles + buffer * FRAGS * 64 + lane;
 
-            const ValueScale scales(fvs, ev);
+            const ValueScale scales = value_scale<SPLIT>(fvs);
 
             // four fragments ahead of the products that take them, sums that depend on each other 8 products apart
             half8v frag[2][4];
@@ -772,12 +775,6 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
             }
             __builtin_amdgcn_s_setprio(0);
             half8v p[CT][2], pl[CT][2];
-            if (scales.e != ev) {  // a larger scale of values than any before
-#pragma unroll
-                for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                    for (int i = 0; i < 4 * DN; i++) o[ct][i] *= ldexpf(1.0f, ev - scales.e);
-            }
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
                 Factor fk = times<SPLIT>(factor[ct], fs);
@@ -785,7 +782,6 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
                 if (!whole) mask_scores(s[ct], fk, v, t0 + 16 * quad, there, g.window > 0 ? hi[ct] - g.window : 0, hi[ct]);
                 weights_of<SPLIT>(s[ct], fk, v, m[ct], l[ct], o[ct], p[ct], pl[ct]);
             }
-            ev = scales.e;
             put(buffer ^ 1);
 #pragma unroll
             for (int j = 0; j < 2 * DN; j++) {
@@ -817,7 +813,7 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
             if (f.many.splits > 1 && split == 0 && row < rows && quad == 0)
                 f.parts[(long)(sp.start + i) * g.q.heads + kv * g.group + row - i * g.group] = make_int2(0, ns);
             store_row<T, DN>(f, sp, kv, row, rows, ns > 1, f.many_at(split, sp.start + i, kv * g.group + row - i * g.group), m[ct],
-                             l[ct], ev, o[ct]);
+                             l[ct], o[ct]);
         }
     }
 }
