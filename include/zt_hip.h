@@ -709,9 +709,11 @@ typedef struct zt_kv8_cache {
 } zt_kv8_cache;
 
 /* Puts the keys and values of `tokens` tokens at their slots (page *
- * page_tokens + place; outside the cache: that token is left out).  Tokens of
- * one page stand next to each other in ascending order, and no page comes
- * twice, as zt_kv8_plan gives them.  A page's scale becomes the largest of
+ * page_tokens + place; outside the cache, -1 for one: that token is left out).
+ * Tokens of one page stand next to each other, as zt_kv8_plan gives them; those
+ * left out may stand between, and places may be passed over.  A page whose
+ * tokens stand in two places, or a slot that comes twice, gives values without
+ * a meaning in that page.  A page's scale becomes the largest of
  * what it was (0 if the page's first place is among the slots: it starts
  * anew, its other places become 0) and the new values' largest magnitude
  * times 1/127; where it grows, the codes that the page holds are taken over as

@@ -152,26 +152,38 @@ __device__ __forceinline__ int code_of(float x, float scale) {
     return (int)fminf(fmaxf(q, -127.0f), 127.0f);
 }
 
-// The n tokens from t on, which go to one page from place `off` on: the page's
-// new scale, and its codes by way of an image of it in LDS.
+// The tokens of one page: n of them, from token t on.
+struct Run {
+    int t, n, page, off;
+    bool fresh;  // one of them is the page's first
+    // tokens and places one after the other, from t and `off` on; else as listed: tokens from t on, and their places
+    bool dense;
+    const int* listed;
+    const uint8_t* places;
+    __device__ __forceinline__ int token(int i) const { return t + (dense ? i : listed[i]); }
+    __device__ __forceinline__ int place(int i) const { return dense ? off + i : places[i]; }
+};
+
+// A run's tokens into their page: its new scale, and its codes by way of an image
+// of it in LDS.
 template <class T, int V, bool VALUES>
-__device__ __forceinline__ void append_page(const AppendArgs& g, int t, int n, int page, int off, int head,
-                                            uint32_t* image, float* red) {
+__device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run, int head, uint32_t* image, float* red) {
     const Kv8& c = g.c;
     const Rows& x = g.x[VALUES];
     Turn turn = g.turn;
     if (VALUES) turn.half = 0;
     const int units = units_of<V>(c.dim, turn.half);
-    const T* rows = (const T*)x.p + (long)t * x.token + (long)head * x.head;
+    const int n = run.n;
+    const T* rows = (const T*)x.p + (long)head * x.head;
     float a[V], b[V];
     int first, second;
 
     float m = 0.0f;
     bool bad = false;
     for (int i = threadIdx.x; i < n * units; i += kThreads) {
-        const int tl = i / units, u = i - tl * units;
-        const int pos = turn.half ? turn.positions[t + tl] : 0;
-        turned<T, V>(rows + tl * x.token, u, pos, turn, a, b, first, second);
+        const int tl = i / units, u = i - tl * units, t = run.token(tl);
+        const int pos = turn.half ? turn.positions[t] : 0;
+        turned<T, V>(rows + (long)t * x.token, u, pos, turn, a, b, first, second);
 #pragma unroll
         for (int j = 0; j < V; j++) {
             m = fmaxf(m, fmaxf(fabsf(a[j]), fabsf(b[j])));
@@ -181,14 +193,16 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, int t, int n, i
     block_peak(m, bad, red);
 
     float* scales = VALUES ? c.v_scale : c.k_scale;
-    const long place = (long)page * c.heads + head;
-    const bool fresh = off == 0;
-    const float had = fresh ? 0.0f : scales[place];
+    const long at = (long)run.page * c.heads + head;
+    const bool fresh = run.fresh;
+    const float had = fresh ? 0.0f : scales[at];
     const float now = bad || had != had ? __builtin_nanf("") : fmaxf(had, m * (1.0f / 127.0f));
     const bool grown = now > had, whole = fresh || grown;
-    u32x4* codes = reinterpret_cast<u32x4*>((VALUES ? c.v : c.k) + c.at(page, head));
+    u32x4* codes = reinterpret_cast<u32x4*>((VALUES ? c.v : c.k) + c.at(run.page, head));
     u32x4* image4 = reinterpret_cast<u32x4*>(image);
-    const int pieces = c.bytes() / 16;
+    // 16 bytes each: all of the page, or, of keys of a page that goes on with its scale, the new tokens' rows
+    const int row = c.dp / 16, pieces = whole ? c.bytes() / 16 : n * row;
+    auto piece = [&](int i) { return whole ? i : run.dense ? run.off * row + i : run.place(i / row) * row + i % row; };
     const float ratio = grown ? had / now : 0.0f;
     if (grown && !fresh) {
         for (int i = threadIdx.x; i < pieces; i += kThreads) {
@@ -204,43 +218,112 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, int t, int n, i
             image4[i] = w;
         }
     } else if (whole || !VALUES) {  // zeros where nothing new comes; of a page that goes on, its new keys' rows
-        const int lo = whole ? 0 : off * c.dp / 16, hi = whole ? pieces : (off + n) * c.dp / 16;
-        for (int i = lo + threadIdx.x; i < hi; i += kThreads) image4[i] = (u32x4){0, 0, 0, 0};
+        for (int i = threadIdx.x; i < pieces; i += kThreads) image4[piece(i)] = (u32x4){0, 0, 0, 0};
     }
     __syncthreads();  // (the scale has been read by everybody, too)
 
     int8_t* bytes = reinterpret_cast<int8_t*>(image);
     const float step = now > 0.0f ? now : 1.0f;  // 1 for a NaN, whose codes nobody takes for values
     for (int i = threadIdx.x; i < n * units; i += kThreads) {
-        const int tl = i / units, u = i - tl * units;
-        const int pos = turn.half ? turn.positions[t + tl] : 0;
-        turned<T, V>(rows + tl * x.token, u, pos, turn, a, b, first, second);
+        const int tl = i / units, u = i - tl * units, t = run.token(tl);
+        const int pos = turn.half ? turn.positions[t] : 0;
+        turned<T, V>(rows + (long)t * x.token, u, pos, turn, a, b, first, second);
+        const int place = run.place(tl);
 #pragma unroll
         for (int j = 0; j < V; j++) {
             const int p = code_of(a[j], step), q = code_of(b[j], step);
             if (VALUES) {
-                bytes[(first + j) * c.page + off + tl] = (int8_t)p;
-                bytes[(second + j) * c.page + off + tl] = (int8_t)q;
+                bytes[(first + j) * c.page + place] = (int8_t)p;
+                bytes[(second + j) * c.page + place] = (int8_t)q;
             } else {
-                bytes[(off + tl) * c.dp + first + j] = (int8_t)p;
-                bytes[(off + tl) * c.dp + second + j] = (int8_t)q;
+                bytes[place * c.dp + first + j] = (int8_t)p;
+                bytes[place * c.dp + second + j] = (int8_t)q;
             }
         }
     }
     __syncthreads();
 
     if (whole || !VALUES) {
-        const int lo = whole ? 0 : off * c.dp / 16, hi = whole ? pieces : (off + n) * c.dp / 16;
-        for (int i = lo + threadIdx.x; i < hi; i += kThreads) codes[i] = image4[i];
+        for (int i = threadIdx.x; i < pieces; i += kThreads) codes[piece(i)] = image4[piece(i)];
     } else {
         int8_t* out = reinterpret_cast<int8_t*>(codes);
         for (int i = threadIdx.x; i < c.dim * n; i += kThreads) {
-            const int d = i / n, at = d * c.page + off + i - d * n;
-            out[at] = bytes[at];
+            const int d = i / n, to = d * c.page + run.place(i - d * n);
+            out[to] = bytes[to];
         }
     }
-    if (threadIdx.x == 0) scales[place] = now;
+    if (threadIdx.x == 0) scales[at] = now;
     __syncthreads();  // the image is free again
+}
+
+// The page of a slot; none (-1) of one outside the cache.
+__device__ __forceinline__ int page_of(const Kv8& c, long slot) {
+    return slot >= 0 && slot < (long)c.pages << c.shift ? (int)(slot >> c.shift) : -1;
+}
+
+struct Found {
+    int dense;  // tokens from the run's first on, one after the other
+    int end;    // the first token of another page
+    int last;   // the last token of this one's
+    int count;  // of a list
+    int fresh;
+};
+
+// The tokens on the page of token t, whose slot is s: up to the first that is on
+// another page, without those that are left out.
+__device__ __forceinline__ Run run_from(const AppendArgs& g, int t, long s, Found& found, int* listed, uint8_t* places) {
+    const Kv8& c = g.c;
+    const int tid = threadIdx.x, left = g.tokens - t;
+    Run run{t, 0, (int)(s >> c.shift), (int)(s & (c.page - 1)), false, true, listed, places};
+    const int most = min(c.page - run.off, left);
+    if (tid == 0) found = {most, left, 0, 0, 0};
+    __syncthreads();
+    auto look = [&](int i, long x, bool first) {  // token t + i, of the 64 of this wave, has slot x
+        const int p = i < left ? page_of(c, x) : -1, from = i - (tid & 63);
+        const uint64_t other = __ballot(p >= 0 && p != run.page), same = __ballot(p == run.page);
+        const uint64_t gap = first ? __ballot(i < most && x != s + i) : 0;
+        if ((tid & 63) == 0) {
+            if (gap) atomicMin(&found.dense, from + __builtin_ctzll(gap));
+            if (other) atomicMin(&found.end, from + __builtin_ctzll(other));
+            if (same) atomicMax(&found.last, from + 63 - __builtin_clzll(same));
+        }
+    };
+    look(tid, tid < left ? g.slots[t + tid] : -1, true);
+    __syncthreads();
+    // (a page that ends the step, or is followed by many tokens that are left out)
+    constexpr int kAhead = 8;
+    for (int i0 = kThreads; i0 < left && found.end >= i0; i0 += kAhead * kThreads) {
+        long x[kAhead];
+#pragma unroll
+        for (int e = 0; e < kAhead; e++) x[e] = i0 + e * kThreads + tid < left ? g.slots[(long)t + i0 + e * kThreads + tid] : -1;
+        __syncthreads();  // everybody has seen that the run goes on
+#pragma unroll
+        for (int e = 0; e < kAhead; e++) look(i0 + e * kThreads + tid, x[e], false);
+        __syncthreads();
+    }
+    run.n = found.dense;
+    run.fresh = run.off == 0;
+    const int end = min(found.end, found.last + 1);
+    if (end <= run.n) return run;
+    // some of its tokens come after a gap: a list of all
+    run.dense = false;
+    for (int i0 = 0; i0 < end; i0 += kThreads) {
+        const long x = i0 + tid < end ? g.slots[(long)t + i0 + tid] : -1;
+        const bool mine = page_of(c, x) == run.page;
+        const uint64_t all = __ballot(mine);
+        int at = 0;
+        if ((tid & 63) == 0 && all) at = atomicAdd(&found.count, __builtin_popcountll(all));
+        at = __shfl(at, 0) + __builtin_popcountll(all & ((1ull << (tid & 63)) - 1));
+        if (mine && at < c.page) {  // (more would be a slot that comes twice)
+            listed[at] = i0 + tid;
+            places[at] = (uint8_t)(x & (c.page - 1));
+            if ((x & (c.page - 1)) == 0) found.fresh = 1;
+        }
+    }
+    __syncthreads();
+    run.n = min(found.count, c.page);
+    run.fresh = found.fresh;
+    return run;
 }
 
 // A page's scale s' = max(s, amax / 127), its codes rint(c s / s') where it grew,
@@ -250,9 +333,10 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, int t, int n, i
 // lie token-minor, and go out as whole 16 bytes instead of one byte a line.
 // No atomics on memory, and no order among workgroups.
 //
-// A workgroup looks at 64 tokens: those that do not go on from the one before,
-// in its page, begin a page's tokens.  It takes every turns-th of them.  q's
-// rotation rides along as more workgroups, instead of a launch of its own.
+// A workgroup looks at 64 tokens: those whose page is not that of the one before
+// (tokens that are left out do not come between) begin a page's tokens.  It takes
+// every turns-th of them, each with all that follow on its page.  q's rotation
+// rides along as more workgroups, instead of a launch of its own.
 //
 // One token for each of 64 sequences (8 heads of 128, pages of 64, fp32): 10.4
 // us, where a page that grows is read and written, and the chain slot - scale -
@@ -262,7 +346,9 @@ template <class T, int V, int VQ>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, RopeArgs q) {
     extern __shared__ __align__(16) uint32_t image[];  // of one page and head
     __shared__ float red[4];
-    __shared__ int count;
+    __shared__ Found found;
+    __shared__ int listed[128];
+    __shared__ uint8_t places[128];
     if (blockIdx.x >= g.blocks) {
         rope_block<T, VQ>(q, blockIdx.x - g.blocks);
         return;
@@ -272,27 +358,31 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, RopeArgs
     const int values = b & 1, head = (b >> 1) % c.heads;
     b = (b >> 1) / c.heads;
     const int turn = b % g.turns, from = b / g.turns * 64, lane = threadIdx.x & 63;
-    const long slots = (long)c.pages << c.shift;
-    const long here = from + lane < g.tokens ? g.slots[from + lane] : -1;
-    long last = __shfl_up(here, 1);
-    if (lane == 0) last = from > 0 ? g.slots[from - 1] : -1;
-    const bool goes_on = (here & (c.page - 1)) != 0 && last == here - 1;
-    uint64_t begin = __ballot(here >= 0 && here < slots && !goes_on);
+    auto slot = [&](long t) { return t >= 0 && t < g.tokens ? g.slots[t] : -1l; };
+    const long here = slot(from + lane), behind = slot((long)from - 1 - lane);
+    const int page = page_of(c, here);
+    const uint64_t stored = __ballot(page >= 0);
+    if (!stored) return;
+    // the page of the last token before these that is stored
+    int last = page_of(c, behind);
+    uint64_t any = __ballot(last >= 0);
+    for (long t = (long)from - 65; !any && t >= 0; t -= 64) {
+        last = page_of(c, slot(t - lane));
+        any = __ballot(last >= 0);
+    }
+    last = any ? __shfl(last, __builtin_ctzll(any)) : -1;
+    const uint64_t below = stored & ((1ull << lane) - 1);
+    const int before = __shfl(page, below ? 63 - __builtin_clzll(below) : lane);
+    uint64_t begin = __ballot(page >= 0 && page != (below ? before : last));
     for (int left = turn; begin; begin &= begin - 1) {
         if (left-- > 0) continue;
         left = g.turns - 1;
-        const int i = __builtin_ctzll(begin), t = from + i;
-        const long s = __shfl(here, i);
-        const int off = (int)(s & (c.page - 1));
-        if (threadIdx.x == 0) count = min(c.page - off, g.tokens - t);
-        __syncthreads();
-        if ((int)threadIdx.x < count && g.slots[t + threadIdx.x] != s + threadIdx.x) atomicMin(&count, (int)threadIdx.x);
-        __syncthreads();
-        const int n = count, page = (int)(s >> c.shift);
+        const int i = __builtin_ctzll(begin);
+        const Run run = run_from(g, from + i, __shfl(here, i), found, listed, places);
         if (values)
-            append_page<T, V, true>(g, t, n, page, off, head, image, red);
+            append_page<T, V, true>(g, run, head, image, red);
         else
-            append_page<T, V, false>(g, t, n, page, off, head, image, red);
+            append_page<T, V, false>(g, run, head, image, red);
     }
 }
 

@@ -217,8 +217,11 @@ class DecodeOps:
         into a new tensor or q_out, which is returned.
 
         A page's scale grows where the new values need it, and the codes that
-        it holds are rounded to the new scale; a page that starts anew forgets
-        what it held.  Tokens whose slot is outside the cache are left out."""
+        it holds are rounded to the new scale; a page that starts anew (its
+        first place is among the slots) forgets what it held.  Tokens whose
+        slot is outside the cache (-1) are left out, wherever they stand: a
+        step's rejected tokens for instance.  The others of one page stand
+        next to each other but for those, each slot once."""
         rows, pack = self._rows, _ROWS.pack
         krows, vrows = rows(k, "k"), rows(v, "v")
         tokens, heads, dim = k.shape
