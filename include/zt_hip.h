@@ -742,8 +742,8 @@ int zt_kv8_dequant(const zt_kv8_cache* cache, const int* pages, int n, float* ke
  * row (or whose length would pass 2^31 - 1), gets none: its tokens' slots are
  * -1 and its length stays.  Tokens past the last request's, up to `tokens`,
  * get slot -1 and position 0.  Negative lengths count as 0.  free_capacity: the
- * entries of free_pages.  kv_lens_out and free_count_out are not kv_lens and
- * free_count, else InvalidValue. */
+ * entries of free_pages.  What is written shares no bytes with what is read, but
+ * for table_out that is table, nor with each other, else InvalidValue. */
 int zt_kv8_plan(const int* kv_lens, const int* add, const int* table, int requests, int width, const int* free_pages,
                 const int* free_count, int free_capacity, int page_tokens, int tokens, int* table_out, long* slots,
                 int* positions, int* q_start, int* kv_lens_out, int* free_count_out, zt_stream_t stream);

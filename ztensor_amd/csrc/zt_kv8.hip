@@ -609,6 +609,15 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs g) {
 
 }  // namespace zt
 
+struct Bytes {
+    const void* p;
+    long n;
+    bool meets(const Bytes& o) const {
+        const uintptr_t a = (uintptr_t)p, b = (uintptr_t)o.p;
+        return n > 0 && o.n > 0 && a < b + o.n && b < a + n;
+    }
+};
+
 ZT_EXPORT int zt_kv8_plan(const int* kv_lens, const int* add, const int* table, int requests, int width,
                           const int* free_pages, const int* free_count, int free_capacity, int page_tokens, int tokens,
                           int* table_out, long* slots, int* positions, int* q_start, int* kv_lens_out,
@@ -624,8 +633,17 @@ ZT_EXPORT int zt_kv8_plan(const int* kv_lens, const int* add, const int* table, 
     for (const void* p : ints)
         if ((uintptr_t)p & 3) return kInvalid;
     if ((uintptr_t)slots & 7) return kInvalid;
-    // other workgroups read these while one writes (a table's row has one workgroup)
-    if ((requests && kv_lens_out == kv_lens) || free_count_out == free_count) return kInvalid;
+    // what one workgroup writes the others do not read (a table's row has one workgroup: it may be written in place)
+    const long row = 4l * requests, rows = row * width;
+    const Bytes in[] = {{kv_lens, row}, {add, row}, {free_pages, 4l * free_capacity}, {free_count, 4}, {table, rows}};
+    const Bytes out[] = {{slots, 8l * tokens},  {positions, 4l * tokens}, {q_start, row + 4},
+                         {kv_lens_out, row}, {free_count_out, 4},      {table_out, rows}};
+    for (const Bytes& o : out) {
+        for (const Bytes& i : in)
+            if (o.meets(i) && !(o.p == table_out && i.p == table && table_out == table)) return kInvalid;
+        for (const Bytes& other : out)
+            if (&other < &o && o.meets(other)) return kInvalid;
+    }
     PlanArgs g{kv_lens,  add,     table,     free_pages, free_count, requests,    width,         free_capacity, __builtin_ctz(page_tokens),
                tokens,   table_out, positions, q_start,  kv_lens_out, free_count_out, slots};
     plan_kernel<<<requests + 1, kThreads, 0, stream>>>(g);
