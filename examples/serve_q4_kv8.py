@@ -77,10 +77,12 @@ class Server:
         self.free, self.free_count = torch.arange(pages, **i32), torch.tensor([pages], **i32)
 
     def step(self, tokens, new, max_q, max_kv):
-        """Hidden states of `tokens`, new[r] of them of request r."""
+        """Hidden states of `tokens`, new[r] of them of request r.  Where self.took[r] is false the pages did not suffice:
+        the request's length stays, and its hidden states have no meaning."""
         p = self.m.e.kv8_plan(self.lens, new, self.table, self.free, self.free_count, self.page_tokens, tokens.numel(),
                               in_place=True)
         x = self.m.forward(tokens, p, self.caches, max_q, max_kv)
+        self.took = p.kv_lens == self.lens + new
         self.lens.copy_(p.kv_lens)
         self.free_count.copy_(p.free_count)
         return x, p
@@ -94,27 +96,31 @@ class Server:
         self.lens[r] = 0
 
 
-def generate(engine, prompts, steps, layers=2, seed=1, **sampling):
-    """Tokens of each request: the prompts together, then one token of each a step."""
+def generate(engine, prompts, steps, layers=2, seed=1, pages=64, **sampling):
+    """Tokens of each request: the prompts together, then one token of each a step; -1 in steps for which a request got
+    no page (it goes on where it was once there is one)."""
     with torch.cuda.stream(engine.stream):
         model = Model(engine, layers=layers)
         r = len(prompts)
-        server = Server(model, r)
+        server = Server(model, r, pages)
         most = max(map(len, prompts)) + steps
         dev = engine.device
         gen = torch.Generator(device=dev).manual_seed(seed)
         new = torch.tensor([len(p) for p in prompts], dtype=torch.int32, device=dev)
         x, p = server.step(torch.tensor(sum(prompts, []), device=dev), new, max(map(len, prompts)), most)
+        if not bool(server.took.all()):
+            raise RuntimeError(f"{pages} pages do not hold the prompts")
         logits = engine.matmul(x[p.q_start[1:].long() - 1], model.head)
         token, _ = engine.sample(logits, torch.rand(r, device=dev, generator=gen), **sampling)
-        out = [token.clone()]
+        out, given = [token.clone()], token.clone()
         one = torch.ones(r, dtype=torch.int32, device=dev)
         u = torch.empty(r, device=dev)
 
         def decode():
             x, _ = server.step(token, one, 1, most)
             t, _ = engine.sample(engine.matmul(x, model.head), u, **sampling)
-            token.copy_(t)
+            given.copy_(torch.where(server.took, t, -1))
+            token.copy_(torch.where(server.took, t, token))
 
         graph = None
         for i in range(steps - 1):
@@ -127,7 +133,7 @@ def generate(engine, prompts, steps, layers=2, seed=1, **sampling):
                 decode()
             else:
                 graph.replay()
-            out.append(token.clone())
+            out.append(given.clone())
         torch.cuda.synchronize()
         return model, server, torch.stack(out, 1)
 

@@ -738,9 +738,11 @@ int zt_kv8_dequant(const zt_kv8_cache* cache, const int* pages, int n, float* ke
  * Token t of the step, the requests' tokens in their order, gets its slot and
  * its position, request r's are q_start[r] .. q_start[r + 1] - 1 (requests + 1
  * values), kv_lens_out[r] = kv_lens[r] + add[r], and free_count_out is what is
- * left of the list.  A request whose pages are not there, or do not fit its
- * row (or whose length would pass 2^31 - 1), gets none: its tokens' slots are
- * -1 and its length stays.  Tokens past the last request's, up to `tokens`,
+ * left of the list.  A request whose pages are not there (or were not for one
+ * before it), or do not fit its row (or whose length would pass 2^31 - 1), gets
+ * none: its tokens' slots are -1 and its length stays, by which a caller can
+ * tell.  Its rows are in q_start all the same, and what zt_kv8_attention makes
+ * of them has no meaning.  Tokens past the last request's, up to `tokens`,
  * get slot -1 and position 0.  Negative lengths count as 0.  free_capacity: the
  * entries of free_pages.  What is written shares no bytes with what is read, but
  * for table_out that is table, nor with each other, else InvalidValue. */
@@ -757,7 +759,8 @@ int zt_kv8_plan(const int* kv_lens, const int* add, const int* table, int reques
  * and softmax in fp32.  A row that sees nothing (no length, pages outside the
  * cache) gives zeros, and so do rows that belong to no request (before
  * q_start[0], or past the last one's).  A request's rows past `tokens` are not
- * there; starts that are not in order give values without a meaning.  Tokens on a
+ * there; starts that are not in order give values without a meaning, and so do
+ * rows whose tokens zt_kv8_plan refused: they would be the last held.  Tokens on a
  * page outside the cache are not seen.  max_q and max_kv are bounds that the
  * host knows for the largest n and length (they choose the launch; a larger
  * one is still computed).  Workspace: zt_kv8_attention_workspace_bytes (-1

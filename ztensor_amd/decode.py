@@ -274,8 +274,11 @@ class DecodeOps:
         all (or more: the rest get slot -1).  New pages come off the end of the
         first free_count (int32 [1]) of free_pages; a request that finds too
         few, or whose row of block_table (int32 [requests, width]) is full,
-        gets none: its slots are -1 and its length stays.  in_place: the new
-        pages are written into block_table itself, not a copy."""
+        gets none, nor do those after it that want some: their slots are -1
+        and their lengths stay (kv_lens[r] as it was, though new[r] > 0).
+        Their rows in q_start are still theirs; what kv8_attention gives for
+        them has no meaning, and no token is to be drawn from it.  in_place:
+        the new pages are written into block_table itself, not a copy."""
         r, width = block_table.shape
         dense, i32, one = self._dense, torch.int32, (r,)
         args = (dense(kv_lens, "kv_lens", i32, one), dense(new, "new", i32, one),
@@ -303,7 +306,8 @@ class DecodeOps:
         [1] on the device, 1 / sqrt(head_dim) without.  max_q, max_kv: bounds
         of the rows and the length of one request (without, what q and
         block_table allow): they choose the launch, not the result's meaning.
-        Rows that see nothing are zeros."""
+        Rows that see nothing are zeros.  A request whose step kv8_plan
+        refused has rows, but no tokens for them: values without a meaning."""
         if out is None:
             out = _like(q)
         elif out.shape != q.shape:
