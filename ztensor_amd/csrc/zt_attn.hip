@@ -37,6 +37,7 @@ struct Work {
     AttnArgs a;
     int most;    // requests of up to so many rows (a row: a token and one of the heads of a group) are the few kernel's
     int shares;  // waves of the few kernel
+    int empties; // workgroups of a key/value head for the rows of no request
     bool single; // each takes whole heads
     Split many;
     int qtiles;  // workgroups along the rows of the other kernel
@@ -409,14 +410,16 @@ __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queri
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int blocks = (f.shares + 3) / 4, share = block * 4 + wave;
     if (block >= blocks) {  // rows of no request: those before the first one's, and past the last one's
-        const int kv = block - blocks, upto = g.requests ? row_bound(g, 0) : 0;
-        const int from = g.requests ? max(upto, row_bound(g, g.requests)) : 0;
-        for (int t = upto ? 0 : from; t < g.tokens; t = t + 1 == upto ? from : t + 1)
+        const int kv = (block - blocks) % c.heads, upto = g.requests ? row_bound(g, 0) : 0;
+        const int from = g.requests ? max(upto, row_bound(g, g.requests)) : 0, rows = upto + g.tokens - from;
+        for (long row = (block - blocks) / c.heads; row < rows; row += f.empties) {
+            const int t = (int)(row < upto ? row : from + row - upto);
             for (int i = threadIdx.x; i < g.group * c.dim; i += 256) {
                 const int h = i / c.dim;
                 if (i - h * c.dim == 0) f.parts[(long)t * g.q.heads + kv * g.group + h] = make_int2(0, 1);
                 ((T*)g.out.p)[(long)t * g.out.token + (long)(kv * g.group + h) * g.out.head + i - h * c.dim] = (T)0.0f;
             }
+        }
         return;
     }
     if (share >= f.shares) return;
@@ -958,7 +961,7 @@ static bool attn_ok(const zt_kv8_attn* a) {
 // How a call is launched.
 struct AttnPlan {
     int ct;  // column tiles of a wave of the few kernel
-    int most, shares, qtiles;
+    int most, shares, qtiles, empties;
     int few_n, many_n;  // bounds of the tokens of one request
     bool single, wide;
     Split many;
@@ -989,6 +992,9 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
     // eight waves to join a row of more than 16 parts (one sequence of 40011 tokens, 128 parts: 26 us, with one 37), else
     // one (64 sequences 70 us, with eight 80)
     p.wide = p.shares > 16 * requests * heads * groups;
+    // Any row may be of no request (a batch padded to a graph's size): a workgroup zeroes one in 0.3 us (8 heads, group
+    // 4), so one for 16 rows, up to about the card's 1024 in all (4096 padded rows 50 us, by one a head 1210).
+    p.empties = (int)std::max(1l, std::min({(a->tokens + 15) / 16l, 64l, 1024 / heads}));
     p.others = 2l * p.shares * 16 * p.ct;
     p.many_n = std::max(1, std::min(a->max_q, a->tokens));
     p.few_n = std::max(1, std::min(p.many_n, 64 / group));
@@ -1024,7 +1030,7 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
 template <class T, int DN>
 static int launch(const Work& f, const AttnPlan& p, hipStream_t stream) {
     const long tiled = (long)p.qtiles * p.many.splits * f.a.c.heads * f.a.requests;
-    const int few = (f.shares + 3) / 4 + f.a.c.heads;
+    const int few = (f.shares + 3) / 4 + f.a.c.heads * f.empties;
     if (tiled + few >= 1l << 31) return kInvalid;
     constexpr int column = DN * 2 * (sizeof(T) / 2) * 4096;  // LDS of the few kernel, at most 64 KB in all
     if (tiled) {
@@ -1073,7 +1079,7 @@ ZT_EXPORT int zt_kv8_attention(const zt_kv8_attn* a, void* workspace, long works
     const AttnArgs g{kv8_of(a->cache), rows_of(a->q), rows_of(a->out), a->table, a->kv_lens, a->q_start, a->scale,
                      a->requests,      a->width,      a->tokens,       a->window, a->q.heads / a->cache.kv_heads,
                      (float)unit,      (float)(unit - (double)(float)unit)};
-    const Work f{g,        p.most, p.shares, p.single, p.many, p.qtiles, rows_vector(a->q, 4, a->type) && rows_vector(a->out, 4, a->type),
+    const Work f{g,        p.most, p.shares, p.empties, p.single, p.many, p.qtiles, rows_vector(a->q, 4, a->type) && rows_vector(a->out, 4, a->type),
                  p.others, p.places, std::max(p.shares, p.many.splits), (float*)workspace, (float2*)((char*)workspace + p.part),
                  (int2*)((char*)workspace + p.part + p.stat)};
     const bool f32 = a->type == ZT_F32;
