@@ -765,7 +765,8 @@ int zt_kv8_plan(const int* kv_lens, const int* add, const int* table, int reques
  * host knows for the largest n and length (they choose the launch; a larger
  * one is still computed).  Workspace: zt_kv8_attention_workspace_bytes (-1
  * for a call that is refused), 16-byte aligned; short or missing ->
- * InvalidValue.  Results do not depend on what else runs. */
+ * InvalidValue, and so are 2^31 - 256 or more rows of heads.  Results do not
+ * depend on what else runs. */
 typedef struct zt_kv8_attn {
     zt_kv8_cache cache;
     zt_rows q;

@@ -137,6 +137,12 @@ struct Span {
     int tile0, tile1;   // tiles of 64 tokens that any row sees
 };
 __device__ __forceinline__ int row_bound(const AttnArgs& g, int r) { return min(max(0, g.q_start[r]), g.tokens); }
+// The first token that token i of a request's n sees.  (Lengths and windows may be up to 2^31 - 1: what may pass that is
+// a long, or unsigned.)
+__device__ __forceinline__ int first_seen(const AttnArgs& g, int len, int n, int i) {
+    return g.window > 0 ? (int)max(0l, (long)len - n + i + 1 - g.window) : 0;
+}
+__device__ __forceinline__ int tiles_up_to(int token) { return (int)(((unsigned)token + 63) >> 6); }
 __device__ __forceinline__ Span span_of(const AttnArgs& g, int r) {
     Span s;
     s.start = row_bound(g, r);
@@ -145,9 +151,8 @@ __device__ __forceinline__ Span span_of(const AttnArgs& g, int r) {
     // (rows that q does not have are the last ones of their request: what only they would see is as good as not there)
     const long cut = max(0, g.q_start[r + 1]) - (long)(s.start + s.n);
     s.len = g.c.pages ? (int)max(0l, min((long)max(0, g.kv_lens[r]), most) - max(0l, cut)) : 0;
-    const int lo = g.window > 0 ? max(0, s.len - s.n + 1 - g.window) : 0;
-    s.tile0 = lo >> 6;
-    s.tile1 = max((s.len + 63) >> 6, s.tile0 + 1);  // (one where there is nothing to see: it gives zeros)
+    s.tile0 = first_seen(g, s.len, s.n, 0) >> 6;
+    s.tile1 = max(tiles_up_to(s.len), s.tile0 + 1);  // (one where there is nothing to see: it gives zeros)
     return s;
 }
 
@@ -229,16 +234,17 @@ struct Base {
 };
 
 // Of a tile's 16 tokens in this lane, t on, what a row does not see: tokens that
-// are not `there`, before lo or from hi on.  Their scores become -inf; of a lane
-// in which it sees none the scales may be anything, and are set aside.
-__device__ __forceinline__ void mask_scores(float4v (&s)[4], Factor& fk, ValueScale& v, int t, bool there, int lo, int hi) {
-    if (!there || max(t, lo) >= min(t + 16, hi)) {
+// are not `there`, from hi on, or (window > 0) not among the last `window` before
+// that.  Their scores become -inf; of a lane in which it sees none the scales may
+// be anything, and are set aside.
+__device__ __forceinline__ void mask_scores(float4v (&s)[4], Factor& fk, ValueScale& v, int t, bool there, int window, int hi) {
+    hi -= t;
+    const int lo = window > 0 ? hi - window : 0;
+    if (!there || hi <= 0 || lo >= 16) {
         fk = {1.0f, 1e-37f};
         v = {1.0f, 1000.0f};  // (a logarithm that asks for nothing: see weights_of)
         hi = 0;
     }
-    lo -= t;
-    hi -= t;
 #pragma unroll
     for (int k = 0; k < 16; k++)
         if (k < lo || k >= hi) s[k >> 2][k & 3] = kNone;
@@ -323,8 +329,8 @@ __device__ __forceinline__ void weights_of(const float4v (&s)[4], const Factor& 
 struct Pages {
     const int* row;
     int len, shift;
-    __device__ __forceinline__ int operator()(int token) const { return len > 0 ? row[min(token, len - 1) >> shift] : -1; }
-    __device__ __forceinline__ bool seen(const Kv8& c, int page, int token) const { return token < len && c.holds(page); }
+    __device__ __forceinline__ int operator()(unsigned token) const { return len > 0 ? row[min(token, (unsigned)len - 1) >> shift] : -1; }
+    __device__ __forceinline__ bool seen(const Kv8& c, int page, unsigned token) const { return token < (unsigned)len && c.holds(page); }
 };
 
 // What a lane holds of a row, dims 16 i + 4 (lane / 16) .. +4: the result, or
@@ -505,7 +511,7 @@ __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queri
         // every row of these columns sees tokens all_lo .. all_hi - 1
         const int row0 = cg * 16 * CT, row1 = min(rows, row0 + 16 * CT) - 1;
         const int all_hi = sp.len - sp.n + row0 / g.group + 1;
-        const int all_lo = g.window > 0 ? max(0, sp.len - sp.n + row1 / g.group + 1 - g.window) : 0;
+        const int all_lo = first_seen(g, sp.len, sp.n, row1 / g.group);
 
         float4v o[CT][4 * DN];
         Base m[CT];
@@ -534,10 +540,10 @@ __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queri
             const float ks = c.k_scale[(long)at * c.heads + kv], vs = c.v_scale[(long)at * c.heads + kv];
 #pragma unroll
             for (int i = 0; i < 4 * DN; i++) vw[i] = *reinterpret_cast<const u32x4*>(vp + (long)16 * i * c.page);
-            const bool whole = t0 + 64 <= all_hi && t0 >= all_lo && __all(seen);
+            const bool whole = t0 <= all_hi - 64 && t0 >= all_lo && __all(seen);
             // the next tile's pages, while this one's codes are on their way
-            pk = page_of(t0 + 64 + (col >> 2) * 16);
-            pv = page_of(t0 + 64 + quad * 16);
+            pk = page_of(t0 + 64u + (col >> 2) * 16);
+            pv = page_of(t0 + 64u + quad * 16);
 
             const ValueScale scales = value_scale<SPLIT>(vs);
 
@@ -565,7 +571,7 @@ __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queri
             for (int ct = 0; ct < CT; ct++) {
                 Factor fk = times<SPLIT>(factor[ct], ks);
                 ValueScale v = scales;
-                if (!whole) mask_scores(s[ct], fk, v, t0 + 16 * quad, seen, g.window > 0 ? hi[ct] - g.window : 0, hi[ct]);
+                if (!whole) mask_scores(s[ct], fk, v, t0 + 16 * quad, seen, g.window, hi[ct]);
                 weights_of<SPLIT>(s[ct], fk, v, m[ct], l[ct], o[ct], p[ct], pl[ct]);
             }
 #pragma unroll
@@ -617,9 +623,8 @@ __device__ __forceinline__ RowTiles tiles_of(const AttnArgs& g, const Span& sp, 
     RowTiles w;
     w.row0 = row / kRows<DN> * kRows<DN>;
     const int last = min(w.row0 + kRows<DN>, sp.n * g.group) - 1;
-    const int lo = g.window > 0 ? max(0, sp.len - sp.n + w.row0 / g.group + 1 - g.window) : 0;
-    w.tile0 = lo >> 6;
-    w.tile1 = max((max(0, sp.len - sp.n + last / g.group + 1) + 63) >> 6, w.tile0);
+    w.tile0 = first_seen(g, sp.len, sp.n, w.row0 / g.group) >> 6;
+    w.tile1 = max(tiles_up_to(max(0, sp.len - sp.n + last / g.group + 1)), w.tile0);
     return w;
 }
 
@@ -675,7 +680,7 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
         for (int ct = 0; ct < CT; ct++)
             load_query<T, DN>(f, sp, kv, row0 + 16 * ct + col, rows, scale, q[ct], ql[ct], factor[ct], hi[ct]);
         const int all_hi = sp.len - sp.n + row0 / g.group + 1;
-        const int all_lo = g.window > 0 ? max(0, sp.len - sp.n + row1 / g.group + 1 - g.window) : 0;
+        const int all_lo = first_seen(g, sp.len, sp.n, row1 / g.group);
 
         float4v o[CT][4 * DN];
         Base m[CT];
@@ -697,7 +702,7 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
         const uint32_t k_lane = ((krow + 4 * wave) & (c.page - 1)) * c.dp + 16 * quad + head_bytes;
         const uint32_t v_lane = (16 * DN * wave + col) * c.page + ((16 * quad) & (c.page - 1)) + head_bytes;
         auto fetch = [&](int tile, int pk, int pv) {
-            const int t0 = tile * 64, in = t0 & (c.page - 1);
+            const unsigned t0 = tile * 64u, in = t0 & (c.page - 1);
             seen = page_of.seen(c, pv, t0 + 16 * quad);
             const uint32_t p = seen ? pv : 0, q = page_of.seen(c, pk, t0 + (col >> 2) * 16) ? pk : 0;
             const int8_t* kp = c.k + ((uint64_t)q * page_bytes + (k_lane + in * c.dp));
@@ -725,8 +730,8 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
         __syncthreads();  // nobody reads the buffers of the rows before any more
         if (first < last) {
             fetch(first, pk, pv);
-            pk = page_of(first * 64 + 64 + (col >> 2) * 16);
-            pv = page_of(first * 64 + 64 + quad * 16);
+            pk = page_of(first * 64 + 64u + (col >> 2) * 16);
+            pv = page_of(first * 64 + 64u + quad * 16);
             put(0);
         }
         __syncthreads();
@@ -734,11 +739,11 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
             const int t0 = tile * 64;
             const float fs = ks, fvs = vs;
             const bool there = seen;
-            const bool whole = t0 + 64 <= all_hi && t0 >= all_lo && __all(there);
+            const bool whole = t0 <= all_hi - 64 && t0 >= all_lo && __all(there);
             // (past the last tile: of the last token's page, for nobody)
             fetch(tile + 1, pk, pv);
-            pk = page_of(t0 + 128 + (col >> 2) * 16);
-            pv = page_of(t0 + 128 + quad * 16);
+            pk = page_of(t0 + 128u + (col >> 2) * 16);
+            pv = page_of(t0 + 128u + quad * 16);
             const half8v* from = tiles + buffer * FRAGS * 64 + lane;
 
             const ValueScale scales = value_scale<SPLIT>(fvs);
@@ -782,7 +787,7 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
             for (int ct = 0; ct < CT; ct++) {
                 Factor fk = times<SPLIT>(factor[ct], fs);
                 ValueScale v = scales;
-                if (!whole) mask_scores(s[ct], fk, v, t0 + 16 * quad, there, g.window > 0 ? hi[ct] - g.window : 0, hi[ct]);
+                if (!whole) mask_scores(s[ct], fk, v, t0 + 16 * quad, there, g.window, hi[ct]);
                 weights_of<SPLIT>(s[ct], fk, v, m[ct], l[ct], o[ct], p[ct], pl[ct]);
             }
             put(buffer ^ 1);
@@ -955,7 +960,7 @@ static bool attn_ok(const zt_kv8_attn* a) {
     return a && kv8_ok(a->cache) && type_ok(a->type) && a->reserved == 0 && a->requests >= 0 && a->width >= 1 &&
            a->tokens >= 0 && a->max_q >= 0 && a->max_kv >= 0 && a->window >= 0 && a->q.heads >= 1 &&
            a->q.heads == a->out.heads && a->q.heads % a->cache.kv_heads == 0 && a->q.heads <= 1 << 16 &&
-           (long)a->tokens * a->q.heads < (1l << 31) && (long)a->requests * a->width < (1l << 31);
+           (long)a->tokens * a->q.heads < (1l << 31) - 256 && (long)a->requests * a->width < (1l << 31);
 }
 
 // How a call is launched.

@@ -323,7 +323,7 @@ class DecodeOps:
         a = _ATTN.pack(*c, *qrows, *orows, dense(block_table, "block_table", i32, (r, width)),
                        dense(kv_lens, "kv_lens", i32, (r,)), dense(q_start, "q_start", i32, (r + 1,)),
                        dense(scale, "scale", torch.float32, (1,)), r, width, tokens, tokens if max_q is None else max_q,
-                       width * c[7] if max_kv is None else max_kv, window, t, 0)
+                       min(width * c[7], 0x7FFFFFFF) if max_kv is None else max_kv, window, t, 0)
         ws, wsb = self._workspace(self.lib.zt_kv8_attention_workspace_bytes(a))
         self.lib.call("zt_kv8_attention", a, ws, wsb, self._s)
         return out
