@@ -721,7 +721,8 @@ typedef struct zt_kv8_cache {
  * that is not finite makes its page's scale NaN, so that no reader takes the
  * page for sound.  With `table` the keys are turned first (zt_rope's rule
  * in fp32, not rounded in between), and q into q_out in the same launch; q,
- * q_out NULL: none.  table NULL: keys as they are, positions are not read. */
+ * q_out NULL: none.  table NULL: keys as they are, positions are not read.
+ * tokens below 2^30, else InvalidValue. */
 int zt_kv8_append(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v, const long* slots, const zt_rows* q,
                   const zt_rows* q_out, const int* positions, const float* table, int tokens, int rot_dim, int max_pos,
                   int type, int flags, zt_stream_t stream);
@@ -745,7 +746,8 @@ int zt_kv8_dequant(const zt_kv8_cache* cache, const int* pages, int n, float* ke
  * of them has no meaning.  Tokens past the last request's, up to `tokens`,
  * get slot -1 and position 0.  Negative lengths count as 0.  free_capacity: the
  * entries of free_pages.  What is written shares no bytes with what is read, but
- * for table_out that is table, nor with each other, else InvalidValue. */
+ * for table_out that is table, nor with each other, and requests * width is
+ * below 2^31 - 256, requests below 2^24, else InvalidValue. */
 int zt_kv8_plan(const int* kv_lens, const int* add, const int* table, int requests, int width, const int* free_pages,
                 const int* free_count, int free_capacity, int page_tokens, int tokens, int* table_out, long* slots,
                 int* positions, int* q_start, int* kv_lens_out, int* free_count_out, zt_stream_t stream);

@@ -698,7 +698,7 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
         float ks, vs;
         bool seen;
         // (a tile begins at a multiple of 64: what a lane adds to that stays in the page, or is taken modulo its tokens)
-        const uint32_t page_bytes = (uint32_t)(c.heads * c.bytes()), head_bytes = (uint32_t)(kv * c.bytes());
+        const uint32_t page_bytes = (uint32_t)c.heads * c.bytes(), head_bytes = (uint32_t)kv * c.bytes();
         const uint32_t k_lane = ((krow + 4 * wave) & (c.page - 1)) * c.dp + 16 * quad + head_bytes;
         const uint32_t v_lane = (16 * DN * wave + col) * c.page + ((16 * quad) & (c.page - 1)) + head_bytes;
         auto fetch = [&](int tile, int pk, int pv) {

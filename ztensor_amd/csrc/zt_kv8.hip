@@ -391,7 +391,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, RopeArgs
 ZT_EXPORT int zt_kv8_append(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v, const long* slots,
                             const zt_rows* q, const zt_rows* q_out, const int* positions, const float* table, int tokens,
                             int rot_dim, int max_pos, int type, int flags, zt_stream_t stream) {
-    if (!cache || !kv8_ok(*cache) || !k || !v || tokens < 0 || !type_ok(type) || (flags & ~ZT_ROPE_INTERLEAVED) ||
+    if (!cache || !kv8_ok(*cache) || !k || !v || tokens < 0 || tokens >= 1l << 30 || !type_ok(type) || (flags & ~ZT_ROPE_INTERLEAVED) ||
         (q == nullptr) != (q_out == nullptr) || (q && !table))
         return kInvalid;
     const int dim = cache->head_dim, half = table ? rot_dim / 2 : 0;
@@ -623,7 +623,7 @@ ZT_EXPORT int zt_kv8_plan(const int* kv_lens, const int* add, const int* table, 
                           int* table_out, long* slots, int* positions, int* q_start, int* kv_lens_out,
                           int* free_count_out, zt_stream_t stream) {
     if (requests < 0 || width < 1 || tokens < 0 || free_capacity < 0 || !page_tokens_ok(page_tokens) ||
-        (long)requests * width >= 1l << 31 || requests >= 1 << 24)
+        (long)requests * width >= (1l << 31) - 256 || requests >= 1 << 24)
         return kInvalid;
     if (requests && (!kv_lens || !add || !table || !table_out || !kv_lens_out)) return kInvalid;
     if ((free_capacity && !free_pages) || !free_count || !free_count_out || !q_start || (tokens && (!slots || !positions)))
