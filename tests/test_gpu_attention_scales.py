@@ -190,3 +190,23 @@ def test_large_values_of_no_weight(eng, new, dtype):  # noqa: F811
         host.scales[1, table[r, 1]] = 2.0 ** 40
     q, starts = queries(rng, new, 8, 128)
     check(eng, 1 + 0.01 * q, host, table, LENS, starts, dtype)
+
+
+@pytest.mark.parametrize("new", [1, 2, 5])
+@pytest.mark.parametrize("before", [0, 63, 200])
+def test_a_weight_that_is_all_is_one(eng, before, new):  # noqa: F811
+    """fp16 rows that see one token, or give the others nothing: its values, rounded once (and fp32 sums), since the
+    sum's weight is rounded as the product's is.  The columns beside them have no rows, or rows that see nothing."""
+    rng = np.random.default_rng(before)
+    host, table = paged(rng, [before + new], 16, 1, 128)
+    host.codes[0], host.scales[0] = 0, 0.1
+    for i in range(new):  # token before + i answers to value i of a query alone
+        host.codes[0, table[0, (before + i) // 16], 0, (before + i) % 16, i] = 127
+    q = np.zeros((new, 4, 128))
+    for i in range(new):
+        q[i, :, i] = 60
+    qd = cuda(q.astype(np.float16))
+    want, _ = attend(q, host, table, [before + new], [0, new], True)
+    out = eng.kv8_attention(qd, host.device(torch), i32(table), i32([before + new]), i32([0, new]))
+    far = np.abs(out.double().cpu().numpy() - want)
+    assert (far <= np.abs(want) * (2.0 ** -11 + 2.0 ** -18) + 2.0 ** -25).all(), float((far / np.abs(want)).max())

@@ -302,9 +302,10 @@ __device__ __forceinline__ void weights_of(const float4v (&s)[4], const Factor& 
         // rounding is the same above and below, but for pages whose scale is so far below that fp16 holds too little of
         // what they add to it: off by at most 2^-25 each where they are small, from 2^kSumBits on that is 2^-29 of l's unit
         // for a token, 2^-13 for 65536 of them.
-        const float at = v.log - unit;
+        // (Of a row that has seen nothing, base and unit are the same: it does not ask for that.)
+        const float at = v.log - unit, bits = v.log + kWeightBits + (from - b.unit);
         const half2v one = {(_Float16)1.0f, (_Float16)1.0f};
-        const bool apart = __any(at + from < kSumBits);
+        const bool apart = __any(bits < kSumBits);
 #pragma unroll
         for (int k = 0; k < 16; k += 2) {
             const half2v w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 2][k & 3], fk.hi, at)),
@@ -313,7 +314,7 @@ __device__ __forceinline__ void weights_of(const float4v (&s)[4], const Factor& 
             p[k >> 3][k & 7] = w[0];
             p[k >> 3][(k & 7) + 1] = w[1];
         }
-        sum *= __builtin_amdgcn_exp2f(-(at + from));
+        sum *= __builtin_amdgcn_exp2f(-bits);
         if (apart) {
             sum = 0.0f;
 #pragma unroll
