@@ -77,7 +77,8 @@ constexpr float kLog2e = 1.44269504088896340736f, kLog2eLo = (float)(1.442695040
 
 // What makes a product of a query and a key a score in units of log 2, to 48
 // bits: an error in it is one of every score in the same direction, and grows
-// with them.
+// with them.  fp16 rows take the first 24 (lo stays out): a score of 100 is then
+// off by 2^-17, far below the 11 bits that its weight is held in.
 struct Factor {
     float hi, lo;
 };
@@ -364,8 +365,8 @@ __device__ __forceinline__ void store_row(const Work& f, const Span& sp, int kv,
 // ends: sequences of any lengths keep all CUs busy to the end.  What a share
 // holds of a head's tiles goes to `out` if it is all of them, else to the
 // share's place for its first part or its last.
-// That place counts as four tiles: 64 sequences of up to 8000 tokens, fp16, 87 us at one, 74 at two, 68 at four or
-// seven; fp32 74, 68, 67 and 68.  Where the host knows of few tiles, a head's are one place: nothing is split, nothing
+// That place counts as four tiles: 64 sequences of up to 8000 tokens, fp16, 89 us at one, 77 at two, 70 at four or
+// seven; fp32 80, 70, 72 and 73.  Where the host knows of few tiles, a head's are one place: nothing is split, nothing
 // to be joined.
 constexpr int kBegin = 4;
 __device__ __forceinline__ int begin_of(const Work& f) { return f.single ? 0 : kBegin; }
@@ -403,10 +404,11 @@ __device__ __forceinline__ long wave_scan(long v) {
 // 32 bits below it.  fp32 rows: queries and weights in two fp16 parts (22 bits).
 //
 // The codes bound it: 64 sequences of up to 8000 tokens (8 heads of 128, fp32,
-// pages of 32) 306 MB in 63 us, 4.9 TB/s, the rate of a large copy; one of 40011
-// (fp16, pages of 64) 82 MB in 21.6 us, 3.8 TB/s, of which about 5 us are the
-// launch and the chain from the lengths to the first codes; 37 tokens 8.6 us, all
-// of it that chain.
+// pages of 32) 306 MB in 65 us, 4.7 TB/s, near the rate of a large copy; one of
+// 40011 (fp16, pages of 64) 82 MB in 20.3 us, 4.0 TB/s, of which about 5 us are
+// the launch and the chain from the lengths to the first codes; 37 tokens 8.9 us,
+// all of it that chain.  fp32 rows of two columns keep 24 registers in memory at
+// 128 dims, and fp32 rows 78, fp16 rows 25 at 256.
 template <class T, int DN, int CT>
 __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queries) {  // [4 waves][CT][DN][2][PARTS][64]
     constexpr bool SPLIT = sizeof(T) == 4;
@@ -638,13 +640,14 @@ __device__ __forceinline__ RowTiles tiles_of(const AttnArgs& g, const Span& sp, 
 // buffer after it: one barrier a tile.
 //
 // Two workgroups a CU.  Three prompts (187 GFLOP, 32 heads over 8 of 128, fp16)
-// 247 us, 0.75 PFLOP/s, one call after the other (up to 290 as the first).  A tile of one wave
-// is 64 matrix instructions (1024 cycles) and some 340 of the vector unit (1800
-// cycles with the exponentials), which bounds it: 80 decode its share of the
-// codes, 5 for each of its scores are the softmax's.  The last fifth of the time
-// is a tail with half of the workgroups; splitting those along their tokens makes
-// parts to be joined and costs more (272 us: 387 with tiles in 24s, 474 in 32s),
-// dealing a late row tile and an early one to one workgroup 273.
+// 243 us, 0.77 PFLOP/s, one call after the other (290 for the first ones, before
+// the clock has settled).  A tile of one wave is 64 matrix instructions (1024
+// cycles) and some 360 of the vector unit (1800 cycles with the exponentials),
+// which bounds it: 80 decode its share of the codes, 5 for each of its scores are
+// the softmax's.  The last fifth of the time is a tail with half of the
+// workgroups.  fp32 rows take twice the products in two fp16 parts: 364 us, 1.03
+// PFLOP/s of them, with 38 registers kept in memory; at 256 dims those are 84, of
+// fp16 rows 24.
 template <class T, int DN>
 __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {  // [2][FRAGS][64]
     constexpr bool SPLIT = sizeof(T) == 4;
@@ -827,8 +830,7 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
     }
 }
 
-// The other kernel's workgroups come last in the same launch: they are there while the tiled ones run out (a prompt of
-// 100 tokens 13.5 us, with two launches 15.6; three of up to 4096 252 and 258).
+// The other kernel's workgroups come last in the same launch: they are there while the tiled ones run out.
 template <class T, int DN>
 __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f, int tiled) {
     extern __shared__ __align__(16) half8v shared[];
@@ -846,7 +848,7 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f, int tiled) {
 // the other kernel's.
 //
 // It reads the parts (512 bytes each at 128 dims) after where they are, two loads
-// that wait for each other: the 64 rows of one long sequence, in 128 parts, 4.2
+// that wait for each other: the 64 rows of one long sequence, in 128 parts, 4.3
 // us; 64 sequences' 2048 rows 4.8.
 enum class Join { ROWS, FEW, MANY };
 template <class T, int DN, int W>
@@ -981,22 +983,22 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
     const int group = a->q.heads / a->cache.kv_heads, dp = (a->cache.head_dim + 63) & ~63;
     const long requests = std::max(1, a->requests), heads = a->cache.kv_heads;
     const long most = (long)std::min(a->max_q, a->tokens) * group;
-    // up to 64 rows by the few kernel: 32 requests of 3000 tokens, 64 rows 91 us, by the other 95; 128 rows 136 and 110
+    // up to 64 rows by the few kernel: 32 requests of 3000 tokens, 64 rows 88 us, by the other 97; 128 rows 124 and 103
     p.most = most <= 64 ? 0x7FFFFFFF : 64;
-    // of more than 16 rows two columns of them share what is read of a tile (those requests, 32 rows: 67 us, one by one
-    // 81); past 128 dims their sums would leave no registers
+    // of more than 16 rows two columns of them share what is read of a tile (those requests, 32 rows: 66 us, one by one
+    // 80); past 128 dims their sums would leave no registers
     p.ct = most > 16 && dp <= 128 ? 2 : 1;
     long kv = std::min((long)a->max_kv, (long)a->width * a->cache.page_tokens);
     if (a->window > 0) kv = std::min(kv, (long)a->window + a->max_q + 63);
     const long tiles = std::max(1l, (kv + 63) / 64);
     // A tile each as far as the bounds go, up to a wave for each SIMD: fewer leave some without work, each more makes
-    // parts to be joined (one sequence of 40011 tokens 25.6 us, with 512 32.6, with 2048 27.4; 64 of up to 8000 68, 96
-    // and 70).
+    // parts to be joined (one sequence of 40011 tokens 25.4 us, with 512 29.7, with 2048 28.1; 64 of up to 8000 69, 95
+    // and 73).
     const long groups = (std::max(1l, std::min(most, 64l)) + 16 * p.ct - 1) / (16 * p.ct);
     p.single = tiles <= 2;
     p.shares = (int)std::min(1024l, requests * heads * groups * (p.single ? 1 : tiles + kBegin));
-    // eight waves to join a row of more than 16 parts (one sequence of 40011 tokens, 128 parts: 26 us, with one 37), else
-    // one (64 sequences 70 us, with eight 80)
+    // eight waves to join a row of more than 16 parts (one sequence of 40011 tokens, 128 parts: 25 us, with one 39), else
+    // one (64 sequences 70 us, with eight 81)
     p.wide = p.shares > 16 * requests * heads * groups;
     // Any row may be of no request (a batch padded to a graph's size): a workgroup zeroes one in 0.3 us (8 heads, group
     // 4), so one for 16 rows, up to about the card's 1024 in all (4096 padded rows 50 us, by one a head 1210).
@@ -1009,8 +1011,8 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
         p.qtiles = ceil_div(most, dp <= 128 ? 128 : 64);
         // Along the tokens where that is less time: a tile of 128 rows and dims is 2.2 us while the card's 512 workgroups
         // are not passed, the parts are written and read at 4.5 TB/s, a launch 4 us.  (32 heads over 8 of 128, fp16, one
-        // sequence: 100 tokens onto 4000 42 us in 16 splits, 124 whole; 1000 onto 4000 129 in two, 151 whole; 1500 from
-        // the beginning 83 in two, 63 whole.)
+        // sequence: 100 tokens onto 4000 41 us in 16 splits, 120 whole; 1000 onto 4000 127 in two, 150 whole; 700 from
+        // the beginning 40 in two, 32 whole.)
         const long have = requests * heads * p.qtiles;
         const double tile = 2.2 * dp / (dp <= 128 ? 128 : 256), part = 8.0 * a->tokens * a->q.heads * dp / 4.5e6;
         long splits = 1;

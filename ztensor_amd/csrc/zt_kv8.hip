@@ -338,10 +338,11 @@ __device__ __forceinline__ Run run_from(const AppendArgs& g, int t, long s, Foun
 // every turns-th of them, each with all that follow on its page.  q's rotation
 // rides along as more workgroups, instead of a launch of its own.
 //
-// One token for each of 64 sequences (8 heads of 128, pages of 64, fp32): 10.4
-// us, where a page that grows is read and written, and the chain slot - scale -
-// page - codes is what a workgroup waits for.  Prompts of 1955 tokens in all
-// (fp16, 64 + 8 heads, pages of 16): 76 MB, 64 of them q, in 23 us, 3.3 TB/s.
+// One token for each of 64 sequences (8 heads of 128, pages of 64, fp32): 10.3
+// us, where a page that grows is read and written; a workgroup waits for its
+// slots, its rows, their largest, the scale and the codes one after the other.
+// Prompts of 1955 tokens in all (fp16, 64 + 8 heads, pages of 16): 76 MB, 64 of
+// them q, in 22.6 us, 3.4 TB/s.
 template <class T, int V, int VQ>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, RopeArgs q) {
     extern __shared__ __align__(16) uint32_t image[];  // of one page and head
@@ -416,9 +417,9 @@ ZT_EXPORT int zt_kv8_append(const zt_kv8_cache* cache, const zt_rows* k, const z
     g.turn = {positions, table, half, max_pos, flags};
     g.tokens = tokens;
     // a workgroup for each token while they are few (a batch's next tokens, each on a page of its own: with the pages'
-    // values read back, 64 sequences 28 us, with 8 workgroups for 64 tokens 47), else for eight: a prompt's tokens mostly
+    // values read back, 64 sequences 28 us, with 8 workgroups for 64 tokens 45), else for eight: a prompt's tokens mostly
     // go on in their page, and a workgroup that finds none to do costs its launch (pages of 16, prompts of 1955 tokens:
-    // 38 us, with 16 43, 32 52, 4 36; but 512 sequences' single tokens 154, 154, 157 and 176)
+    // 38 us, with 16 44, 32 55, 4 36; but 512 sequences' single tokens 150, 152, 152 and 169)
     g.turns = tokens <= 256 ? 64 : 8;
     g.blocks = 2l * cache->kv_heads * ceil_div(tokens, 64) * g.turns;
     const int lds = g.c.bytes();

@@ -241,9 +241,9 @@ __device__ __forceinline__ void sample_row(const SampleArgs& g, int b, const Sco
 // The logits are read three times, from the Infinity Cache after the first: 128
 // rows of 100003 fp32 (51 MB) take 10.4 us in (1), the rate of a copy, 16.6 in
 // (2), bound by LDS atomics and exponentials, 24 in (3), 5 of them until its cuts
-// are known, and 20 in (4), most of it the sort of up to 2048 tokens (23 with a
-// barrier after each of its steps).  One row, 50 tokens to sort: 3.5, 2.5, 8.4
-// and 8.1 us, chains of a few loads, sums over a workgroup, and launches.
+// are known, and 20 in (4), most of it the sort of up to 2048 tokens; (4) keeps 6
+// registers in memory.  One row, 50 tokens to sort: 3.5, 2.5, 8.5 and 8.1 us,
+// chains of a few loads, sums over a workgroup, and launches.
 constexpr int kBins = kSampleThreads;
 constexpr int kSplits = 64;    // most workgroups of a row
 constexpr int kWaves = kSampleThreads / 64;
