@@ -4,13 +4,13 @@
  * operators of a decode step between those matmuls.
  *
  * Every entry point takes plain pointers and integers (floats only by device
- * pointer), allocates nothing, launches asynchronously on `stream` and
- * returns a hipError_t as int: 0 on success, 1 (hipErrorInvalidValue) for a
- * shape, alignment or null-pointer violation (nothing is launched then), or
- * the launch error.  This is the contract of the reference's CUDA launchers
- * (internal/cuda/kernels/gemm_q4.cu:163-201) and of the purego layer that
- * calls them (internal/cuda/kernels/gemm_q4_purego.go:15-28: integer /
- * pointer arguments only, nonzero -> Go error -> CPU fallback).
+ * pointer or in a host structure), allocates nothing, launches asynchronously
+ * on `stream` and returns a hipError_t as int: 0 on success, 1
+ * (hipErrorInvalidValue) for a shape, alignment or null-pointer violation
+ * (nothing is launched then), or the launch error.  This is the contract of the
+ * reference's CUDA launchers (internal/cuda/kernels/gemm_q4.cu:163-201) and of
+ * the purego layer that calls them (internal/cuda/kernels/gemm_q4_purego.go:15-28:
+ * integer / pointer arguments only, nonzero -> Go error -> CPU fallback).
  *
  * Matrix convention (the one GemmQ4F32 / GemmQ8F32 use,
  * internal/gpuapi/kernels.go:45-48,79-81): C[M,N] = dequant(A)[M,K] * B[K,N],
@@ -693,6 +693,21 @@ typedef struct zt_rows {
 int zt_rope(const zt_rows* in, const zt_rows* out, int n, const int* positions, const float* table, int tokens,
             int head_dim, int rot_dim, int max_pos, int type, int flags, zt_stream_t stream);
 
+/* The same with each head normed before it is turned: x r w, r = 1 / sqrt(mean
+ * of the head's squares + eps), the squares summed in 64 bits, r rounded to fp32
+ * once, x r and then its product with w each rounded to fp32.  q and k are the
+ * weights of in[0] and in[1], fp32 [head_dim] on the device, NULL: ones.  table
+ * NULL: nothing is turned, positions are not read.  head_dim even and at most
+ * 256, eps above 0 and finite, flags ZT_ROPE_INTERLEAVED or 0, else as zt_rope. */
+typedef struct zt_head_norm {
+    const float* q;
+    const float* k;
+    double eps;
+} zt_head_norm;
+int zt_norm_rope(const zt_rows* in, const zt_rows* out, int n, const zt_head_norm* norm, const int* positions,
+                 const float* table, int tokens, int head_dim, int rot_dim, int max_pos, int type, int flags,
+                 zt_stream_t stream);
+
 /* The cache: pages of page_tokens (16, 32, 64 or 128) tokens, a value is its
  * code times the scale of its page and head.  Dp = head_dim to the next
  * multiple of 64; codes past head_dim are 0, and a scale is not negative (it
@@ -726,6 +741,13 @@ typedef struct zt_kv8_cache {
 int zt_kv8_append(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v, const long* slots, const zt_rows* q,
                   const zt_rows* q_out, const int* positions, const float* table, int tokens, int rot_dim, int max_pos,
                   int type, int flags, zt_stream_t stream);
+
+/* The same with the keys normed before they are turned, and q into q_out
+ * likewise (zt_norm_rope's rule; keys are not rounded in between).  q may go
+ * without a table here. */
+int zt_kv8_append_norm(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v, const long* slots, const zt_rows* q,
+                       const zt_rows* q_out, const zt_head_norm* norm, const int* positions, const float* table,
+                       int tokens, int rot_dim, int max_pos, int type, int flags, zt_stream_t stream);
 
 /* The values of n pages: keys and values fp32 [n][kv_heads][page_tokens]
  * [head_dim], code * scale.  A page outside the cache gives NaN. */

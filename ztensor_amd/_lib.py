@@ -134,6 +134,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "zt_gemm_wide_f32": (I, [I, P, L, L, P, I, P, I, P, I, I, I, P, L, P]),
     "zt_rope": (I, [P, P, I, P, P, I, I, I, I, I, I, P]),
     "zt_kv8_append": (I, [P, P, P, P, P, P, P, P, I, I, I, I, I, P]),
+    "zt_norm_rope": (I, [P, P, I, P, P, P, I, I, I, I, I, I, P]),
+    "zt_kv8_append_norm": (I, [P, P, P, P, P, P, P, P, P, I, I, I, I, I, P]),
     "zt_kv8_dequant": (I, [P, P, I, P, P, P]),
     "zt_kv8_plan": (I, [P, P, P, I, I, P, P, I, I, I, P, P, P, P, P, P, P]),
     "zt_kv8_attention_workspace_bytes": (L, [P]),
@@ -204,6 +206,12 @@ class Rows(C.Structure):
 
     _fields_ = [("p", C.c_void_p), ("token_stride", C.c_long), ("head_stride", C.c_long), ("heads", C.c_int),
                 ("reserved", C.c_int)]
+
+
+class HeadNorm(C.Structure):
+    """zt_head_norm: the weights of q's and k's norms, and what is added to a mean of squares."""
+
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("eps", C.c_double)]
 
 
 class KV8(C.Structure):

@@ -90,17 +90,11 @@ __host__ __device__ __forceinline__ int units_of(int dim, int half) {
 // Whether units of 2 V values divide a head of this size.
 __host__ inline bool units_fit(int V, int dim, int half) { return half % V == 0 && (dim - 2 * half) % (2 * V) == 0; }
 
-// Unit u of one head: its values in pairs (a[i], b[i]), turned by position pos;
-// first and second: where a and b lie, as V neighbours each, or (second < 0)
-// interleaved from `first` on.  Each product and sum is rounded by itself: a
-// plain program's values to the bit.
+// Unit u of one head as it lies in memory: first and second, where its two
+// sets of V neighbours begin.
 template <class T, int V>
-__device__ __forceinline__ void turned(const T* x, int u, int pos, const Turn& r, float (&a)[V], float (&b)[V], int& first,
-                                       int& second) {
-#pragma clang fp contract(off)
-    const int n = r.half / V;
-    const bool pairs = u < n, inter = pairs && (r.flags & ZT_ROPE_INTERLEAVED);
-    if (pairs && !inter) {
+__device__ __forceinline__ void load_unit(const T* x, int u, const Turn& r, float (&a)[V], float (&b)[V], int& first, int& second) {
+    if (u < r.half / V && !(r.flags & ZT_ROPE_INTERLEAVED)) {
         first = u * V;
         second = first + r.half;
     } else {
@@ -109,6 +103,14 @@ __device__ __forceinline__ void turned(const T* x, int u, int pos, const Turn& r
     }
     load_values<T, V>(x + first, a);
     load_values<T, V>(x + second, b);
+}
+
+// The same, its pairs (a[i], b[i]) turned by position pos: each product and sum
+// is rounded by itself, a plain program's values to the bit.
+template <int V>
+__device__ __forceinline__ void turn_unit(int u, int pos, const Turn& r, float (&a)[V], float (&b)[V]) {
+#pragma clang fp contract(off)
+    const bool pairs = u < r.half / V, inter = pairs && (r.flags & ZT_ROPE_INTERLEAVED);
     if (!pairs) return;
     if (inter) {
         float e[V], o[V];
@@ -156,6 +158,60 @@ __device__ __forceinline__ void turned(const T* x, int u, int pos, const Turn& r
             b[i] = hi[i];
         }
     }
+}
+
+template <class T, int V>
+__device__ __forceinline__ void turned(const T* x, int u, int pos, const Turn& r, float (&a)[V], float (&b)[V], int& first,
+                                       int& second) {
+    load_unit<T, V>(x, u, r, a, b, first, second);
+    turn_unit<V>(u, pos, r, a, b);
+}
+
+// A head's norm: x r w with r = 1 / sqrt(mean x^2 + eps).  The squares are
+// summed in 64 bits and r is rounded once, so that r does not depend on how the
+// sum is dealt out: a key's code lies next to a border often enough that an r
+// with another last bit is another code.  w NULL: ones.
+struct HeadNorm {
+    const float* w;
+    double eps;
+};
+
+// r of the head at x, in each of the L lanes that share it (neighbours, a power
+// of two of them); lane l has units l and, N == 2, l + L, as load_unit gives
+// them: a and b, first and second.
+template <class T, int V, int N>
+__device__ __forceinline__ float load_head(const T* x, int l, int L, int units, int dim, const Turn& turn, double eps,
+                                           float (&a)[N][V], float (&b)[N][V], int (&first)[N], int (&second)[N]) {
+    double sum = 0;
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const int u = l + k * L;
+        if (u < units) {
+            load_unit<T, V>(x, u, turn, a[k], b[k], first[k], second[k]);
+#pragma unroll
+            for (int i = 0; i < V; i++) sum += (double)a[k][i] * a[k][i] + (double)b[k][i] * b[k][i];
+        }
+    }
+    for (int o = L / 2; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+    return (float)(1.0 / sqrt(sum / dim + eps));
+}
+
+template <int V>
+__device__ __forceinline__ void scale_unit(const HeadNorm& n, float r, int at, float (&a)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        a[i] *= r;
+        if (n.w) a[i] *= n.w[at + i];
+    }
+}
+
+// Lanes that share a head of so many units, and units of one of them.
+template <int V>
+constexpr int kHeadUnits = V == 1 ? 2 : 1;
+__host__ inline int head_lanes(int units) {
+    int l = 1;
+    while (l < units && l < 64) l *= 2;
+    return l;
 }
 
 // A [tokens, heads, dim] operand as kernels take it.

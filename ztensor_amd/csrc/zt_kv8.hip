@@ -5,6 +5,8 @@
 // All of it moves bytes: a page holds, for each head, page x Dp codes of keys
 // [token][dim] and as many of values [dim][token] (the order in which the
 // attention's two products read them), and one fp32 scale of each.
+#include <type_traits>
+
 #include "zt_kv8.h"
 
 namespace zt {
@@ -77,9 +79,102 @@ __host__ inline int rope_width(const zt_rows* const* r, int n, int dim, int half
     return 1;
 }
 
+// -------------------------------------------------------- rotary, normed heads
+
+struct NormArgs {
+    RopeArgs r;
+    const float* w[2];
+    double eps;
+    int lanes;  // of one head: a power of two
+};
+
+// A head for g.lanes lanes.
+template <class T, int V>
+__device__ __forceinline__ void norm_block(const NormArgs& g, int block) {
+    constexpr int N = kHeadUnits<V>;
+    const int l = threadIdx.x & (g.lanes - 1), heads = g.r.all;
+    const long item = ((long)block * kThreads + threadIdx.x) / g.lanes, t = item / heads;
+    if (t >= g.r.tokens) return;
+    int h = (int)(item - t * heads);
+    const int second_in = h >= g.r.in[0].heads;
+    h -= second_in ? g.r.in[0].heads : 0;
+    const Rows &x = g.r.in[second_in], &y = g.r.out[second_in];
+    const HeadNorm norm{g.w[second_in], g.eps};
+    float a[N][V], b[N][V];
+    int first[N], second[N];
+    const int pos = g.r.turn.half ? g.r.turn.positions[t] : 0;
+    const float r = load_head<T, V, N>((const T*)x.p + t * x.token + h * x.head, l, g.lanes, g.r.units, g.r.dim, g.r.turn, g.eps, a, b, first, second);
+    T* o = (T*)y.p + t * y.token + h * y.head;
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        if (l + k * g.lanes >= g.r.units) continue;
+        scale_unit<V>(norm, r, first[k], a[k]);
+        scale_unit<V>(norm, r, second[k], b[k]);
+        turn_unit<V>(l + k * g.lanes, pos, g.r.turn, a[k], b[k]);
+        store_values<T, V>(o + first[k], a[k]);
+        store_values<T, V>(o + second[k], b[k]);
+    }
+}
+
+template <class T, int V>
+__global__ __launch_bounds__(kThreads) void norm_kernel(NormArgs g) {
+    norm_block<T, V>(g, blockIdx.x);
+}
+
+// The launch of n operands whose heads are normed.
+__host__ inline long norm_blocks(NormArgs& g, int n, int V) {
+    g.r.units = g.r.turn.half / V + (g.r.dim - 2 * g.r.turn.half) / (2 * V);
+    g.r.all = g.r.in[0].heads + (n > 1 ? g.r.in[1].heads : 0);
+    g.lanes = head_lanes(g.r.units);
+    return ((long)g.r.tokens * g.r.all * g.lanes + kThreads - 1) / kThreads;
+}
+
+__host__ inline bool norm_ok(const zt_head_norm* n) {
+    return n && n->eps > 0 && n->eps <= 1e30 && (((uintptr_t)n->q | (uintptr_t)n->k) & 3) == 0;
+}
+
 }  // namespace zt
 
 using namespace zt;
+
+ZT_EXPORT int zt_norm_rope(const zt_rows* in, const zt_rows* out, int n, const zt_head_norm* norm, const int* positions,
+                           const float* table, int tokens, int head_dim, int rot_dim, int max_pos, int type, int flags,
+                           zt_stream_t stream) {
+    if (!in || !out || n < 1 || n > 2 || !norm_ok(norm) || tokens < 0 || head_dim < 2 || head_dim % 2 || head_dim > 256 ||
+        !type_ok(type) || (flags & ~ZT_ROPE_INTERLEAVED) ||
+        (table && (rot_dim < 2 || rot_dim % 2 || rot_dim > head_dim || max_pos < 1)))
+        return kInvalid;
+    const zt_rows* all[4];
+    for (int i = 0; i < n; i++) {
+        if (in[i].heads != out[i].heads || in[i].heads > (1 << 20) / head_dim) return kInvalid;
+        all[2 * i] = in + i;
+        all[2 * i + 1] = out + i;
+    }
+    if (tokens == 0) return 0;
+    for (int i = 0; i < 2 * n; i++)
+        if (!rows_ok(*all[i], type)) return kInvalid;
+    if (table && (!positions || ((uintptr_t)positions & 3) || ((uintptr_t)table & 3))) return kInvalid;
+    NormArgs g{};
+    for (int i = 0; i < n; i++) {
+        g.r.in[i] = rows_of(in[i]);
+        g.r.out[i] = rows_of(out[i]);
+    }
+    g.r.turn = {positions, table, table ? rot_dim / 2 : 0, max_pos, flags};
+    g.r.tokens = tokens;
+    g.r.dim = head_dim;
+    g.w[0] = norm->q;
+    g.w[1] = norm->k;
+    g.eps = norm->eps;
+    const int v = rope_width(all, 2 * n, head_dim, g.r.turn.half, type);
+    const long blocks = norm_blocks(g, n, v);
+    if (blocks >= 1l << 31) return kInvalid;
+    auto run = [&](auto kernel) { kernel<<<blocks, kThreads, 0, stream>>>(g); };
+    if (type == ZT_F32)
+        v == 4 ? run(norm_kernel<float, 4>) : run(norm_kernel<float, 1>);
+    else
+        v == 8 ? run(norm_kernel<_Float16, 8>) : v == 4 ? run(norm_kernel<_Float16, 4>) : run(norm_kernel<_Float16, 1>);
+    return (int)hipGetLastError();
+}
 
 ZT_EXPORT int zt_rope(const zt_rows* in, const zt_rows* out, int n, const int* positions, const float* table, int tokens,
                       int head_dim, int rot_dim, int max_pos, int type, int flags, zt_stream_t stream) {
@@ -131,6 +226,8 @@ struct AppendArgs {
     Rows x[2];  // keys, values
     const long* slots;
     Turn turn;  // half == 0: keys as they are
+    HeadNorm norm;  // of the keys, where the kernel norms them
+    int lanes;      // that share a key for that
     int tokens;
     int turns;  // workgroups that the pages which 64 tokens begin are dealt out to, for one head of keys or of values
     long blocks;
@@ -166,8 +263,8 @@ struct Run {
 
 // A run's tokens into their page: its new scale, and its codes by way of an image
 // of it in LDS.
-template <class T, int V, bool VALUES>
-__device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run, int head, uint32_t* image, float* red) {
+template <class T, int V, bool VALUES, bool NORM>
+__device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run, int head, uint32_t* image, float* red, float* factors) {
     const Kv8& c = g.c;
     const Rows& x = g.x[VALUES];
     Turn turn = g.turn;
@@ -177,13 +274,32 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run,
     const T* rows = (const T*)x.p + (long)head * x.head;
     float a[V], b[V];
     int first, second;
+    if constexpr (NORM) {
+        const int l = threadIdx.x & (g.lanes - 1);
+        for (int i = threadIdx.x / g.lanes; i < n; i += kThreads / g.lanes) {
+            constexpr int N = kHeadUnits<V>;
+            float a[N][V], b[N][V];
+            int first[N], second[N];
+            const float r = load_head<T, V, N>(rows + (long)run.token(i) * x.token, l, g.lanes, units, c.dim, turn, g.norm.eps, a, b, first, second);
+            if (l == 0) factors[i] = r;
+        }
+        __syncthreads();
+    }
+    auto unit = [&](int tl, int u, int t) {
+        const int pos = turn.half ? turn.positions[t] : 0;
+        load_unit<T, V>(rows + (long)t * x.token, u, turn, a, b, first, second);
+        if constexpr (NORM) {
+            scale_unit<V>(g.norm, factors[tl], first, a);
+            scale_unit<V>(g.norm, factors[tl], second, b);
+        }
+        turn_unit<V>(u, pos, turn, a, b);
+    };
 
     float m = 0.0f;
     bool bad = false;
     for (int i = threadIdx.x; i < n * units; i += kThreads) {
         const int tl = i / units, u = i - tl * units, t = run.token(tl);
-        const int pos = turn.half ? turn.positions[t] : 0;
-        turned<T, V>(rows + (long)t * x.token, u, pos, turn, a, b, first, second);
+        unit(tl, u, t);
 #pragma unroll
         for (int j = 0; j < V; j++) {
             m = fmaxf(m, fmaxf(fabsf(a[j]), fabsf(b[j])));
@@ -226,8 +342,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run,
     const float step = now > 0.0f ? now : 1.0f;  // 1 for a NaN, whose codes nobody takes for values
     for (int i = threadIdx.x; i < n * units; i += kThreads) {
         const int tl = i / units, u = i - tl * units, t = run.token(tl);
-        const int pos = turn.half ? turn.positions[t] : 0;
-        turned<T, V>(rows + (long)t * x.token, u, pos, turn, a, b, first, second);
+        unit(tl, u, t);
         const int place = run.place(tl);
 #pragma unroll
         for (int j = 0; j < V; j++) {
@@ -343,15 +458,23 @@ __device__ __forceinline__ Run run_from(const AppendArgs& g, int t, long s, Foun
 // slots, its rows, their largest, the scale and the codes one after the other.
 // Prompts of 1955 tokens in all (fp16, 64 + 8 heads, pages of 16): 76 MB, 64 of
 // them q, in 22.6 us, 3.4 TB/s.
-template <class T, int V, int VQ>
-__global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, RopeArgs q) {
+//
+// Normed keys: a head's factor once for all, in LDS, from one more reading of the
+// rows.
+template <class T, int V, int VQ, class Q>
+__global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, Q q) {
+    constexpr bool NORM = std::is_same_v<Q, NormArgs>;
     extern __shared__ __align__(16) uint32_t image[];  // of one page and head
+    __shared__ float factors[NORM ? 128 : 1];
     __shared__ float red[4];
     __shared__ Found found;
     __shared__ int listed[128];
     __shared__ uint8_t places[128];
     if (blockIdx.x >= g.blocks) {
-        rope_block<T, VQ>(q, blockIdx.x - g.blocks);
+        if constexpr (NORM)
+            norm_block<T, VQ>(q, blockIdx.x - g.blocks);
+        else
+            rope_block<T, VQ>(q, blockIdx.x - g.blocks);
         return;
     }
     const Kv8& c = g.c;
@@ -381,19 +504,37 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, RopeArgs
         const int i = __builtin_ctzll(begin);
         const Run run = run_from(g, from + i, __shfl(here, i), found, listed, places);
         if (values)
-            append_page<T, V, true>(g, run, head, image, red);
+            append_page<T, V, true, false>(g, run, head, image, red, factors);
         else
-            append_page<T, V, false>(g, run, head, image, red);
+            append_page<T, V, false, NORM>(g, run, head, image, red, factors);
     }
 }
 
 }  // namespace zt
 
-ZT_EXPORT int zt_kv8_append(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v, const long* slots,
-                            const zt_rows* q, const zt_rows* q_out, const int* positions, const float* table, int tokens,
-                            int rot_dim, int max_pos, int type, int flags, zt_stream_t stream) {
+template <class Q>
+static int launch_append(const AppendArgs& g, const Q& q, long blocks, int type, int width, int q_width, hipStream_t stream) {
+    if (blocks >= 1l << 31) return kInvalid;
+    const int lds = g.c.bytes();
+    auto run = [&](auto kernel) { kernel<<<blocks, kThreads, lds, stream>>>(g, q); };
+    if (type == ZT_F32) {
+        if (width == 4)
+            q_width == 4 ? run(append_kernel<float, 4, 4, Q>) : run(append_kernel<float, 4, 1, Q>);
+        else
+            q_width == 4 ? run(append_kernel<float, 1, 4, Q>) : run(append_kernel<float, 1, 1, Q>);
+    } else if (width == 4) {
+        q_width == 8 ? run(append_kernel<_Float16, 4, 8, Q>) : q_width == 4 ? run(append_kernel<_Float16, 4, 4, Q>) : run(append_kernel<_Float16, 4, 1, Q>);
+    } else {
+        q_width == 8 ? run(append_kernel<_Float16, 1, 8, Q>) : q_width == 4 ? run(append_kernel<_Float16, 1, 4, Q>) : run(append_kernel<_Float16, 1, 1, Q>);
+    }
+    return (int)hipGetLastError();
+}
+
+static int append(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v, const long* slots, const zt_rows* q,
+                  const zt_rows* q_out, const zt_head_norm* norm, const int* positions, const float* table, int tokens,
+                  int rot_dim, int max_pos, int type, int flags, hipStream_t stream) {
     if (!cache || !kv8_ok(*cache) || !k || !v || tokens < 0 || tokens >= 1l << 30 || !type_ok(type) || (flags & ~ZT_ROPE_INTERLEAVED) ||
-        (q == nullptr) != (q_out == nullptr) || (q && !table))
+        (q == nullptr) != (q_out == nullptr) || (q && !table && !norm))
         return kInvalid;
     const int dim = cache->head_dim, half = table ? rot_dim / 2 : 0;
     if (table && (rot_dim < 2 || rot_dim % 2 || rot_dim > dim || max_pos < 1)) return kInvalid;
@@ -422,30 +563,37 @@ ZT_EXPORT int zt_kv8_append(const zt_kv8_cache* cache, const zt_rows* k, const z
     // 38 us, with 16 44, 32 55, 4 36; but 512 sequences' single tokens 150, 152, 152 and 169)
     g.turns = tokens <= 256 ? 64 : 8;
     g.blocks = 2l * cache->kv_heads * ceil_div(tokens, 64) * g.turns;
-    const int lds = g.c.bytes();
     RopeArgs r{};
-    long blocks = g.blocks;
+    r.turn = g.turn;
+    r.tokens = tokens;
+    r.dim = dim;
     if (q) {
         r.in[0] = rows_of(*q);
         r.out[0] = rows_of(*q_out);
-        r.turn = g.turn;
-        r.tokens = tokens;
-        r.dim = dim;
-        blocks += rope_blocks(r, 1, q_width);
     }
-    if (blocks >= 1l << 31) return kInvalid;
-    auto run = [&](auto kernel) { kernel<<<blocks, kThreads, lds, stream>>>(g, r); };
-    if (type == ZT_F32) {
-        if (width == 4)
-            q_width == 4 ? run(append_kernel<float, 4, 4>) : run(append_kernel<float, 4, 1>);
-        else
-            q_width == 4 ? run(append_kernel<float, 1, 4>) : run(append_kernel<float, 1, 1>);
-    } else if (width == 4) {
-        q_width == 8 ? run(append_kernel<_Float16, 4, 8>) : q_width == 4 ? run(append_kernel<_Float16, 4, 4>) : run(append_kernel<_Float16, 4, 1>);
-    } else {
-        q_width == 8 ? run(append_kernel<_Float16, 1, 8>) : q_width == 4 ? run(append_kernel<_Float16, 1, 4>) : run(append_kernel<_Float16, 1, 1>);
+    if (!norm) {
+        const long more = q ? rope_blocks(r, 1, q_width) : 0;
+        return launch_append(g, r, g.blocks + more, type, width, q_width, stream);
     }
-    return (int)hipGetLastError();
+    g.norm = {norm->k, norm->eps};
+    g.lanes = head_lanes(half / width + (dim - 2 * half) / (2 * width));
+    NormArgs m{r, {norm->q, nullptr}, norm->eps, 1};
+    const long more = q ? norm_blocks(m, 1, q_width) : 0;
+    return launch_append(g, m, g.blocks + more, type, width, q_width, stream);
+}
+
+ZT_EXPORT int zt_kv8_append(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v, const long* slots,
+                            const zt_rows* q, const zt_rows* q_out, const int* positions, const float* table, int tokens,
+                            int rot_dim, int max_pos, int type, int flags, zt_stream_t stream) {
+    return append(cache, k, v, slots, q, q_out, nullptr, positions, table, tokens, rot_dim, max_pos, type, flags, stream);
+}
+
+ZT_EXPORT int zt_kv8_append_norm(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v, const long* slots,
+                                 const zt_rows* q, const zt_rows* q_out, const zt_head_norm* norm, const int* positions,
+                                 const float* table, int tokens, int rot_dim, int max_pos, int type, int flags,
+                                 zt_stream_t stream) {
+    if (!norm_ok(norm)) return kInvalid;
+    return append(cache, k, v, slots, q, q_out, norm, positions, table, tokens, rot_dim, max_pos, type, flags, stream);
 }
 
 // ------------------------------------------------------------------ dequant

@@ -2,7 +2,7 @@
 int8 paged key/value cache and attention over it, the pages' bookkeeping, and
 the choice of a token.
 
-The kernels are zt_rope, zt_kv8_* and zt_sample of libzt_hip.so; DecodeOps
+The kernels are zt_rope, zt_norm_rope, zt_kv8_* and zt_sample of libzt_hip.so; DecodeOps
 holds the engine's methods for them.  A step of a batch of requests:
 
     p = engine.kv8_plan(kv_lens, new, block_table, free_pages, free_count, page_tokens, tokens)
@@ -46,6 +46,15 @@ class KV8Cache(NamedTuple):
                    torch.zeros((pages, kv_heads, dp, page_tokens), dtype=torch.int8, device=device),
                    torch.zeros((pages, kv_heads), dtype=torch.float32, device=device),
                    torch.zeros((pages, kv_heads), dtype=torch.float32, device=device))
+
+
+class HeadNorm(NamedTuple):
+    """The norms of q's and k's heads: each over the root of the mean of its
+    squares + eps, times weights (float32 [head_dim]; None: ones)."""
+
+    q: torch.Tensor | None
+    k: torch.Tensor | None
+    eps: float = 1e-6
 
 
 class KV8Plan(NamedTuple):
@@ -122,6 +131,7 @@ def rope_table(rot_dim: int, max_pos: int, base: float = 10000.0, scaling: dict 
 # costs a third of building a ctypes.Structure (0.5 us of a call's 10 instead of 2).
 _ROWS = struct.Struct("@Pqqii")
 _ROWS2 = struct.Struct("@PqqiiPqqii")
+_NORM = struct.Struct("@PPd")
 _CACHE = struct.Struct("@PPPPiiii")
 _ATTN = struct.Struct("@PPPPiiiiPqqiiPqqiiPPPPiiiiiiii")
 
@@ -159,6 +169,11 @@ class DecodeOps:
         if t is None:
             raise TypeError(f"{name} takes float32 or float16 tensors of one type")
         return t
+
+    def _norm(self, norm: HeadNorm, dim: int) -> bytes:
+        """zt_head_norm."""
+        dense, f32, one = self._dense, torch.float32, (dim,)
+        return _NORM.pack(dense(norm[0], "norm.q", f32, one), dense(norm[1], "norm.k", f32, one), norm[2])
 
     def _kv8(self, cache, head_dim: int) -> tuple:
         """zt_kv8_cache's fields."""
@@ -207,14 +222,53 @@ class DecodeOps:
         return q_out, k_out if n == 2 else None
 
     @_on_engine_stream
+    def norm_rope(self, q: torch.Tensor, k: torch.Tensor | None, norm: HeadNorm, positions: torch.Tensor | None = None,
+                  table: torch.Tensor | None = None, *, interleaved: bool = False, q_out: torch.Tensor | None = None,
+                  k_out: torch.Tensor | None = None):
+        """rope of q and k whose heads (of an even size up to 256) are normed
+        first, in the same pass; without a table normed only.  The norm's
+        squares are summed in 64 bits, and its factor, the products and the
+        rotation rounded to 32 one by one; the result is rounded once to the
+        tensors' type.  q_out and k_out may be q and k themselves."""
+        if q_out is None:
+            q_out = _like(q)
+        rows = self._rows
+        if k is None:
+            t, n = self._type("norm_rope", q, q_out), 1
+            ins, outs = _ROWS.pack(*rows(q, "q")), _ROWS.pack(*rows(q_out, "q_out"))
+        else:
+            if k_out is None:
+                k_out = _like(k)
+            t, n = self._type("norm_rope", q, k, q_out, k_out), 2
+            ins = _ROWS2.pack(*rows(q, "q"), *rows(k, "k"))
+            outs = _ROWS2.pack(*rows(q_out, "q_out"), *rows(k_out, "k_out"))
+            if k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k_out.shape != k.shape:
+                raise ValueError("norm_rope: q, k and their outputs have the same tokens and head size")
+        if q_out.shape != q.shape:
+            raise ValueError("norm_rope: q, k and their outputs have the same tokens and head size")
+        tokens, _, dim = q.shape
+        pos = tab = half = most = 0
+        if table is not None:
+            if positions is None:
+                raise ValueError("norm_rope: a rope table needs positions")
+            pos = self._dense(positions, "positions", torch.int32, (tokens,))
+            tab = self._dense(table, "table", torch.float32, (None, 2, None))
+            most, _, half = table.shape
+        self.lib.call("zt_norm_rope", ins, outs, n, self._norm(norm, dim), pos, tab, tokens, dim, 2 * half, most, t,
+                      _lib.ROPE_INTERLEAVED if interleaved else 0, self._s)
+        return q_out, k_out if n == 2 else None
+
+    @_on_engine_stream
     def kv8_append(self, k: torch.Tensor, v: torch.Tensor, cache, slots: torch.Tensor, *,
                    positions: torch.Tensor | None = None, table: torch.Tensor | None = None,
                    interleaved: bool = False, q: torch.Tensor | None = None,
-                   q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+                   q_out: torch.Tensor | None = None, norm: HeadNorm | None = None) -> torch.Tensor | None:
         """Puts a step's keys and values ([tokens, kv_heads, head_dim]) into
         the cache at their slots (int64 [tokens], kv8_plan's).  With a rope
         table the keys are turned by their positions first, and q, if given,
-        into a new tensor or q_out, which is returned.
+        into a new tensor or q_out, which is returned.  With norm the heads of
+        keys and q are normed before that (norm_rope's rule); q may then go
+        without a table.
 
         A page's scale grows where the new values need it, and the codes that
         it holds are rounded to the new scale; a page that starts anew (its
@@ -229,8 +283,8 @@ class DecodeOps:
             raise ValueError("kv8_append: k and v have one shape")
         qr = qo = None
         if q is not None:
-            if table is None or q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != dim:
-                raise ValueError("kv8_append: q goes with a rope table, and has k's tokens and head size")
+            if (table is None and norm is None) or q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != dim:
+                raise ValueError("kv8_append: q goes with a rope table or a norm, and has k's tokens and head size")
             if q_out is None:
                 q_out = _like(q)
             elif q_out.shape != q.shape:
@@ -251,9 +305,10 @@ class DecodeOps:
             pos = self._dense(positions, "positions", torch.int32, (tokens,))
             tab = self._dense(table, "table", torch.float32, (None, 2, None))
             most, _, half = table.shape
-        self.lib.call("zt_kv8_append", _CACHE.pack(*c), pack(*krows), pack(*vrows),
-                      self._dense(slots, "slots", torch.int64, (tokens,)), qr, qo, pos, tab, tokens, 2 * half, most, t,
-                      _lib.ROPE_INTERLEAVED if interleaved else 0, self._s)
+        name, norms = ("zt_kv8_append", ()) if norm is None else ("zt_kv8_append_norm", (self._norm(norm, dim),))
+        self.lib.call(name, _CACHE.pack(*c), pack(*krows), pack(*vrows),
+                      self._dense(slots, "slots", torch.int64, (tokens,)), qr, qo, *norms, pos, tab, tokens, 2 * half,
+                      most, t, _lib.ROPE_INTERLEAVED if interleaved else 0, self._s)
         return q_out
 
     @_on_engine_stream
