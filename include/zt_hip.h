@@ -811,6 +811,114 @@ typedef struct zt_kv8_attn {
 long zt_kv8_attention_workspace_bytes(const zt_kv8_attn* a);
 int zt_kv8_attention(const zt_kv8_attn* a, void* workspace, long workspace_bytes, zt_stream_t stream);
 
+/* Positions and masks of a step's drafted trees.  parents [tokens]: of each row
+ * the row of its own request that it continues, an earlier one (counted from the
+ * request's first row; anything else: none, it continues the context).  Of a
+ * request's n rows, q_start[r] .. q_start[r + 1] - 1, which are the last of its
+ * kv_lens[r] tokens: positions = kv_lens[r] - n and the rows above it (0 where
+ * that is negative), mask [tokens][words]: its bit and those of the rows above it
+ * among the first 64 words.  Rows of no request get position 0 and no bits.
+ * words from 1 to ZT_TREE_WORDS; outputs share no bytes with inputs nor with each
+ * other, else InvalidValue. */
+#define ZT_TREE_WORDS 16
+int zt_kv8_tree(const int* parents, const int* kv_lens, const int* q_start, int requests, int tokens, int words,
+                int* positions, uint64_t* mask, zt_stream_t stream);
+
+/* The same for the rows of a drafted tree, which are not in a line.  A request's
+ * n rows stand behind its context, the first kv_lens[r] - n tokens.  Row i sees
+ * the context and, of the request's own rows, row j where bit j % 64 of word
+ * j / 64 of mask[i] is set (its ancestors and itself, as zt_kv8_tree gives them;
+ * any other set of rows does too, an empty one among them); bits from n on are
+ * ignored, and a row from 64 words on is seen by none.  With window > 0 it sees,
+ * of the context, the last tokens from position - window + 1 on, where its
+ * position is the context's length and the rows that it sees, less one; its own
+ * request's rows are seen as the mask says.  mask: [tokens][words] on the device,
+ * 8-byte aligned, words from 1 to ZT_TREE_WORDS, else InvalidValue.  The
+ * workspace is zt_kv8_attention_workspace_bytes'. */
+int zt_kv8_tree_attention(const zt_kv8_attn* a, const uint64_t* mask, int words, void* workspace, long workspace_bytes,
+                          zt_stream_t stream);
+
+/* The path of each request's tree that the drawn tokens accept.  Row 0 of a
+ * request is a token that stands; from row i the path goes on to the first row
+ * whose parent it is (zt_kv8_tree's rule; parents NULL: a chain, each row's is the
+ * one before it) and whose token drafted[] is drawn[i], what was sampled after
+ * row i; a drawn token below 0 is nobody's.  path[q_start[r] + k]: the path's
+ * rows, counted from the request's first, then -1; kept[r]: how many; last[r]: the
+ * last one, counted from the step's first row; token[r]: drawn there.  A request
+ * without rows, or whose first row's slot is below 0 (slots NULL: none is; it got
+ * no pages), has kept 0 and last and token -1.  Rows of no request: path -1. */
+int zt_tree_accept(const long* drafted, const long* drawn, const int* parents, const int* q_start, const long* slots,
+                   int requests, int tokens, int* path, int* kept, int* last, long* token, zt_stream_t stream);
+
+/* Moves the kept rows of a step to their contexts' ends, in the caches of all
+ * layers (which have one shape, and the same tables).  Request r held held[r]
+ * tokens before the step, and its n rows stand behind them.  Row path[q_start[r] +
+ * k] goes to place held[r] + k for k below kept[r] (at most n); an entry that is
+ * not above k, or not below n, stays out: that place keeps what it has.
+ * kv_lens_out[r] = held[r] + kept[r].  On its own page a code stays as it is.
+ * From another page its value does, code times that page's scale in fp32: the
+ * page's scale becomes the largest of what it was and those values' largest
+ * magnitude times 1/127, and codes are taken over or rounded to it as
+ * zt_kv8_append does it (a scale that is not a number goes on to the page).  What
+ * stands behind the kept rows has no meaning.  Entries of tables outside the cache
+ * are not read or written. */
+int zt_kv8_compact(const zt_kv8_cache* caches, int layers, const int* table, int requests, int width, const int* held,
+                   const int* q_start, const int* path, const int* kept, int tokens, int* kv_lens_out,
+                   zt_stream_t stream);
+
+/* Copies page from[i] to page to[i], codes and scales, in the caches of all
+ * layers (of one shape); either of them outside the cache: none.  No page is
+ * copied to twice, or both from and to. */
+int zt_kv8_copy(const zt_kv8_cache* caches, int layers, const int* from, const int* to, int n, zt_stream_t stream);
+
+/* Gives pages back.  Request r holds kv_lens[r] tokens in the pages of its row of
+ * table and keeps the first keep[r] of them: the pages that only the others are
+ * on become -1 in table_out (which is table else, or table itself), and go to the
+ * end of the free list, in the order of their numbers.  free_pages has room for
+ * all pages, `pages` entries of which the first free_count are there; entries
+ * of the table outside 0 .. pages - 1 stay as they are.  refs[p]: how many
+ * sequences hold page p besides one (zt_kv8_fork counts them up); a page that is
+ * given back fewer times than it has holders stays, with as many fewer.  NULL:
+ * nobody shares.  pages at most 2^20; outputs (free_pages and refs among them)
+ * share no bytes with inputs nor with each other, but for table_out that is table,
+ * else InvalidValue. */
+int zt_kv8_trim(const int* kv_lens, const int* keep, const int* table, int requests, int width, int* free_pages,
+                const int* free_count, int pages, int page_tokens, int* refs, int* table_out, int* free_count_out,
+                zt_stream_t stream);
+
+/* Sequences that go on from others: row target[i] of the table gets what row
+ * source[i] held before the call.  Full pages are shared, refs[p] one more each; a
+ * last page that is not full needs a page of its own off the end of the free
+ * list, in the order of i, and copy_from[i] and copy_to[i] say what zt_kv8_copy is
+ * to do for it (-1: nothing).  A fork that finds no page gets no tokens: length 0,
+ * its row all -1; so does one whose source is outside the table or holds nothing,
+ * or more than its row.  The other rows, and a row forked from itself, stay as
+ * they are.  A row's old pages are not given back (zt_kv8_trim does that), and
+ * each row is a target once at most.  `pages`: the entries of free_pages and refs.
+ * Outputs (refs among them) share no bytes with inputs nor with each other, else
+ * InvalidValue. */
+typedef struct zt_kv8_fork_call {
+    const int* source; /* [n] */
+    const int* target; /* [n] */
+    const int* kv_lens; /* [rows] */
+    const int* table;   /* [rows][width] */
+    const int* free_pages;
+    const int* free_count;
+    int* refs;
+    int* table_out;
+    int* kv_lens_out;
+    int* free_count_out;
+    int* copy_from; /* [n] */
+    int* copy_to;   /* [n] */
+    int n;
+    int rows;
+    int width;
+    int pages;
+    int page_tokens;
+    int reserved; /* 0 */
+} zt_kv8_fork_call;
+int zt_kv8_fork(const zt_kv8_fork_call* a, zt_stream_t stream);
+
 /* A token of each row of logits [rows][vocab] (row_stride elements apart) from
  * u[row] in [0, 1).  With z the row's values (NaN counts as -inf) and m their
  * largest, token i weighs w_i = exp((z_i - m) / T), taken down to a whole

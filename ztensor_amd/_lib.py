@@ -140,6 +140,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "zt_kv8_plan": (I, [P, P, P, I, I, P, P, I, I, I, P, P, P, P, P, P, P]),
     "zt_kv8_attention_workspace_bytes": (L, [P]),
     "zt_kv8_attention": (I, [P, P, L, P]),
+    "zt_kv8_tree": (I, [P, P, P, I, I, I, P, P, P]),
+    "zt_tree_accept": (I, [P, P, P, P, P, I, I, P, P, P, P, P]),
+    "zt_kv8_compact": (I, [P, I, P, I, I, P, P, P, P, I, P, P]),
+    "zt_kv8_copy": (I, [P, I, P, P, I, P]),
+    "zt_kv8_trim": (I, [P, P, P, I, I, P, P, I, I, P, P, P, P]),
+    "zt_kv8_fork": (I, [P, P]),
+    "zt_kv8_tree_attention": (I, [P, P, I, P, L, P]),
     "zt_sample_workspace_bytes": (L, [I, I]),
     "zt_sample": (I, [P, L, I, I, I, P, P, P, P, P, P, P, P, L, P]),
     "zt_gemm_int8_f32": (I, [P, P, P, I, I, I, P]),
@@ -199,6 +206,7 @@ def w4a16_gemv_descs(entries) -> C.Array:
 
 F32, F16 = 0, 1  # ZT_F32, ZT_F16
 ROPE_INTERLEAVED, ROPE_INVERSE = 1, 2  # ZT_ROPE_*
+TREE_WORDS = 16  # ZT_TREE_WORDS
 
 
 class Rows(C.Structure):
@@ -228,6 +236,14 @@ class KV8Attn(C.Structure):
                 ("q_start", C.c_void_p), ("scale", C.c_void_p), ("requests", C.c_int), ("width", C.c_int),
                 ("tokens", C.c_int), ("max_q", C.c_int), ("max_kv", C.c_int), ("window", C.c_int),
                 ("type", C.c_int), ("reserved", C.c_int)]
+
+
+class KV8Fork(C.Structure):
+    """zt_kv8_fork_call: one call of zt_kv8_fork."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("source", "target", "kv_lens", "table", "free_pages", "free_count", "refs",
+                                          "table_out", "kv_lens_out", "free_count_out", "copy_from", "copy_to")] + [
+        (n, C.c_int) for n in ("n", "rows", "width", "pages", "page_tokens", "reserved")]
 
 
 class ZTError(RuntimeError):

@@ -23,6 +23,8 @@ struct AttnArgs {
     const float* scale;
     int requests, width, tokens, window, group;
     float unit, unit_lo;  // log2(e) / sqrt(dim) in two parts: a score's factor where no scale is given
+    const uint64_t* mask;  // [tokens][words] of a tree's rows: bit j, its request's row j is seen
+    int words;
 };
 
 // ------------------------------------------------- few rows: a long axis split
@@ -144,6 +146,51 @@ __device__ __forceinline__ int first_seen(const AttnArgs& g, int len, int n, int
     return g.window > 0 ? (int)max(0l, (long)len - n + i + 1 - g.window) : 0;
 }
 __device__ __forceinline__ int tiles_up_to(int token) { return (int)(((unsigned)token + 63) >> 6); }
+
+// A tree's rows stand behind their context, tokens 0 .. len - n - 1: a row sees
+// that (with a window, the last of it before the row's own position, which is the
+// context's end and the rows that its mask has, less one) and, of the tokens
+// behind it, those whose bits its mask has.
+__device__ __forceinline__ int tree_first(const AttnArgs& g, int len, int n) {  // no row sees a token before
+    return g.window > 0 ? max(0, len - n - g.window) : 0;
+}
+struct TreeRow {
+    int row, lo;  // of the masks (-1: no such row), and the first token of the context that it sees
+};
+__device__ __forceinline__ TreeRow tree_row(const AttnArgs& g, const Span& sp, int i, bool there) {
+    TreeRow r{there ? sp.start + i : -1, 0};
+    if (!there || g.window <= 0) return r;
+    const uint64_t* mask = g.mask + (long)r.row * g.words;
+    int seen = 0;
+    for (int w = 0; w < g.words && 64 * w < sp.n; w++) {
+        const int left = sp.n - 64 * w;
+        seen += __builtin_popcountll(mask[w] & (left < 64 ? (1ull << left) - 1 : ~0ull));
+    }
+    const int context = sp.len - sp.n;
+    r.lo = (int)min((long)context, max(0l, (long)context + seen - g.window));
+    return r;
+}
+// Which of tokens t .. t + 15 it sees.
+__device__ __forceinline__ uint32_t tree_seen(const AttnArgs& g, const Span& sp, const TreeRow& r, int t) {
+    if (r.row < 0 || t >= sp.len) return 0;
+    const int d = t - (sp.len - sp.n);  // the first one's bit
+    uint32_t seen = 0xFFFFu;
+    if (d > -16) {
+        const uint64_t* mask = g.mask + (long)r.row * g.words;
+        if (d < 0) {
+            seen = (uint32_t)(mask[0] << -d) | ((1u << -d) - 1);
+        } else {
+            const int w = d >> 6, at = d & 63;
+            uint64_t x = w < g.words ? mask[w] >> at : 0;
+            if (at > 48 && w + 1 < g.words) x |= mask[w + 1] << (64 - at);
+            seen = (uint32_t)x;
+        }
+    }
+    if (r.lo > t) seen &= r.lo - t < 16 ? ~0u << (r.lo - t) : 0;
+    return seen & (sp.len - t < 16 ? (1u << (sp.len - t)) - 1 : 0xFFFFu);
+}
+
+template <bool TREE>
 __device__ __forceinline__ Span span_of(const AttnArgs& g, int r) {
     Span s;
     s.start = row_bound(g, r);
@@ -152,7 +199,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs& g, int r) {
     // (rows that q does not have are the last ones of their request: what only they would see is as good as not there)
     const long cut = max(0, g.q_start[r + 1]) - (long)(s.start + s.n);
     s.len = g.c.pages ? (int)max(0l, min((long)max(0, g.kv_lens[r]), most) - max(0l, cut)) : 0;
-    s.tile0 = first_seen(g, s.len, s.n, 0) >> 6;
+    s.tile0 = (TREE ? tree_first(g, s.len, s.n) : first_seen(g, s.len, s.n, 0)) >> 6;
     s.tile1 = max(tiles_up_to(s.len), s.tile0 + 1);  // (one where there is nothing to see: it gives zeros)
     return s;
 }
@@ -249,6 +296,18 @@ __device__ __forceinline__ void mask_scores(float4v (&s)[4], Factor& fk, ValueSc
 #pragma unroll
     for (int k = 0; k < 16; k++)
         if (k < lo || k >= hi) s[k >> 2][k & 3] = kNone;
+}
+
+// The same of a tree's row.
+__device__ __forceinline__ void mask_scores(float4v (&s)[4], Factor& fk, ValueScale& v, bool there, uint32_t seen) {
+    if (!there || seen == 0) {
+        fk = {1.0f, 1e-37f};
+        v = {1.0f, 1000.0f};
+        seen = 0;
+    }
+#pragma unroll
+    for (int k = 0; k < 16; k++)
+        if (!(seen >> k & 1)) s[k >> 2][k & 3] = kNone;
 }
 
 // The weights of a tile's 16 tokens in this lane for one row: scores s times fk
@@ -409,7 +468,7 @@ __device__ __forceinline__ long wave_scan(long v) {
 // the launch and the chain from the lengths to the first codes; 37 tokens 8.9 us,
 // all of it that chain.  fp32 rows of two columns keep 24 registers in memory at
 // 128 dims, and fp32 rows 78, fp16 rows 25 at 256.
-template <class T, int DN, int CT>
+template <class T, int DN, int CT, bool TREE>
 __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queries) {  // [4 waves][CT][DN][2][PARTS][64]
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int PARTS = SPLIT ? 2 : 1;
@@ -437,7 +496,7 @@ __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queri
     long all = 0, before = 0, upto = 0, places = 0;
     auto load_spans = [&](int r0) {
         span = Span{};
-        if (r0 + lane < g.requests) span = span_of(g, r0 + lane);
+        if (r0 + lane < g.requests) span = span_of<TREE>(g, r0 + lane);
         places = places_of(f, span, 16 * CT);
         upto = wave_scan(places);
     };
@@ -499,10 +558,13 @@ __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queri
         half8v* mine_q = queries + wave * (CT * DN * 2 * PARTS * 64);
         Factor factor[CT];
         int hi[CT];
+        TreeRow tree[CT];
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             half8v q[DN][2], ql[DN][2];
-            load_query<T, DN>(f, sp, kv, (cg * CT + ct) * 16 + col, rows, scale, q, ql, factor[ct], hi[ct]);
+            const int row = (cg * CT + ct) * 16 + col;
+            load_query<T, DN>(f, sp, kv, row, rows, scale, q, ql, factor[ct], hi[ct]);
+            if constexpr (TREE) tree[ct] = tree_row(g, sp, row / g.group, row < rows);
 #pragma unroll
             for (int d = 0; d < DN; d++)
 #pragma unroll
@@ -513,8 +575,8 @@ __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queri
         }
         // every row of these columns sees tokens all_lo .. all_hi - 1
         const int row0 = cg * 16 * CT, row1 = min(rows, row0 + 16 * CT) - 1;
-        const int all_hi = sp.len - sp.n + row0 / g.group + 1;
-        const int all_lo = first_seen(g, sp.len, sp.n, row1 / g.group);
+        const int all_hi = TREE ? sp.len - sp.n : sp.len - sp.n + row0 / g.group + 1;
+        const int all_lo = first_seen(g, sp.len, sp.n, TREE ? sp.n - 1 : row1 / g.group);
 
         float4v o[CT][4 * DN];
         Base m[CT];
@@ -574,7 +636,12 @@ __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queri
             for (int ct = 0; ct < CT; ct++) {
                 Factor fk = times<SPLIT>(factor[ct], ks);
                 ValueScale v = scales;
-                if (!whole) mask_scores(s[ct], fk, v, t0 + 16 * quad, seen, g.window, hi[ct]);
+                if (!whole) {
+                    if constexpr (TREE)
+                        mask_scores(s[ct], fk, v, seen, tree_seen(g, sp, tree[ct], t0 + 16 * quad));
+                    else
+                        mask_scores(s[ct], fk, v, t0 + 16 * quad, seen, g.window, hi[ct]);
+                }
                 weights_of<SPLIT>(s[ct], fk, v, m[ct], l[ct], o[ct], p[ct], pl[ct]);
             }
 #pragma unroll
@@ -603,10 +670,10 @@ __device__ __forceinline__ void few_rows(const Work& f, int block, half8v* queri
     }
 }
 
-template <class T, int DN, int CT>
+template <class T, int DN, int CT, bool TREE>
 __global__ __launch_bounds__(256, 2) void attn_few_kernel(Work f) {
     extern __shared__ __align__(16) half8v shared[];
-    few_rows<T, DN, CT>(f, blockIdx.x, shared);
+    few_rows<T, DN, CT, TREE>(f, blockIdx.x, shared);
 }
 
 // ------------------------------------------------------------ prompts: tiled
@@ -621,10 +688,15 @@ constexpr int kRows = 64 * kCols<DN>;  // rows of a workgroup
 struct RowTiles {
     int row0, tile0, tile1;
 };
-template <int DN>
+template <int DN, bool TREE>
 __device__ __forceinline__ RowTiles tiles_of(const AttnArgs& g, const Span& sp, int row) {
     RowTiles w;
     w.row0 = row / kRows<DN> * kRows<DN>;
+    if (TREE) {
+        w.tile0 = tree_first(g, sp.len, sp.n) >> 6;
+        w.tile1 = max(tiles_up_to(sp.len), w.tile0);
+        return w;
+    }
     const int last = min(w.row0 + kRows<DN>, sp.n * g.group) - 1;
     w.tile0 = first_seen(g, sp.len, sp.n, w.row0 / g.group) >> 6;
     w.tile1 = max(tiles_up_to(max(0, sp.len - sp.n + last / g.group + 1)), w.tile0);
@@ -648,7 +720,7 @@ __device__ __forceinline__ RowTiles tiles_of(const AttnArgs& g, const Span& sp, 
 // workgroups.  fp32 rows take twice the products in two fp16 parts: 364 us, 1.03
 // PFLOP/s of them, with 38 registers kept in memory; at 256 dims those are 84, of
 // fp16 rows 24.
-template <class T, int DN>
+template <class T, int DN, bool TREE>
 __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {  // [2][FRAGS][64]
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int CT = kCols<DN>, FRAGS = 16 * DN;  // fragments of 64 lanes x 16 bytes in a buffer: keys', then values'
@@ -661,7 +733,7 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
     const int split = b % f.many.splits;
     b /= f.many.splits;
     const int r = b % g.requests, at = b / g.requests;  // (the longest rows of all requests first)
-    const Span sp = span_of(g, r);
+    const Span sp = span_of<TREE>(g, r);
     const int rows = sp.n * g.group;
     if (sp.n <= 0 || rows <= f.most) return;
     const Factor scale = factor_of(g);
@@ -671,7 +743,7 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
     // the later a row, the more tokens it sees: those first
     const int all = (rows + kRows<DN> - 1) / kRows<DN>;
     for (int qt = all - 1 - at; qt >= 0; qt -= f.qtiles) {
-        const RowTiles w = tiles_of<DN>(g, sp, qt * kRows<DN>);
+        const RowTiles w = tiles_of<DN, TREE>(g, sp, qt * kRows<DN>);
         const int ns = splits_of(f.many, w.tile1 - w.tile0);
         if (split >= ns) continue;
         const int first = w.tile0 + split * f.many.tiles, last = split == ns - 1 ? w.tile1 : first + f.many.tiles;
@@ -679,12 +751,16 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
         half8v q[CT][DN][2], ql[CT][DN][2];
         Factor factor[CT];
         int hi[CT];
+        TreeRow tree[CT];
         const int row0 = w.row0 + wave * 16 * CT, row1 = min(rows, row0 + 16 * CT) - 1;
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++)
-            load_query<T, DN>(f, sp, kv, row0 + 16 * ct + col, rows, scale, q[ct], ql[ct], factor[ct], hi[ct]);
-        const int all_hi = sp.len - sp.n + row0 / g.group + 1;
-        const int all_lo = first_seen(g, sp.len, sp.n, row1 / g.group);
+        for (int ct = 0; ct < CT; ct++) {
+            const int row = row0 + 16 * ct + col;
+            load_query<T, DN>(f, sp, kv, row, rows, scale, q[ct], ql[ct], factor[ct], hi[ct]);
+            if constexpr (TREE) tree[ct] = tree_row(g, sp, row / g.group, row < rows);
+        }
+        const int all_hi = TREE ? sp.len - sp.n : sp.len - sp.n + row0 / g.group + 1;
+        const int all_lo = first_seen(g, sp.len, sp.n, TREE ? sp.n - 1 : row1 / g.group);
 
         float4v o[CT][4 * DN];
         Base m[CT];
@@ -791,7 +867,12 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
             for (int ct = 0; ct < CT; ct++) {
                 Factor fk = times<SPLIT>(factor[ct], fs);
                 ValueScale v = scales;
-                if (!whole) mask_scores(s[ct], fk, v, t0 + 16 * quad, there, g.window, hi[ct]);
+                if (!whole) {
+                    if constexpr (TREE)
+                        mask_scores(s[ct], fk, v, there, tree_seen(g, sp, tree[ct], t0 + 16 * quad));
+                    else
+                        mask_scores(s[ct], fk, v, t0 + 16 * quad, there, g.window, hi[ct]);
+                }
                 weights_of<SPLIT>(s[ct], fk, v, m[ct], l[ct], o[ct], p[ct], pl[ct]);
             }
             put(buffer ^ 1);
@@ -831,13 +912,13 @@ __device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
 }
 
 // The other kernel's workgroups come last in the same launch: they are there while the tiled ones run out.
-template <class T, int DN>
+template <class T, int DN, bool TREE>
 __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f, int tiled) {
     extern __shared__ __align__(16) half8v shared[];
     if ((int)blockIdx.x < tiled)
-        many_rows<T, DN>(f, blockIdx.x, shared);
+        many_rows<T, DN, TREE>(f, blockIdx.x, shared);
     else
-        few_rows<T, DN, (DN <= 2 ? 2 : 1)>(f, blockIdx.x - tiled, shared);
+        few_rows<T, DN, (DN <= 2 ? 2 : 1), TREE>(f, blockIdx.x - tiled, shared);
 }
 
 // Joins what several waves or workgroups hold of a row, in their order: W waves
@@ -1035,7 +1116,7 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
     return p;
 }
 
-template <class T, int DN>
+template <class T, int DN, bool TREE>
 static int launch(const Work& f, const AttnPlan& p, hipStream_t stream) {
     const long tiled = (long)p.qtiles * p.many.splits * f.a.c.heads * f.a.requests;
     const int few = (f.shares + 3) / 4 + f.a.c.heads * f.empties;
@@ -1046,14 +1127,14 @@ static int launch(const Work& f, const AttnPlan& p, hipStream_t stream) {
         constexpr int lds = 2 * 16 * DN * 1024;
         static_assert(lds >= column * (DN <= 2 ? 2 : 1));
         if constexpr (lds > 65536) {
-            const hipError_t rc = raise_lds((const void*)attn_many_kernel<T, DN>, lds, raised);
+            const hipError_t rc = raise_lds((const void*)attn_many_kernel<T, DN, TREE>, lds, raised);
             if (rc != hipSuccess) return (int)rc;
         }
-        attn_many_kernel<T, DN><<<(unsigned)(tiled + few), 256, lds, stream>>>(f, (int)tiled);
+        attn_many_kernel<T, DN, TREE><<<(unsigned)(tiled + few), 256, lds, stream>>>(f, (int)tiled);
     } else if (p.ct == 2) {
-        if constexpr (DN <= 2) attn_few_kernel<T, DN, 2><<<few, 256, 2 * column, stream>>>(f);
+        if constexpr (DN <= 2) attn_few_kernel<T, DN, 2, TREE><<<few, 256, 2 * column, stream>>>(f);
     } else {
-        attn_few_kernel<T, DN, 1><<<few, 256, column, stream>>>(f);
+        attn_few_kernel<T, DN, 1, TREE><<<few, 256, column, stream>>>(f);
     }
     const auto join = [&](Join which, int each, bool wide) {
         each = (int)std::min((long)each, std::max(1l, ((1l << 31) - 1) / (std::max(1l, (long)f.a.requests) * f.a.q.heads)));
@@ -1074,7 +1155,9 @@ ZT_EXPORT long zt_kv8_attention_workspace_bytes(const zt_kv8_attn* a) {
     return p.part + p.stat + p.parts;
 }
 
-ZT_EXPORT int zt_kv8_attention(const zt_kv8_attn* a, void* workspace, long workspace_bytes, zt_stream_t stream) {
+template <bool TREE>
+static int attention(const zt_kv8_attn* a, const uint64_t* mask, int words, void* workspace, long workspace_bytes,
+                     hipStream_t stream) {
     if (!attn_ok(a)) return kInvalid;
     if (a->tokens == 0) return 0;
     if (!rows_ok(a->q, a->type) || !rows_ok(a->out, a->type) || !a->q_start ||
@@ -1086,15 +1169,25 @@ ZT_EXPORT int zt_kv8_attention(const zt_kv8_attn* a, void* workspace, long works
     const double unit = 1.44269504088896340736 / std::sqrt((double)a->cache.head_dim);
     const AttnArgs g{kv8_of(a->cache), rows_of(a->q), rows_of(a->out), a->table, a->kv_lens, a->q_start, a->scale,
                      a->requests,      a->width,      a->tokens,       a->window, a->q.heads / a->cache.kv_heads,
-                     (float)unit,      (float)(unit - (double)(float)unit)};
+                     (float)unit,      (float)(unit - (double)(float)unit), mask, words};
     const Work f{g,        p.most, p.shares, p.empties, p.single, p.many, p.qtiles, rows_vector(a->q, 4, a->type) && rows_vector(a->out, 4, a->type),
                  p.others, p.places, std::max(p.shares, p.many.splits), (float*)workspace, (float2*)((char*)workspace + p.part),
                  (int2*)((char*)workspace + p.part + p.stat)};
     const bool f32 = a->type == ZT_F32;
     switch (g.c.dp) {
-        case 64: return f32 ? launch<float, 1>(f, p, stream) : launch<_Float16, 1>(f, p, stream);
-        case 128: return f32 ? launch<float, 2>(f, p, stream) : launch<_Float16, 2>(f, p, stream);
-        case 192: return f32 ? launch<float, 3>(f, p, stream) : launch<_Float16, 3>(f, p, stream);
-        default: return f32 ? launch<float, 4>(f, p, stream) : launch<_Float16, 4>(f, p, stream);
+        case 64: return f32 ? launch<float, 1, TREE>(f, p, stream) : launch<_Float16, 1, TREE>(f, p, stream);
+        case 128: return f32 ? launch<float, 2, TREE>(f, p, stream) : launch<_Float16, 2, TREE>(f, p, stream);
+        case 192: return f32 ? launch<float, 3, TREE>(f, p, stream) : launch<_Float16, 3, TREE>(f, p, stream);
+        default: return f32 ? launch<float, 4, TREE>(f, p, stream) : launch<_Float16, 4, TREE>(f, p, stream);
     }
+}
+
+ZT_EXPORT int zt_kv8_attention(const zt_kv8_attn* a, void* workspace, long workspace_bytes, zt_stream_t stream) {
+    return attention<false>(a, nullptr, 0, workspace, workspace_bytes, stream);
+}
+
+ZT_EXPORT int zt_kv8_tree_attention(const zt_kv8_attn* a, const uint64_t* mask, int words, void* workspace,
+                                    long workspace_bytes, zt_stream_t stream) {
+    if (words < 1 || words > ZT_TREE_WORDS || ((uintptr_t)mask & 7) || (a && a->tokens > 0 && !mask)) return kInvalid;
+    return attention<true>(a, mask, words, workspace, workspace_bytes, stream);
 }

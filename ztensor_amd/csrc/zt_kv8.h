@@ -48,6 +48,27 @@ __host__ inline bool rows_vector(const zt_rows& r, int n, int type) {
     return ((uintptr_t)r.p & (n * (type == ZT_F16 ? 2 : 4) - 1)) == 0 && r.token_stride % n == 0 && r.head_stride % n == 0;
 }
 
+// Buffers of a call, and whether what it writes shares no bytes with what it
+// reads, nor with each other.
+struct Bytes {
+    const void* p;
+    long n;
+    bool meets(const Bytes& o) const {
+        const uintptr_t a = (uintptr_t)p, b = (uintptr_t)o.p;
+        return n > 0 && o.n > 0 && a < b + o.n && b < a + n;
+    }
+};
+template <int I, int O>
+__host__ inline bool apart(const Bytes (&in)[I], const Bytes (&out)[O]) {
+    for (int i = 0; i < O; i++) {
+        for (const Bytes& b : in)
+            if (out[i].meets(b)) return false;
+        for (int j = 0; j < i; j++)
+            if (out[i].meets(out[j])) return false;
+    }
+    return true;
+}
+
 template <class T, int V>
 __device__ __forceinline__ void load_values(const T* p, float (&v)[V]) {
     typedef T vec __attribute__((ext_vector_type(V)));
@@ -212,6 +233,22 @@ __host__ inline int head_lanes(int units) {
     int l = 1;
     while (l < units && l < 64) l *= 2;
     return l;
+}
+
+// The largest m of a workgroup of four waves, and whether any of its threads said bad.
+__device__ __forceinline__ void block_peak(float& m, bool& bad, float* red) {
+    bad = __any(bad);
+    m = max_step<1>(max_step<2>(max_step<4>(max_step<8>(max_step<16>(max_step<32>(m))))));
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) red[wave] = bad ? __builtin_inff() : m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    bad = m > kMaxFloat;
+}
+
+__device__ __forceinline__ int code_of(float x, float scale) {
+    const float q = rintf(x / scale);
+    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
 }
 
 // A [tokens, heads, dim] operand as kernels take it.

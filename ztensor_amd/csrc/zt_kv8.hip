@@ -233,22 +233,6 @@ struct AppendArgs {
     long blocks;
 };
 
-// The largest m of the workgroup, and whether any of its threads said bad.
-__device__ __forceinline__ void block_peak(float& m, bool& bad, float* red) {
-    bad = __any(bad);
-    m = max_step<1>(max_step<2>(max_step<4>(max_step<8>(max_step<16>(max_step<32>(m))))));
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) red[wave] = bad ? __builtin_inff() : m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    bad = m > kMaxFloat;
-}
-
-__device__ __forceinline__ int code_of(float x, float scale) {
-    const float q = rintf(x / scale);
-    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
-}
-
 // The tokens of one page: n of them, from token t on.
 struct Run {
     int t, n, page, off;
@@ -757,15 +741,6 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs g) {
 }
 
 }  // namespace zt
-
-struct Bytes {
-    const void* p;
-    long n;
-    bool meets(const Bytes& o) const {
-        const uintptr_t a = (uintptr_t)p, b = (uintptr_t)o.p;
-        return n > 0 && o.n > 0 && a < b + o.n && b < a + n;
-    }
-};
 
 ZT_EXPORT int zt_kv8_plan(const int* kv_lens, const int* add, const int* table, int requests, int width,
                           const int* free_pages, const int* free_count, int free_capacity, int page_tokens, int tokens,

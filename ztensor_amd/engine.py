@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 from ._stream import _on_engine_stream
-from .decode import DecodeOps
+from .drafts import DraftOps
 from .storage import (
     AWQStorage,
     Float16Storage,
@@ -64,7 +64,7 @@ def _tiled_cached(s: Any, key: tuple):
     return None
 
 
-class ROCmEngine(DecodeOps):
+class ROCmEngine(DraftOps):
     def __init__(self, device: int = 0, stream: torch.cuda.Stream | None = None, q6k_split: bool = True,
                  split_reserve_bytes: int = 1 << 30, token_copies: bool = True):
         """q6k_split: Q6_K batch 1 on a split copy of the super-blocks (35-55%
