@@ -833,8 +833,9 @@ int zt_kv8_tree(const int* parents, const int* kv_lens, const int* q_start, int 
  * of the context, the last tokens from position - window + 1 on, where its
  * position is the context's length and the rows that it sees, less one; its own
  * request's rows are seen as the mask says.  mask: [tokens][words] on the device,
- * 8-byte aligned, words from 1 to ZT_TREE_WORDS, else InvalidValue.  The
- * workspace is zt_kv8_attention_workspace_bytes'. */
+ * 8-byte aligned, words from 1 to ZT_TREE_WORDS, else InvalidValue.  Workspace:
+ * zt_kv8_tree_attention_workspace_bytes, as above. */
+long zt_kv8_tree_attention_workspace_bytes(const zt_kv8_attn* a);
 int zt_kv8_tree_attention(const zt_kv8_attn* a, const uint64_t* mask, int words, void* workspace, long workspace_bytes,
                           zt_stream_t stream);
 

@@ -146,6 +146,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "zt_kv8_copy": (I, [P, I, P, P, I, P]),
     "zt_kv8_trim": (I, [P, P, P, I, I, P, P, I, I, P, P, P, P]),
     "zt_kv8_fork": (I, [P, P]),
+    "zt_kv8_tree_attention_workspace_bytes": (L, [P]),
     "zt_kv8_tree_attention": (I, [P, P, I, P, L, P]),
     "zt_sample_workspace_bytes": (L, [I, I]),
     "zt_sample": (I, [P, L, I, I, I, P, P, P, P, P, P, P, P, L, P]),

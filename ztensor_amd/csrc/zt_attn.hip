@@ -8,9 +8,12 @@
 // several waves have of one row.  A call whose requests have at most 64 rows of a
 // key/value head (tokens x the group of its q heads) is the first kernel's, which
 // reads a tile for 16 or 32 of them; in a call of longer ones those of up to 64
-// still are, and the others' rows are the second's, up to 128 at a time.
+// still are, and the others' rows are the second's, up to 128 at a time.  A drafted
+// tree's rows, which masks tell apart, are the second's from 17 on, dealt out as
+// the first kernel's are.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "zt_kv8.h"
 
@@ -43,6 +46,8 @@ struct Work {
     bool single; // each takes whole heads
     Split many;
     int qtiles;  // workgroups along the rows of the other kernel
+    int tree_shares, tree_rows;  // or, of trees, its workgroups in all and the rows of one
+    bool tree_whole;  // each of which takes whole segments
     int vec;     // q and out in pieces of 4 values
     long others; // rows of sums that the few kernel has room for; the other kernel's follow
     long places; // of both
@@ -170,21 +175,20 @@ __device__ __forceinline__ TreeRow tree_row(const AttnArgs& g, const Span& sp, i
     r.lo = (int)min((long)context, max(0l, (long)context + seen - g.window));
     return r;
 }
-// Which of tokens t .. t + 15 it sees.
-__device__ __forceinline__ uint32_t tree_seen(const AttnArgs& g, const Span& sp, const TreeRow& r, int t) {
+// Which of tokens t .. t + 15 it sees.  (Few tiles ask: what it needs is worked out here, not held in registers.)
+__device__ __forceinline__ uint32_t tree_seen(const AttnArgs& g, const Span& sp, TreeRow r, int t) {
+    asm volatile("" : "+v"(r.row), "+v"(r.lo), "+v"(t));
     if (r.row < 0 || t >= sp.len) return 0;
     const int d = t - (sp.len - sp.n);  // the first one's bit
     uint32_t seen = 0xFFFFu;
     if (d > -16) {
         const uint64_t* mask = g.mask + (long)r.row * g.words;
-        if (d < 0) {
-            seen = (uint32_t)(mask[0] << -d) | ((1u << -d) - 1);
-        } else {
-            const int w = d >> 6, at = d & 63;
-            uint64_t x = w < g.words ? mask[w] >> at : 0;
-            if (at > 48 && w + 1 < g.words) x |= mask[w + 1] << (64 - at);
-            seen = (uint32_t)x;
-        }
+        const int w = max(d, 0) >> 6, at = d & 63;
+        const uint64_t lo = mask[min(w, g.words - 1)], hi = mask[min(w + 1, g.words - 1)];  // (both asked for at once)
+        if (d < 0)
+            seen = (uint32_t)(lo << -d) | ((1u << -d) - 1);
+        else
+            seen = (uint32_t)((w < g.words ? lo >> at : 0) | (at > 48 && w + 1 < g.words ? hi << (64 - at) : 0));
     }
     if (r.lo > t) seen &= r.lo - t < 16 ? ~0u << (r.lo - t) : 0;
     return seen & (sp.len - t < 16 ? (1u << (sp.len - t)) - 1 : 0xFFFFu);
@@ -683,20 +687,20 @@ template <int DN>
 constexpr int kCols = DN <= 2 ? 2 : 1;
 template <int DN>
 constexpr int kRows = 64 * kCols<DN>;  // rows of a workgroup
+// Of trees: what a tile counts for, whose waves have so many columns, and a segment's beginning.
+template <int COLS>
+constexpr int kTreeTile = COLS == 2 ? 5 : 4;
+template <int COLS>
+constexpr int kTreeBegin = COLS == 2 ? 29 : 18;
 
 // The workgroup's rows that `row` is among: the tiles that they see.
 struct RowTiles {
     int row0, tile0, tile1;
 };
-template <int DN, bool TREE>
+template <int DN>
 __device__ __forceinline__ RowTiles tiles_of(const AttnArgs& g, const Span& sp, int row) {
     RowTiles w;
     w.row0 = row / kRows<DN> * kRows<DN>;
-    if (TREE) {
-        w.tile0 = tree_first(g, sp.len, sp.n) >> 6;
-        w.tile1 = max(tiles_up_to(sp.len), w.tile0);
-        return w;
-    }
     const int last = min(w.row0 + kRows<DN>, sp.n * g.group) - 1;
     w.tile0 = first_seen(g, sp.len, sp.n, w.row0 / g.group) >> 6;
     w.tile1 = max(tiles_up_to(max(0, sp.len - sp.n + last / g.group + 1)), w.tile0);
@@ -720,205 +724,372 @@ __device__ __forceinline__ RowTiles tiles_of(const AttnArgs& g, const Span& sp, 
 // workgroups.  fp32 rows take twice the products in two fp16 parts: 364 us, 1.03
 // PFLOP/s of them, with 38 registers kept in memory; at 256 dims those are 84, of
 // fp16 rows 24.
-template <class T, int DN, bool TREE>
-__device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {  // [2][FRAGS][64]
+// What of them a workgroup works on at a time: rows row0 on of a request and a
+// key/value head, tiles first .. last - 1; their sums are the rows' own, or go to
+// `part` (its place of row 0).
+struct Tiles {
+    int r, kv, row0, first, last;
+};
+template <class T, int DN, int CT, bool TREE, class Done>
+__device__ __forceinline__ void many_tiles(const Work& f, const Span& sp, const Tiles& w, half8v* tiles, Done done) {  // [2][FRAGS][64]
     constexpr bool SPLIT = sizeof(T) == 4;
-    constexpr int CT = kCols<DN>, FRAGS = 16 * DN;  // fragments of 64 lanes x 16 bytes in a buffer: keys', then values'
+    constexpr int FRAGS = 16 * DN;  // fragments of 64 lanes x 16 bytes in a buffer: keys', then values'
     const AttnArgs& g = f.a;
     const Kv8& c = g.c;
     const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kv = b % c.heads;
-    b /= c.heads;
-    const int split = b % f.many.splits;
-    b /= f.many.splits;
-    const int r = b % g.requests, at = b / g.requests;  // (the longest rows of all requests first)
-    const Span sp = span_of<TREE>(g, r);
-    const int rows = sp.n * g.group;
-    if (sp.n <= 0 || rows <= f.most) return;
+    const int kv = w.kv, rows = sp.n * g.group, first = w.first, last = w.last;
     const Factor scale = factor_of(g);
     const int krow = (col >> 2) * 16 + (col & 3);
-    const Pages page_of{g.table + (long)r * g.width, sp.len, c.shift};
+    const Pages page_of{g.table + (long)w.r * g.width, sp.len, c.shift};
 
-    // the later a row, the more tokens it sees: those first
-    const int all = (rows + kRows<DN> - 1) / kRows<DN>;
-    for (int qt = all - 1 - at; qt >= 0; qt -= f.qtiles) {
-        const RowTiles w = tiles_of<DN, TREE>(g, sp, qt * kRows<DN>);
-        const int ns = splits_of(f.many, w.tile1 - w.tile0);
-        if (split >= ns) continue;
-        const int first = w.tile0 + split * f.many.tiles, last = split == ns - 1 ? w.tile1 : first + f.many.tiles;
-
-        half8v q[CT][DN][2], ql[CT][DN][2];
-        Factor factor[CT];
-        int hi[CT];
-        TreeRow tree[CT];
-        const int row0 = w.row0 + wave * 16 * CT, row1 = min(rows, row0 + 16 * CT) - 1;
+    // this wave's share of a tile: key tile j = wave (DN loads), values' dims 16 (DN wave + i) (DN loads).  A tile of one
+    // column is too short for its loads: they are asked for a tile earlier.
+    constexpr int DEPTH = TREE && CT == 1 ? 2 : 1;
+    u32x4 kw[DEPTH][DN], vw[DEPTH][DN];
+    float ks[DEPTH], vs[DEPTH];
+    bool seen[DEPTH];
+    // (a tile begins at a multiple of 64: what a lane adds to that stays in the page, or is taken modulo its tokens)
+    const uint32_t page_bytes = (uint32_t)c.heads * c.bytes(), head_bytes = (uint32_t)kv * c.bytes();
+    const uint32_t k_lane = ((krow + 4 * wave) & (c.page - 1)) * c.dp + 16 * quad + head_bytes;
+    const uint32_t v_lane = (16 * DN * wave + col) * c.page + ((16 * quad) & (c.page - 1)) + head_bytes;
+    auto fetch = [&](int slot, int tile, int pk, int pv) __attribute__((always_inline)) {
+        const unsigned t0 = tile * 64u, in = t0 & (c.page - 1);
+        seen[slot] = page_of.seen(c, pv, t0 + 16 * quad);
+        const uint32_t p = seen[slot] ? pv : 0, q = page_of.seen(c, pk, t0 + (col >> 2) * 16) ? pk : 0;
+        const int8_t* kp = c.k + ((uint64_t)q * page_bytes + (k_lane + in * c.dp));
+        const int8_t* vp = c.v + ((uint64_t)p * page_bytes + (v_lane + in));
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++) {
-            const int row = row0 + 16 * ct + col;
-            load_query<T, DN>(f, sp, kv, row, rows, scale, q[ct], ql[ct], factor[ct], hi[ct]);
-            if constexpr (TREE) tree[ct] = tree_row(g, sp, row / g.group, row < rows);
+        for (int d = 0; d < DN; d++) {
+            kw[slot][d] = *reinterpret_cast<const u32x4*>(kp + 64 * d);
+            vw[slot][d] = *reinterpret_cast<const u32x4*>(vp + 16 * d * c.page);
         }
-        const int all_hi = TREE ? sp.len - sp.n : sp.len - sp.n + row0 / g.group + 1;
-        const int all_lo = first_seen(g, sp.len, sp.n, TREE ? sp.n - 1 : row1 / g.group);
-
-        float4v o[CT][4 * DN];
-        Base m[CT];
-        float l[CT];
+        const uint32_t at = p * c.heads + kv;
+        ks[slot] = c.k_scale[at];
+        vs[slot] = c.v_scale[at];
+    };
+    auto put = [&](int slot, int buffer) __attribute__((always_inline)) {
+        half8v* to = tiles + buffer * FRAGS * 64 + lane;
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++) {
-            m[ct] = {kNothing, kNothing};
-            l[ct] = 0.0f;
+        for (int d = 0; d < DN; d++)
 #pragma unroll
-            for (int i = 0; i < 4 * DN; i++) o[ct][i] = (float4v){0, 0, 0, 0};
-        }
-
-        // this wave's share of a tile: key tile j = wave (DN loads), values' dims 16 (DN wave + i) (DN loads)
-        u32x4 kw[DN], vw[DN];
-        float ks, vs;
-        bool seen;
-        // (a tile begins at a multiple of 64: what a lane adds to that stays in the page, or is taken modulo its tokens)
-        const uint32_t page_bytes = (uint32_t)c.heads * c.bytes(), head_bytes = (uint32_t)kv * c.bytes();
-        const uint32_t k_lane = ((krow + 4 * wave) & (c.page - 1)) * c.dp + 16 * quad + head_bytes;
-        const uint32_t v_lane = (16 * DN * wave + col) * c.page + ((16 * quad) & (c.page - 1)) + head_bytes;
-        auto fetch = [&](int tile, int pk, int pv) {
-            const unsigned t0 = tile * 64u, in = t0 & (c.page - 1);
-            seen = page_of.seen(c, pv, t0 + 16 * quad);
-            const uint32_t p = seen ? pv : 0, q = page_of.seen(c, pk, t0 + (col >> 2) * 16) ? pk : 0;
-            const int8_t* kp = c.k + ((uint64_t)q * page_bytes + (k_lane + in * c.dp));
-            const int8_t* vp = c.v + ((uint64_t)p * page_bytes + (v_lane + in));
-#pragma unroll
-            for (int d = 0; d < DN; d++) {
-                kw[d] = *reinterpret_cast<const u32x4*>(kp + 64 * d);
-                vw[d] = *reinterpret_cast<const u32x4*>(vp + 16 * d * c.page);
+            for (int h = 0; h < 2; h++) {
+                to[((wave * DN + d) * 2 + h) * 64] = codes8(kw[slot][d][2 * h], kw[slot][d][2 * h + 1]);
+                to[(8 * DN + (wave * DN + d) * 2 + h) * 64] = codes8(vw[slot][d][2 * h], vw[slot][d][2 * h + 1]);
             }
-            const uint32_t at = p * c.heads + kv;
-            ks = c.k_scale[at];
-            vs = c.v_scale[at];
-        };
-        auto put = [&](int buffer) {
-            half8v* to = tiles + buffer * FRAGS * 64 + lane;
-#pragma unroll
-            for (int d = 0; d < DN; d++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    to[((wave * DN + d) * 2 + h) * 64] = codes8(kw[d][2 * h], kw[d][2 * h + 1]);
-                    to[(8 * DN + (wave * DN + d) * 2 + h) * 64] = codes8(vw[d][2 * h], vw[d][2 * h + 1]);
-                }
-        };
-        int pk = page_of(first * 64 + (col >> 2) * 16), pv = page_of(first * 64 + quad * 16);
-        __syncthreads();  // nobody reads the buffers of the rows before any more
-        if (first < last) {
-            fetch(first, pk, pv);
-            pk = page_of(first * 64 + 64u + (col >> 2) * 16);
-            pv = page_of(first * 64 + 64u + quad * 16);
-            put(0);
+    };
+    // the pages of a tile's keys and values in this lane (of a tree without a condition, whose branch would wait for them)
+    const unsigned last_token = max(sp.len, 1) - 1;
+    auto page_at = [&](unsigned token) __attribute__((always_inline)) {
+        return TREE ? page_of.row[min(token, last_token) >> c.shift] : page_of(token);
+    };
+    auto key_page = [&](int tile) __attribute__((always_inline)) { return page_at(tile * 64u + (col >> 2) * 16); };
+    auto value_page = [&](int tile) __attribute__((always_inline)) { return page_at(tile * 64u + quad * 16); };
+    int pk = key_page(first), pv = value_page(first);
+    if (first < last) {
+        int nk = 0, nv = 0;
+        if (DEPTH == 2) {
+            nk = key_page(first + 1);
+            nv = value_page(first + 1);
         }
-        __syncthreads();
-        for (int tile = first, buffer = 0; tile < last; tile++, buffer ^= 1) {
-            const int t0 = tile * 64;
-            const float fs = ks, fvs = vs;
-            const bool there = seen;
-            const bool whole = t0 <= all_hi - 64 && t0 >= all_lo && __all(there);
-            // (past the last tile: of the last token's page, for nobody)
-            fetch(tile + 1, pk, pv);
-            pk = page_of(t0 + 128u + (col >> 2) * 16);
-            pv = page_of(t0 + 128u + quad * 16);
-            const half8v* from = tiles + buffer * FRAGS * 64 + lane;
+        fetch(0, first, pk, pv);
+        if (DEPTH == 2) {
+            pk = key_page(first + 2);
+            pv = value_page(first + 2);
+            fetch(DEPTH - 1, first + 1, nk, nv);
+        } else {
+            pk = key_page(first + 1);
+            pv = value_page(first + 1);
+        }
+    }
 
-            const ValueScale scales = value_scale<SPLIT>(fvs);
+    half8v q[CT][DN][2], ql[CT][DN][2];
+    Factor factor[CT];
+    int hi[CT];
+    TreeRow tree[CT];
+    const int row0 = w.row0 + wave * 16 * CT, row1 = min(rows, row0 + 16 * CT) - 1;
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        const int row = row0 + 16 * ct + col;
+        load_query<T, DN>(f, sp, kv, row, rows, scale, q[ct], ql[ct], factor[ct], hi[ct]);
+        if constexpr (TREE) tree[ct] = tree_row(g, sp, row / g.group, row < rows);
+    }
+    const int all_hi = TREE ? sp.len - sp.n : sp.len - sp.n + row0 / g.group + 1;
+    const int all_lo = first_seen(g, sp.len, sp.n, TREE ? sp.n - 1 : row1 / g.group);
 
-            // four fragments ahead of the products that take them, sums that depend on each other 8 products apart
-            half8v frag[2][4];
-            auto keys = [&](int to, int k) {
+    float4v o[CT][4 * DN];
+    Base m[CT];
+    float l[CT];
 #pragma unroll
-                for (int j = 0; j < 4; j++) frag[to][j] = from[(j * 2 * DN + k) * 64];
-            };
-            auto values = [&](int to, int at) {
+    for (int ct = 0; ct < CT; ct++) {
+        m[ct] = {kNothing, kNothing};
+        l[ct] = 0.0f;
 #pragma unroll
-                for (int k = 0; k < 4; k++) frag[to][k] = from[(8 * DN + 4 * at + k) * 64];
-            };
-            __builtin_amdgcn_s_setprio(1);  // the other workgroup's wave has the vector unit meanwhile
-            float4v s[CT][4];
+        for (int i = 0; i < 4 * DN; i++) o[ct][i] = (float4v){0, 0, 0, 0};
+    }
+
+    __syncthreads();  // nobody reads the buffers of the rows before any more
+    if (first < last) put(0, 0);
+    __syncthreads();
+    auto step = [&](int tile, int buffer, int slot) __attribute__((always_inline)) {  // the slot of this tile, and of tile + DEPTH
+        const int t0 = tile * 64;
+        const float fs = ks[slot], fvs = vs[slot];
+        const bool there = seen[slot];
+        const bool whole = t0 <= all_hi - 64 && t0 >= all_lo && __all(there);
+        // (past the last tile: of the last token's page, for nobody)
+        if (DEPTH == 2) {  // loads come back in their order: the pages' numbers, which are waited for first, before codes
+            const int nk = key_page(tile + 3), nv = value_page(tile + 3);
+            __builtin_amdgcn_sched_barrier(0);
+            fetch(slot, tile + 2, pk, pv);
+            pk = nk;
+            pv = nv;
+        } else {
+            fetch(slot, tile + 1, pk, pv);
+            pk = key_page(tile + 2);
+            pv = value_page(tile + 2);
+        }
+        const half8v* from = tiles + buffer * FRAGS * 64 + lane;
+
+        const ValueScale scales = value_scale<SPLIT>(fvs);
+
+        // four fragments ahead of the products that take them, sums that depend on each other 8 products apart
+        half8v frag[2][4];
+        auto keys = [&](int to, int k) {
 #pragma unroll
-            for (int ct = 0; ct < CT; ct++)
+            for (int j = 0; j < 4; j++) frag[to][j] = from[(j * 2 * DN + k) * 64];
+        };
+        auto values = [&](int to, int at) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) s[ct][j] = (float4v){0, 0, 0, 0};
-            keys(0, 0);
+            for (int k = 0; k < 4; k++) frag[to][k] = from[(8 * DN + 4 * at + k) * 64];
+        };
+        __builtin_amdgcn_s_setprio(1);  // the other workgroup's wave has the vector unit meanwhile
+        float4v s[CT][4];
 #pragma unroll
-            for (int k = 0; k < 2 * DN; k++) {
-                if (k + 1 < 2 * DN) keys((k + 1) & 1, k + 1); else values((k + 1) & 1, 0);
+        for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) s[ct][j] = (float4v){0, 0, 0, 0};
+        keys(0, 0);
+#pragma unroll
+        for (int k = 0; k < 2 * DN; k++) {
+            if (k + 1 < 2 * DN) keys((k + 1) & 1, k + 1); else values((k + 1) & 1, 0);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) s[ct][j] = mfma(frag[k & 1][j], q[ct][k >> 1][k & 1], s[ct][j]);
+            if constexpr (SPLIT) {
 #pragma unroll
                 for (int j = 0; j < 4; j++)
 #pragma unroll
-                    for (int ct = 0; ct < CT; ct++) s[ct][j] = mfma(frag[k & 1][j], q[ct][k >> 1][k & 1], s[ct][j]);
+                    for (int ct = 0; ct < CT; ct++) s[ct][j] = mfma(frag[k & 1][j], ql[ct][k >> 1][k & 1], s[ct][j]);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 4 * CT * (SPLIT ? 2 : 1), 0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        half8v p[CT][2], pl[CT][2];
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            Factor fk = times<SPLIT>(factor[ct], fs);
+            ValueScale v = scales;
+            if (!whole) {
+                if constexpr (TREE)
+                    mask_scores(s[ct], fk, v, there, tree_seen(g, sp, tree[ct], t0 + 16 * quad));
+                else
+                    mask_scores(s[ct], fk, v, t0 + 16 * quad, there, g.window, hi[ct]);
+            }
+            weights_of<SPLIT>(s[ct], fk, v, m[ct], l[ct], o[ct], p[ct], pl[ct]);
+        }
+        put(DEPTH == 2 ? slot ^ 1 : slot, buffer ^ 1);
+#pragma unroll
+        for (int j = 0; j < 2 * DN; j++) {
+            if (j + 1 < 2 * DN) values((j + 1) & 1, j + 1);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++)
+                        o[ct][2 * j + e] = mfma(frag[j & 1][2 * e + h], p[ct][h], o[ct][2 * j + e]);
                 if constexpr (SPLIT) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-#pragma unroll
-                        for (int ct = 0; ct < CT; ct++) s[ct][j] = mfma(frag[k & 1][j], ql[ct][k >> 1][k & 1], s[ct][j]);
-                }
-                __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-                __builtin_amdgcn_sched_group_barrier(0x008, 4 * CT * (SPLIT ? 2 : 1), 0);
-            }
-            __builtin_amdgcn_s_setprio(0);
-            half8v p[CT][2], pl[CT][2];
-#pragma unroll
-            for (int ct = 0; ct < CT; ct++) {
-                Factor fk = times<SPLIT>(factor[ct], fs);
-                ValueScale v = scales;
-                if (!whole) {
-                    if constexpr (TREE)
-                        mask_scores(s[ct], fk, v, there, tree_seen(g, sp, tree[ct], t0 + 16 * quad));
-                    else
-                        mask_scores(s[ct], fk, v, t0 + 16 * quad, there, g.window, hi[ct]);
-                }
-                weights_of<SPLIT>(s[ct], fk, v, m[ct], l[ct], o[ct], p[ct], pl[ct]);
-            }
-            put(buffer ^ 1);
-#pragma unroll
-            for (int j = 0; j < 2 * DN; j++) {
-                if (j + 1 < 2 * DN) values((j + 1) & 1, j + 1);
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
 #pragma unroll
                     for (int e = 0; e < 2; e++)
 #pragma unroll
                         for (int ct = 0; ct < CT; ct++)
-                            o[ct][2 * j + e] = mfma(frag[j & 1][2 * e + h], p[ct][h], o[ct][2 * j + e]);
-                    if constexpr (SPLIT) {
-#pragma unroll
-                        for (int e = 0; e < 2; e++)
-#pragma unroll
-                            for (int ct = 0; ct < CT; ct++)
-                                o[ct][2 * j + e] = mfma(frag[j & 1][2 * e + h], pl[ct][h], o[ct][2 * j + e]);
-                    }
+                            o[ct][2 * j + e] = mfma(frag[j & 1][2 * e + h], pl[ct][h], o[ct][2 * j + e]);
                 }
             }
-            __syncthreads();
         }
+        __syncthreads();
+    };
+    if constexpr (DEPTH == 2) {
+        for (int tile = first; tile < last; tile += 2) {
+            step(tile, 0, 0);
+            if (tile + 1 < last) step(tile + 1, 1, DEPTH - 1);
+        }
+    } else {
+        for (int tile = first, buffer = 0; tile < last; tile++, buffer ^= 1) step(tile, buffer, 0);
+    }
 
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++) {
-            l[ct] += __shfl_xor(l[ct], 16);
-            l[ct] += __shfl_xor(l[ct], 32);
-            const int row = row0 + 16 * ct + col, i = row / g.group;
-            if (f.many.splits > 1 && split == 0 && row < rows && quad == 0)
-                f.parts[(long)(sp.start + i) * g.q.heads + kv * g.group + row - i * g.group] = make_int2(0, ns);
-            store_row<T, DN>(f, sp, kv, row, rows, ns > 1, f.many_at(split, sp.start + i, kv * g.group + row - i * g.group), m[ct],
-                             l[ct], o[ct]);
-        }
+    for (int ct = 0; ct < CT; ct++) {
+        l[ct] += __shfl_xor(l[ct], 16);
+        l[ct] += __shfl_xor(l[ct], 32);
+        done(row0 + 16 * ct + col, (wave * CT + ct) * 16 + col, m[ct], l[ct], o[ct]);
     }
 }
 
-// The other kernel's workgroups come last in the same launch: they are there while the tiled ones run out.
-template <class T, int DN, bool TREE>
+template <class T, int DN>
+__device__ __forceinline__ void many_rows(const Work& f, int b, half8v* tiles) {
+    const AttnArgs& g = f.a;
+    const int kv = b % g.c.heads;
+    b /= g.c.heads;
+    const int split = b % f.many.splits;
+    b /= f.many.splits;
+    const int r = b % g.requests, at = b / g.requests;  // (the longest rows of all requests first)
+    const Span sp = span_of<false>(g, r);
+    const int rows = sp.n * g.group;
+    if (sp.n <= 0 || rows <= f.most) return;
+
+    // the later a row, the more tokens it sees: those first
+    const int all = (rows + kRows<DN> - 1) / kRows<DN>;
+    for (int qt = all - 1 - at; qt >= 0; qt -= f.qtiles) {
+        const RowTiles w = tiles_of<DN>(g, sp, qt * kRows<DN>);
+        const int ns = splits_of(f.many, w.tile1 - w.tile0);
+        if (split >= ns) continue;
+        const int first = w.tile0 + split * f.many.tiles, last = split == ns - 1 ? w.tile1 : first + f.many.tiles;
+        many_tiles<T, DN, kCols<DN>, false>(f, sp, {r, kv, w.row0, first, last}, tiles, [&](int row, int, const Base& m, float l, const float4v (&o)[4 * DN]) {
+            const int i = row / g.group, t = sp.start + i, h = kv * g.group + row - i * g.group;
+            if (f.many.splits > 1 && split == 0 && row < rows && (threadIdx.x & 48) == 0)
+                f.parts[(long)t * g.q.heads + h] = make_int2(0, ns);
+            store_row<T, DN>(f, sp, kv, row, rows, ns > 1, f.many_at(split, t, h), m, l, o);
+        });
+    }
+}
+
+// ------------------------------------------------------------- trees: tiled
+
+// A wave's value of what all of its lanes have, in scalar registers.
+__device__ __forceinline__ int one_of(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ long one_of(long v) {
+    return (long)((uint64_t)(uint32_t)one_of((int)(v >> 32)) << 32 | (uint32_t)one_of((int)v));
+}
+
+// Columns of 16 rows that a wave holds at most, and rows of a workgroup: two columns where the registers allow it (fp32
+// rows of 128 dims, which keep 54 in memory then: 24 trees of 64 495 us, with one column 470; fp16 rows 293 and 344).
+template <class T, int DN>
+constexpr int kTreeCols = DN == 1 || (DN == 2 && sizeof(T) == 2) ? 2 : 1;
+template <class T, int DN>
+constexpr int kTreeRows = 64 * kTreeCols<T, DN>;
+
+// A tree's rows all see its whole context, and contexts may be of any lengths: as
+// in the few kernel every workgroup takes an equal share of a row of tiles, request
+// after request, of each its heads and of these its groups of kTreeRows rows, each
+// with all of its tiles after a place for its beginning.  A last group of up to 64
+// rows has one column, whose tile takes 1.67 us while the card is full, one of two
+// columns 2.05; a beginning (the page's number, then the codes, the masked tiles,
+// the end's sums) takes about 12, so they count 4, 5 and 29, and, where there is
+// one column only, 4 and 18.  64 requests' spans lie in LDS at a time.
+//
+// 24 trees of up to 64 rows, 64 heads over 8 of 128, on contexts of up to 12000
+// (fp16, 185 GFLOP): 285 us, 0.65 PFLOP/s; with workgroups that take whole groups
+// 472.  What bounds it: a tile of two columns is 64 matrix instructions (1024
+// cycles) and some 320 of the vector unit, and beside a full stream of matrix
+// instructions that issues one each 8.5 cycles (5.2 alone); 2.05 us at 1.8 GHz are
+// 3700 cycles for the two waves of a SIMD.
+struct TreeSpans {
+    Span span[64];
+    long upto[64];
+};
+template <class T, int DN>
+__device__ __forceinline__ void tree_rows(const Work& f, int share, half8v* tiles, TreeSpans& in) {
+    const AttnArgs& g = f.a;
+    const int lane = threadIdx.x & 63;
+    const bool whole = f.tree_whole;
+    constexpr int ROWS = kTreeRows<T, DN>, COLS = kTreeCols<T, DN>;
+    auto groups = [&](const Span& sp) { return (sp.n * g.group + ROWS - 1) / ROWS; };
+    // of a request: columns of its last group's waves, and the places of a group of so many columns
+    auto columns = [&](const Span& sp) { return COLS == 2 && sp.n * g.group - (groups(sp) - 1) * ROWS > 64 ? 2 : 1; };
+    auto length = [&](const Span& sp, int cols) { return whole ? 1 : (sp.tile1 - sp.tile0) * (cols == 2 ? kTreeTile<2> : kTreeTile<1>) + kTreeBegin<COLS>; };
+    auto of_head = [&](const Span& sp) { return (groups(sp) - 1l) * length(sp, COLS) + length(sp, columns(sp)); };
+    auto load = [&](int r0) {
+        Span sp{};
+        if (r0 + lane < g.requests) sp = span_of<true>(g, r0 + lane);
+        const bool mine = sp.n > 0 && sp.n * g.group > f.most;
+        const long upto = wave_scan(mine ? of_head(sp) * g.c.heads : 0);
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            in.span[lane] = sp;
+            in.upto[lane] = upto;
+        }
+        __syncthreads();
+        return __shfl(upto, 63);
+    };
+    long all = 0;
+    for (int r0 = 0; r0 < g.requests; r0 += 64) all += load(r0);
+    const long each = one_of(max(whole ? 1l : kTreeTile<COLS>, (all + f.tree_shares - 1) / f.tree_shares)), end = one_of(min(all, share * each + each));
+    long pos = share * each, block = 0;  // block: places before the 64 requests
+    if (pos >= end) return;
+    int r = 0, r0 = 0;
+    if (g.requests > 64) load(0);
+    while (pos < end) {
+        for (;;) {
+            const long upto = block + one_of(in.upto[r]);
+            if (upto > pos) break;
+            if (++r < 64) continue;
+            block = upto;
+            r0 += 64;
+            r = 0;
+            load(r0);
+        }
+        const long before = block + (r ? one_of(in.upto[r - 1]) : 0);
+        const Span sp{one_of(in.span[r].start), one_of(in.span[r].n), one_of(in.span[r].len), one_of(in.span[r].tile0), one_of(in.span[r].tile1)};
+        const int count = sp.tile1 - sp.tile0, begin = whole ? 0 : kTreeBegin<COLS>, per = groups(sp), rows = sp.n * g.group;
+        const long head = of_head(sp);
+        const int kv = (int)((pos - before) / head);
+        const long in_head = pos - before - kv * head;
+        const int group = (int)min(in_head / length(sp, COLS), per - 1l), cols = group == per - 1 ? columns(sp) : COLS;
+        const int len = length(sp, cols), at0 = (int)(in_head - (long)group * length(sp, COLS)), at1 = (int)min(at0 + end - pos, (long)len);
+        // a tile is the share's that has its first place
+        const int each_tile = cols == 2 ? kTreeTile<2> : kTreeTile<1>;
+        auto tile_of = [&](int at) { return (max(0, at - begin) + each_tile - 1) / each_tile; };
+        const int into = whole ? 0 : tile_of(at0), n = whole ? count : tile_of(at1) - into;
+        const long first_place = pos - at0 + begin;
+        pos += at1 - at0;
+        if (n <= 0) continue;
+        const int parts = whole ? 1 : (int)((first_place + (long)each_tile * (count - 1)) / each) - share + 1;  // (of the first part's share)
+        const int first = sp.tile0 + into, last = g.c.pages ? first + n : first;
+        const long place = f.others + ((long)share * 2 + (into == 0)) * ROWS;
+        const auto done = [&](int row, int in_group, const Base& m, float l, const float4v (&o)[4 * DN]) {
+            const int i = row / g.group;
+            if (into == 0 && row < rows && (threadIdx.x & 48) == 0)
+                f.parts[(long)(sp.start + i) * g.q.heads + kv * g.group + row - i * g.group] = make_int2((int)(place + in_group), parts);
+            store_row<T, DN>(f, sp, kv, row, rows, n < count, place + in_group, m, l, o);
+        };
+        const Tiles w{r0 + r, kv, group * ROWS, first, last};
+        if (cols == 2)
+            many_tiles<T, DN, COLS, true>(f, sp, w, tiles, done);
+        else
+            many_tiles<T, DN, 1, true>(f, sp, w, tiles, done);
+    }
+}
+
+template <class T, int DN>
+__global__ __launch_bounds__(256, 2) void attn_tree_kernel(Work f) {
+    extern __shared__ __align__(16) half8v shared[];
+    __shared__ TreeSpans spans;
+    if ((int)blockIdx.x < f.tree_shares)
+        tree_rows<T, DN>(f, xcd_contiguous(blockIdx.x, f.tree_shares), shared, spans);
+    else
+        few_rows<T, DN, 1, true>(f, blockIdx.x - f.tree_shares, shared);
+}
+
+template <class T, int DN>
 __global__ __launch_bounds__(256, 2) void attn_many_kernel(Work f, int tiled) {
     extern __shared__ __align__(16) half8v shared[];
     if ((int)blockIdx.x < tiled)
-        many_rows<T, DN, TREE>(f, blockIdx.x, shared);
+        many_rows<T, DN>(f, blockIdx.x, shared);
     else
-        few_rows<T, DN, (DN <= 2 ? 2 : 1), TREE>(f, blockIdx.x - tiled, shared);
+        few_rows<T, DN, (DN <= 2 ? 2 : 1), false>(f, blockIdx.x - tiled, shared);
 }
 
 // Joins what several waves or workgroups hold of a row, in their order: W waves
@@ -964,8 +1135,9 @@ __global__ __launch_bounds__(512) void attn_join_kernel(Work f, int rows_of_grou
         if (ns <= 1 || ns > f.most_parts) continue;
         // the place of the first part, of the second, and on from there
         const long at0 = which == Join::MANY ? f.many_at(0, t, h) : of.x;
-        const long at = which == Join::MANY ? f.many_at(1, t, h) : at0 + rows_of_group;
-        const long step = which == Join::MANY ? at - at0 : 2l * rows_of_group;
+        const int next = of.x < f.others ? rows_of_group : f.tree_rows;  // (a tree's places follow the few kernel's)
+        const long at = which == Join::MANY ? f.many_at(1, t, h) : at0 + next;
+        const long step = which == Join::MANY ? at - at0 : 2l * next;
         float top = kNone, l = 0.0f;
         float4 sum = make_float4(0, 0, 0, 0);
         if (group < G) {
@@ -1036,6 +1208,61 @@ __global__ __launch_bounds__(512) void attn_join_kernel(Work f, int rows_of_grou
     }
 }
 
+// The same for a tree's rows, which are many and in few parts each: 16 DN lanes a
+// row and q head, 4 dims each, and up to eight parts at a time.
+template <class T, int DN>
+__global__ __launch_bounds__(256) void tree_join_kernel(Work f, int rows_of_group) {
+    constexpr int LANES = DN == 3 ? 64 : 16 * DN, LOADS = 8;
+    const AttnArgs& g = f.a;
+    const int piece = threadIdx.x % LANES;
+    const long row = ((long)blockIdx.x * 256 + threadIdx.x) / LANES;
+    if (row >= (long)g.tokens * g.q.heads || piece >= 16 * DN) return;
+    const int2 of = f.parts[row];
+    const int ns = of.y;
+    if (ns <= 1 || ns > f.most_parts) return;
+    const int next = of.x < f.others ? rows_of_group : f.tree_rows;  // (the other kernel's places follow the few kernel's)
+    float top = kNone, l = 0.0f;
+    float4 sum = make_float4(0, 0, 0, 0);
+    for (int s = 0; s < ns; s += LOADS) {
+        float2 st[LOADS];
+        float4 x[LOADS];
+#pragma unroll
+        for (int e = 0; e < LOADS; e++) {
+            const int k = s + e;
+            const long place = k ? (long)of.x + next + 2l * (k - 1) * next : of.x;
+            st[e] = make_float2(kNone, 0.0f);
+            x[e] = make_float4(0, 0, 0, 0);
+            if (k < ns && place >= 0 && place < f.places) {  // (a starts' array out of order may lead past them)
+                st[e] = f.stat[place];
+                x[e] = reinterpret_cast<const float4*>(f.part + place * g.c.dp)[piece];
+            }
+        }
+        float m = top;
+#pragma unroll
+        for (int e = 0; e < LOADS; e++) m = fmaxf(m, st[e].x);
+        const float base = m == kNone ? 0.0f : m, old = __builtin_amdgcn_exp2f(top - base);
+        top = m;
+        l *= old;
+        sum.x *= old;
+        sum.y *= old;
+        sum.z *= old;
+        sum.w *= old;
+#pragma unroll
+        for (int e = 0; e < LOADS; e++) {
+            const float w = __builtin_amdgcn_exp2f(st[e].x - base);
+            l += st[e].y * w;
+            sum.x += x[e].x * w;
+            sum.y += x[e].y * w;
+            sum.z += x[e].z * w;
+            sum.w += x[e].w * w;
+        }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int t = (int)(row / g.q.heads), h = (int)(row - (long)t * g.q.heads);
+    store4<T>((T*)g.out.p + (long)t * g.out.token + (long)h * g.out.head, 4 * piece, g.c.dim, f.vec,
+              {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv});
+}
+
 }  // namespace zt
 
 using namespace zt;
@@ -1053,19 +1280,22 @@ struct AttnPlan {
     int most, shares, qtiles, empties;
     int few_n, many_n;  // bounds of the tokens of one request
     bool single, wide;
+    int tree_rows, tree_shares;  // of trees: the rows of the other kernel's workgroups, and how many of these,
+    bool tree_whole;             // each of whole segments or an equal share
     Split many;
     long others;
     long part, stat, parts;  // bytes of the parts' sums, and of where they are
     long places;
 };
 
-static AttnPlan attn_plan(const zt_kv8_attn* a) {
+static AttnPlan attn_plan(const zt_kv8_attn* a, bool tree) {
     AttnPlan p{};
     const int group = a->q.heads / a->cache.kv_heads, dp = (a->cache.head_dim + 63) & ~63;
     const long requests = std::max(1, a->requests), heads = a->cache.kv_heads;
     const long most = (long)std::min(a->max_q, a->tokens) * group;
     // up to 64 rows by the few kernel: 32 requests of 3000 tokens, 64 rows 88 us, by the other 97; 128 rows 124 and 103
-    p.most = most <= 64 ? 0x7FFFFFFF : 64;
+    const long few = tree ? 16 : 64;
+    p.most = most <= few ? 0x7FFFFFFF : (int)few;
     // of more than 16 rows two columns of them share what is read of a tile (those requests, 32 rows: 66 us, one by one
     // 80); past 128 dims their sums would leave no registers
     p.ct = most > 16 && dp <= 128 ? 2 : 1;
@@ -1075,7 +1305,7 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
     // A tile each as far as the bounds go, up to a wave for each SIMD: fewer leave some without work, each more makes
     // parts to be joined (one sequence of 40011 tokens 25.4 us, with 512 29.7, with 2048 28.1; 64 of up to 8000 69, 95
     // and 73).
-    const long groups = (std::max(1l, std::min(most, 64l)) + 16 * p.ct - 1) / (16 * p.ct);
+    const long groups = (std::max(1l, std::min(most, few)) + 16 * p.ct - 1) / (16 * p.ct);
     p.single = tiles <= 2;
     p.shares = (int)std::min(1024l, requests * heads * groups * (p.single ? 1 : tiles + kBegin));
     // eight waves to join a row of more than 16 parts (one sequence of 40011 tokens, 128 parts: 25 us, with one 39), else
@@ -1085,10 +1315,20 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
     // 4), so one for 16 rows, up to about the card's 1024 in all (4096 padded rows 50 us, by one a head 1210).
     p.empties = (int)std::max(1l, std::min({(a->tokens + 15) / 16l, 64l, 1024 / heads}));
     p.others = 2l * p.shares * 16 * p.ct;
+    long all = p.others;
     p.many_n = std::max(1, std::min(a->max_q, a->tokens));
-    p.few_n = std::max(1, std::min(p.many_n, 64 / group));
+    p.few_n = std::max(1, std::min(p.many_n, (int)few / group));
     p.many = {1, 1};
-    if (most > 64) {
+    if (most > few && tree) {
+        p.tree_rows = dp == 64 || (dp == 128 && a->type == ZT_F16) ? 128 : 64;
+        const long segments = requests * heads * ceil_div(most, p.tree_rows);
+        p.tree_whole = tiles <= 4;
+        // all that the card holds at a time (24 trees of 64, 8 of 128: 512 293 us, with 384 368, 1024 307)
+        const long all_cus = dp <= 128 ? 512 : 256;
+        p.tree_shares = (int)(p.tree_whole ? std::min(1l << 20, segments) : std::min(all_cus, segments * std::max(1l, tiles / 4)));
+        p.wide = p.tree_shares > 16 * segments;
+        if (!p.tree_whole) all += 2l * p.tree_shares * p.tree_rows;
+    } else if (most > few) {
         p.qtiles = ceil_div(most, dp <= 128 ? 128 : 64);
         // Along the tokens where that is less time: a tile of 128 rows and dims is 2.2 us while the card's 512 workgroups
         // are not passed, the parts are written and read at 4.5 TB/s, a launch 4 us.  (32 heads over 8 of 128, fp16, one
@@ -1108,7 +1348,7 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
         p.many.tiles = (int)((tiles + splits - 1) / splits);
         p.many.splits = (int)((tiles + p.many.tiles - 1) / p.many.tiles);
     }
-    const long all = p.others + (p.many.splits > 1 ? (long)p.many.splits * a->tokens * a->q.heads : 0);
+    if (p.many.splits > 1) all += (long)p.many.splits * a->tokens * a->q.heads;
     p.stat = (all * 8 + 15) & ~15l;
     p.part = all * dp * 4;
     p.places = all;
@@ -1116,7 +1356,7 @@ static AttnPlan attn_plan(const zt_kv8_attn* a) {
     return p;
 }
 
-template <class T, int DN, bool TREE>
+template <class T, int DN>
 static int launch(const Work& f, const AttnPlan& p, hipStream_t stream) {
     const long tiled = (long)p.qtiles * p.many.splits * f.a.c.heads * f.a.requests;
     const int few = (f.shares + 3) / 4 + f.a.c.heads * f.empties;
@@ -1127,14 +1367,14 @@ static int launch(const Work& f, const AttnPlan& p, hipStream_t stream) {
         constexpr int lds = 2 * 16 * DN * 1024;
         static_assert(lds >= column * (DN <= 2 ? 2 : 1));
         if constexpr (lds > 65536) {
-            const hipError_t rc = raise_lds((const void*)attn_many_kernel<T, DN, TREE>, lds, raised);
+            const hipError_t rc = raise_lds((const void*)attn_many_kernel<T, DN>, lds, raised);
             if (rc != hipSuccess) return (int)rc;
         }
-        attn_many_kernel<T, DN, TREE><<<(unsigned)(tiled + few), 256, lds, stream>>>(f, (int)tiled);
+        attn_many_kernel<T, DN><<<(unsigned)(tiled + few), 256, lds, stream>>>(f, (int)tiled);
     } else if (p.ct == 2) {
-        if constexpr (DN <= 2) attn_few_kernel<T, DN, 2, TREE><<<few, 256, 2 * column, stream>>>(f);
+        if constexpr (DN <= 2) attn_few_kernel<T, DN, 2, false><<<few, 256, 2 * column, stream>>>(f);
     } else {
-        attn_few_kernel<T, DN, 1, TREE><<<few, 256, column, stream>>>(f);
+        attn_few_kernel<T, DN, 1, false><<<few, 256, column, stream>>>(f);
     }
     const auto join = [&](Join which, int each, bool wide) {
         each = (int)std::min((long)each, std::max(1l, ((1l << 31) - 1) / (std::max(1l, (long)f.a.requests) * f.a.q.heads)));
@@ -1149,9 +1389,40 @@ static int launch(const Work& f, const AttnPlan& p, hipStream_t stream) {
     return (int)hipGetLastError();
 }
 
+template <class T, int DN>
+static int launch_tree(const Work& f, const AttnPlan& p, hipStream_t stream) {
+    const long blocks = (long)p.tree_shares + (f.shares + 3) / 4 + f.a.c.heads * f.empties;
+    if (blocks >= 1l << 31) return kInvalid;
+    if (p.tree_shares) {
+        static std::atomic<uint64_t> raised{0};
+        constexpr int lds = 2 * 16 * DN * 1024;
+        if constexpr (lds > 48 << 10) {  // (beside the kernel's own)
+            const hipError_t rc = raise_lds((const void*)attn_tree_kernel<T, DN>, lds, raised);
+            if (rc != hipSuccess) return (int)rc;
+        }
+        attn_tree_kernel<T, DN><<<(unsigned)blocks, 256, lds, stream>>>(f);
+    } else {
+        attn_few_kernel<T, DN, 1, true><<<(unsigned)blocks, 256, DN * 2 * (sizeof(T) / 2) * 4096, stream>>>(f);
+    }
+    if (f.a.requests && (!p.single || (p.tree_shares && !p.tree_whole))) {
+        const long rows = (long)f.a.tokens * f.a.q.heads;
+        if (p.wide)
+            attn_join_kernel<T, DN, 8><<<(unsigned)rows, 512, 0, stream>>>(f, 16, 1, Join::ROWS);
+        else
+            tree_join_kernel<T, DN><<<(unsigned)((rows * (DN == 3 ? 64 : 16 * DN) + 255) / 256), 256, 0, stream>>>(f, 16);
+    }
+    return (int)hipGetLastError();
+}
+
 ZT_EXPORT long zt_kv8_attention_workspace_bytes(const zt_kv8_attn* a) {
     if (!attn_ok(a)) return -1;
-    const AttnPlan p = attn_plan(a);
+    const AttnPlan p = attn_plan(a, false);
+    return p.part + p.stat + p.parts;
+}
+
+ZT_EXPORT long zt_kv8_tree_attention_workspace_bytes(const zt_kv8_attn* a) {
+    if (!attn_ok(a)) return -1;
+    const AttnPlan p = attn_plan(a, true);
     return p.part + p.stat + p.parts;
 }
 
@@ -1164,21 +1435,28 @@ static int attention(const zt_kv8_attn* a, const uint64_t* mask, int words, void
         (a->requests && (!a->table || !a->kv_lens)) ||
         (((uintptr_t)a->table | (uintptr_t)a->kv_lens | (uintptr_t)a->q_start | (uintptr_t)a->scale) & 3))
         return kInvalid;
-    const AttnPlan p = attn_plan(a);
+    const AttnPlan p = attn_plan(a, TREE);
     if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.part + p.stat + p.parts) return kInvalid;
     const double unit = 1.44269504088896340736 / std::sqrt((double)a->cache.head_dim);
     const AttnArgs g{kv8_of(a->cache), rows_of(a->q), rows_of(a->out), a->table, a->kv_lens, a->q_start, a->scale,
                      a->requests,      a->width,      a->tokens,       a->window, a->q.heads / a->cache.kv_heads,
                      (float)unit,      (float)(unit - (double)(float)unit), mask, words};
-    const Work f{g,        p.most, p.shares, p.empties, p.single, p.many, p.qtiles, rows_vector(a->q, 4, a->type) && rows_vector(a->out, 4, a->type),
-                 p.others, p.places, std::max(p.shares, p.many.splits), (float*)workspace, (float2*)((char*)workspace + p.part),
+    const Work f{g,        p.most, p.shares, p.empties, p.single, p.many, p.qtiles, p.tree_shares, p.tree_rows, p.tree_whole, rows_vector(a->q, 4, a->type) && rows_vector(a->out, 4, a->type),
+                 p.others, p.places, std::max({p.shares, p.many.splits, p.tree_shares}), (float*)workspace, (float2*)((char*)workspace + p.part),
                  (int2*)((char*)workspace + p.part + p.stat)};
-    const bool f32 = a->type == ZT_F32;
+    const auto run = [&](auto type, auto dn) {
+        using T = decltype(type);
+        if constexpr (TREE)
+            return launch_tree<T, decltype(dn)::value>(f, p, stream);
+        else
+            return launch<T, decltype(dn)::value>(f, p, stream);
+    };
+    const auto of_type = [&](auto dn) { return a->type == ZT_F32 ? run(0.0f, dn) : run((_Float16)0.0f, dn); };
     switch (g.c.dp) {
-        case 64: return f32 ? launch<float, 1, TREE>(f, p, stream) : launch<_Float16, 1, TREE>(f, p, stream);
-        case 128: return f32 ? launch<float, 2, TREE>(f, p, stream) : launch<_Float16, 2, TREE>(f, p, stream);
-        case 192: return f32 ? launch<float, 3, TREE>(f, p, stream) : launch<_Float16, 3, TREE>(f, p, stream);
-        default: return f32 ? launch<float, 4, TREE>(f, p, stream) : launch<_Float16, 4, TREE>(f, p, stream);
+        case 64: return of_type(std::integral_constant<int, 1>{});
+        case 128: return of_type(std::integral_constant<int, 2>{});
+        case 192: return of_type(std::integral_constant<int, 3>{});
+        default: return of_type(std::integral_constant<int, 4>{});
     }
 }
 

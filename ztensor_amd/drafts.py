@@ -129,7 +129,7 @@ class DraftOps(DecodeOps):
                        dense(kv_lens, "kv_lens", i32, (r,)), dense(q_start, "q_start", i32, (r + 1,)),
                        dense(scale, "scale", torch.float32, (1,)), r, width, tokens, tokens if max_q is None else max_q,
                        min(width * c[7], 0x7FFFFFFF) if max_kv is None else max_kv, window, t, 0)
-        ws, wsb = self._workspace(self.lib.zt_kv8_attention_workspace_bytes(a))
+        ws, wsb = self._workspace(self.lib.zt_kv8_tree_attention_workspace_bytes(a))
         self.lib.call("zt_kv8_tree_attention", a, bits, mask.shape[1], ws, wsb, self._s)
         return out
 
