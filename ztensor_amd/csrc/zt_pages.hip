@@ -159,22 +159,42 @@ struct CompactArgs {
     int* kv_lens_out;  // NULL: another launch writes them
 };
 
-// Where the code of a place of a page comes from.
-struct Source {
-    int page, place;  // page -1: it stays
+// Where the codes of a page's places come from.
+struct Sources {
+    int page[128];  // -1: they stay
+    uint8_t place[128];
+    float scale[128];  // of that page
+    uint8_t rows[128];  // the places that are written, in their order
 };
 
-// One workgroup: a request's rows of one head of keys or of values, page after
-// page of those that they go to.  A row never comes from a page before the one
-// that it goes to, so what is still to be read has not been written; inside a
-// page all is read before anything is.
+// A code as this page takes it over: what it holds itself by the growth of its
+// scale, what comes from another page by its value.
+struct TakeOver {
+    float ratio, step;  // ratio 1: the scale stays
+    __device__ __forceinline__ int operator()(int code, bool far, float by) const {
+        return far ? code_of((float)code * by, step) : ratio != 1.0f ? (int)rintf((float)code * ratio) : code;
+    }
+};
+__device__ __forceinline__ int code_at(const u32x4& w, int k) { return (int8_t)(w[k >> 2] >> 8 * (k & 3)); }
+__device__ __forceinline__ void set_code(u32x4& w, int k, int code) {
+    w[k >> 2] = (w[k >> 2] & ~(0xFFu << 8 * (k & 3))) | ((uint32_t)code & 0xFFu) << 8 * (k & 3);
+}
+
+// One wave: a request's rows of one head of keys or of values, page after page of
+// those that they go to.  A row comes from behind the place that it goes to, and
+// places are written in their order, each by the lane that has read what goes
+// there (of values a lane has a dim of all places): nothing is written before it
+// has been read.
 //
 // On its own page a code stays what it is; from another page its value comes,
 // and the page's scale grows where that needs it, as the cache's writer has it.
-__global__ __launch_bounds__(kThreads) void compact_kernel(CompactArgs g, Layers layers) {
-    __shared__ Source from[128];
-    __shared__ float red[4];
+//
+// Loads that wait for each other bound it: starts and counts, the path, the pages,
+// their scales, the codes.
+__global__ __launch_bounds__(64) void compact_kernel(CompactArgs g, Layers layers) {
+    __shared__ Sources from;
     const Kv8& c = g.c;
+    const int lane = threadIdx.x;
     int b = blockIdx.x;
     const int values = b & 1, head = (b >> 1) % c.heads;
     b = (b >> 1) / c.heads;
@@ -182,99 +202,133 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(CompactArgs g, Layers
     const RowSpan s = rows_of_request(g.q_start, r, g.tokens);
     const long base = max(0, g.held[r]);
     const int kept = min(max(0, g.kept[r]), s.n);
-    if (g.kv_lens_out && layer == 0 && head == 0 && !values && threadIdx.x == 0)
-        g.kv_lens_out[r] = (int)min(base + kept, 0x7FFFFFFFl);
+    if (g.kv_lens_out && layer == 0 && head == 0 && !values && lane == 0) g.kv_lens_out[r] = (int)min(base + kept, 0x7FFFFFFFl);
     int8_t* codes = values ? layers.v[layer] : layers.k[layer];
     float* scales = values ? layers.v_scale[layer] : layers.k_scale[layer];
     const int* row = g.table + (long)r * g.width;
     const long end = min(base + kept, (long)g.width << c.shift);
-    const int mask = c.page - 1;
     for (long p = base >> c.shift; p << c.shift < end; p++) {
         const int page = row[p];
-        const long first = p << c.shift;  // the page's first position
-        bool any = false, far = false;
-        if ((int)threadIdx.x < c.page) {
-            const long at = first + threadIdx.x;
-            Source x{-1, 0};
-            if (at >= base && at < end) {
+        uint64_t moved[2] = {0, 0}, far[2] = {0, 0};
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const int place = 64 * half + lane;
+            const long at = (p << c.shift) + place;
+            int src_page = -1;
+            if (place < c.page && at >= base && at < end) {
                 const int j = (int)(at - base), k = g.path[s.start + j];
                 const long src = base + k;
                 if (k > j && k < s.n && src < (long)g.width << c.shift) {
-                    x = {row[src >> c.shift], (int)(src & mask)};
-                    if (!c.holds(x.page) || !c.holds(page)) x.page = -1;
+                    src_page = row[src >> c.shift];
+                    if (!c.holds(src_page) || !c.holds(page)) src_page = -1;
+                    from.place[place] = (uint8_t)(src & (c.page - 1));
+                    from.scale[place] = src_page < 0 ? 0.0f : scales[(long)src_page * c.heads + head];
                 }
             }
-            from[threadIdx.x] = x;
-            any = x.page >= 0;
-            far = any && x.page != page;
+            if (place < c.page) from.page[place] = src_page;
+            moved[half] = __ballot(src_page >= 0);
+            far[half] = __ballot(src_page >= 0 && src_page != page);
         }
-        if (!__syncthreads_or(any)) continue;
+        if (!(moved[0] | moved[1])) continue;
+        __syncthreads();
 
         const long at = (long)page * c.heads + head;
         const float had = scales[at];
         float now = had;
-        if (__syncthreads_or(far)) {
+        if (far[0] | far[1]) {
             float m = 0.0f;
             bool bad = false;
-            for (int i = threadIdx.x; i < c.page * c.dp; i += kThreads) {
-                const int place = i / c.dp, d = i - place * c.dp;
-                const Source x = from[place];
-                if (x.page < 0 || x.page == page) continue;
-                const int8_t* src = codes + c.at(x.page, head);
-                const float value = fabsf((float)src[values ? d * c.page + x.place : x.place * c.dp + d] * scales[(long)x.page * c.heads + head]);
+            auto look = [&](int code, float by) {
+                const float value = fabsf((float)code * by);
                 m = fmaxf(m, value);
                 bad |= !(value <= kMaxFloat);
+            };
+            uint64_t left[2] = {far[0], far[1]};
+            while (left[0] | left[1]) {
+                // four places at a time (the last ones again where there are fewer); of each 4 dims a lane
+                uint32_t w[4];
+                float by[4];
+                int z = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int half = left[0] ? 0 : 1;
+                    if (left[half]) {
+                        z = 64 * half + __builtin_ctzll(left[half]);
+                        left[half] &= left[half] - 1;
+                    }
+                    const int8_t* src = codes + c.at(from.page[z], head);
+                    const int in = from.place[z];
+                    by[e] = from.scale[z];
+                    w[e] = 0;
+                    if (!values) {
+                        if (4 * lane < c.dp) w[e] = *reinterpret_cast<const uint32_t*>(src + in * c.dp + 4 * lane);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            if (lane + 64 * k < c.dp) w[e] |= (uint32_t)(uint8_t)src[(lane + 64 * k) * c.page + in] << 8 * k;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) look((int8_t)(w[e] >> 8 * k), by[e]);
             }
-            block_peak(m, bad, red);
+            bad = __any(bad);
+            m = max_step<1>(max_step<2>(max_step<4>(max_step<8>(max_step<16>(max_step<32>(m))))));
             now = bad || had != had ? __builtin_nanf("") : fmaxf(had, m * (1.0f / 127.0f));
         }
         const bool grown = now > had;
-        const float ratio = grown ? had / now : 0.0f, step = now > 0.0f ? now : 1.0f;
-        // 16 codes at a time, of keys: a place's dims, of values: a dim's places
-        const int pieces = c.bytes() / 16, per = values ? c.page / 16 : c.dp / 16;
+        const TakeOver take{grown ? had / now : 1.0f, now > 0.0f ? now : 1.0f};
         u32x4* out = reinterpret_cast<u32x4*>(codes + c.at(page, head));
-        constexpr int kMost = 128 * 256 / 16 / kThreads;
-        u32x4 w[kMost];
-        bool write[kMost];
+        if (!values) {  // rows of dp codes, as many at a time as the lanes have
+            int count = 0;
 #pragma unroll
-        for (int e = 0; e < kMost; e++) {
-            const int i = threadIdx.x + e * kThreads;
-            write[e] = false;
-            if (i >= pieces) continue;
-            const int line = i / per, in = (i - line * per) * 16;
-            u32x4 old = out[i];
-            if (values) {
-                bool moved = false;
-#pragma unroll
-                for (int k = 0; k < 16; k++) moved |= from[in + k].page >= 0;
-                write[e] = moved || grown;
-            } else {
-                write[e] = from[line].page >= 0 || grown;
+            for (int half = 0; half < 2; half++) {
+                const uint64_t some = grown ? c.page - 64 * half >= 64 ? ~0ull : c.page <= 64 * half ? 0 : (1ull << (c.page - 64 * half)) - 1
+                                            : moved[half];
+                if (some >> lane & 1) from.rows[count + __builtin_popcountll(some & ((1ull << lane) - 1))] = (uint8_t)(64 * half + lane);
+                count += __builtin_popcountll(some);
             }
-            if (!write[e]) continue;
+            __syncthreads();
+            const int per = c.dp / 16, rows = 64 / per, mine = lane / per, piece = lane - mine * per;
+            for (int i = mine; i < count; i += rows) {
+                if (mine >= rows) break;  // (of 192 dims 60 lanes)
+                const int z = from.rows[i], src_page = from.page[z];
+                const bool other = src_page >= 0 && src_page != page;
+                u32x4 w = *(reinterpret_cast<const u32x4*>(codes + c.at(src_page < 0 ? page : src_page, head)) + (src_page < 0 ? z : from.place[z]) * per + piece);
+                if (other || grown) {
+                    const float by = other ? from.scale[z] : 0.0f;
 #pragma unroll
-            for (int k = 0; k < 16; k++) {
-                const Source x = values ? from[in + k] : from[line];
-                const int d = values ? line : in + k;
-                int code = (int8_t)(old[k >> 2] >> 8 * (k & 3));
-                float by = 0.0f;  // another page's scale
-                if (x.page >= 0) {
-                    code = codes[c.at(x.page, head) + (values ? d * c.page + x.place : x.place * c.dp + d)];
-                    if (x.page != page) by = scales[(long)x.page * c.heads + head];
+                    for (int k = 0; k < 16; k++) set_code(w, k, take(code_at(w, k), other, by));
                 }
-                if (x.page >= 0 && x.page != page)
-                    code = code_of((float)code * by, step);
-                else if (grown)
-                    code = (int)rintf((float)code * ratio);
-                old[k >> 2] = (old[k >> 2] & ~(0xFFu << 8 * (k & 3))) | ((uint32_t)code & 0xFFu) << 8 * (k & 3);
+                out[z * per + piece] = w;
             }
-            w[e] = old;
-        }
-        __syncthreads();
+        } else {  // 16 places of a dim
+            const int per = c.page / 16;
+            for (int chunk = 0; chunk < per; chunk++) {
+                const uint32_t some = (uint32_t)(moved[chunk >> 2] >> 16 * (chunk & 3)) & 0xFFFFu;
+                if (!some && !grown) continue;
+                for (int d = lane; d < c.dp; d += 64) {
+                    u32x4 w = out[d * per + chunk];
+                    int8_t in[16];
 #pragma unroll
-        for (int e = 0; e < kMost; e++)
-            if (write[e]) out[threadIdx.x + e * kThreads] = w[e];
-        if (threadIdx.x == 0 && !(now == had)) scales[at] = now;
+                    for (int k = 0; k < 16; k++) {
+                        const int z = 16 * chunk + k;
+                        in[k] = some >> k & 1 ? codes[c.at(from.page[z], head) + d * c.page + from.place[z]] : 0;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        const int z = 16 * chunk + k;
+                        if (some >> k & 1)
+                            set_code(w, k, take(in[k], from.page[z] != page, from.scale[z]));
+                        else if (grown)
+                            set_code(w, k, take(code_at(w, k), false, 0.0f));
+                    }
+                    out[d * per + chunk] = w;
+                }
+            }
+        }
+        if (lane == 0 && !(now == had)) scales[at] = now;
         __syncthreads();  // `from` is free again
     }
 }
@@ -563,7 +617,7 @@ ZT_EXPORT int zt_kv8_compact(const zt_kv8_cache* caches, int layers, const int* 
     if (blocks * std::min(layers, kLayers) >= 1l << 31) return kInvalid;
     return for_layers(caches, layers, [&](const Layers& l, int n, bool first) {
         const CompactArgs g{kv8_of(*caches), table, held, q_start, path, kept, requests, width, tokens, first ? kv_lens_out : nullptr};
-        compact_kernel<<<(unsigned)(blocks * n), kThreads, 0, stream>>>(g, l);
+        compact_kernel<<<(unsigned)(blocks * n), 64, 0, stream>>>(g, l);
     });
 }
 
