@@ -111,11 +111,19 @@ __host__ __device__ __forceinline__ int units_of(int dim, int half) {
 // Whether units of 2 V values divide a head of this size.
 __host__ inline bool units_fit(int V, int dim, int half) { return half % V == 0 && (dim - 2 * half) % (2 * V) == 0; }
 
+// How a head's pairs lie: as the flags of a call say, or known to the compiler
+// (HALVES, INTERLEAVED: and they are turned forwards).
+enum class Pairs { FLAGS, HALVES, INTERLEAVED };
+template <Pairs P>
+__device__ __forceinline__ bool interleaved(const Turn& r) {
+    return P == Pairs::FLAGS ? r.flags & ZT_ROPE_INTERLEAVED : P == Pairs::INTERLEAVED;
+}
+
 // Unit u of one head as it lies in memory: first and second, where its two
 // sets of V neighbours begin.
-template <class T, int V>
+template <class T, int V, Pairs P = Pairs::FLAGS>
 __device__ __forceinline__ void load_unit(const T* x, int u, const Turn& r, float (&a)[V], float (&b)[V], int& first, int& second) {
-    if (u < r.half / V && !(r.flags & ZT_ROPE_INTERLEAVED)) {
+    if (u < r.half / V && !interleaved<P>(r)) {
         first = u * V;
         second = first + r.half;
     } else {
@@ -126,12 +134,29 @@ __device__ __forceinline__ void load_unit(const T* x, int u, const Turn& r, floa
     load_values<T, V>(x + second, b);
 }
 
-// The same, its pairs (a[i], b[i]) turned by position pos: each product and sum
-// is rounded by itself, a plain program's values to the bit.
+// Unit u's cosines and sines of position pos (of one that is not turned: nothing).
 template <int V>
-__device__ __forceinline__ void turn_unit(int u, int pos, const Turn& r, float (&a)[V], float (&b)[V]) {
+__device__ __forceinline__ void load_angles(int u, int pos, const Turn& r, float (&c)[V], float (&s)[V]) {
+    if (u >= r.half / V) return;
+    if ((unsigned)pos < (unsigned)r.max_pos) {
+        const float* row = r.table + (long)pos * 2 * r.half + u * V;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            c[i] = row[i];
+            s[i] = row[r.half + i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) c[i] = s[i] = __builtin_nanf("");
+    }
+}
+
+// Its pairs (a[i], b[i]) turned by them: each product and sum is rounded by
+// itself, a plain program's values to the bit.
+template <int V, Pairs P = Pairs::FLAGS>
+__device__ __forceinline__ void turn_by(int u, const Turn& r, const float (&c)[V], const float (&s)[V], float (&a)[V], float (&b)[V]) {
 #pragma clang fp contract(off)
-    const bool pairs = u < r.half / V, inter = pairs && (r.flags & ZT_ROPE_INTERLEAVED);
+    const bool pairs = u < r.half / V, inter = pairs && interleaved<P>(r);
     if (!pairs) return;
     if (inter) {
         float e[V], o[V];
@@ -147,21 +172,9 @@ __device__ __forceinline__ void turn_unit(int u, int pos, const Turn& r, float (
             b[i] = o[i];
         }
     }
-    float c[V], s[V];
-    if ((unsigned)pos < (unsigned)r.max_pos) {
-        const float* row = r.table + (long)pos * 2 * r.half + u * V;
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            c[i] = row[i];
-            s[i] = row[r.half + i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; i++) c[i] = s[i] = __builtin_nanf("");
-    }
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        const float si = (r.flags & ZT_ROPE_INVERSE) ? -s[i] : s[i];
+        const float si = P == Pairs::FLAGS && (r.flags & ZT_ROPE_INVERSE) ? -s[i] : s[i];
         const float ac = a[i] * c[i], bs = b[i] * si, bc = b[i] * c[i], as = a[i] * si;
         a[i] = ac - bs;
         b[i] = bc + as;
@@ -181,6 +194,13 @@ __device__ __forceinline__ void turn_unit(int u, int pos, const Turn& r, float (
     }
 }
 
+template <int V, Pairs P = Pairs::FLAGS>
+__device__ __forceinline__ void turn_unit(int u, int pos, const Turn& r, float (&a)[V], float (&b)[V]) {
+    float c[V], s[V];
+    load_angles<V>(u, pos, r, c, s);
+    turn_by<V, P>(u, r, c, s, a, b);
+}
+
 template <class T, int V>
 __device__ __forceinline__ void turned(const T* x, int u, int pos, const Turn& r, float (&a)[V], float (&b)[V], int& first,
                                        int& second) {
@@ -194,36 +214,76 @@ __device__ __forceinline__ void turned(const T* x, int u, int pos, const Turn& r
 // with another last bit is another code.  w NULL: ones.
 struct HeadNorm {
     const float* w;
-    double eps;
+    double eps, share;  // share: 1 / the head's size
 };
 
-// r of the head at x, in each of the L lanes that share it (neighbours, a power
-// of two of them); lane l has units l and, N == 2, l + L, as load_unit gives
-// them: a and b, first and second.
-template <class T, int V, int N>
-__device__ __forceinline__ float load_head(const T* x, int l, int L, int units, int dim, const Turn& turn, double eps,
-                                           float (&a)[N][V], float (&b)[N][V], int (&first)[N], int (&second)[N]) {
+// v + v(partner), in lanes that differ in bit OFF where those that differ in lower bits have the same v.
+template <int OFF>
+__device__ __forceinline__ double sum_step(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const int lo = (int)(uint32_t)u, hi = (int)(uint32_t)(u >> 32);
+    int other_lo, other_hi;
+    if constexpr (OFF >= 16) {
+        other_lo = __shfl_xor(lo, OFF);
+        other_hi = __shfl_xor(hi, OFF);
+    } else {  // in a row of 16: l ^ 1, l ^ 2, 7 - l, 15 - l
+        constexpr int ctrl = OFF == 8 ? 0x140 : OFF == 4 ? 0x141 : OFF == 2 ? 0x4E : 0xB1;
+        other_lo = __builtin_amdgcn_update_dpp(0, lo, ctrl, 0xF, 0xF, false);
+        other_hi = __builtin_amdgcn_update_dpp(0, hi, ctrl, 0xF, 0xF, false);
+    }
+    return v + __builtin_bit_cast(double, (uint64_t)(uint32_t)other_hi << 32 | (uint32_t)other_lo);
+}
+
+// 1 / sqrt(x) of x > 0 by two steps of Newton's from the instruction's 23 bits or more: to the last bits of a double.
+__device__ __forceinline__ double inverse_root(double x) {
+    double y = __builtin_amdgcn_rsq(x);
+    if (y == 0.0) return 0.0;  // of infinity
+    y *= __builtin_fma(-0.5 * x * y, y, 1.5);
+    return y * __builtin_fma(-0.5 * x * y, y, 1.5);
+}
+
+// The head at x in L lanes that share it (neighbours, a power of two of them):
+// lane l has units l and, N == 2, l + L, as load_unit gives them; past the last
+// unit another one.
+template <class T, int V, int N, Pairs P>
+__device__ __forceinline__ void load_head(const T* x, int l, int L, int units, const Turn& turn, float (&a)[N][V], float (&b)[N][V],
+                                          int (&first)[N], int (&second)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; k++) load_unit<T, V, P>(x, l + k * L < units ? l + k * L : 0, turn, a[k], b[k], first[k], second[k]);
+}
+
+// Its r, in each of the lanes.
+template <int V, int N>
+__device__ __forceinline__ float head_factor(int l, int L, int units, const HeadNorm& norm, const float (&a)[N][V], const float (&b)[N][V]) {
     double sum = 0;
 #pragma unroll
     for (int k = 0; k < N; k++) {
-        const int u = l + k * L;
-        if (u < units) {
-            load_unit<T, V>(x, u, turn, a[k], b[k], first[k], second[k]);
+        double some[2] = {0, 0};  // (a product of two fp32 values is exact)
 #pragma unroll
-            for (int i = 0; i < V; i++) sum += (double)a[k][i] * a[k][i] + (double)b[k][i] * b[k][i];
+        for (int i = 0; i < V; i++) {
+            some[0] = __builtin_fma((double)a[k][i], (double)a[k][i], some[0]);
+            some[1] = __builtin_fma((double)b[k][i], (double)b[k][i], some[1]);
         }
+        sum += l + k * L < units ? some[0] + some[1] : 0.0;
     }
-    for (int o = L / 2; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
-    return (float)(1.0 / sqrt(sum / dim + eps));
+    if (L > 1) sum = sum_step<1>(sum);
+    if (L > 2) sum = sum_step<2>(sum);
+    if (L > 4) sum = sum_step<4>(sum);
+    if (L > 8) sum = sum_step<8>(sum);
+    if (L > 16) sum = sum_step<16>(sum);
+    if (L > 32) sum = sum_step<32>(sum);
+    return (float)inverse_root(__builtin_fma(sum, norm.share, norm.eps));
 }
 
 template <int V>
-__device__ __forceinline__ void scale_unit(const HeadNorm& n, float r, int at, float (&a)[V]) {
+__device__ __forceinline__ void load_weights(const HeadNorm& n, int at, float (&w)[V]) {
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        a[i] *= r;
-        if (n.w) a[i] *= n.w[at + i];
-    }
+    for (int i = 0; i < V; i++) w[i] = n.w ? n.w[at + i] : 1.0f;
+}
+template <int V>
+__device__ __forceinline__ void scale_unit(float r, const float (&w)[V], float (&a)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) a[i] = a[i] * r * w[i];
 }
 
 // Lanes that share a head of so many units, and units of one of them.

@@ -82,49 +82,63 @@ __host__ inline int rope_width(const zt_rows* const* r, int n, int dim, int half
 // -------------------------------------------------------- rotary, normed heads
 
 struct NormArgs {
-    RopeArgs r;
-    const float* w[2];
-    double eps;
+    RopeArgs r;  // (its `all`: chunks of heads of one token)
+    HeadNorm norm[2];
     int lanes;  // of one head: a power of two
 };
 
-// A head for g.lanes lanes.
-template <class T, int V>
+// g.lanes lanes have kHeads heads of one token, whose weights and angles are the
+// same: those are read once, and the heads' loads wait together.  Bytes bound it.
+constexpr int kHeads = 4;
+template <class T, int V, Pairs P>
 __device__ __forceinline__ void norm_block(const NormArgs& g, int block) {
     constexpr int N = kHeadUnits<V>;
-    const int l = threadIdx.x & (g.lanes - 1), heads = g.r.all;
-    const long item = ((long)block * kThreads + threadIdx.x) / g.lanes, t = item / heads;
+    const int l = threadIdx.x & (g.lanes - 1);
+    const long item = ((long)block * kThreads + threadIdx.x) / g.lanes, t = item / g.r.all;
     if (t >= g.r.tokens) return;
-    int h = (int)(item - t * heads);
-    const int second_in = h >= g.r.in[0].heads;
-    h -= second_in ? g.r.in[0].heads : 0;
-    const Rows &x = g.r.in[second_in], &y = g.r.out[second_in];
-    const HeadNorm norm{g.w[second_in], g.eps};
-    float a[N][V], b[N][V];
+    int chunk = (int)(item - t * g.r.all);
+    const int chunks = (g.r.in[0].heads + kHeads - 1) / kHeads, which = chunk >= chunks;
+    chunk -= which ? chunks : 0;
+    const Rows &x = g.r.in[which], &y = g.r.out[which];
+    const HeadNorm& norm = g.norm[which];
+    const int h0 = chunk * kHeads, n = min(kHeads, x.heads - h0);
+    float a[kHeads][N][V], b[kHeads][N][V], w[N][2][V], cs[N][2][V];
     int first[N], second[N];
     const int pos = g.r.turn.half ? g.r.turn.positions[t] : 0;
-    const float r = load_head<T, V, N>((const T*)x.p + t * x.token + h * x.head, l, g.lanes, g.r.units, g.r.dim, g.r.turn, g.eps, a, b, first, second);
-    T* o = (T*)y.p + t * y.token + h * y.head;
+#pragma unroll
+    for (int h = 0; h < kHeads; h++)  // (past the last head: that one again)
+        load_head<T, V, N, P>((const T*)x.p + t * x.token + (h0 + min(h, n - 1)) * x.head, l, g.lanes, g.r.units, g.r.turn, a[h], b[h], first, second);
 #pragma unroll
     for (int k = 0; k < N; k++) {
-        if (l + k * g.lanes >= g.r.units) continue;
-        scale_unit<V>(norm, r, first[k], a[k]);
-        scale_unit<V>(norm, r, second[k], b[k]);
-        turn_unit<V>(l + k * g.lanes, pos, g.r.turn, a[k], b[k]);
-        store_values<T, V>(o + first[k], a[k]);
-        store_values<T, V>(o + second[k], b[k]);
+        load_weights<V>(norm, first[k], w[k][0]);
+        load_weights<V>(norm, second[k], w[k][1]);
+        load_angles<V>(l + k * g.lanes, pos, g.r.turn, cs[k][0], cs[k][1]);
+    }
+#pragma unroll
+    for (int h = 0; h < kHeads; h++) {
+        const float r = head_factor<V, N>(l, g.lanes, g.r.units, norm, a[h], b[h]);
+        T* o = (T*)y.p + t * y.token + (h0 + h) * y.head;
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            if (h >= n || l + k * g.lanes >= g.r.units) continue;
+            scale_unit<V>(r, w[k][0], a[h][k]);
+            scale_unit<V>(r, w[k][1], b[h][k]);
+            turn_by<V, P>(l + k * g.lanes, g.r.turn, cs[k][0], cs[k][1], a[h][k], b[h][k]);
+            store_values<T, V>(o + first[k], a[h][k]);
+            store_values<T, V>(o + second[k], b[h][k]);
+        }
     }
 }
 
-template <class T, int V>
+template <class T, int V, Pairs P>
 __global__ __launch_bounds__(kThreads) void norm_kernel(NormArgs g) {
-    norm_block<T, V>(g, blockIdx.x);
+    norm_block<T, V, P>(g, blockIdx.x);
 }
 
 // The launch of n operands whose heads are normed.
 __host__ inline long norm_blocks(NormArgs& g, int n, int V) {
     g.r.units = g.r.turn.half / V + (g.r.dim - 2 * g.r.turn.half) / (2 * V);
-    g.r.all = g.r.in[0].heads + (n > 1 ? g.r.in[1].heads : 0);
+    g.r.all = ceil_div(g.r.in[0].heads, kHeads) + (n > 1 ? ceil_div(g.r.in[1].heads, kHeads) : 0);
     g.lanes = head_lanes(g.r.units);
     return ((long)g.r.tokens * g.r.all * g.lanes + kThreads - 1) / kThreads;
 }
@@ -162,17 +176,20 @@ ZT_EXPORT int zt_norm_rope(const zt_rows* in, const zt_rows* out, int n, const z
     g.r.turn = {positions, table, table ? rot_dim / 2 : 0, max_pos, flags};
     g.r.tokens = tokens;
     g.r.dim = head_dim;
-    g.w[0] = norm->q;
-    g.w[1] = norm->k;
-    g.eps = norm->eps;
+    g.norm[0] = {norm->q, norm->eps, 1.0 / head_dim};
+    g.norm[1] = {norm->k, norm->eps, 1.0 / head_dim};
     const int v = rope_width(all, 2 * n, head_dim, g.r.turn.half, type);
     const long blocks = norm_blocks(g, n, v);
     if (blocks >= 1l << 31) return kInvalid;
     auto run = [&](auto kernel) { kernel<<<blocks, kThreads, 0, stream>>>(g); };
-    if (type == ZT_F32)
-        v == 4 ? run(norm_kernel<float, 4>) : run(norm_kernel<float, 1>);
-    else
-        v == 8 ? run(norm_kernel<_Float16, 8>) : v == 4 ? run(norm_kernel<_Float16, 4>) : run(norm_kernel<_Float16, 1>);
+    auto with = [&](auto pairs) {
+        constexpr Pairs P = decltype(pairs)::value;
+        if (type == ZT_F32)
+            v == 4 ? run(norm_kernel<float, 4, P>) : run(norm_kernel<float, 1, P>);
+        else
+            v == 8 ? run(norm_kernel<_Float16, 8, P>) : v == 4 ? run(norm_kernel<_Float16, 4, P>) : run(norm_kernel<_Float16, 1, P>);
+    };
+    flags & ZT_ROPE_INTERLEAVED ? with(std::integral_constant<Pairs, Pairs::INTERLEAVED>{}) : with(std::integral_constant<Pairs, Pairs::HALVES>{});
     return (int)hipGetLastError();
 }
 
@@ -247,7 +264,7 @@ struct Run {
 
 // A run's tokens into their page: its new scale, and its codes by way of an image
 // of it in LDS.
-template <class T, int V, bool VALUES, bool NORM>
+template <class T, int V, bool VALUES, bool NORM, Pairs P>
 __device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run, int head, uint32_t* image, float* red, float* factors) {
     const Kv8& c = g.c;
     const Rows& x = g.x[VALUES];
@@ -258,36 +275,54 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run,
     const T* rows = (const T*)x.p + (long)head * x.head;
     float a[V], b[V];
     int first, second;
-    if constexpr (NORM) {
-        const int l = threadIdx.x & (g.lanes - 1);
-        for (int i = threadIdx.x / g.lanes; i < n; i += kThreads / g.lanes) {
-            constexpr int N = kHeadUnits<V>;
-            float a[N][V], b[N][V];
-            int first[N], second[N];
-            const float r = load_head<T, V, N>(rows + (long)run.token(i) * x.token, l, g.lanes, units, c.dim, turn, g.norm.eps, a, b, first, second);
-            if (l == 0) factors[i] = r;
-        }
-        __syncthreads();
-    }
-    auto unit = [&](int tl, int u, int t) {
-        const int pos = turn.half ? turn.positions[t] : 0;
-        load_unit<T, V>(rows + (long)t * x.token, u, turn, a, b, first, second);
-        if constexpr (NORM) {
-            scale_unit<V>(g.norm, factors[tl], first, a);
-            scale_unit<V>(g.norm, factors[tl], second, b);
-        }
-        turn_unit<V>(u, pos, turn, a, b);
-    };
-
     float m = 0.0f;
     bool bad = false;
-    for (int i = threadIdx.x; i < n * units; i += kThreads) {
-        const int tl = i / units, u = i - tl * units, t = run.token(tl);
-        unit(tl, u, t);
+    auto look = [&](const float (&a)[V], const float (&b)[V]) {
 #pragma unroll
         for (int j = 0; j < V; j++) {
             m = fmaxf(m, fmaxf(fabsf(a[j]), fabsf(b[j])));
             bad |= !(fabsf(a[j]) <= kMaxFloat) || !(fabsf(b[j]) <= kMaxFloat);
+        }
+    };
+    auto unit = [&](int tl, int u, int t) {
+        const int pos = turn.half ? turn.positions[t] : 0;
+        load_unit<T, V, P>(rows + (long)t * x.token, u, turn, a, b, first, second);
+        if constexpr (NORM) {
+            float w[2][V];
+            load_weights<V>(g.norm, first, w[0]);
+            load_weights<V>(g.norm, second, w[1]);
+            scale_unit<V>(factors[tl], w[0], a);
+            scale_unit<V>(factors[tl], w[1], b);
+        }
+        turn_unit<V, P>(u, pos, turn, a, b);
+    };
+    if constexpr (NORM) {
+        constexpr int N = kHeadUnits<V>;
+        const int l = threadIdx.x & (g.lanes - 1);
+        for (int i = threadIdx.x / g.lanes; i < n; i += kThreads / g.lanes) {
+            float a[N][V], b[N][V];
+            int first[N], second[N];
+            const int t = run.token(i), pos = turn.half ? turn.positions[t] : 0;
+            load_head<T, V, N, P>(rows + (long)t * x.token, l, g.lanes, units, turn, a, b, first, second);
+            const float r = head_factor<V, N>(l, g.lanes, units, g.norm, a, b);
+            if (l == 0) factors[i] = r;
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                if (l + k * g.lanes >= units) continue;
+                float w[2][V];
+                load_weights<V>(g.norm, first[k], w[0]);
+                load_weights<V>(g.norm, second[k], w[1]);
+                scale_unit<V>(r, w[0], a[k]);
+                scale_unit<V>(r, w[1], b[k]);
+                turn_unit<V, P>(l + k * g.lanes, pos, turn, a[k], b[k]);
+                look(a[k], b[k]);
+            }
+        }
+    } else {
+        for (int i = threadIdx.x; i < n * units; i += kThreads) {
+            const int tl = i / units, u = i - tl * units;
+            unit(tl, u, run.token(tl));
+            look(a, b);
         }
     }
     block_peak(m, bad, red);
@@ -443,9 +478,9 @@ __device__ __forceinline__ Run run_from(const AppendArgs& g, int t, long s, Foun
 // Prompts of 1955 tokens in all (fp16, 64 + 8 heads, pages of 16): 76 MB, 64 of
 // them q, in 22.6 us, 3.4 TB/s.
 //
-// Normed keys: a head's factor once for all, in LDS, from one more reading of the
-// rows.
-template <class T, int V, int VQ, class Q>
+// Normed keys: a row is dealt out to lanes that share its sum of squares, and its
+// factor kept in LDS for the second reading.
+template <class T, int V, int VQ, class Q, Pairs P>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, Q q) {
     constexpr bool NORM = std::is_same_v<Q, NormArgs>;
     extern __shared__ __align__(16) uint32_t image[];  // of one page and head
@@ -456,7 +491,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, Q q) {
     __shared__ uint8_t places[128];
     if (blockIdx.x >= g.blocks) {
         if constexpr (NORM)
-            norm_block<T, VQ>(q, blockIdx.x - g.blocks);
+            norm_block<T, VQ, P>(q, blockIdx.x - g.blocks);
         else
             rope_block<T, VQ>(q, blockIdx.x - g.blocks);
         return;
@@ -488,28 +523,28 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, Q q) {
         const int i = __builtin_ctzll(begin);
         const Run run = run_from(g, from + i, __shfl(here, i), found, listed, places);
         if (values)
-            append_page<T, V, true, false>(g, run, head, image, red, factors);
+            append_page<T, V, true, false, P>(g, run, head, image, red, factors);
         else
-            append_page<T, V, false, NORM>(g, run, head, image, red, factors);
+            append_page<T, V, false, NORM, P>(g, run, head, image, red, factors);
     }
 }
 
 }  // namespace zt
 
-template <class Q>
+template <Pairs P, class Q>
 static int launch_append(const AppendArgs& g, const Q& q, long blocks, int type, int width, int q_width, hipStream_t stream) {
     if (blocks >= 1l << 31) return kInvalid;
     const int lds = g.c.bytes();
     auto run = [&](auto kernel) { kernel<<<blocks, kThreads, lds, stream>>>(g, q); };
     if (type == ZT_F32) {
         if (width == 4)
-            q_width == 4 ? run(append_kernel<float, 4, 4, Q>) : run(append_kernel<float, 4, 1, Q>);
+            q_width == 4 ? run(append_kernel<float, 4, 4, Q, P>) : run(append_kernel<float, 4, 1, Q, P>);
         else
-            q_width == 4 ? run(append_kernel<float, 1, 4, Q>) : run(append_kernel<float, 1, 1, Q>);
+            q_width == 4 ? run(append_kernel<float, 1, 4, Q, P>) : run(append_kernel<float, 1, 1, Q, P>);
     } else if (width == 4) {
-        q_width == 8 ? run(append_kernel<_Float16, 4, 8, Q>) : q_width == 4 ? run(append_kernel<_Float16, 4, 4, Q>) : run(append_kernel<_Float16, 4, 1, Q>);
+        q_width == 8 ? run(append_kernel<_Float16, 4, 8, Q, P>) : q_width == 4 ? run(append_kernel<_Float16, 4, 4, Q, P>) : run(append_kernel<_Float16, 4, 1, Q, P>);
     } else {
-        q_width == 8 ? run(append_kernel<_Float16, 1, 8, Q>) : q_width == 4 ? run(append_kernel<_Float16, 1, 4, Q>) : run(append_kernel<_Float16, 1, 1, Q>);
+        q_width == 8 ? run(append_kernel<_Float16, 1, 8, Q, P>) : q_width == 4 ? run(append_kernel<_Float16, 1, 4, Q, P>) : run(append_kernel<_Float16, 1, 1, Q, P>);
     }
     return (int)hipGetLastError();
 }
@@ -557,13 +592,14 @@ static int append(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v,
     }
     if (!norm) {
         const long more = q ? rope_blocks(r, 1, q_width) : 0;
-        return launch_append(g, r, g.blocks + more, type, width, q_width, stream);
+        return launch_append<Pairs::FLAGS>(g, r, g.blocks + more, type, width, q_width, stream);
     }
-    g.norm = {norm->k, norm->eps};
+    g.norm = {norm->k, norm->eps, 1.0 / dim};
     g.lanes = head_lanes(half / width + (dim - 2 * half) / (2 * width));
-    NormArgs m{r, {norm->q, nullptr}, norm->eps, 1};
+    NormArgs m{r, {{norm->q, norm->eps, 1.0 / dim}, {}}, 1};
     const long more = q ? norm_blocks(m, 1, q_width) : 0;
-    return launch_append(g, m, g.blocks + more, type, width, q_width, stream);
+    if (flags & ZT_ROPE_INTERLEAVED) return launch_append<Pairs::INTERLEAVED>(g, m, g.blocks + more, type, width, q_width, stream);
+    return launch_append<Pairs::HALVES>(g, m, g.blocks + more, type, width, q_width, stream);
 }
 
 ZT_EXPORT int zt_kv8_append(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v, const long* slots,
