@@ -138,16 +138,13 @@ __device__ __forceinline__ void load_unit(const T* x, int u, const Turn& r, floa
 template <int V>
 __device__ __forceinline__ void load_angles(int u, int pos, const Turn& r, float (&c)[V], float (&s)[V]) {
     if (u >= r.half / V) return;
-    if ((unsigned)pos < (unsigned)r.max_pos) {
-        const float* row = r.table + (long)pos * 2 * r.half + u * V;
+    const bool in = (unsigned)pos < (unsigned)r.max_pos;
+    const float* row = r.table + (in ? (long)pos * 2 * r.half + u * V : 0);
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            c[i] = row[i];
-            s[i] = row[r.half + i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; i++) c[i] = s[i] = __builtin_nanf("");
+    for (int i = 0; i < V; i++) {
+        const float ci = row[i], si = row[r.half + i];  // loaded in any case, so that neighbours' loads are one
+        c[i] = in ? ci : __builtin_nanf("");
+        s[i] = in ? si : __builtin_nanf("");
     }
 }
 

@@ -246,7 +246,8 @@ struct AppendArgs {
     HeadNorm norm;  // of the keys, where the kernel norms them
     int lanes;      // that share a key for that
     int tokens;
-    int turns;  // workgroups that the pages which 64 tokens begin are dealt out to, for one head of keys or of values
+    int windows;  // of 64 tokens
+    int turns;    // workgroups that the pages which 64 tokens begin are dealt out to, for one head of keys or of values
     long blocks;
 };
 
@@ -273,18 +274,16 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run,
     const int units = units_of<V>(c.dim, turn.half);
     const int n = run.n;
     const T* rows = (const T*)x.p + (long)head * x.head;
-    float a[V], b[V];
-    int first, second;
     float m = 0.0f;
     bool bad = false;
-    auto look = [&](const float (&a)[V], const float (&b)[V]) {
+    auto look = [&](const float (&a)[V], const float (&b)[V]) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < V; j++) {
             m = fmaxf(m, fmaxf(fabsf(a[j]), fabsf(b[j])));
             bad |= !(fabsf(a[j]) <= kMaxFloat) || !(fabsf(b[j]) <= kMaxFloat);
         }
     };
-    auto unit = [&](int tl, int u, int t) {
+    auto unit = [&](int tl, int u, int t, float (&a)[V], float (&b)[V], int& first, int& second) __attribute__((always_inline)) {
         const int pos = turn.half ? turn.positions[t] : 0;
         load_unit<T, V, P>(rows + (long)t * x.token, u, turn, a, b, first, second);
         if constexpr (NORM) {
@@ -296,32 +295,53 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run,
         }
         turn_unit<V, P>(u, pos, turn, a, b);
     };
+    // Normed keys: lanes share a row, and kHeld rows' loads wait together.
+    constexpr int N = kHeadUnits<V>, kHeld = NORM ? 2 : 1;
+    float ha[kHeld][N][V], hb[kHeld][N][V];
+    int first_of[N], second_of[N];
+    const int l = NORM ? threadIdx.x & (g.lanes - 1) : 0, at_once = NORM ? kThreads / g.lanes : 1, mine = NORM ? threadIdx.x / g.lanes : 0;
     if constexpr (NORM) {
-        constexpr int N = kHeadUnits<V>;
-        const int l = threadIdx.x & (g.lanes - 1);
-        for (int i = threadIdx.x / g.lanes; i < n; i += kThreads / g.lanes) {
-            float a[N][V], b[N][V];
-            int first[N], second[N];
-            const int t = run.token(i), pos = turn.half ? turn.positions[t] : 0;
-            load_head<T, V, N, P>(rows + (long)t * x.token, l, g.lanes, units, turn, a, b, first, second);
-            const float r = head_factor<V, N>(l, g.lanes, units, g.norm, a, b);
-            if (l == 0) factors[i] = r;
+        float w[N][2][V];
+        for (int i0 = mine; i0 < n + mine; i0 += kHeld * at_once) {
+            float cs[kHeld][N][2][V];
+            int pos[kHeld];
+#pragma unroll
+            for (int e = 0; e < kHeld; e++) {
+                if (e && i0 - mine + e * at_once >= n) break;  // (the same for the workgroup)
+                const int t = run.token(min(i0 + e * at_once, n - 1));
+                pos[e] = turn.half ? turn.positions[t] : 0;
+                load_head<T, V, N, P>(rows + (long)t * x.token, l, g.lanes, units, turn, ha[e], hb[e], first_of, second_of);
+            }
 #pragma unroll
             for (int k = 0; k < N; k++) {
-                if (l + k * g.lanes >= units) continue;
-                float w[2][V];
-                load_weights<V>(g.norm, first[k], w[0]);
-                load_weights<V>(g.norm, second[k], w[1]);
-                scale_unit<V>(r, w[0], a[k]);
-                scale_unit<V>(r, w[1], b[k]);
-                turn_unit<V, P>(l + k * g.lanes, pos, turn, a[k], b[k]);
-                look(a[k], b[k]);
+                load_weights<V>(g.norm, first_of[k], w[k][0]);
+                load_weights<V>(g.norm, second_of[k], w[k][1]);
+#pragma unroll
+                for (int e = 0; e < kHeld; e++) {
+                    if (e && i0 - mine + e * at_once >= n) break;
+                    load_angles<V>(l + k * g.lanes, pos[e], turn, cs[e][k][0], cs[e][k][1]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < kHeld; e++) {
+                if (e && i0 - mine + e * at_once >= n) break;
+                const float r = head_factor<V, N>(l, g.lanes, units, g.norm, ha[e], hb[e]);
+                if (l == 0 && i0 + e * at_once < n) factors[i0 + e * at_once] = r;
+#pragma unroll
+                for (int k = 0; k < N; k++) {
+                    scale_unit<V>(r, w[k][0], ha[e][k]);
+                    scale_unit<V>(r, w[k][1], hb[e][k]);
+                    turn_by<V, P>(l + k * g.lanes, turn, cs[e][k][0], cs[e][k][1], ha[e][k], hb[e][k]);
+                    if (i0 + e * at_once < n && l + k * g.lanes < units) look(ha[e][k], hb[e][k]);
+                }
             }
         }
     } else {
         for (int i = threadIdx.x; i < n * units; i += kThreads) {
             const int tl = i / units, u = i - tl * units;
-            unit(tl, u, run.token(tl));
+            float a[V], b[V];
+            int first, second;
+            unit(tl, u, run.token(tl), a, b, first, second);
             look(a, b);
         }
     }
@@ -359,10 +379,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run,
 
     int8_t* bytes = reinterpret_cast<int8_t*>(image);
     const float step = now > 0.0f ? now : 1.0f;  // 1 for a NaN, whose codes nobody takes for values
-    for (int i = threadIdx.x; i < n * units; i += kThreads) {
-        const int tl = i / units, u = i - tl * units, t = run.token(tl);
-        unit(tl, u, t);
-        const int place = run.place(tl);
+    auto write = [&](int place, const float (&a)[V], const float (&b)[V], int first, int second) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < V; j++) {
             const int p = code_of(a[j], step), q = code_of(b[j], step);
@@ -373,6 +390,22 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run,
                 bytes[place * c.dp + first + j] = (int8_t)p;
                 bytes[place * c.dp + second + j] = (int8_t)q;
             }
+        }
+    };
+    if (NORM && n <= kHeld * at_once) {
+#pragma unroll
+        for (int e = 0; e < kHeld; e++)
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                if (mine + e * at_once < n && l + k * g.lanes < units)
+                    write(run.place(mine + e * at_once), ha[e][k], hb[e][k], first_of[k], second_of[k]);
+    } else {
+        for (int i = threadIdx.x; i < n * units; i += kThreads) {
+            const int tl = i / units, u = i - tl * units;
+            float a[V], b[V];
+            int first, second;
+            unit(tl, u, run.token(tl), a, b, first, second);
+            write(run.place(tl), a, b, first, second);
         }
     }
     __syncthreads();
@@ -475,11 +508,13 @@ __device__ __forceinline__ Run run_from(const AppendArgs& g, int t, long s, Foun
 // One token for each of 64 sequences (8 heads of 128, pages of 64, fp32): 10.3
 // us, where a page that grows is read and written; a workgroup waits for its
 // slots, its rows, their largest, the scale and the codes one after the other.
-// Prompts of 1955 tokens in all (fp16, 64 + 8 heads, pages of 16): 76 MB, 64 of
-// them q, in 22.6 us, 3.4 TB/s.
+// Prompts of 1955 tokens in all (fp16, 32 + 8 heads of 128, pages of 16): 16.2 us.
 //
-// Normed keys: a row is dealt out to lanes that share its sum of squares, and its
-// factor kept in LDS for the second reading.
+// Normed keys: a row is dealt out to lanes that share its sum of squares, two
+// rows at a time (four: 3218 tokens of prompts 30.4 us instead of 31.0, but 48
+// sequences' tokens 12.0 instead of 10.3, for code that most of them skip).  A run
+// that is as short as that stays in registers, others' factors are kept in LDS
+// for the second reading.
 template <class T, int V, int VQ, class Q, Pairs P>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, Q q) {
     constexpr bool NORM = std::is_same_v<Q, NormArgs>;
@@ -500,7 +535,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, Q q) {
     int b = blockIdx.x;
     const int values = b & 1, head = (b >> 1) % c.heads;
     b = (b >> 1) / c.heads;
-    const int turn = b % g.turns, from = b / g.turns * 64, lane = threadIdx.x & 63;
+    const int turn = b / g.windows, from = (b - turn * g.windows) * 64, lane = threadIdx.x & 63;
     auto slot = [&](long t) { return t >= 0 && t < g.tokens ? g.slots[t] : -1l; };
     const long here = slot(from + lane), behind = slot((long)from - 1 - lane);
     const int page = page_of(c, here);
@@ -576,12 +611,18 @@ static int append(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v,
     g.slots = slots;
     g.turn = {positions, table, half, max_pos, flags};
     g.tokens = tokens;
+    g.windows = ceil_div(tokens, 64);
     // a workgroup for each token while they are few (a batch's next tokens, each on a page of its own: with the pages'
-    // values read back, 64 sequences 28 us, with 8 workgroups for 64 tokens 45), else for eight: a prompt's tokens mostly
-    // go on in their page, and a workgroup that finds none to do costs its launch (pages of 16, prompts of 1955 tokens:
-    // 38 us, with 16 44, 32 55, 4 36; but 512 sequences' single tokens 150, 152, 152 and 169)
-    g.turns = tokens <= 256 ? 64 : 8;
-    g.blocks = 2l * cache->kv_heads * ceil_div(tokens, 64) * g.turns;
+    // values read back, 64 sequences 28 us, with 8 workgroups for 64 tokens 45), else as many as give each CU four, and no
+    // fewer than pages that 64 tokens of one sequence begin.  One that finds none to do costs its launch and its look at
+    // 64 slots: all the first ones come first, so that they are spread over the CUs, the idle ones behind them, q last (fp16,
+    // with q, four heads for each of keys, pages of 64; us with these and with 8 in turn for each 64 tokens: 8 heads, a prompt
+    // of 16000 tokens 93 and 166, of 1955 15.5 and 24.7, 300 sequences' single tokens 25 and 33, 2048 135 and 127, where four
+    // times as many take 121 but prompts of 1955 on pages of 16 18.6 instead of 16.2; 2 heads, 26 and 91, 10.4 and 16.2, 12 and
+    // 29, 34 and 37)
+    const long wide = 1024 / (2l * cache->kv_heads * g.windows), most = tokens <= 256 ? 64 : 32;
+    g.turns = tokens <= 256 || wide > most ? most : max((int)wide, max(64 / g.c.page, 1));
+    g.blocks = 2l * cache->kv_heads * g.windows * g.turns;
     RopeArgs r{};
     r.turn = g.turn;
     r.tokens = tokens;
