@@ -104,6 +104,14 @@ def check(eng, rng, counts, contexts, heads, kv, dim, page, dtype, window=0, wor
     return got
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 4])
+@pytest.mark.parametrize("counts,contexts", [((12, 5), (-2, 6)), ((40,), (-9,)), ((90, 7), (-70, -3))])
+def test_the_largest_window(eng, counts, contexts, window):
+    """Requests that hold fewer tokens than they have rows: no first token, before or behind an int's end."""
+    for dtype in DT:
+        assert np.abs(check(eng, np.random.default_rng(3), counts, contexts, 2, 1, 64, 16, dtype, window=window)).max() > 0
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("counts,contexts,heads,kv,dim,page", [
     ((1,), (0,), 4, 2, 64, 16), ((1,), (37,), 8, 2, 128, 16), ((8,), (60,), 8, 2, 128, 32), ((7, 1, 13), (5, 200, 0), 4, 1, 64, 64),

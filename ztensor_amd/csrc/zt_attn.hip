@@ -157,7 +157,7 @@ __device__ __forceinline__ int tiles_up_to(int token) { return (int)(((unsigned)
 // context's end and the rows that its mask has, less one) and, of the tokens
 // behind it, those whose bits its mask has.
 __device__ __forceinline__ int tree_first(const AttnArgs& g, int len, int n) {  // no row sees a token before
-    return g.window > 0 ? max(0, len - n - g.window) : 0;
+    return g.window > 0 ? (int)max(0l, (long)len - n - g.window) : 0;
 }
 struct TreeRow {
     int row, lo;  // of the masks (-1: no such row), and the first token of the context that it sees
