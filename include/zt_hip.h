@@ -879,8 +879,9 @@ int zt_kv8_copy(const zt_kv8_cache* caches, int layers, const int* from, const i
  * all pages, `pages` entries of which the first free_count are there; entries
  * of the table outside 0 .. pages - 1 stay as they are.  refs[p]: how many
  * sequences hold page p besides one (zt_kv8_fork counts them up); a page that is
- * given back fewer times than it has holders stays, with as many fewer.  NULL:
- * nobody shares.  pages at most 2^20; outputs (free_pages and refs among them)
+ * given back fewer times than it has holders stays, with as many fewer (and one
+ * that keep[r] ends in and others hold is theirs too: no step may write there;
+ * zt_kv8_fork of the request copies it).  NULL: nobody shares.  pages at most 2^20; outputs (free_pages and refs among them)
  * share no bytes with inputs nor with each other, but for table_out that is table,
  * else InvalidValue. */
 int zt_kv8_trim(const int* kv_lens, const int* keep, const int* table, int requests, int width, int* free_pages,
@@ -894,7 +895,8 @@ int zt_kv8_trim(const int* kv_lens, const int* keep, const int* table, int reque
  * to do for it (-1: nothing).  A fork that finds no page gets no tokens: length 0,
  * its row all -1; so does one whose source is outside the table or holds nothing,
  * or more than its row.  The other rows, and a row forked from itself, stay as
- * they are.  A row's old pages are not given back (zt_kv8_trim does that), and
+ * they are.  A row's old pages are not given back (zt_kv8_trim does that, before
+ * this or after it with the table as it was), and
  * each row is a target once at most.  `pages`: the entries of free_pages and refs.
  * Outputs (refs among them) share no bytes with inputs nor with each other, else
  * InvalidValue. */

@@ -346,6 +346,61 @@ def test_forks_are_copies(eng):
     assert sorted(a.free.tolist()) == list(range(96))
 
 
+def test_beams(eng):
+    """Rows that go on from others while they hold something themselves: forks first, then what they held by the old table."""
+    a, b = Requests(eng, 4), Requests(eng, 4)
+    for each in (a, b):
+        _, p = each.step(torch.arange(21 * 4, device="cuda") % 50, [21] * 4)
+        each.lens, each.table, each.count = p.kv_lens, p.block_table, p.free_count
+    order = [0, 0, 3, 0]  # row 2 goes on from 3, 1 and 3 from 0
+    for step in range(3):
+        f = eng.kv8_fork(i32(order), i32(range(4)), a.lens, a.table, a.refs, a.free, a.count, a.page)
+        eng.kv8_copy(a.caches, f.copy_from, f.copy_to)
+        keep = i32([n if order[r] == r else 0 for r, n in enumerate(a.lens.tolist())])
+        left = eng.kv8_trim(a.lens, keep, a.table, a.free, f.free_count, a.page, refs=a.refs)
+        a.lens, a.table, a.count = f.kv_lens, f.block_table, left.free_count
+        text = torch.tensor([7 + step, 8, 9, 10], device="cuda")
+        x, p = a.step(text, [1] * 4)
+        a.lens, a.table, a.count = p.kv_lens, p.block_table, p.free_count
+        if step == 0:  # what rows of their own leave, which had the sources' tokens all along
+            y, _ = b.step(torch.cat([text[:1], text[3:]]), [1, 0, 0, 1])
+            assert torch.equal(x[0], y[0])
+        held = a.table[a.table >= 0].tolist()
+        assert len(a.free[:a.count.item()].unique()) == a.count.item()
+        assert sorted(set(held) | set(a.free[:a.count.item()].tolist())) == list(range(96))
+        assert sum(a.refs.tolist()) == len(held) - len(set(held)) and not set(held) & set(a.free[:a.count.item()].tolist())
+    left = eng.kv8_trim(a.lens, i32([0] * 4), a.table, a.free, a.count, a.page, refs=a.refs)
+    assert left.free_count.item() == 96 and a.refs.sum().item() == 0
+
+
+def test_a_cut_into_a_shared_page_goes_on_as_a_fork(eng):
+    a, b = Requests(eng, 3), Requests(eng, 1)
+    text = torch.arange(40, device="cuda")
+    for each, new in ((a, [40, 0, 0]), (b, [40])):
+        _, p = each.step(text, new)
+        each.lens, each.table, each.count = p.kv_lens, p.block_table, p.free_count
+    def fork(source, target):
+        f = eng.kv8_fork(i32([source]), i32([target]), a.lens, a.table, a.refs, a.free, a.count, a.page)
+        eng.kv8_copy(a.caches, f.copy_from, f.copy_to)
+        a.lens, a.table, a.count = f.kv_lens, f.block_table, f.free_count
+    def cut(keep):
+        left = eng.kv8_trim(a.lens, i32(keep), a.table, a.free, a.count, a.page, refs=a.refs)
+        a.lens, a.table, a.count = i32(keep), left.block_table, left.free_count
+    fork(0, 1)
+    cut([40, 20, 0])  # on page 1, which row 0 holds too
+    fork(1, 2)
+    cut([40, 0, 20])
+    assert a.table[0, 0] == a.table[2, 0] and a.table[0, 1] != a.table[2, 1]
+    for i in range(14):  # over the end of the page
+        x, p = a.step(torch.tensor([3, 44], device="cuda"), [1, 0, 1])
+        a.lens, a.table, a.count = p.kv_lens, p.block_table, p.free_count
+        y, p = b.step(torch.tensor([3], device="cuda"), [1])
+        b.lens, b.table, b.count = p.kv_lens, p.block_table, p.free_count
+        assert torch.equal(x[0], y[0])
+    cut([0, 0, 0])
+    assert a.count.item() == 96 and a.refs.sum().item() == 0
+
+
 def test_captured(eng):
     """The bookkeeping of a step in a graph, replayed over other lengths."""
     rng = np.random.default_rng(1)

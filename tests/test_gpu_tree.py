@@ -301,3 +301,15 @@ def test_accept_of_tokens_that_are_nobodys(eng):
     assert [x.tolist() for x in got] == [[0, 1, 2], [3], [2], [5]]
     none = eng.tree_accept(i64([]), i64([]), i32([0, 0]))
     assert [x.tolist() for x in none] == [[], [0], [-1], [-1]]
+
+
+def test_accept_refuses(eng):
+    one = i64([1, 2, 3])
+    with pytest.raises(ValueError, match="q_start"):
+        eng.tree_accept(one, one, i32([]))
+    with pytest.raises(ValueError, match="drawn"):
+        eng.tree_accept(one, one[:2].contiguous(), i32([0, 3]))
+    with pytest.raises(ValueError, match="parents"):
+        eng.tree_accept(one, one, i32([0, 3]), parents=one)
+    none = eng.tree_accept(one[:0], one[:0], i32([0]))
+    assert [x.numel() for x in none] == [0, 0, 0, 0]

@@ -23,7 +23,16 @@ one:
     f = engine.kv8_fork(source, target, kv_lens, block_table, refs, free_pages, free_count, page_tokens)
     engine.kv8_copy(caches, f.copy_from, f.copy_to)
 
-and kv8_trim with refs gives a page back when its last holder does.
+and kv8_trim with refs gives a page back when its last holder does.  Beams, whose
+targets held something else: the forks first, then what those rows held goes back
+by the table from before (keep 0 for the targets, the others' lengths for them):
+
+    left = engine.kv8_trim(kv_lens, keep, block_table, free_pages, f.free_count, page_tokens, refs=refs)
+    # on with f.block_table, f.kv_lens and left.free_count
+
+A step writes into the page that a sequence's last tokens are on, if it is not
+full, so that page has to be its own: who is cut in the middle of a page that
+others hold too goes on as a fork of itself, in another row.
 """
 from __future__ import annotations
 
@@ -142,6 +151,8 @@ class DraftOps(DecodeOps):
         (drawn, int64 [tokens]: a sample of every row).  parents None: a chain.
         slots (kv8_plan's): a request without pages keeps nothing."""
         tokens, r, i32, i64 = drafted.shape[0], q_start.shape[0] - 1, torch.int32, torch.int64
+        if r < 0:
+            raise ValueError("tree_accept: q_start has an entry more than there are requests")
         dense, one = self._dense, (tokens,)
         args = (dense(drafted, "drafted", i64, one), dense(drawn, "drawn", i64, one), dense(parents, "parents", i32, one),
                 dense(q_start, "q_start", i32, (None,)), dense(slots, "slots", i64, one), r, tokens)
@@ -189,7 +200,9 @@ class DraftOps(DecodeOps):
         free_count (int32 [1]) entries are there.  free_pages (int32 [pages])
         has room for all pages and is written in place.  refs (int32 [pages],
         in place too): a page that others hold as well stays, with one holder
-        fewer.  in_place: the -1 are written into block_table itself."""
+        fewer (one that keep[r] ends in is not to be written to then: a fork of
+        the request has its own).  in_place: the -1 are written into block_table
+        itself."""
         r, width = block_table.shape
         dense, i32, one = self._dense, torch.int32, (r,)
         pages = free_pages.shape[0]
@@ -210,7 +223,8 @@ class DraftOps(DecodeOps):
         shared (refs, int32 [pages], one more, in place); a last page that is
         not full gets a page of its own, and copy_from / copy_to are what
         kv8_copy is to do for it.  A fork that finds no free page gets length 0.
-        What a target's row held is not given back: kv8_trim does that, before."""
+        What a target's row held is not given back: kv8_trim does that, before,
+        or after with block_table as it was."""
         n, (r, width), i32, dense = source.shape[0], block_table.shape, torch.int32, self._dense
         pages = free_pages.shape[0]
         args = (dense(source, "source", i32, (n,)), dense(target, "target", i32, (n,)), dense(kv_lens, "kv_lens", i32, (r,)),
