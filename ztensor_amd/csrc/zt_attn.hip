@@ -722,7 +722,7 @@ __device__ __forceinline__ RowTiles tiles_of(const AttnArgs& g, const Span& sp, 
 // which bounds it: 80 decode its share of the codes, 5 for each of its scores are
 // the softmax's.  The last fifth of the time is a tail with half of the
 // workgroups.  fp32 rows take twice the products in two fp16 parts: 364 us, 1.03
-// PFLOP/s of them, with 38 registers kept in memory; at 256 dims those are 84, of
+// PFLOP/s of them, with 42 registers kept in memory; at 256 dims those are 81, of
 // fp16 rows 24.
 // What of them a workgroup works on at a time: rows row0 on of a request and a
 // key/value head, tiles first .. last - 1; their sums are the rows' own, or go to
@@ -991,7 +991,7 @@ constexpr int kTreeRows = 64 * kTreeCols<T, DN>;
 // one column only, 4 and 18.  64 requests' spans lie in LDS at a time.
 //
 // 24 trees of up to 64 rows, 64 heads over 8 of 128, on contexts of up to 12000
-// (fp16, 185 GFLOP): 285 us, 0.65 PFLOP/s; with workgroups that take whole groups
+// (fp16, 185 GFLOP): 284 us, 0.65 PFLOP/s; with workgroups that take whole groups
 // 472.  What bounds it: a tile of two columns is 64 matrix instructions (1024
 // cycles) and some 320 of the vector unit, and beside a full stream of matrix
 // instructions that issues one each 8.5 cycles (5.2 alone); 2.05 us at 1.8 GHz are
@@ -1209,7 +1209,8 @@ __global__ __launch_bounds__(512) void attn_join_kernel(Work f, int rows_of_grou
 }
 
 // The same for a tree's rows, which are many and in few parts each: 16 DN lanes a
-// row and q head, 4 dims each, and up to eight parts at a time.
+// row and q head, 4 dims each, and up to eight parts at a time.  24 trees of up to
+// 64 rows, 64 heads of 128: 18.2 us of the call's 284.
 template <class T, int DN>
 __global__ __launch_bounds__(256) void tree_join_kernel(Work f, int rows_of_group) {
     constexpr int LANES = DN == 3 ? 64 : 16 * DN, LOADS = 8;

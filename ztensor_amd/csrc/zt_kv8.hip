@@ -88,7 +88,10 @@ struct NormArgs {
 };
 
 // g.lanes lanes have kHeads heads of one token, whose weights and angles are the
-// same: those are read once, and the heads' loads wait together.  Bytes bound it.
+// same: those are read once, and the heads' loads wait together.  Bytes bound it:
+// 4099 tokens, 64 + 4 heads of 128 of which 64 dims are turned, fp16, 144 MB in 30
+// us, 4.8 TB/s, 26 where half of it is in the Infinity Cache (one head at a time
+// 42); one token 3.8 us, the launch and the chain from its position to the angles.
 constexpr int kHeads = 4;
 template <class T, int V, Pairs P>
 __device__ __forceinline__ void norm_block(const NormArgs& g, int block) {
