@@ -401,6 +401,36 @@ def test_a_cut_into_a_shared_page_goes_on_as_a_fork(eng):
     assert a.count.item() == 96 and a.refs.sum().item() == 0
 
 
+def test_past_32_bits(eng):
+    """Pages that lie more than 2 GiB into the cache: copied, their rows moved, a tree over them."""
+    rng = np.random.default_rng(8)
+    page, dim, heads = 128, 128, 4
+    pages = (1 << 31) // (page * dim) + 4
+    host = ref.Cache(3, 1, dim, page, rng)
+    cache = KV8Cache(*(torch.empty(x, dtype=torch.int8, device="cuda") for x in ((pages, 1, page, dim), (pages, 1, dim, page))),
+                     *(torch.empty((pages, 1), device="cuda") for _ in range(2)))
+    for t, d in zip(cache, host.device(torch)):
+        t[1:4] = d
+    far = [pages - 1, pages - 3, pages - 2]
+    eng.kv8_copy([cache], i32([1, 2, 3]), i32(far))
+    for t in cache:
+        assert torch.equal(t[1:4], t[far])
+    held, n, lens = 150, 130, 280
+    starts, table = [0, n], np.array([[0, 1, 2]])
+    parents = np.array([-1] + [int(rng.integers(max(0, i - 4), i)) for i in range(1, n)])
+    mask = draft_ref.tree(parents, [lens], starts, n, 3)[1]
+    q = rng.standard_normal((n, heads, dim)).astype(np.float32)
+    want, most, big = draft_ref.attend(q, host, table, [lens], starts, mask)
+    got = eng.kv8_tree_attention(torch.from_numpy(q).cuda(), cache, i32([far]), i32([lens]), i32(starts), torch.from_numpy(mask).cuda())
+    assert (np.abs(got.cpu().numpy() - want) <= ref.attend_bound(want, most, big, False)).all()
+    path = np.full(n, -1)
+    path[:120] = some_path(rng, n, 120)
+    assert eng.kv8_compact([cache], i32([far]), i32([held]), i32(starts), i32(path), i32([120])).tolist() == [270]
+    draft_ref.compact(host, table, [held], starts, path, [120])
+    for t, d in zip(cache, host.device(torch)):
+        assert torch.equal(t[far], d)
+
+
 def test_captured(eng):
     """The bookkeeping of a step in a graph, replayed over other lengths."""
     rng = np.random.default_rng(1)

@@ -238,6 +238,28 @@ def test_strides_scale_bounds_and_out(eng):
         eng.kv8_tree_attention(q, *args[:-1], torch.zeros(9, 17, dtype=torch.int64, device="cuda"))
 
 
+@pytest.mark.parametrize("heads,most,longest", [(2, 40, 800), (8, 40, 800), (8, 1, 64), (8, 40, 100)])
+def test_starts_out_of_order(eng, heads, most, longest):
+    """No meaning, but nothing outside the buffers is read or written: finite values, and the guard rows untouched."""
+    rng = np.random.default_rng(most)
+    lens = [100, 800, 40, 300]
+    table, pages = paged(rng, lens, 16)
+    cache = ref.Cache(pages, 2, 128, 16, rng).device(torch)
+    q = torch.from_numpy(rng.standard_normal((60, heads, 128)).astype(np.float32)).cuda()
+    mask = torch.from_numpy(rng.integers(-2 ** 63, 2 ** 63 - 1, (60, 1)))
+    tokens = torch.from_numpy(rng.integers(0, 3, (2, 60))).cuda()
+    parents = i32(rng.integers(-1, 20, 60))
+    whole = torch.full((64, heads, 128), 7.0, device="cuda")
+    for starts in ([-9, 5, 2, 9, 60], [2 ** 31 - 1, -2 ** 31, 30, -2, 2 ** 31 - 1], [50, 40, 30, 20, 10], [-2 ** 31] * 5):
+        print(starts, flush=True)
+        out = eng.kv8_tree_attention(q, cache, i32(table), i32(lens), i32(starts), mask.cuda(), max_q=most, max_kv=longest, out=whole[2:62])
+        assert torch.isfinite(out).all() and (whole[:2] == 7).all() and (whole[62:] == 7).all()
+        eng.kv8_tree(parents, i32(lens), i32(starts), 60)
+        took = eng.tree_accept(tokens[0], tokens[1], i32(starts), parents=parents)
+        eng.kv8_compact([cache], i32(table), i32([2 ** 31 - 1, 700, 0, 5]), i32(starts), took.path, took.kept)
+        torch.cuda.synchronize()
+
+
 def test_attention_again_and_captured(eng):
     """The same bits every call, and in replays whose lengths, masks and starts change."""
     rng = np.random.default_rng(11)
