@@ -47,7 +47,7 @@ def some_path(rng, n, m):
 @pytest.mark.parametrize("heads,dim,page,held,counts,layers", [
     (2, 64, 16, (5, 16, 0), (12, 30, 1), 1), (1, 128, 16, (30, 3), (64, 40), 2), (3, 80, 32, (31, 64, 7), (33, 20, 5), 1),
     (2, 256, 128, (120, 0), (20, 200), 1), (1, 72, 64, (60, 63), (5, 2), 3), (2, 128, 64, (1, 2, 3, 500), (70, 9, 0, 64), 1),
-    (1, 64, 16, (7,), (9,), 40)])
+    (1, 64, 16, (7,), (9,), 40), (2, 192, 32, (3, 90), (100, 37), 1), (1, 136, 128, (200, 5), (150, 300), 2)])
 def test_compact(eng, heads, dim, page, held, counts, layers):
     rng = np.random.default_rng(dim + page)
     lens = [h + n for h, n in zip(held, counts)]

@@ -183,6 +183,44 @@ __device__ __forceinline__ int code_at(const u32x4& w, int k) { return (int8_t)(
 __device__ __forceinline__ void set_code(u32x4& w, int k, int code) {
     w[k >> 2] = (w[k >> 2] & ~(0xFFu << 8 * (k & 3))) | ((uint32_t)code & 0xFFu) << 8 * (k & 3);
 }
+// The same where k is one for the wave, but not known to the compiler.
+__device__ __forceinline__ int code_at_any(const u32x4& w, int k) {
+    return (int8_t)((k & 8 ? k & 4 ? w[3] : w[2] : k & 4 ? w[1] : w[0]) >> 8 * (k & 3));
+}
+__device__ __forceinline__ void set_code_any(u32x4& w, int k, int code) {
+    const uint32_t mask = 0xFFu << 8 * (k & 3), to = ((uint32_t)code & 0xFFu) << 8 * (k & 3);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (k >> 2 == i) w[i] = (w[i] & ~mask) | to;
+}
+
+// Values' places that come from the same 16 of the same page as the first of
+// `left`, which they are taken from: loaded at once, a dim of all 16 a lane.
+struct Sixteen {
+    int page, piece;
+    float scale;
+    uint64_t places[2];
+};
+// (of place 64 half + lane: `from`'s values in a lane's registers, which others read without LDS's wait)
+struct Lanes {
+    int page[2], place[2];
+    float scale[2];
+    __device__ __forceinline__ int place_of(int half, uint64_t bits) const {
+        return __builtin_amdgcn_readlane(place[half], __builtin_ctzll(bits));
+    }
+};
+__device__ __forceinline__ Sixteen first_sixteen(const Lanes& from, uint64_t (&left)[2]) {
+    const int z = __builtin_ctzll(left[0] ? left[0] : left[1]);
+    Sixteen x{__builtin_amdgcn_readlane(left[0] ? from.page[0] : from.page[1], z),
+              __builtin_amdgcn_readlane(left[0] ? from.place[0] : from.place[1], z) >> 4,
+              __int_as_float(__builtin_amdgcn_readlane(__float_as_int(left[0] ? from.scale[0] : from.scale[1]), z)), {0, 0}};
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+        x.places[half] = left[half] & __ballot(from.page[half] == x.page && from.place[half] >> 4 == x.piece);
+        left[half] &= ~x.places[half];
+    }
+    return x;
+}
 
 // One wave: a request's rows of one head of keys or of values, page after page of
 // those that they go to.  A row comes from behind the place that it goes to, and
@@ -194,9 +232,11 @@ __device__ __forceinline__ void set_code(u32x4& w, int k, int code) {
 // and the page's scale grows where that needs it, as the cache's writer has it.
 //
 // Loads that wait for each other bound it: starts and counts, the path, the pages,
-// their scales, the codes.  Codes go in pieces of 16 bytes (of 128 requests with
-// trees of 48 rows, 8 heads of 128, pages of 16, two layers: 24.9 us, code by code
-// 139); 8 requests of 12 rows, pages of 64: 7.4 us.
+// their scales, the codes.  Codes go in pieces of 16 bytes, of values those of 16
+// places of a dim, however many of them are wanted (of 128 requests with trees of
+// 48 rows, 8 heads of 128, pages of 16, two layers: 20.4 us; values' codes read one
+// by one, lanes 16 bytes apart, 24.7; all codes one by one 139); 8 requests of 12
+// rows, pages of 64: 5.9 us.
 __global__ __launch_bounds__(64) void compact_kernel(CompactArgs g, Layers layers) {
     __shared__ Sources from;
     const Kv8& c = g.c;
@@ -216,22 +256,30 @@ __global__ __launch_bounds__(64) void compact_kernel(CompactArgs g, Layers layer
     for (long p = base >> c.shift; p << c.shift < end; p++) {
         const int page = row[p];
         uint64_t moved[2] = {0, 0}, far[2] = {0, 0};
+        Lanes lanes;
 #pragma unroll
         for (int half = 0; half < 2; half++) {
             const int place = 64 * half + lane;
             const long at = (p << c.shift) + place;
             int src_page = -1;
+            lanes.place[half] = 0;
+            lanes.scale[half] = 0.0f;
             if (place < c.page && at >= base && at < end) {
                 const int j = (int)(at - base), k = g.path[s.start + j];
                 const long src = base + k;
                 if (k > j && k < s.n && src < (long)g.width << c.shift) {
                     src_page = row[src >> c.shift];
                     if (!c.holds(src_page) || !c.holds(page)) src_page = -1;
-                    from.place[place] = (uint8_t)(src & (c.page - 1));
-                    from.scale[place] = src_page < 0 ? 0.0f : scales[(long)src_page * c.heads + head];
+                    lanes.place[half] = (int)(src & (c.page - 1));
+                    if (src_page >= 0) lanes.scale[half] = scales[(long)src_page * c.heads + head];
                 }
             }
-            if (place < c.page) from.page[place] = src_page;
+            lanes.page[half] = src_page;
+            if (place < c.page) {
+                from.page[place] = src_page;
+                from.place[place] = (uint8_t)lanes.place[half];
+                from.scale[place] = lanes.scale[half];
+            }
             moved[half] = __ballot(src_page >= 0);
             far[half] = __ballot(src_page >= 0 && src_page != page);
         }
@@ -241,6 +289,7 @@ __global__ __launch_bounds__(64) void compact_kernel(CompactArgs g, Layers layer
         const long at = (long)page * c.heads + head;
         const float had = scales[at];
         float now = had;
+        auto sixteen = [&](const Sixteen& x) { return reinterpret_cast<const u32x4*>(codes + c.at(x.page, head)) + x.piece; };
         if (far[0] | far[1]) {
             float m = 0.0f;
             bool bad = false;
@@ -250,7 +299,7 @@ __global__ __launch_bounds__(64) void compact_kernel(CompactArgs g, Layers layer
                 bad |= !(value <= kMaxFloat);
             };
             uint64_t left[2] = {far[0], far[1]};
-            while (left[0] | left[1]) {
+            while (!values && (left[0] | left[1])) {
                 // four places at a time (the last ones again where there are fewer); of each 4 dims a lane
                 uint32_t w[4];
                 float by[4];
@@ -262,22 +311,27 @@ __global__ __launch_bounds__(64) void compact_kernel(CompactArgs g, Layers layer
                         z = 64 * half + __builtin_ctzll(left[half]);
                         left[half] &= left[half] - 1;
                     }
-                    const int8_t* src = codes + c.at(from.page[z], head);
-                    const int in = from.place[z];
                     by[e] = from.scale[z];
                     w[e] = 0;
-                    if (!values) {
-                        if (4 * lane < c.dp) w[e] = *reinterpret_cast<const uint32_t*>(src + in * c.dp + 4 * lane);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            if (lane + 64 * k < c.dp) w[e] |= (uint32_t)(uint8_t)src[(lane + 64 * k) * c.page + in] << 8 * k;
-                    }
+                    if (4 * lane < c.dp) w[e] = *reinterpret_cast<const uint32_t*>(codes + c.at(from.page[z], head) + from.place[z] * c.dp + 4 * lane);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; e++)
 #pragma unroll
                     for (int k = 0; k < 4; k++) look((int8_t)(w[e] >> 8 * k), by[e]);
+            }
+            while (left[0] | left[1]) {
+                const Sixteen x = first_sixteen(lanes, left);
+                const u32x4* src = sixteen(x);
+                int most = 0;  // (the largest product is the largest code's)
+                for (int d = lane; d < c.dp; d += 64) {
+                    const u32x4 w = src[d * (c.page / 16)];
+#pragma unroll
+                    for (int half = 0; half < 2; half++)
+                        for (uint64_t bits = x.places[half]; bits; bits &= bits - 1)
+                            most = max(most, abs(code_at_any(w, lanes.place_of(half, bits) & 15)));
+                }
+                look(most, x.scale);
             }
             bad = __any(bad);
             m = max_step<1>(max_step<2>(max_step<4>(max_step<8>(max_step<16>(max_step<32>(m))))));
@@ -316,19 +370,19 @@ __global__ __launch_bounds__(64) void compact_kernel(CompactArgs g, Layers layer
                 if (!some && !grown) continue;
                 for (int d = lane; d < c.dp; d += 64) {
                     u32x4 w = out[d * per + chunk];
-                    int8_t in[16];
+                    if (grown) {
 #pragma unroll
-                    for (int k = 0; k < 16; k++) {
-                        const int z = 16 * chunk + k;
-                        in[k] = some >> k & 1 ? codes[c.at(from.page[z], head) + d * c.page + from.place[z]] : 0;
+                        for (int k = 0; k < 16; k++) set_code(w, k, take(code_at(w, k), false, 0.0f));
                     }
+                    const uint64_t bits16 = (uint64_t)some << 16 * (chunk & 3);
+                    uint64_t left[2] = {chunk < 4 ? bits16 : 0, chunk < 4 ? 0 : bits16};
+                    while (left[0] | left[1]) {
+                        const Sixteen x = first_sixteen(lanes, left);
+                        const u32x4 in = sixteen(x)[d * per];
 #pragma unroll
-                    for (int k = 0; k < 16; k++) {
-                        const int z = 16 * chunk + k;
-                        if (some >> k & 1)
-                            set_code(w, k, take(in[k], from.page[z] != page, from.scale[z]));
-                        else if (grown)
-                            set_code(w, k, take(code_at(w, k), false, 0.0f));
+                        for (int half = 0; half < 2; half++)
+                            for (uint64_t bits = x.places[half]; bits; bits &= bits - 1)
+                                set_code_any(w, __builtin_ctzll(bits) & 15, take(code_at_any(in, lanes.place_of(half, bits) & 15), x.page != page, x.scale));
                     }
                     out[d * per + chunk] = w;
                 }
