@@ -411,7 +411,7 @@ __global__ __launch_bounds__(kThreads) void copy_kernel(Kv8 c, Layers layers, co
     float* scales = values ? layers.v_scale[layer] : layers.k_scale[layer];
     const u32x4* src = reinterpret_cast<const u32x4*>(codes + c.at(a, 0));
     u32x4* dst = reinterpret_cast<u32x4*>(codes + c.at(z, 0));
-    const int pieces = c.heads * c.bytes() / 16, first = chunk * kCopyPieces * kThreads + threadIdx.x;
+    const int pieces = (int)((long)c.heads * c.bytes() / 16), first = chunk * kCopyPieces * kThreads + threadIdx.x;
     u32x4 w[kCopyPieces];
 #pragma unroll
     for (int e = 0; e < kCopyPieces; e++)
