@@ -5,6 +5,7 @@
 // All of it moves bytes: a page holds, for each head, page x Dp codes of keys
 // [token][dim] and as many of values [dim][token] (the order in which the
 // attention's two products read them), and one fp32 scale of each.
+#include <algorithm>
 #include <type_traits>
 
 #include "zt_kv8.h"
@@ -250,7 +251,9 @@ struct AppendArgs {
     int lanes;      // that share a key for that
     int tokens;
     int windows;  // of 64 tokens
-    int turns;    // workgroups that the pages which 64 tokens begin are dealt out to, for one head of keys or of values
+    // workgroups that a window's pages are dealt out to, for one head of keys or of values; where that is one, it takes the
+    // first `first` of them, and `helpers` share the further ones of every groups-th window
+    int turns, first, groups, helpers;
     long blocks;
 };
 
@@ -269,7 +272,7 @@ struct Run {
 // A run's tokens into their page: its new scale, and its codes by way of an image
 // of it in LDS.
 template <class T, int V, bool VALUES, bool NORM, Pairs P>
-__device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run, int head, uint32_t* image, float* red, float* factors) {
+__device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run, int head, int tid, uint32_t* image, float* red, float* factors) {
     const Kv8& c = g.c;
     const Rows& x = g.x[VALUES];
     Turn turn = g.turn;
@@ -302,7 +305,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run,
     constexpr int N = kHeadUnits<V>, kHeld = NORM ? 2 : 1;
     float ha[kHeld][N][V], hb[kHeld][N][V];
     int first_of[N], second_of[N];
-    const int l = NORM ? threadIdx.x & (g.lanes - 1) : 0, at_once = NORM ? kThreads / g.lanes : 1, mine = NORM ? threadIdx.x / g.lanes : 0;
+    const int shift = NORM ? __builtin_ctz(g.lanes) : 0, l = tid & ((1 << shift) - 1), at_once = kThreads >> shift, mine = tid >> shift;
     if constexpr (NORM) {
         float w[N][2][V];
         for (int i0 = mine; i0 < n + mine; i0 += kHeld * at_once) {
@@ -340,7 +343,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run,
             }
         }
     } else {
-        for (int i = threadIdx.x; i < n * units; i += kThreads) {
+        for (int i = tid; i < n * units; i += kThreads) {
             const int tl = i / units, u = i - tl * units;
             float a[V], b[V];
             int first, second;
@@ -363,7 +366,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run,
     auto piece = [&](int i) { return whole ? i : run.dense ? run.off * row + i : run.place(i / row) * row + i % row; };
     const float ratio = grown ? had / now : 0.0f;
     if (grown && !fresh) {
-        for (int i = threadIdx.x; i < pieces; i += kThreads) {
+        for (int i = tid; i < pieces; i += kThreads) {
             u32x4 w = codes[i];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -376,7 +379,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run,
             image4[i] = w;
         }
     } else if (whole || !VALUES) {  // zeros where nothing new comes; of a page that goes on, its new keys' rows
-        for (int i = threadIdx.x; i < pieces; i += kThreads) image4[piece(i)] = (u32x4){0, 0, 0, 0};
+        for (int i = tid; i < pieces; i += kThreads) image4[piece(i)] = (u32x4){0, 0, 0, 0};
     }
     __syncthreads();  // (the scale has been read by everybody, too)
 
@@ -403,7 +406,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run,
                 if (mine + e * at_once < n && l + k * g.lanes < units)
                     write(run.place(mine + e * at_once), ha[e][k], hb[e][k], first_of[k], second_of[k]);
     } else {
-        for (int i = threadIdx.x; i < n * units; i += kThreads) {
+        for (int i = tid; i < n * units; i += kThreads) {
             const int tl = i / units, u = i - tl * units;
             float a[V], b[V];
             int first, second;
@@ -414,15 +417,15 @@ __device__ __forceinline__ void append_page(const AppendArgs& g, const Run& run,
     __syncthreads();
 
     if (whole || !VALUES) {
-        for (int i = threadIdx.x; i < pieces; i += kThreads) codes[piece(i)] = image4[piece(i)];
+        for (int i = tid; i < pieces; i += kThreads) codes[piece(i)] = image4[piece(i)];
     } else {
         int8_t* out = reinterpret_cast<int8_t*>(codes);
-        for (int i = threadIdx.x; i < c.dim * n; i += kThreads) {
+        for (int i = tid; i < c.dim * n; i += kThreads) {
             const int d = i / n, to = d * c.page + run.place(i - d * n);
             out[to] = bytes[to];
         }
     }
-    if (threadIdx.x == 0) scales[at] = now;
+    if (tid == 0) scales[at] = now;
     __syncthreads();  // the image is free again
 }
 
@@ -441,9 +444,9 @@ struct Found {
 
 // The tokens on the page of token t, whose slot is s: up to the first that is on
 // another page, without those that are left out.
-__device__ __forceinline__ Run run_from(const AppendArgs& g, int t, long s, Found& found, int* listed, uint8_t* places) {
+__device__ __forceinline__ Run run_from(const AppendArgs& g, int t, long s, int tid, Found& found, int* listed, uint8_t* places) {
     const Kv8& c = g.c;
-    const int tid = threadIdx.x, left = g.tokens - t;
+    const int left = g.tokens - t;
     Run run{t, 0, (int)(s >> c.shift), (int)(s & (c.page - 1)), false, true, listed, places};
     const int most = min(c.page - run.off, left);
     if (tid == 0) found = {most, left, 0, 0, 0};
@@ -496,6 +499,15 @@ __device__ __forceinline__ Run run_from(const AppendArgs& g, int t, long s, Foun
     return run;
 }
 
+// What a workgroup helps with, of each of its waves: the tokens that begin pages, and their slots.  A wave looks at kLooks
+// windows at a time, and has a helper's part of each one's at most 64 pages.
+constexpr int kLooks = 4;
+struct Jobs {
+    long slot[4][16 * kLooks];
+    int token[4][16 * kLooks];
+    int n[4];
+};
+
 // A page's scale s' = max(s, amax / 127), its codes rint(c s / s') where it grew,
 // new ones rint(x / s'): one workgroup has a page of one head, keys or values,
 // whole, since all of its codes wait for one maximum.  It reads its new rows
@@ -503,22 +515,26 @@ __device__ __forceinline__ Run run_from(const AppendArgs& g, int t, long s, Foun
 // lie token-minor, and go out as whole 16 bytes instead of one byte a line.
 // No atomics on memory, and no order among workgroups.
 //
-// A workgroup looks at 64 tokens: those whose page is not that of the one before
-// (tokens that are left out do not come between) begin a page's tokens.  It takes
-// every turns-th of them, each with all that follow on its page.  q's rotation
-// rides along as more workgroups, instead of a launch of its own.
+// A workgroup looks at a window of 64 tokens: those whose page is not that of the
+// one before (tokens that are left out do not come between) begin a page's tokens.
+// It takes every turns-th of them, each with all that follow on its page; or
+// (HELP) the first few, and the first workgroups also take their part of what
+// crowded windows have besides: of one that others share too, page i of window k of
+// the group is helper (61 k + i) % helpers', which spreads them evenly, whatever
+// their number in a window.  q's rotation rides along as more workgroups, instead
+// of a launch of its own.
 //
 // One token for each of 64 sequences (8 heads of 128, pages of 64, fp32): 10.3
 // us, where a page that grows is read and written; a workgroup waits for its
 // slots, its rows, their largest, the scale and the codes one after the other.
-// Prompts of 1955 tokens in all (fp16, 32 + 8 heads of 128, pages of 16): 16.2 us.
+// Prompts of 1955 tokens in all (fp16, 32 + 8 heads of 128, pages of 16): 18.5 us.
 //
 // Normed keys: a row is dealt out to lanes that share its sum of squares, two
 // rows at a time (four: 3218 tokens of prompts 30.4 us instead of 31.0, but 48
 // sequences' tokens 12.0 instead of 10.3, for code that most of them skip).  A run
 // that is as short as that stays in registers, others' factors are kept in LDS
 // for the second reading.
-template <class T, int V, int VQ, class Q, Pairs P>
+template <class T, int V, int VQ, class Q, Pairs P, bool HELP>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, Q q) {
     constexpr bool NORM = std::is_same_v<Q, NormArgs>;
     extern __shared__ __align__(16) uint32_t image[];  // of one page and head
@@ -538,32 +554,114 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, Q q) {
     int b = blockIdx.x;
     const int values = b & 1, head = (b >> 1) % c.heads;
     b = (b >> 1) / c.heads;
-    const int turn = b / g.windows, from = (b - turn * g.windows) * 64, lane = threadIdx.x & 63;
+    int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    auto lower = [&](uint64_t bits) { return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(bits >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bits, 0)); };  // of lanes before this one
     auto slot = [&](long t) { return t >= 0 && t < g.tokens ? g.slots[t] : -1l; };
-    const long here = slot(from + lane), behind = slot((long)from - 1 - lane);
-    const int page = page_of(c, here);
-    const uint64_t stored = __ballot(page >= 0);
-    if (!stored) return;
-    // the page of the last token before these that is stored
-    int last = page_of(c, behind);
-    uint64_t any = __ballot(last >= 0);
-    for (long t = (long)from - 65; !any && t >= 0; t -= 64) {
-        last = page_of(c, slot(t - lane));
-        any = __ballot(last >= 0);
-    }
-    last = any ? __shfl(last, __builtin_ctzll(any)) : -1;
-    const uint64_t below = stored & ((1ull << lane) - 1);
-    const int before = __shfl(page, below ? 63 - __builtin_clzll(below) : lane);
-    uint64_t begin = __ballot(page >= 0 && page != (below ? before : last));
-    for (int left = turn; begin; begin &= begin - 1) {
-        if (left-- > 0) continue;
-        left = g.turns - 1;
-        const int i = __builtin_ctzll(begin);
-        const Run run = run_from(g, from + i, __shfl(here, i), found, listed, places);
+    // of 64 tokens, whose slots are `here` (and `before` that of the one before them), those that begin a page and are wanted
+    // by that page's number among these
+    auto begun = [&](long from, long here, long before, auto wanted) __attribute__((always_inline)) {
+        const int page = page_of(c, here);
+        const uint64_t stored = __ballot(page >= 0), below = stored & ((1ull << lane) - 1);
+        if (!stored) return (uint64_t)0;
+        int last = page_of(c, before);  // the page of the last token before these that is stored
+        for (long t = from - 2; last < 0 && t >= 0; t -= 64) {
+            const int p = page_of(c, slot(t - lane));
+            const uint64_t any = __ballot(p >= 0);
+            if (any) last = __shfl(p, __builtin_ctzll(any));
+        }
+        const int prior = __shfl(page, below ? 63 - __builtin_clzll(below) : lane);
+        const bool begins = page >= 0 && page != (below ? prior : last);
+        const int i = lower(__ballot(begins));
+        return (uint64_t)__ballot(begins && wanted(i));
+    };
+    auto append = [&](int t, long s) __attribute__((always_inline)) {
+        int tid = threadIdx.x;
+        // (worked out for each page, not held in registers meanwhile: eight waves a SIMD instead of seven; normed keys', which
+        // have more to work out, are four anyway)
+        if constexpr (!NORM) asm volatile("" : "+v"(tid));
+        const Run run = run_from(g, t, s, tid, found, listed, places);
         if (values)
-            append_page<T, V, true, false, P>(g, run, head, image, red, factors);
+            append_page<T, V, true, false, P>(g, run, head, tid, image, red, factors);
         else
-            append_page<T, V, false, NORM, P>(g, run, head, image, red, factors);
+            append_page<T, V, false, NORM, P>(g, run, head, tid, image, red, factors);
+    };
+    if constexpr (!HELP) {
+        const int turn = b / g.windows, from = (b - turn * g.windows) * 64;
+        const long here = slot(from + lane), behind = slot((long)from - 1);
+        uint64_t todo = begun(from, here, behind, [&](int) { return true; });
+        for (int left = turn; todo; todo &= todo - 1) {
+            if (left-- > 0) continue;
+            left = g.turns - 1;
+            const int i = __builtin_ctzll(todo);
+            append(from + i, __shfl(here, i));
+        }
+    } else {
+        __shared__ Jobs jobs;
+        const long own = b < g.windows ? 64l * b : -64;
+        const long here = slot(own + lane), behind = slot(own - 1);
+        int group = 0, help = 0, count = 0;  // the windows that it helps with
+        if (b < g.groups * g.helpers) {
+            help = b / g.groups;
+            group = b - help * g.groups;
+            count = (g.windows - group + g.groups - 1) / g.groups;
+        }
+        uint64_t todo = 0;
+        for (int k0 = 0;; k0 += 4 * kLooks) {
+            asm volatile("" : "+v"(lane));  // (what depends on it is worked out here, not held in registers while pages are written)
+            auto from = [&](int e) { return 64l * (group + (long)(k0 + kLooks * wave + e) * g.groups); };
+            long x[kLooks];
+            if (k0 < count) {
+#pragma unroll
+                for (int e = 0; e < kLooks; e++) x[e] = slot(from(e) + lane);
+            }
+            if (k0 == 0) todo = begun(own, here, behind, [&](int i) { return i < g.first; });
+            int w = 4, n = 0;
+            if (k0 < count) {
+                uint32_t more = 0;  // windows with more than `first` tokens that are not on the page of the one before
+#pragma unroll
+                for (int e = 0; e < kLooks; e++) {
+                    const int page = page_of(c, x[e]), before = __shfl_up(page, 1);
+                    if (__builtin_popcountll(__ballot(page >= 0 && (lane == 0 || page != before))) > g.first) more |= 1u << e;
+                }
+                for (; more; more &= more - 1) {
+                    const int e = __builtin_ctz(more);
+                    const uint32_t k = k0 + kLooks * wave + e;
+                    const long at = slot(from(e) + lane);
+                    const uint64_t all = begun(from(e), at, slot(from(e) - 1), [&](int i) { return i >= g.first && (61 * k + i) % (uint32_t)g.helpers == (uint32_t)help; });
+                    if (all >> lane & 1) {
+                        const int j = n + lower(all);
+                        jobs.token[wave][j] = (int)from(e) + lane;
+                        jobs.slot[wave][j] = at;
+                    }
+                    n += __builtin_popcountll(all);
+                }
+                if (lane == 0) jobs.n[wave] = n;
+                __syncthreads();
+                w = n = 0;
+            }
+            for (;;) {
+                int t;
+                long s;
+                if (todo) {
+                    const int i = __builtin_ctzll(todo);
+                    todo &= todo - 1;
+                    t = (int)own + i;
+                    s = __shfl(here, i);
+                } else {
+                    while (w < 4 && n == __builtin_amdgcn_readfirstlane(jobs.n[w])) {
+                        w++;
+                        n = 0;
+                    }
+                    if (w == 4) break;
+                    t = __builtin_amdgcn_readfirstlane(jobs.token[w][n]);
+                    s = jobs.slot[w][n++];
+                }
+                append(t, (long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(s >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)s)));
+            }
+            if (k0 + 4 * kLooks >= count) break;
+            __syncthreads();  // nobody reads the list any more
+        }
     }
 }
 
@@ -574,16 +672,20 @@ static int launch_append(const AppendArgs& g, const Q& q, long blocks, int type,
     if (blocks >= 1l << 31) return kInvalid;
     const int lds = g.c.bytes();
     auto run = [&](auto kernel) { kernel<<<blocks, kThreads, lds, stream>>>(g, q); };
-    if (type == ZT_F32) {
-        if (width == 4)
-            q_width == 4 ? run(append_kernel<float, 4, 4, Q, P>) : run(append_kernel<float, 4, 1, Q, P>);
-        else
-            q_width == 4 ? run(append_kernel<float, 1, 4, Q, P>) : run(append_kernel<float, 1, 1, Q, P>);
-    } else if (width == 4) {
-        q_width == 8 ? run(append_kernel<_Float16, 4, 8, Q, P>) : q_width == 4 ? run(append_kernel<_Float16, 4, 4, Q, P>) : run(append_kernel<_Float16, 4, 1, Q, P>);
-    } else {
-        q_width == 8 ? run(append_kernel<_Float16, 1, 8, Q, P>) : q_width == 4 ? run(append_kernel<_Float16, 1, 4, Q, P>) : run(append_kernel<_Float16, 1, 1, Q, P>);
-    }
+    auto with = [&](auto help) {
+        constexpr bool H = decltype(help)::value;
+        if (type == ZT_F32) {
+            if (width == 4)
+                q_width == 4 ? run(append_kernel<float, 4, 4, Q, P, H>) : run(append_kernel<float, 4, 1, Q, P, H>);
+            else
+                q_width == 4 ? run(append_kernel<float, 1, 4, Q, P, H>) : run(append_kernel<float, 1, 1, Q, P, H>);
+        } else if (width == 4) {
+            q_width == 8 ? run(append_kernel<_Float16, 4, 8, Q, P, H>) : q_width == 4 ? run(append_kernel<_Float16, 4, 4, Q, P, H>) : run(append_kernel<_Float16, 4, 1, Q, P, H>);
+        } else {
+            q_width == 8 ? run(append_kernel<_Float16, 1, 8, Q, P, H>) : q_width == 4 ? run(append_kernel<_Float16, 1, 4, Q, P, H>) : run(append_kernel<_Float16, 1, 1, Q, P, H>);
+        }
+    };
+    g.helpers ? with(std::true_type{}) : with(std::false_type{});
     return (int)hipGetLastError();
 }
 
@@ -615,17 +717,25 @@ static int append(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v,
     g.turn = {positions, table, half, max_pos, flags};
     g.tokens = tokens;
     g.windows = ceil_div(tokens, 64);
-    // a workgroup for each token while they are few (a batch's next tokens, each on a page of its own: with the pages'
-    // values read back, 64 sequences 28 us, with 8 workgroups for 64 tokens 45), else as many as give each CU four, and no
-    // fewer than pages that 64 tokens of one sequence begin.  One that finds none to do costs its launch and its look at
-    // 64 slots: all the first ones come first, so that they are spread over the CUs, the idle ones behind them, q last (fp16,
-    // with q, four heads for each of keys, pages of 64; us with these and with 8 in turn for each 64 tokens: 8 heads, a prompt
-    // of 16000 tokens 93 and 166, of 1955 15.5 and 24.7, 300 sequences' single tokens 25 and 33, 2048 135 and 127, where four
-    // times as many take 121 but prompts of 1955 on pages of 16 18.6 instead of 16.2; 2 heads, 26 and 91, 10.4 and 16.2, 12 and
-    // 29, 34 and 37)
-    const long wide = 1024 / (2l * cache->kv_heads * g.windows), most = tokens <= 256 ? 64 : 32;
-    g.turns = tokens <= 256 || wide > most ? most : max((int)wide, max(64 / g.c.page, 1));
-    g.blocks = 2l * cache->kv_heads * g.windows * g.turns;
+    // A workgroup for each token while they are few (a batch's next tokens, each on a page of its own: with the pages'
+    // values read back, 64 sequences 28 us, with 8 workgroups for 64 tokens 45), then as many as give each CU four, at
+    // least eight for 64 tokens (2048 sequences' single tokens, 8 heads, pages of 16: 92 us, with four 105).  One that finds
+    // none to do costs its launch and its look at 64 slots, and prompts begin few pages.  So where eight for each 64 tokens
+    // are more than twice what the card holds at a time, there is one, which takes the pages that a prompt begins there, and
+    // as many as are surely at work at a time share the others (fp16, with q, four heads for each of keys, pages of 64; us
+    // with these, with eight in any case, and with one alone: 8 heads, a prompt of 16000 tokens 97, 131 and 94; 8192
+    // sequences' single tokens 492, 492 and 614; 300 of them before a prompt of 8000 58, 84 and 200).
+    const long pairs = 2l * cache->kv_heads, held = norm ? 1024 : 2048;  // (at work at a time)
+    g.turns = tokens <= 256 ? 64 : 8 * pairs * g.windows > 2 * held ? 1 : (int)std::min(32l, std::max(8l, 1024 / (pairs * g.windows)));
+    if (g.turns == 1) {
+        g.first = std::max(64 / g.c.page + 1, 4);
+        // (4096 single tokens 255 us; with 1792 of them, some of which begin when others have ended, 349)
+        const int all = std::max(8, (norm ? 1024 : 1536) / (int)pairs);
+        // enough groups for one look at each one's windows, and for all helpers; at least six of these in each
+        g.groups = std::min({g.windows, all / 6, std::max(ceil_div(g.windows, 4 * kLooks), ceil_div(all, 64))});
+        g.helpers = std::min(64, all / g.groups);
+    }
+    g.blocks = pairs * std::max((long)g.windows * g.turns, (long)g.groups * g.helpers);
     RopeArgs r{};
     r.turn = g.turn;
     r.tokens = tokens;
