@@ -824,6 +824,13 @@ int zt_kv8_attention(const zt_kv8_attn* a, void* workspace, long workspace_bytes
 int zt_kv8_tree(const int* parents, const int* kv_lens, const int* q_start, int requests, int tokens, int words,
                 int* positions, uint64_t* mask, zt_stream_t stream);
 
+/* The same for attention with a window (above 0; 0: as above): of the rows above a
+ * row those window or more steps up have no bit.  With these masks and the same
+ * window zt_kv8_tree_attention gives each row what zt_kv8_attention gives it where
+ * its path is all that follows the context. */
+int zt_kv8_tree_window(const int* parents, const int* kv_lens, const int* q_start, int requests, int tokens, int words,
+                       int window, int* positions, uint64_t* mask, zt_stream_t stream);
+
 /* The same for the rows of a drafted tree, which are not in a line.  A request's
  * n rows stand behind its context, the first kv_lens[r] - n tokens.  Row i sees
  * the context and, of the request's own rows, row j where bit j % 64 of word
@@ -832,7 +839,8 @@ int zt_kv8_tree(const int* parents, const int* kv_lens, const int* q_start, int 
  * ignored, and a row from 64 words on is seen by none.  With window > 0 it sees,
  * of the context, the last tokens from position - window + 1 on, where its
  * position is the context's length and the rows that it sees, less one; its own
- * request's rows are seen as the mask says.  mask: [tokens][words] on the device,
+ * request's rows are seen as the mask says, however far up (zt_kv8_tree_window's
+ * masks leave out those that the window does).  mask: [tokens][words] on the device,
  * 8-byte aligned, words from 1 to ZT_TREE_WORDS, else InvalidValue.  Workspace:
  * zt_kv8_tree_attention_workspace_bytes, as above. */
 long zt_kv8_tree_attention_workspace_bytes(const zt_kv8_attn* a);

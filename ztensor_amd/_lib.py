@@ -141,6 +141,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "zt_kv8_attention_workspace_bytes": (L, [P]),
     "zt_kv8_attention": (I, [P, P, L, P]),
     "zt_kv8_tree": (I, [P, P, P, I, I, I, P, P, P]),
+    "zt_kv8_tree_window": (I, [P, P, P, I, I, I, I, P, P, P]),
     "zt_tree_accept": (I, [P, P, P, P, P, I, I, P, P, P, P, P]),
     "zt_kv8_compact": (I, [P, I, P, I, I, P, P, P, P, I, P, P]),
     "zt_kv8_copy": (I, [P, I, P, P, I, P]),

@@ -39,7 +39,7 @@ __device__ __forceinline__ void rows_of_none(const int* q_start, int requests, i
 
 struct TreeArgs {
     const int *parents, *kv_lens, *q_start;
-    int requests, tokens, words;
+    int requests, tokens, words, window;  // window: rows that a row sees, itself and those right above it (0: all)
     int* positions;
     uint64_t* mask;
 };
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(kThreads) void tree_kernel(TreeArgs g) {
                 out[w] = bits;
                 bits = 0;
             }
-            if (x == w) bits |= 1ull << (at & 63);
+            if (x == w && (g.window == 0 || depth < g.window)) bits |= 1ull << (at & 63);
             at = parent_of(at < kNear ? near[at] : parents[at], at);
         }
         for (; w >= 0; w--) {
@@ -606,9 +606,9 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(ForkArgs g) {
 
 using namespace zt;
 
-ZT_EXPORT int zt_kv8_tree(const int* parents, const int* kv_lens, const int* q_start, int requests, int tokens, int words,
-                          int* positions, uint64_t* mask, zt_stream_t stream) {
-    if (requests < 0 || requests >= 1 << 24 || tokens < 0 || words < 1 || words > ZT_TREE_WORDS || !q_start) return kInvalid;
+ZT_EXPORT int zt_kv8_tree_window(const int* parents, const int* kv_lens, const int* q_start, int requests, int tokens, int words,
+                                 int window, int* positions, uint64_t* mask, zt_stream_t stream) {
+    if (requests < 0 || requests >= 1 << 24 || tokens < 0 || words < 1 || words > ZT_TREE_WORDS || window < 0 || !q_start) return kInvalid;
     if (tokens == 0) return 0;
     if (!parents || !positions || !mask || (requests && !kv_lens) ||
         (((uintptr_t)parents | (uintptr_t)kv_lens | (uintptr_t)q_start | (uintptr_t)positions) & 3) || ((uintptr_t)mask & 7))
@@ -616,8 +616,13 @@ ZT_EXPORT int zt_kv8_tree(const int* parents, const int* kv_lens, const int* q_s
     const Bytes in[] = {{parents, 4l * tokens}, {kv_lens, 4l * requests}, {q_start, 4l * requests + 4}};
     const Bytes out[] = {{positions, 4l * tokens}, {mask, 8l * tokens * words}};
     if (!apart(in, out)) return kInvalid;
-    tree_kernel<<<requests + 1, kThreads, 0, stream>>>({parents, kv_lens, q_start, requests, tokens, words, positions, mask});
+    tree_kernel<<<requests + 1, kThreads, 0, stream>>>({parents, kv_lens, q_start, requests, tokens, words, window, positions, mask});
     return (int)hipGetLastError();
+}
+
+ZT_EXPORT int zt_kv8_tree(const int* parents, const int* kv_lens, const int* q_start, int requests, int tokens, int words,
+                          int* positions, uint64_t* mask, zt_stream_t stream) {
+    return zt_kv8_tree_window(parents, kv_lens, q_start, requests, tokens, words, 0, positions, mask, stream);
 }
 
 ZT_EXPORT int zt_tree_accept(const long* drafted, const long* drawn, const int* parents, const int* q_start,

@@ -5,7 +5,7 @@ row is the token that it stands at, the others are drafts that continue an
 earlier row of it (its parent).  With `held` the lengths before the step:
 
     p = engine.kv8_plan(held, new, block_table, free_pages, free_count, page_tokens, tokens)
-    t = engine.kv8_tree(parents, p.kv_lens, p.q_start, max_q)
+    t = engine.kv8_tree(parents, p.kv_lens, p.q_start, max_q)  # (window= for a model that has one, here and in the attention)
     for each layer:
         q = engine.kv8_append(k, v, cache, p.slots, positions=t.positions, table=rope, q=q)
         a = engine.kv8_tree_attention(q, cache, p.block_table, p.kv_lens, p.q_start, t.mask, max_q=..., max_kv=...)
@@ -93,13 +93,15 @@ class DraftOps(DecodeOps):
         return b"".join(packed), len(packed)
 
     @_on_engine_stream
-    def kv8_tree(self, parents: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.Tensor, max_q: int) -> KV8Tree:
+    def kv8_tree(self, parents: torch.Tensor, kv_lens: torch.Tensor, q_start: torch.Tensor, max_q: int, *,
+                 window: int = 0) -> KV8Tree:
         """Positions and masks of a step's trees.  parents (int32 [tokens]): the
         row of its request that a row continues, counted from the request's
         first row and before it (else, -1 for instance, the context).  kv_lens
         and q_start: kv8_plan's, the step's tokens included.  max_q, at most
         1024: a bound of the rows of one request; a row that is past the mask's
-        words (64 rows each) is seen by none."""
+        words (64 rows each) is seen by none.  window: the attention's; rows
+        that many steps above a row, or more, are not in its mask."""
         tokens, r, i32 = parents.shape[0], kv_lens.shape[0], torch.int32
         words = max(1, -(-max_q // 64))
         dense = self._dense
@@ -107,7 +109,7 @@ class DraftOps(DecodeOps):
                 dense(q_start, "q_start", i32, (r + 1,)), r, tokens, words)
         positions = torch.empty(tokens, dtype=i32, device=self.device)
         mask = torch.empty((tokens, words), dtype=torch.int64, device=self.device)
-        self.lib.call("zt_kv8_tree", *args, positions.data_ptr(), mask.data_ptr(), self._s)
+        self.lib.call("zt_kv8_tree_window", *args, window, positions.data_ptr(), mask.data_ptr(), self._s)
         return KV8Tree(positions, mask)
 
     @_on_engine_stream
@@ -120,7 +122,8 @@ class DraftOps(DecodeOps):
         rows, row j where bit j % 64 of mask[i, j // 64] is set (int64 [tokens,
         words]; kv8_tree's, or any other).  window > 0: of the context the
         tokens after position - window, its position being the context's length
-        and the rows that it sees, less one.  A row that sees nothing is zeros."""
+        and the rows that it sees, less one; of the request's rows what the mask
+        has (give kv8_tree the same window).  A row that sees nothing is zeros."""
         if out is None:
             out = _like(q)
         elif out.shape != q.shape:
