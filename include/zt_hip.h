@@ -904,8 +904,8 @@ int zt_kv8_trim(const int* kv_lens, const int* keep, const int* table, int reque
  * its row all -1; so does one whose source is outside the table or holds nothing,
  * or more than its row.  The other rows, and a row forked from itself, stay as
  * they are.  A row's old pages are not given back (zt_kv8_trim does that, before
- * this or after it with the table as it was), and
- * each row is a target once at most.  `pages`: the entries of free_pages and refs.
+ * this or after it with the table as it was).  Of forks that have one target the
+ * first is done, the others are nothing.  `pages`: the entries of free_pages and refs.
  * Outputs (refs among them) share no bytes with inputs nor with each other, else
  * InvalidValue. */
 typedef struct zt_kv8_fork_call {

@@ -544,46 +544,65 @@ __device__ __forceinline__ Forked forked(const ForkArgs& g, int i) {
 
 // Workgroup r: row r of the table, which is a fork's or stays.  How many forks
 // before it take a page it counts by itself, as the step's plan does: loads that
-// wait for each other, no second launch.  4 forks of 500 tokens 4.2 us, 160 of
-// 1500 6.4.
+// wait for each other, no second launch.  A fork whose target an earlier one has
+// takes none; whether there may be any, a bit of LDS for each row says (past 2^18
+// rows two may share one: then the earlier forks are looked through for nothing).
+// 4 forks of 500 tokens 4.2 us, 160 of 1500 6.4.
+constexpr int kMet = 1 << 18;  // rows that have bits of their own
 __global__ __launch_bounds__(kThreads) void fork_kernel(ForkArgs g) {
-    __shared__ int chosen, wanted;
+    extern __shared__ uint32_t met[];  // of min(rows, kMet) bits
+    __shared__ int chosen, wanted, twice;
     const int r = blockIdx.x, free = min(max(0, *g.a.free_count), g.a.pages);
     if (threadIdx.x == 0) {
-        chosen = g.a.n;
-        wanted = 0;
+        chosen = r == g.a.rows ? 0 : g.a.n;
+        wanted = twice = 0;
     }
     __syncthreads();
-    if (r == g.a.rows) {
-        int mine = 0;
-        for (int i = threadIdx.x; i < g.a.n; i += kThreads) {
-            mine += forked(g, i).part;
-            if ((unsigned)g.a.target[i] >= (unsigned)g.a.rows) g.a.copy_from[i] = g.a.copy_to[i] = -1;
-        }
-        atomicAdd(&wanted, mine);
-        __syncthreads();
-        if (threadIdx.x == 0) *g.a.free_count_out = free - min(free, wanted);
-        return;
-    }
-    for (int i = threadIdx.x; i < g.a.n; i += kThreads)
-        if (g.a.target[i] == r) atomicMin(&chosen, i);
+    if (r < g.a.rows)
+        for (int i = threadIdx.x; i < g.a.n; i += kThreads)
+            if (g.a.target[i] == r) atomicMin(&chosen, i);
     __syncthreads();
     const int i = chosen;
     const int* row = g.a.table + (long)r * g.a.width;
     int* out = g.a.table_out + (long)r * g.a.width;
-    const bool itself = i < g.a.n && g.a.source[i] == r;
-    for (int k = threadIdx.x; k < g.a.n; k += kThreads)  // (a row that comes twice: the first of them)
-        if (g.a.target[k] == r && (k != i || itself)) g.a.copy_from[k] = g.a.copy_to[k] = -1;
-    if (i >= g.a.n || itself) {
-        for (int j = threadIdx.x; j < g.a.width; j += kThreads) out[j] = row[j];
-        if (threadIdx.x == 0) g.a.kv_lens_out[r] = g.a.kv_lens[r];
+    const bool itself = r < g.a.rows && i < g.a.n && g.a.source[i] == r;
+    if (r < g.a.rows) {
+        for (int k = threadIdx.x; k < g.a.n; k += kThreads)  // (a row that comes twice: the first of them)
+            if (g.a.target[k] == r && (k != i || itself)) g.a.copy_from[k] = g.a.copy_to[k] = -1;
+        if (i >= g.a.n || itself) {
+            for (int j = threadIdx.x; j < g.a.width; j += kThreads) out[j] = row[j];
+            if (threadIdx.x == 0) g.a.kv_lens_out[r] = g.a.kv_lens[r];
+            return;
+        }
+    }
+    // the pages that forks before this one take, or (of no row) all
+    const int n = r < g.a.rows ? i : g.a.n;
+    for (int k = threadIdx.x; 32 * k < min(g.a.rows, kMet); k += kThreads) met[k] = 0;
+    __syncthreads();
+    int mine = 0;
+    for (int k = threadIdx.x; k < n; k += kThreads) {
+        mine += forked(g, k).part;
+        const int t = g.a.target[k];
+        if ((unsigned)t < (unsigned)g.a.rows && atomicOr(&met[t % kMet / 32], 1u << (t & 31)) >> (t & 31) & 1) twice = 1;
+    }
+    __syncthreads();
+    if (twice) {
+        mine = 0;
+        for (int k = threadIdx.x; k < n; k += kThreads) {
+            bool first = forked(g, k).part;
+            for (int e = 0; e < k && first; e++) first = g.a.target[e] != g.a.target[k];
+            mine += first;
+        }
+    }
+    if (mine) atomicAdd(&wanted, mine);
+    __syncthreads();
+    if (r == g.a.rows) {
+        for (int k = threadIdx.x; k < n; k += kThreads)
+            if ((unsigned)g.a.target[k] >= (unsigned)g.a.rows) g.a.copy_from[k] = g.a.copy_to[k] = -1;
+        if (threadIdx.x == 0) *g.a.free_count_out = free - min(free, wanted);
         return;
     }
     const Forked f = forked(g, i);
-    int mine = 0;
-    for (int k = threadIdx.x; k < i; k += kThreads) mine += forked(g, k).part;
-    if (mine) atomicAdd(&wanted, mine);
-    __syncthreads();
     const bool done = f.held > 0 && (!f.part || wanted < free);
     const int full = f.held >> g.shift, fresh = done && f.part ? g.a.free_pages[free - 1 - wanted] : -1;
     const int* from = g.a.table + (long)(f.held ? f.source : r) * g.a.width;
@@ -745,6 +764,6 @@ ZT_EXPORT int zt_kv8_fork(const zt_kv8_fork_call* a, zt_stream_t stream) {
     const Bytes in[] = {{a->source, forks}, {a->target, forks}, {a->kv_lens, row}, {a->table, row * a->width}, {a->free_pages, list}, {a->free_count, 4}};
     const Bytes out[] = {{a->refs, list}, {a->kv_lens_out, row}, {a->table_out, row * a->width}, {a->free_count_out, 4}, {a->copy_from, forks}, {a->copy_to, forks}};
     if (!apart(in, out)) return kInvalid;
-    fork_kernel<<<a->rows + 1, kThreads, 0, stream>>>({*a, __builtin_ctz(a->page_tokens)});
+    fork_kernel<<<a->rows + 1, kThreads, (std::min(a->rows, kMet) + 31) / 32 * 4, stream>>>({*a, __builtin_ctz(a->page_tokens)});
     return (int)hipGetLastError();
 }

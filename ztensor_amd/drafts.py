@@ -222,7 +222,8 @@ class DraftOps(DecodeOps):
     def kv8_fork(self, source: torch.Tensor, target: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
                  refs: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor, page_tokens: int) -> KV8Fork:
         """Row target[i] of block_table goes on from what row source[i] holds
-        before the call (int32 [forks] both; each target once).  Full pages are
+        before the call (int32 [forks] both; of forks with one target the first
+        is done, the others are nothing).  Full pages are
         shared (refs, int32 [pages], one more, in place); a last page that is
         not full gets a page of its own, and copy_from / copy_to are what
         kv8_copy is to do for it.  A fork that finds no free page gets length 0.
