@@ -1298,8 +1298,8 @@ static AttnPlan attn_plan(const zt_kv8_attn* a, bool tree) {
     const long few = tree ? 16 : 64;
     p.most = most <= few ? 0x7FFFFFFF : (int)few;
     // of more than 16 rows two columns of them share what is read of a tile (those requests, 32 rows: 66 us, one by one
-    // 80); past 128 dims their sums would leave no registers
-    p.ct = most > 16 && dp <= 128 ? 2 : 1;
+    // 80); past 128 dims their sums would leave no registers; a tree's rows are one column here, others the tiled kernel's
+    p.ct = most > 16 && dp <= 128 && !tree ? 2 : 1;
     long kv = std::min((long)a->max_kv, (long)a->width * a->cache.page_tokens);
     if (a->window > 0) kv = std::min(kv, (long)a->window + a->max_q + 63);
     const long tiles = std::max(1l, (kv + 63) / 64);
