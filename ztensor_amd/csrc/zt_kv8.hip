@@ -6,6 +6,7 @@
 // [token][dim] and as many of values [dim][token] (the order in which the
 // attention's two products read them), and one fp32 scale of each.
 #include <algorithm>
+#include <limits>
 #include <type_traits>
 
 #include "zt_kv8.h"
@@ -148,7 +149,7 @@ __host__ inline long norm_blocks(NormArgs& g, int n, int V) {
 }
 
 __host__ inline bool norm_ok(const zt_head_norm* n) {
-    return n && n->eps > 0 && n->eps <= 1e30 && (((uintptr_t)n->q | (uintptr_t)n->k) & 3) == 0;
+    return n && n->eps > 0 && n->eps <= std::numeric_limits<double>::max() && (((uintptr_t)n->q | (uintptr_t)n->k) & 3) == 0;
 }
 
 }  // namespace zt
