@@ -81,3 +81,23 @@ def test_pages_that_others_write(eng, name, dtype, page, norm):  # noqa: F811
     one.append([x[:, h:h + 1].float().cpu().numpy() for x in (k, v)], slots.tolist())
     for x, y in zip(cache, one.device(torch)):
         assert torch.equal(x[:, h:h + 1], y)
+
+
+@pytest.mark.parametrize("heads", [1, 12, 64])
+@pytest.mark.parametrize("lens", [[1] * 20, [1] * 64, [1] * 65, [1] * 100, [1] * 129, [1] * 200, [1] * 256, [1] * 300, [65], [130], [300], [60, 1, 1, 3, 70],
+                                  [1] * 60 + [140], [7] * 31], ids=lambda x: f"{len(x)} of {sum(x)}")
+def test_last_windows_of_few_tokens(eng, lens, heads):  # noqa: F811
+    """A last window of fewer tokens than others has workgroups: all pages are somebody's."""
+    rng = np.random.default_rng(heads + sum(lens))
+    page, need = 16, [-(-n // 16) for n in lens]
+    order, slots, at = rng.permutation(sum(need)), [], 0
+    for n, p in zip(lens, need):
+        slots += [int(order[at + t // page]) * page + t % page for t in range(n)]
+        at += p
+    host = ref.Cache(sum(need), heads, DIM, page)
+    cache = host.device(torch)
+    k, v = rng.standard_normal((2, sum(lens), heads, DIM)).astype(np.float32)
+    eng.kv8_append(cuda(k), cuda(v), cache, torch.tensor(slots, device="cuda"))
+    host.append((k, v), slots)
+    for x, y in zip(cache, host.device(torch)):
+        assert torch.equal(x, y)

@@ -252,9 +252,10 @@ struct AppendArgs {
     int lanes;      // that share a key for that
     int tokens;
     int windows;  // of 64 tokens
-    // workgroups that a window's pages are dealt out to, for one head of keys or of values; where that is one, it takes the
-    // first `first` of them, and `helpers` share the further ones of every groups-th window
-    int turns, first, groups, helpers;
+    // workgroups that a window's pages are dealt out to, for one head of keys or of values, and those of the last window
+    // (no more than its tokens); where that is one, it takes the first `first` of them, and `helpers` share the further ones
+    // of every groups-th window
+    int turns, last, first, groups, helpers;
     long blocks;
 };
 
@@ -528,7 +529,7 @@ struct Jobs {
 // One token for each of 64 sequences (8 heads of 128, pages of 64, fp32): 10.3
 // us, where a page that grows is read and written; a workgroup waits for its
 // slots, its rows, their largest, the scale and the codes one after the other.
-// Prompts of 1955 tokens in all (fp16, 32 + 8 heads of 128, pages of 16): 18.5 us.
+// Prompts of 1955 tokens in all (fp16, 32 + 8 heads of 128, pages of 16): 18.9 us.
 //
 // Normed keys: a row is dealt out to lanes that share its sum of squares, two
 // rows at a time (four: 3218 tokens of prompts 30.4 us instead of 31.0, but 48
@@ -588,7 +589,13 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs g, Q q) {
             append_page<T, V, false, NORM, P>(g, run, head, tid, image, red, factors);
     };
     if constexpr (!HELP) {
-        const int turn = b / g.windows, from = (b - turn * g.windows) * 64;
+        int turn = 0, windows = g.windows;  // all windows' first workgroups come first
+        if (b >= g.last * windows) {
+            turn = g.last;
+            b -= turn * windows--;
+        }
+        const int row = b / windows, from = (b - row * windows) * 64;
+        turn += row;
         const long here = slot(from + lane), behind = slot((long)from - 1);
         uint64_t todo = begun(from, here, behind, [&](int) { return true; });
         for (int left = turn; todo; todo &= todo - 1) {
@@ -718,25 +725,28 @@ static int append(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v,
     g.turn = {positions, table, half, max_pos, flags};
     g.tokens = tokens;
     g.windows = ceil_div(tokens, 64);
-    // A workgroup for each token while they are few (a batch's next tokens, each on a page of its own: with the pages'
-    // values read back, 64 sequences 28 us, with 8 workgroups for 64 tokens 45), then as many as give each CU four, at
-    // least eight for 64 tokens (2048 sequences' single tokens, 8 heads, pages of 16: 92 us, with four 105).  One that finds
-    // none to do costs its launch and its look at 64 slots, and prompts begin few pages.  So where eight for each 64 tokens
-    // are more than twice what the card holds at a time, there is one, which takes the pages that a prompt begins there, and
-    // as many as are surely at work at a time share the others (fp16, with q, four heads for each of keys, pages of 64; us
-    // with these, with eight in any case, and with one alone: 8 heads, a prompt of 16000 tokens 97, 131 and 94; 8192
-    // sequences' single tokens 492, 492 and 614; 300 of them before a prompt of 8000 58, 84 and 200).
-    const long pairs = 2l * cache->kv_heads, held = norm ? 1024 : 2048;  // (at work at a time)
-    g.turns = tokens <= 256 ? 64 : 8 * pairs * g.windows > 2 * held ? 1 : (int)std::min(32l, std::max(8l, 1024 / (pairs * g.windows)));
-    if (g.turns == 1) {
+    // A workgroup for each token (a batch's next tokens, each on a page of its own) as long as all are surely at work at a
+    // time, then as many for 64 tokens as that is, at least eight (us, fp16, with q, four heads for each of keys, pages of 16;
+    // 8 heads, single tokens of 65, 128, 200 and 2048 sequences 9.6, 12.5, 16.3 and 92, with 64 for 64 tokens 14.7, 15.2, 25
+    // and more, with four 105 of 2048).  One that finds no page to begin costs its launch and its look at 64 slots, and
+    // prompts begin few.  So where eight for each 64 tokens are more than twice what the card holds there is one, which takes
+    // the pages that a prompt begins there, and as many as are surely at work at a time share the others (pages of 64; us with
+    // these, with eight in any case, and with one alone: a prompt of 16000 tokens 97, 131 and 94; 8192 sequences' single
+    // tokens 492, 492 and 614; 300 of them before a prompt of 8000 58, 84 and 200; 4096 255, with 1792 workgroups that share,
+    // some of which begin when others have ended, 349).
+    const long pairs = 2l * cache->kv_heads, most = norm ? 1024 : 1536, held = norm ? 1024 : 2048;
+    if (8 * pairs * g.windows <= 2 * held) {
+        g.turns = pairs * tokens <= most ? 64 : (int)std::min(64l, std::max(8l, most / (pairs * g.windows)));
+        g.last = std::min(g.turns, tokens - 64 * (g.windows - 1));
+        g.blocks = pairs * ((long)g.windows * g.turns - (g.turns - g.last));
+    } else {
         g.first = std::max(64 / g.c.page + 1, 4);
-        // (4096 single tokens 255 us; with 1792 of them, some of which begin when others have ended, 349)
-        const int all = std::max(8, (norm ? 1024 : 1536) / (int)pairs);
+        const int all = std::max(8, (int)(most / pairs));
         // enough groups for one look at each one's windows, and for all helpers; at least six of these in each
         g.groups = std::min({g.windows, all / 6, std::max(ceil_div(g.windows, 4 * kLooks), ceil_div(all, 64))});
         g.helpers = std::min(64, all / g.groups);
+        g.blocks = pairs * std::max((long)g.windows, (long)g.groups * g.helpers);
     }
-    g.blocks = pairs * std::max((long)g.windows * g.turns, (long)g.groups * g.helpers);
     RopeArgs r{};
     r.turn = g.turn;
     r.tokens = tokens;
