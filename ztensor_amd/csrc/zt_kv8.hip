@@ -529,7 +529,7 @@ struct Jobs {
 // One token for each of 64 sequences (8 heads of 128, pages of 64, fp32): 10.3
 // us, where a page that grows is read and written; a workgroup waits for its
 // slots, its rows, their largest, the scale and the codes one after the other.
-// Prompts of 1955 tokens in all (fp16, 32 + 8 heads of 128, pages of 16): 18.9 us.
+// Prompts of 1955 tokens in all (fp16, 32 + 8 heads of 128, pages of 16): 17.1 us.
 //
 // Normed keys: a row is dealt out to lanes that share its sum of squares, two
 // rows at a time (four: 3218 tokens of prompts 30.4 us instead of 31.0, but 48
@@ -726,17 +726,17 @@ static int append(const zt_kv8_cache* cache, const zt_rows* k, const zt_rows* v,
     g.tokens = tokens;
     g.windows = ceil_div(tokens, 64);
     // A workgroup for each token (a batch's next tokens, each on a page of its own) as long as all are surely at work at a
-    // time, then as many for 64 tokens as that is, at least eight (us, fp16, with q, four heads for each of keys, pages of 16;
-    // 8 heads, single tokens of 65, 128, 200 and 2048 sequences 9.6, 12.5, 16.3 and 92, with 64 for 64 tokens 14.7, 15.2, 25
-    // and more, with four 105 of 2048).  One that finds no page to begin costs its launch and its look at 64 slots, and
-    // prompts begin few.  So where eight for each 64 tokens are more than twice what the card holds there is one, which takes
-    // the pages that a prompt begins there, and as many as are surely at work at a time share the others (pages of 64; us with
-    // these, with eight in any case, and with one alone: a prompt of 16000 tokens 97, 131 and 94; 8192 sequences' single
-    // tokens 492, 492 and 614; 300 of them before a prompt of 8000 58, 84 and 200; 4096 255, with 1792 workgroups that share,
-    // some of which begin when others have ended, 349).
-    const long pairs = 2l * cache->kv_heads, most = norm ? 1024 : 1536, held = norm ? 1024 : 2048;
-    if (8 * pairs * g.windows <= 2 * held) {
-        g.turns = pairs * tokens <= most ? 64 : (int)std::min(64l, std::max(8l, most / (pairs * g.windows)));
+    // time; then as many for 64 tokens as that is, if at least five, else as twice that is (us, fp16, with q, four heads for
+    // each of keys, pages of 16; 8 heads, single tokens of 65, 128, 200, 1024 and 2048 sequences 10.7, 12.9, 15.7, 47 and 90;
+    // with 64 for 64 tokens 14.7, 15.2 and 25, with eight 59 and 93, with four 57 and 106).  One that finds no page to begin
+    // costs its launch and its look at 64 slots, and prompts begin few.  So where twice would be few, too, there is one, which
+    // takes the pages that a prompt begins there, and as many as are surely at work at a time share the others (pages of 64;
+    // us with these, with eight in any case, and with one alone: a prompt of 16000 tokens 97, 131 and 94; 8192 sequences'
+    // single tokens 492, 492 and 614; 300 of them before a prompt of 8000 58, 84 and 200; 4096 255, with 1792 workgroups that
+    // share, some of which begin when others have ended, 349).
+    const long pairs = 2l * cache->kv_heads, most = norm ? 1024 : 1536, once = most / (pairs * g.windows);
+    if (pairs * g.windows <= (norm ? 256 : 512)) {
+        g.turns = pairs * tokens <= most ? 64 : (int)std::min(64l, once >= 5 ? once : 2 * most / (pairs * g.windows));
         g.last = std::min(g.turns, tokens - 64 * (g.windows - 1));
         g.blocks = pairs * ((long)g.windows * g.turns - (g.turns - g.last));
     } else {
