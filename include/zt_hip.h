@@ -819,7 +819,8 @@ int zt_kv8_attention(const zt_kv8_attn* a, void* workspace, long workspace_bytes
  * that is negative), mask [tokens][words]: its bit and those of the rows above it
  * among the first 64 words.  Rows of no request get position 0 and no bits.
  * words from 1 to ZT_TREE_WORDS; outputs share no bytes with inputs nor with each
- * other, else InvalidValue. */
+ * other, else InvalidValue.  (A row's path is followed step by step, from the
+ * request's row 64 ZT_TREE_WORDS on with a wait for memory each.) */
 #define ZT_TREE_WORDS 16
 int zt_kv8_tree(const int* parents, const int* kv_lens, const int* q_start, int requests, int tokens, int words,
                 int* positions, uint64_t* mask, zt_stream_t stream);
