@@ -520,13 +520,12 @@ struct Jobs {
 // A workgroup looks at a window of 64 tokens: those whose page is not that of the
 // one before (tokens that are left out do not come between) begin a page's tokens.
 // It takes every turns-th of them, each with all that follow on its page; or
-// (HELP) the first few, and the first workgroups also take their part of what
-// crowded windows have besides: of one that others share too, page i of window k of
-// the group is helper (61 k + i) % helpers', which spreads them evenly, whatever
-// their number in a window.  q's rotation rides along as more workgroups, instead
-// of a launch of its own.
+// (HELP) the first few, and the call's first workgroups also take their part of
+// what crowded windows have besides: page i of the k-th window of a group is helper
+// (61 k + i) % helpers', which spreads pages evenly however many a window has.  q's
+// rotation rides along as more workgroups, instead of a launch of its own.
 //
-// One token for each of 64 sequences (8 heads of 128, pages of 64, fp32): 10.3
+// One token for each of 64 sequences (8 heads of 128, pages of 64, fp32): 10.4
 // us, where a page that grows is read and written; a workgroup waits for its
 // slots, its rows, their largest, the scale and the codes one after the other.
 // Prompts of 1955 tokens in all (fp16, 32 + 8 heads of 128, pages of 16): 17.1 us.

@@ -547,7 +547,7 @@ __device__ __forceinline__ Forked forked(const ForkArgs& g, int i) {
 // wait for each other, no second launch.  A fork whose target an earlier one has
 // takes none; whether there may be any, a bit of LDS for each row says (past 2^18
 // rows two may share one: then the earlier forks are looked through for nothing).
-// 4 forks of 500 tokens 4.2 us, 160 of 1500 6.4.
+// 4 forks of 500 tokens 4.0 us, 160 of 1500 6.6.
 constexpr int kMet = 1 << 18;  // rows that have bits of their own
 __global__ __launch_bounds__(kThreads) void fork_kernel(ForkArgs g) {
     extern __shared__ uint32_t met[];  // of min(rows, kMet) bits
